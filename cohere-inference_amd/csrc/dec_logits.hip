@@ -1,0 +1,163 @@
+// Rules on a decoding step's logits, before the greedy choice: penalties for repeated tokens, biases and grammar masks,
+// for gfx950. No counterpart in the reference, which picks from the bare logits (kernels/csrc/decoder_ops.cu:106-159).
+//
+// Row r is slot s = active[r], p = pos[s] the position of its newest token. For token v, seen c times among the slot's
+// tokens at first[s]..p, with (rep, presence, frequency) = pen[s]:
+//   c > 0:  l = l / rep (l > 0) or l rep (otherwise), then l -= c frequency + presence
+//   l += bias[bias_of[s]][v];   l = -inf where the mask row of the grammar's state lacks v
+// in fp32, each operation rounded by itself, the result rounded once to bf16 (what the pick reads).
+//
+// The counts are made anew from the slot's tokens in every call (a workgroup counts, in LDS, the tokens of its own part
+// of the vocabulary): no counts to keep per slot (4 bytes x vocabulary x slots), to clear when a slot is taken over or
+// to wind back. Integer additions: their order does not show.
+// The grammar's state at p is start[s] until the prompt has been read (p < plen[s]), then trans[state at p - 1][class of
+// the token at p]; the state at p is kept in state[s][p % 2] beside the one it came from, so that every workgroup can
+// derive it, a call repeated at one position gives the same, and a captured step needs nothing from the host.
+#include "cohere_hip.h"
+#include "common.h"
+
+#include <string>
+
+namespace {
+
+struct LogitArgs {
+  const uint16_t* x;
+  uint16_t* y;
+  int64_t ldx, ldy;
+  const int32_t *active, *pos;
+  const int64_t* tokens;
+  const int32_t *first, *plen;
+  const float* pen;  // (S, 3) or null
+  const uint16_t* bias;  // (B, V) or null
+  const int32_t* bias_of;
+  const uint8_t* mask;  // (M, 4 ceil(V / 32)) bytes or null
+  const int32_t *classes, *trans, *start;  // classes and trans null: the state stays start[s]
+  int32_t* state;
+  int S, V, OUT, B, M, C;
+};
+
+constexpr int NT = 256;
+
+// J chunks of 8 logits a thread: a workgroup takes J * 2048 logits
+template <int J>
+__global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
+  constexpr int SPAN = J * NT * 8;
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[SPAN];
+  const int r = blockIdx.y, tid = threadIdx.x, v0 = blockIdx.x * SPAN;
+  const uint16_t* xr = a.x + (int64_t)r * a.ldx;
+  uint16_t* yr = a.y + (int64_t)r * a.ldy;
+  uint4 u[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int v = v0 + (j * NT + tid) * 8;
+    u[j] = v < a.V ? *reinterpret_cast<const uint4*>(xr + v) : make_uint4(0, 0, 0, 0);
+  }
+  const int s = a.active[r];
+  const bool known = (unsigned)s < (unsigned)a.S;  // a row of no slot is copied
+  float rep = 1.f, presence = 0.f, freq = 0.f;
+  int p = 0, state = -1, b = -1;
+  bool penal = false;
+  if (known) {
+    p = a.pos[s];
+    if (a.pen) {
+      rep = a.pen[s * (int64_t)3];
+      presence = a.pen[s * (int64_t)3 + 1];
+      freq = a.pen[s * (int64_t)3 + 2];
+      penal = rep != 1.f || presence != 0.f || freq != 0.f;
+    }
+    if (a.bias) b = a.bias_of[s];
+    if (a.mask) {
+      state = a.start[s];
+      if (a.trans && p >= a.plen[s]) {
+        state = a.state[s * (int64_t)2 + ((p + 1) & 1)];
+        const int64_t t = p >= 0 && p < a.OUT ? a.tokens[(int64_t)s * a.OUT + p] : -1;
+        const int cls = t >= 0 && t < a.V ? a.classes[t] : -1;
+        state = (unsigned)state < (unsigned)a.M && (unsigned)cls < (unsigned)a.C
+                    ? a.trans[(int64_t)state * a.C + cls] : -1;
+      }
+      if (a.trans && blockIdx.x == 0 && tid == 0) a.state[s * (int64_t)2 + (p & 1)] = state;
+    }
+  }
+  const int lo = known && penal ? (a.first[s] > 0 ? a.first[s] : 0) : 0, hi = p < a.OUT ? p : a.OUT - 1;
+  penal = penal && lo <= hi;
+  if (penal) {
+#pragma unroll
+    for (int j = 0; j < 2 * J; ++j)
+      *reinterpret_cast<uint4*>(&cnt[(j * NT + tid) * 4]) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const int64_t* t = a.tokens + (int64_t)s * a.OUT;
+    for (int i = lo + tid; i <= hi; i += NT) {
+      const int64_t d = t[i] - v0;
+      if (d >= 0 && d < SPAN) atomicAdd(&cnt[d], 1u);
+    }
+    __syncthreads();
+  }
+  const uint16_t* br = (unsigned)b < (unsigned)a.B ? a.bias + (int64_t)b * a.V : nullptr;
+  const uint8_t* mr =
+      (unsigned)state < (unsigned)a.M ? a.mask + (int64_t)state * ((a.V + 31) / 32 * 4) : nullptr;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int at = (j * NT + tid) * 8, v = v0 + at;
+    if (v >= a.V) continue;
+    const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    if (penal) {
+      const uint4 c0 = *reinterpret_cast<const uint4*>(&cnt[at]), c1 = *reinterpret_cast<const uint4*>(&cnt[at + 4]);
+      const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c[k]) {
+          f[k] = f[k] > 0.f ? f[k] / rep : f[k] * rep;
+          f[k] -= (float)c[k] * freq + presence;
+        }
+    }
+    if (br) {
+      const uint4 t = *reinterpret_cast<const uint4*>(br + v);
+      const uint32_t bw[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] += __uint_as_float(k & 1 ? bw[k >> 1] & 0xffff0000u : bw[k >> 1] << 16);
+    }
+    if (mr) {
+      const uint32_t bits = mr[v >> 3];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (!(bits >> k & 1)) f[k] = -INFINITY;
+    }
+    *reinterpret_cast<uint4*>(yr + v) =
+        make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
+  }
+}
+
+bool al(const void* q, int n) { return (reinterpret_cast<uintptr_t>(q) & (n - 1)) == 0; }
+
+}  // namespace
+
+extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int64_t V,
+                                 const int32_t* active, const int32_t* pos, int64_t slots, const int64_t* tokens,
+                                 int64_t OUT, const int32_t* first, const int32_t* plen, const float* pen,
+                                 const uint16_t* bias, int64_t B, const int32_t* bias_of, const int32_t* mask, int64_t M,
+                                 const int32_t* classes, const int32_t* trans, int64_t C, const int32_t* start,
+                                 int32_t* state, void* stream) {
+  cohere::clear_error();
+  const int64_t top = 0x7fffffff;
+  COHERE_REQUIRE(rows >= 0 && rows <= 65535 && V > 0 && V % 8 == 0 && V < (int64_t(1) << 30) && slots > 0 &&
+                     slots <= top && OUT > 0 && OUT <= top,
+                 "dec_logits: bad sizes (the vocabulary a multiple of 8)");
+  COHERE_REQUIRE(x && y && al(x, 16) && al(y, 16) && ldx >= V && ldy >= V && ldx % 8 == 0 && ldy % 8 == 0,
+                 "dec_logits: logits rows must be 16-byte aligned");
+  COHERE_REQUIRE(active && pos && (!pen || (tokens && first)), "dec_logits: bad pointer");
+  COHERE_REQUIRE(!bias || (bias_of && B > 0 && B <= top && al(bias, 16)), "dec_logits: bias rows need bias_of");
+  COHERE_REQUIRE(!mask || (start && M > 0 && M <= top), "dec_logits: masks need start");
+  COHERE_REQUIRE(!classes == !trans && (!trans || (mask && tokens && plen && state && C > 0 && C <= top)),
+                 "dec_logits: a grammar needs masks, classes, transitions, prompt lengths and states");
+  if (rows == 0) return 0;
+  const LogitArgs a{x, y, ldx, ldy, active, pos, tokens, first, plen, pen, bias, bias_of,
+                    reinterpret_cast<const uint8_t*>(mask), classes, trans, start, state, (int)slots, (int)V, (int)OUT,
+                    (int)B, (int)M, (int)C};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  constexpr int J = 2;
+  dec_logits_kernel<J><<<dim3((unsigned)((V + J * 2048 - 1) / (J * 2048)), (unsigned)rows), NT, 0, s>>>(a);
+  return cohere::check_launch("dec_logits");
+}

@@ -570,7 +570,8 @@ __global__ void __launch_bounds__(256) dec_pick_kernel(const uint16_t* __restric
         }
       const int at = pos0 + 1;
       const bool in_prompt = at < plen0;
-      const int64_t nt = in_prompt ? forced0 : (int64_t)arg;
+      // no logit above -inf (a mask that leaves nothing, NaN): the row ends
+      const int64_t nt = in_prompt ? forced0 : arg == 0x7fffffff ? eos : (int64_t)arg;
       const uint8_t fin = (!in_prompt && (nt == eos || at >= lim0)) ? 1 : 0;
       out[(int64_t)s * OUT + at] = nt;
       tok[s] = nt;

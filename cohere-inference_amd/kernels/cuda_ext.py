@@ -40,7 +40,8 @@ EXPORTS = ("cohere_gemm_i8", "cohere_gemm_sp", "cohere_quantize_rows", "cohere_l
            "cohere_encoder_layers_noalloc", "cohere_dec_linear_fused", "cohere_dec_pick_embed",
            "cohere_gemm_sp_tiled", "cohere_pack_24_tiled_bytes", "cohere_pack_24_tiled", "cohere_sub_conv0_dw_pw",
            "cohere_sub_dw_pw", "cohere_gemm_kv", "cohere_gemm_kv_q8", "cohere_gemm_tile",
-           "cohere_piece_rows")
+           "cohere_piece_rows", "cohere_dec_attention_q4", "cohere_dec_attention_q4_splits", "cohere_dec_scatter_kv_q4",
+           "cohere_dec_gather_kv_q4", "cohere_dec_logits")
 
 
 def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
@@ -71,6 +72,11 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "cohere_dec_add_ln": [P, P, I64, P, P, F, P, I64, I64, P],
         "cohere_dec_attention": [I32, P, I64, P, I64, P, P, P, I64, I64, I64, F, I64, P, I64, P, P],
         "cohere_dec_attention_q8": [I32, P, I64, P, I64, P, P, P, P, P, I64, I64, I64, F, I64, P, I64, P, P],
+        "cohere_dec_attention_q4": [I32, P, I64, P, I64, P, P, P, P, P, I64, I64, I64, I64, F, I64, P, I64, P, P],
+        "cohere_dec_scatter_kv_q4": [P, I64, I64, P, P, P, P, P, P, I64, I64, I64, I64, P],
+        "cohere_dec_gather_kv_q4": [P, P, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
+        "cohere_dec_logits": [P, I64, P, I64, I64, I64, P, P, I64, P, I64, P, P, P, P, I64, P, P, I64, P, P, I64, P, P,
+                              P],
         "cohere_dec_pick": [P, I64, I64, P, I64, P, P, P, P, I64, P, P, P, I64, I64, I64, P],
         "cohere_dec_pick_embed": [P, I64, I64, P, I64, P, P, P, P, I64, P, P, P, I64, I64, I64, P, P, P, P, F, P, P, F,
                                   P, P, I64, P, P],
@@ -98,6 +104,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.cohere_encoder_workspace_bytes.restype = I64
     lib.cohere_encoder_branch_workspace_bytes.argtypes = [I64, I64, I32]
     lib.cohere_encoder_branch_workspace_bytes.restype = I64
+    lib.cohere_dec_attention_q4_splits.argtypes = [I64, I64, I64, I64]
+    lib.cohere_dec_attention_q4_splits.restype = I64
     lib.cohere_logmel_workspace_bytes.argtypes = [I64]
     lib.cohere_logmel_workspace_bytes.restype = I64
     lib.cohere_last_error.restype = ctypes.c_char_p
@@ -114,6 +122,16 @@ def _check(cond: bool, msg: str) -> None:
 
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
+
+
+def _here(what: str, *tensors) -> None:
+    """Every tensor (None: absent) on the current GPU, whose stream the launch takes."""
+    at = {t.get_device() for t in tensors if t is not None}
+    _check(at == {torch.cuda.current_device()} if -1 not in at else False, f"{what}: tensors on the current GPU expected")
+
+
+def _i32(t, n: int) -> bool:
+    return t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n
 
 
 _EMPTY = torch.empty(0)  # an absent per-layer tensor
@@ -623,6 +641,117 @@ class _Ext:
                    "gemm_kv: fp32 scales")
             self._call("cohere_gemm_kv_q8", _ptr(a), a.stride(0), _ptr(w), _ptr(bias), a.shape[0], a.shape[1],
                        _ptr(slot_of), _ptr(frame_of), _ptr(ck), _ptr(cv), _ptr(cks), _ptr(cvs), L, S, H, T, _stream())
+
+    # ---- caches in 4 bits, rules on logits (no counterpart in the reference) -----------------------------------------
+
+    @staticmethod
+    def _q4_checks(what, k4, v4, ks, vs, dims):
+        """The caches' leading sizes: codes uint8 (..., 64) and maxima bf16 (..., 4), keys and values alike."""
+        _check(k4.dim() == dims + 1 and k4.shape == v4.shape and k4.shape[-1] == 64 and
+               k4.dtype == v4.dtype == torch.uint8 and k4.is_contiguous() and v4.is_contiguous(),
+               f"{what}: contiguous uint8 caches of 64 bytes a vector")
+        _check(ks.shape == vs.shape == (*k4.shape[:-1], 4) and ks.dtype == vs.dtype == torch.bfloat16 and
+               ks.is_contiguous() and vs.is_contiguous(), f"{what}: contiguous bf16 maxima, 4 a vector")
+        _check(k4.numel() > 0, f"{what}: empty caches")
+        return k4.shape[:-1]
+
+    def dec_attention_q4_splits(self, rows, heads, kv_heads, T) -> int:
+        """The `splits` that fill the GPU in a dec_attention_q4 call of these sizes."""
+        return int(self._lib.cohere_dec_attention_q4_splits(int(rows), int(heads), int(kv_heads), int(T)))
+
+    def dec_attention_q4(self, self_attn, active, q, k4, v4, ks, vs, n, scale, splits, part, out):
+        """dec_attention over caches in 4 bits: codes k4, v4 uint8 (slots, KV, T, 64) and maxima ks, vs bf16 (slots, KV,
+        T, 4), H = out.shape[1] / 128 query heads, H / KV of them to a key head. Self-attention: q (rows, (H + 2 KV) 128)
+        holds the new token's queries, keys and values, appended at position n[slot] and attended as computed. Rows
+        without keys, of slots out of range or (self-attention) of positions beyond T get zeros. splits > 1 needs part
+        (rows x H x splits x 130 floats). kernels.stream_decoder.quantize_q4 states the form."""
+        S, KV, T = self._q4_checks("dec_attention_q4", k4, v4, ks, vs, 3)
+        _check(q.dim() == 2 and out.dim() == 2 and q.dtype == out.dtype == torch.bfloat16 and
+               (q.stride(1) == 1 or q.shape[1] == 1) and out.is_contiguous() and out.shape[0] == q.shape[0],
+               "dec_attention_q4: bf16 q (rows, ...) with unit column stride, contiguous out (rows, H * 128)")
+        rows, H = q.shape[0], out.shape[1] // 128
+        _check(H > 0 and out.shape[1] % 128 == 0 and H % KV == 0 and
+               q.shape[1] >= (H + (2 * KV if self_attn else 0)) * 128, "dec_attention_q4: heads")
+        splits = int(splits)
+        _check(1 <= splits <= 64 and (splits == 1 or (part is not None and part.dtype == torch.float32 and
+               part.is_contiguous() and part.numel() >= rows * H * splits * 130)),
+               "dec_attention_q4: 1 to 64 splits, more than 1 need part")
+        _check(_i32(active, rows) and _i32(n, S), "dec_attention_q4: int32 active per row, n per slot")
+        if rows == 0:
+            return
+        _here("dec_attention_q4", active, q, k4, v4, ks, vs, n, part, out)
+        self._call("cohere_dec_attention_q4", int(bool(self_attn)), _ptr(active), rows, _ptr(q), q.stride(0), _ptr(k4),
+                   _ptr(v4), _ptr(ks), _ptr(vs), _ptr(n), S, H, KV, T, float(scale), splits, _ptr(part),
+                   part.numel() if part is not None else 0, _ptr(out), _stream())
+
+    def _kv_q4_checks(self, what, kv, slot_of, frame_of, ck, cv, cks, cvs):
+        L, S, H, T = self._q4_checks(what, ck, cv, cks, cvs, 4)
+        _check(kv.dim() == 2 and kv.dtype == torch.bfloat16 and kv.stride(1) == 1 and kv.shape[1] == L * 2 * H * 128,
+               f"{what}: bf16 kv (rows, L * 2 * H * 128) with unit column stride")
+        _check(_i32(slot_of, kv.shape[0]) and _i32(frame_of, kv.shape[0]), f"{what}: int32 slot and position per row")
+        return L, S, H, T
+
+    def dec_scatter_kv_q4(self, kv, slot_of, frame_of, ck, cv, cks, cvs):
+        """dec_scatter_kv into 4-bit caches (L, S, H, T, 64) with maxima (L, S, H, T, 4); rows of slots or positions out
+        of range go nowhere."""
+        L, S, H, T = self._kv_q4_checks("dec_scatter_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
+        if kv.shape[0] == 0:
+            return
+        _here("dec_scatter_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
+        self._call("cohere_dec_scatter_kv_q4", _ptr(kv), kv.stride(0), kv.shape[0], _ptr(slot_of), _ptr(frame_of),
+                   _ptr(ck), _ptr(cv), _ptr(cks), _ptr(cvs), L, S, H, T, _stream())
+
+    def dec_gather_kv_q4(self, slot_of, frame_of, ck, cv, cks, cvs, kv):
+        """What 4-bit caches hold of (slot, position) pairs, as bf16 rows laid out as dec_scatter_kv_q4 takes them (to
+        move a slot to a decoder with other caches, or to look at it); zeros for slots or positions out of range."""
+        L, S, H, T = self._kv_q4_checks("dec_gather_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
+        if kv.shape[0] == 0:
+            return
+        _here("dec_gather_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
+        self._call("cohere_dec_gather_kv_q4", _ptr(slot_of), _ptr(frame_of), kv.shape[0], _ptr(ck), _ptr(cv), _ptr(cks),
+                   _ptr(cvs), L, S, H, T, _ptr(kv), kv.stride(0), _stream())
+
+    def dec_logits(self, logits, y, active, pos, tokens=None, first=None, plen=None, penalties=None, bias=None,
+                   bias_of=None, mask=None, classes=None, trans=None, start=None, state=None):
+        """Rules on a step's logits (rows, V) into y (which may be logits), before dec_pick: of slot s = active[r] at
+        position pos[s], penalties fp32 (slots, 3) (repetition, presence, frequency) for the tokens tokens[s,
+        first[s]..pos[s]], bias row bias_of[s] of bias bf16 (B, V), and -inf for what the mask row of the grammar's state
+        lacks: mask int32 (M, ceil(V / 32)), start int32 (slots), and with classes int32 (V), trans int32 (M, C) and
+        state int32 (slots, 2) the state moves with every token behind the prompt (plen). Absent rules are None; index
+        values out of range switch a rule off for a slot."""
+        _check(logits.dim() == 2 and logits.shape == y.shape and logits.dtype == y.dtype == torch.bfloat16 and
+               logits.stride(1) == y.stride(1) == 1 and logits.shape[1] % 8 == 0 and logits.shape[1] > 0,
+               "dec_logits: bf16 logits and y (rows, V), unit column stride, V % 8 == 0")
+        rows, V = logits.shape
+        S = pos.numel()
+        _check(_i32(active, rows) and _i32(pos, 1) and (first is None or _i32(first, S)) and
+               (plen is None or _i32(plen, S)), "dec_logits: int32 active per row, pos, first, plen per slot")
+        _check(tokens is None or (tokens.dtype == torch.int64 and tokens.dim() == 2 and tokens.shape[0] >= S and
+                                  tokens.shape[1] > 0 and tokens.is_contiguous()),
+               "dec_logits: contiguous int64 tokens (slots, positions)")
+        _check(penalties is None or (penalties.dtype == torch.float32 and penalties.shape == (S, 3) and
+                                     penalties.is_contiguous() and tokens is not None and first is not None),
+               "dec_logits: penalties fp32 (slots, 3) need tokens and first")
+        _check(bias is None or (bias.dtype == torch.bfloat16 and bias.dim() == 2 and bias.shape[0] > 0 and
+                                bias.shape[1] == V and bias.is_contiguous() and bias_of is not None and
+                                _i32(bias_of, S)), "dec_logits: bias bf16 (B, V) needs int32 bias_of per slot")
+        _check(mask is None or (mask.dim() == 2 and mask.shape[0] > 0 and mask.shape[1] == (V + 31) // 32 and
+                                _i32(mask, 1) and start is not None and _i32(start, S)),
+               "dec_logits: mask int32 (M, ceil(V / 32)) needs int32 start per slot")
+        _check((classes is None) == (trans is None) and (classes is None or (
+            mask is not None and classes.numel() == V and _i32(classes, V) and trans.dim() == 2 and
+            trans.shape[0] == mask.shape[0] and trans.shape[1] > 0 and _i32(trans, 1) and state is not None and
+            state.shape == (S, 2) and _i32(state, 1) and tokens is not None and plen is not None)),
+            "dec_logits: a grammar needs mask, classes (V), trans (M, C), state (slots, 2), tokens and plen")
+        if rows == 0:
+            return
+        _here("dec_logits", logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask, classes, trans,
+              start, state)
+        self._call("cohere_dec_logits", _ptr(logits), logits.stride(0), _ptr(y), y.stride(0), rows, V, _ptr(active),
+                   _ptr(pos), S, _ptr(tokens), tokens.shape[1] if tokens is not None else 1, _ptr(first), _ptr(plen),
+                   _ptr(penalties), _ptr(bias), bias.shape[0] if bias is not None else 0, _ptr(bias_of), _ptr(mask),
+                   mask.shape[0] if mask is not None else 0, _ptr(classes), _ptr(trans),
+                   trans.shape[1] if trans is not None else 0, _ptr(start), _ptr(state), _stream())
 
 
 _lib = load_library()

@@ -88,6 +88,29 @@ def bf16_linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, relu: 
     return y
 
 
+# ---- caches in 4 bits -------------------------------------------------------------------------------------------------
+
+def quantize_q4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 vectors (..., 128) in the 4-bit caches' form, as the kernels write it: codes uint8 (..., 64), byte j dimension
+    2j in the low nibble and 2j + 1 in the high one (two's complement), and the maxima m bf16 (..., 4) of the four groups
+    of 32 values. A code is round_half_even(7 x / m), -7..7 (0 where m = 0). A group with a NaN or an infinity holds the
+    maximum NaN and codes 0."""
+    g = x.double().reshape(*x.shape[:-1], 4, 32)
+    m = g.abs().amax(-1, keepdim=True)
+    ok = torch.isfinite(m) & (m > 0)
+    c = torch.where(ok, torch.round(7 * g / torch.where(ok, m, torch.ones_like(m))), torch.zeros_like(g))
+    n = (c.to(torch.int32) & 15).reshape(*x.shape[:-1], 64, 2)
+    held = torch.where(torch.isfinite(m), m, torch.full_like(m, float("nan"))).squeeze(-1).to(torch.bfloat16)
+    return (n[..., 0] | (n[..., 1] << 4)).to(torch.uint8), held
+
+
+def dequantize_q4(codes: torch.Tensor, maxima: torch.Tensor) -> torch.Tensor:
+    """The values c m / 7 (fp32, rounded once) of codes (..., 64) and maxima (..., 4)."""
+    n = torch.stack((codes & 15, codes >> 4), -1).reshape(*codes.shape[:-1], 4, 32).to(torch.float64)
+    c = torch.where(n > 7, n - 16, n)
+    return (c * maxima.double().unsqueeze(-1) / 7).float().reshape(*codes.shape[:-1], 128)
+
+
 # ---- the decoder and its captured step ------------------------------------------------------------------------------
 
 class _Projection:
@@ -461,5 +484,5 @@ class StreamDecoder:
         return sum(p.nbytes for blk in self.blocks for p in blk.projections()) + self.head.nbytes
 
 
-__all__ = ["DEFAULT_CONFIG", "StreamDecoder", "W8_CONFIGS", "W8_PERM", "bf16_linear", "prepare_w8", "unprepare_w8",
-           "w8_config", "w8_linear"]
+__all__ = ["DEFAULT_CONFIG", "StreamDecoder", "W8_CONFIGS", "W8_PERM", "bf16_linear", "dequantize_q4", "prepare_w8",
+           "quantize_q4", "unprepare_w8", "w8_config", "w8_linear"]

@@ -209,7 +209,7 @@ int cohere_dec_attention_q8(int32_t self, const int32_t* active, int64_t rows, c
  * per row (slot s = active[r], skipped when s == dummy or finished[s]): the first index of the maximum of logits bf16
  * [rows, V]; at = pos[s] + 1; the token is forced[s, at] (int64 [slots, FP]) while at < plen[s], else the argmax;
  * out[s, at] = tok[s] = token (out int64 [slots, OUT]); pos[s] = at; finished[s] = 1 at eos or at >= limit[s]
- * outside the prompt. V % 8 == 0. */
+ * outside the prompt. A row without a logit above -inf picks eos. V % 8 == 0. */
 int cohere_dec_pick(const uint16_t* logits, int64_t rows, int64_t V, const int32_t* active, int64_t dummy,
                     int64_t* tok, int32_t* pos, uint8_t* finished, const int64_t* forced, int64_t FP,
                     const int32_t* plen, const int32_t* limit, int64_t* out, int64_t OUT, int64_t pad, int64_t eos,
@@ -252,6 +252,60 @@ int cohere_gemm_kv(const uint16_t* a, int64_t lda, const uint16_t* w, const uint
 int cohere_gemm_kv_q8(const uint16_t* a, int64_t lda, const uint16_t* w, const uint16_t* bias, int64_t M, int64_t K,
                       const int32_t* slot_of, const int32_t* frame_of, int8_t* ck, int8_t* cv, float* cks, float* cvs,
                       int64_t L, int64_t S, int64_t H, int64_t T, void* stream);
+
+/* ---- caches in 4 bits, rules on logits (no counterpart in the reference) --------------------------------------------
+ * A 128-vector in 4 bits: four groups of 32 values, each with its largest magnitude m (bf16) and codes
+ * c = round_half_even(7 x / m) in -7 .. 7 (0 where m = 0), the value held c m / 7. Codes: 64 bytes, byte j dimension 2j
+ * in the low nibble and 2j + 1 in the high one, two's complement; maxima: four bf16 behind each other. A group with a NaN
+ * or an infinity holds the maximum NaN. Codes 16-byte, maxima 8-byte aligned. Slots and positions out of their range are
+ * never read or written: each entry point says what their rows get. */
+
+/* cohere_dec_attention over caches k4, v4 (slots, kv_heads, T, 64) with maxima ks, vs (slots, kv_heads, T, 4), and with
+ * `heads / kv_heads` query heads to a key head (query head h reads key head h / (heads / kv_heads)): out bf16 [rows,
+ * heads * 128]. self != 0: q [rows, ldq] holds heads x 128 queries, then kv_heads x 128 keys, then the values of the new
+ * token, which goes into the caches at position n[s] and is attended as computed, with keys 0 .. n[s] - 1 of the cache;
+ * self == 0: keys 0 .. min(n[s], T) - 1. A row gets zeros if it has no keys, if its slot is out of range, if n[s] < 0 and
+ * (self) if n[s] >= T; nothing is appended then. Two rows of one slot in a self-attention call each get their own
+ * result; the cache holds either's token. splits (1 .. 64) divides each row's keys over workgroups and needs part with
+ * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums. T < 2^26. */
+int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
+                            uint8_t* k4, uint8_t* v4, uint16_t* ks, uint16_t* vs, const int32_t* n, int64_t slots,
+                            int64_t heads, int64_t kv_heads, int64_t T, float scale, int64_t splits, float* part,
+                            int64_t part_len, uint16_t* out, void* stream);
+
+/* The number of splits that fills the GPU for such a call (1 for sizes that the call would refuse). */
+int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, int64_t kv_heads, int64_t T);
+
+/* cohere_dec_scatter_kv into caches ck, cv (L, S, H, T, 64) with maxima (L, S, H, T, 4); kv rows ldkv apart. A row whose
+ * slot or position is out of range goes nowhere; of two rows for one position either stays. */
+int cohere_dec_scatter_kv_q4(const uint16_t* kv, int64_t ldkv, int64_t rows, const int32_t* slot_of,
+                             const int32_t* frame_of, uint8_t* ck, uint8_t* cv, uint16_t* cks, uint16_t* cvs, int64_t L,
+                             int64_t S, int64_t H, int64_t T, void* stream);
+
+/* What such caches hold of position frame_of[i] of slot slot_of[i], rounded to bf16, into row i of kv (laid out as
+ * cohere_dec_scatter_kv_q4 takes it); zeros for a slot or position out of range. */
+int cohere_dec_gather_kv_q4(const int32_t* slot_of, const int32_t* frame_of, int64_t rows, const uint8_t* ck,
+                            const uint8_t* cv, const uint16_t* cks, const uint16_t* cvs, int64_t L, int64_t S, int64_t H,
+                            int64_t T, uint16_t* kv, int64_t ldkv, void* stream);
+
+/* Rules on logits x [rows, V] bf16 (ldx) into y (ldy; y may be x), before cohere_dec_pick. Row r is slot s = active[r]; p =
+ * pos[s] is the position of its newest token, tokens int64 [slots, OUT] what it holds. With c the times that token v is
+ * among tokens[s][max(first[s], 0) .. min(p, OUT - 1)] and (rep, presence, frequency) = pen[s] (fp32 [slots, 3], null:
+ * none), in fp32, one rounding each:
+ *   c > 0: l = l > 0 ? l / rep : l * rep; l = l - (c * frequency + presence)
+ *   l = l + bias[bias_of[s]][v]        (bias bf16 [B, V], null: none; bias_of[s] outside 0 .. B - 1: none)
+ *   l = -inf where mask[state] lacks v (mask int32 [M, ceil(V / 32)], bit v % 32 of word v / 32, null: none; a state
+ *                                       outside 0 .. M - 1 masks nothing)
+ * The state is start[s] (int32 [slots]). With classes (int32 [V]) and trans (int32 [M, C]) it is start[s] while
+ * p < plen[s] and trans[the state at p - 1][classes[tokens[s][p]]] later (-1 where any of these is out of range); the
+ * state at p is written to state[s][p % 2] and the one at p - 1 expected in the other place (state int32 [slots, 2]).
+ * A row whose slot is out of range is copied. V % 8 == 0; 16-byte aligned rows of x, y and bias. Row r of y may be all
+ * -inf: cohere_dec_pick then ends the row. */
+int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int64_t V,
+                      const int32_t* active, const int32_t* pos, int64_t slots, const int64_t* tokens, int64_t OUT,
+                      const int32_t* first, const int32_t* plen, const float* pen, const uint16_t* bias, int64_t B,
+                      const int32_t* bias_of, const int32_t* mask, int64_t M, const int32_t* classes,
+                      const int32_t* trans, int64_t C, const int32_t* start, int32_t* state, void* stream);
 
 /* Number of per-layer tensors of cohere_encoder_layers: the reference's 53 (its enum F,
  * kernels/csrc/encoder_loop.cpp:34-44) followed by 4 of this library's own (the feed-forwards' first linears in 2:4
