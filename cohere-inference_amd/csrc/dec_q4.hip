@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
   const bool slot_ok = (unsigned)s < (unsigned)p.S;
   s = slot_ok ? s : 0;
   int n = p.n[s];
-  const bool row_ok = slot_ok && n >= 0 && n < (SELF ? p.T : 0x7fffffff);
+  const bool row_ok = slot_ok && n >= 0 && (!SELF || n < p.T);
   n = row_ok ? (n < p.T ? n : p.T) : 0;
   const int64_t vec0 = ((int64_t)s * p.KV + kvh) * p.T;
   const char* kb = reinterpret_cast<const char*>(p.k4) + vec0 * VB;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(256) dec_gather_kv_q4_kernel(const KvArgs p) {
   uint4 o = make_uint4(0, 0, 0, 0);
   if (k.in) {
     const uint32_t w = *reinterpret_cast<const uint32_t*>((k.kvi ? p.v4 : p.k4) + k.vec * VB + k.d8 * 4);
-    const float m = bf2f((k.kvi ? p.vs : p.ks)[k.vec * NG + (k.d8 >> 2)]);
+    const Step m = step_of(bf2f((k.kvi ? p.vs : p.ks)[k.vec * NG + (k.d8 >> 2)]));
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = held(code(w, i), m);

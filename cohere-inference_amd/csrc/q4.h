@@ -55,11 +55,16 @@ DEVI uint32_t pack8(const Group& g, const float (&x)[8]) {
 // the code in nibble i (a constant) of a word
 DEVI int code(uint32_t w, int i) { return (int)(w << (28 - 4 * i)) >> 28; }
 
-// c m / 7 in fp32, correctly rounded (c m is exact: 3 + 8 bits)
-DEVI float held(int c, float m) {
-  const float n = (float)c * m, t = n * (1.f / 7.f);
-  return __builtin_fmaf(__builtin_fmaf(-t, 7.f, n), 1.f / 7.f, t);
+// a group's step m / 7 as a sum of two fp32 numbers, and c m / 7 from it with one rounding that matters (the second
+// number is 0 where the step is exact; c m / 7 is otherwise never halfway between two bf16 values)
+struct Step {
+  float hi, lo;
+};
+DEVI Step step_of(float m) {
+  const float hi = m / 7.f;
+  return {hi, __builtin_fmaf(-hi, 7.f, m) / 7.f};
 }
+DEVI float held(int c, const Step& s) { return __builtin_fmaf((float)c, s.hi, (float)c * s.lo); }
 
 DEVI uint32_t max_u(uint32_t a, uint32_t b) { return a > b ? a : b; }
 template <int CTRL>

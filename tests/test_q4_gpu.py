@@ -174,8 +174,8 @@ def _edge_vectors(g, count):
         x[i] = (k * (top.double() / 14)).to(BF)  # every code boundary, as far as bf16 holds it
         x[i, :, 0] = top.to(BF)
     x[1] = 0
-    x[3, 2] = 0
-    x[3, 2, 31] = -2.0
+    x[min(3, count - 1), 2] = 0
+    x[min(3, count - 1), 2, 31] = -2.0
     return x.reshape(count, 128)
 
 
