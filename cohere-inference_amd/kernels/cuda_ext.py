@@ -124,14 +124,25 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _here(what: str, *tensors) -> None:
-    """Every tensor (None: absent) on the current GPU, whose stream the launch takes."""
-    at = {t.get_device() for t in tensors if t is not None}
-    _check(at == {torch.cuda.current_device()} if -1 not in at else False, f"{what}: tensors on the current GPU expected")
+# The methods over 4-bit caches and on logits are called once per layer and step, so their checks are written out: one
+# look at each property, messages made only for a refusal (the checks take more host time than the launch).
+_BF, _U8, _I32, _I64, _F32 = torch.bfloat16, torch.uint8, torch.int32, torch.int64, torch.float32
 
 
-def _i32(t, n: int) -> bool:
-    return t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n
+def _stream_of(what: str, *tensors) -> int:
+    """The current stream of the tensors' GPU (None: absent), which has to be the current one."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise RuntimeError(f"{what}: tensors on the current GPU expected")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _index(t, n: int) -> bool:
+    """At least n int32 values one after the other."""
+    return t.dtype is _I32 and t.numel() >= n and t.is_contiguous()
 
 
 _EMPTY = torch.empty(0)  # an absent per-layer tensor
@@ -645,15 +656,19 @@ class _Ext:
     # ---- caches in 4 bits, rules on logits (no counterpart in the reference) -----------------------------------------
 
     @staticmethod
-    def _q4_checks(what, k4, v4, ks, vs, dims):
+    def _q4_caches(what, k4, v4, ks, vs, dims):
         """The caches' leading sizes: codes uint8 (..., 64) and maxima bf16 (..., 4), keys and values alike."""
-        _check(k4.dim() == dims + 1 and k4.shape == v4.shape and k4.shape[-1] == 64 and
-               k4.dtype == v4.dtype == torch.uint8 and k4.is_contiguous() and v4.is_contiguous(),
-               f"{what}: contiguous uint8 caches of 64 bytes a vector")
-        _check(ks.shape == vs.shape == (*k4.shape[:-1], 4) and ks.dtype == vs.dtype == torch.bfloat16 and
-               ks.is_contiguous() and vs.is_contiguous(), f"{what}: contiguous bf16 maxima, 4 a vector")
-        _check(k4.numel() > 0, f"{what}: empty caches")
-        return k4.shape[:-1]
+        shape = k4.shape
+        if not (len(shape) == dims + 1 and shape[-1] == 64 and v4.shape == shape and k4.dtype is _U8 and
+                v4.dtype is _U8 and k4.is_contiguous() and v4.is_contiguous()):
+            raise RuntimeError(f"{what}: contiguous uint8 caches of 64 bytes a vector")
+        lead = shape[:dims]
+        if not (ks.shape == (*lead, 4) and vs.shape == ks.shape and ks.dtype is _BF and vs.dtype is _BF and
+                ks.is_contiguous() and vs.is_contiguous()):
+            raise RuntimeError(f"{what}: contiguous bf16 maxima, 4 a vector")
+        if 0 in lead:
+            raise RuntimeError(f"{what}: empty caches")
+        return lead
 
     def dec_attention_q4_splits(self, rows, heads, kv_heads, T) -> int:
         """The `splits` that fill the GPU in a dec_attention_q4 call of these sizes."""
@@ -665,51 +680,59 @@ class _Ext:
         holds the new token's queries, keys and values, appended at position n[slot] and attended as computed. Rows
         without keys, of slots out of range or (self-attention) of positions beyond T get zeros. splits > 1 needs part
         (rows x H x splits x 130 floats). kernels.stream_decoder.quantize_q4 states the form."""
-        S, KV, T = self._q4_checks("dec_attention_q4", k4, v4, ks, vs, 3)
-        _check(q.dim() == 2 and out.dim() == 2 and q.dtype == out.dtype == torch.bfloat16 and
-               (q.stride(1) == 1 or q.shape[1] == 1) and out.is_contiguous() and out.shape[0] == q.shape[0],
-               "dec_attention_q4: bf16 q (rows, ...) with unit column stride, contiguous out (rows, H * 128)")
-        rows, H = q.shape[0], out.shape[1] // 128
-        _check(H > 0 and out.shape[1] % 128 == 0 and H % KV == 0 and
-               q.shape[1] >= (H + (2 * KV if self_attn else 0)) * 128, "dec_attention_q4: heads")
-        splits = int(splits)
-        _check(1 <= splits <= 64 and (splits == 1 or (part is not None and part.dtype == torch.float32 and
-               part.is_contiguous() and part.numel() >= rows * H * splits * 130)),
-               "dec_attention_q4: 1 to 64 splits, more than 1 need part")
-        _check(_i32(active, rows) and _i32(n, S), "dec_attention_q4: int32 active per row, n per slot")
+        S, KV, T = self._q4_caches("dec_attention_q4", k4, v4, ks, vs, 3)
+        if not (q.dim() == 2 and out.dim() == 2 and q.dtype is _BF and out.dtype is _BF and q.stride(1) == 1 and
+                out.is_contiguous()):
+            raise RuntimeError("dec_attention_q4: bf16 q (rows, ...) with unit column stride, contiguous out")
+        rows, width = q.shape
+        o_rows, o_width = out.shape
+        H = o_width >> 7
+        if not (o_rows == rows and H > 0 and o_width == H << 7 and H % KV == 0 and
+                width >= (H + (2 * KV if self_attn else 0)) << 7):
+            raise RuntimeError("dec_attention_q4: out (rows, H * 128), H a multiple of the key heads, q as wide as its heads")
+        if not (_index(active, rows) and _index(n, S)):
+            raise RuntimeError("dec_attention_q4: int32 active per row, n per slot")
+        part_len = 0 if part is None else part.numel()
+        if not (1 <= splits <= 64 and (splits == 1 or (part_len >= rows * H * splits * 130 and part.dtype is _F32 and
+                                                       part.is_contiguous()))):
+            raise RuntimeError("dec_attention_q4: 1 to 64 splits, more than 1 need part")
         if rows == 0:
             return
-        _here("dec_attention_q4", active, q, k4, v4, ks, vs, n, part, out)
-        self._call("cohere_dec_attention_q4", int(bool(self_attn)), _ptr(active), rows, _ptr(q), q.stride(0), _ptr(k4),
-                   _ptr(v4), _ptr(ks), _ptr(vs), _ptr(n), S, H, KV, T, float(scale), splits, _ptr(part),
-                   part.numel() if part is not None else 0, _ptr(out), _stream())
+        stream = _stream_of("dec_attention_q4", q, active, k4, v4, ks, vs, n, part, out)
+        if self._lib.cohere_dec_attention_q4(1 if self_attn else 0, active.data_ptr(), rows, q.data_ptr(), q.stride(0),
+                                             k4.data_ptr(), v4.data_ptr(), ks.data_ptr(), vs.data_ptr(), n.data_ptr(), S,
+                                             H, KV, T, scale, splits, None if part is None else part.data_ptr(),
+                                             part_len, out.data_ptr(), stream):
+            raise RuntimeError(self._lib.cohere_last_error().decode())
 
-    def _kv_q4_checks(self, what, kv, slot_of, frame_of, ck, cv, cks, cvs):
-        L, S, H, T = self._q4_checks(what, ck, cv, cks, cvs, 4)
-        _check(kv.dim() == 2 and kv.dtype == torch.bfloat16 and kv.stride(1) == 1 and kv.shape[1] == L * 2 * H * 128,
-               f"{what}: bf16 kv (rows, L * 2 * H * 128) with unit column stride")
-        _check(_i32(slot_of, kv.shape[0]) and _i32(frame_of, kv.shape[0]), f"{what}: int32 slot and position per row")
-        return L, S, H, T
+    def _kv_q4(self, what, kv, slot_of, frame_of, ck, cv, cks, cvs):
+        """(rows, their stride, the caches' sizes, the stream) of a scatter or gather; rows 0: nothing to do."""
+        L, S, H, T = self._q4_caches(what, ck, cv, cks, cvs, 4)
+        if not (kv.dim() == 2 and kv.dtype is _BF and kv.stride(1) == 1 and kv.shape[1] == L * 2 * H * 128):
+            raise RuntimeError(f"{what}: bf16 kv (rows, L * 2 * H * 128) with unit column stride")
+        rows = kv.shape[0]
+        if not (_index(slot_of, rows) and _index(frame_of, rows)):
+            raise RuntimeError(f"{what}: int32 slot and position per row")
+        stream = _stream_of(what, kv, slot_of, frame_of, ck, cv, cks, cvs) if rows else 0
+        return rows, kv.stride(0), L, S, H, T, stream
 
     def dec_scatter_kv_q4(self, kv, slot_of, frame_of, ck, cv, cks, cvs):
         """dec_scatter_kv into 4-bit caches (L, S, H, T, 64) with maxima (L, S, H, T, 4); rows of slots or positions out
         of range go nowhere."""
-        L, S, H, T = self._kv_q4_checks("dec_scatter_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
-        if kv.shape[0] == 0:
-            return
-        _here("dec_scatter_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
-        self._call("cohere_dec_scatter_kv_q4", _ptr(kv), kv.stride(0), kv.shape[0], _ptr(slot_of), _ptr(frame_of),
-                   _ptr(ck), _ptr(cv), _ptr(cks), _ptr(cvs), L, S, H, T, _stream())
+        rows, ld, L, S, H, T, stream = self._kv_q4("dec_scatter_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
+        if rows and self._lib.cohere_dec_scatter_kv_q4(kv.data_ptr(), ld, rows, slot_of.data_ptr(), frame_of.data_ptr(),
+                                                       ck.data_ptr(), cv.data_ptr(), cks.data_ptr(), cvs.data_ptr(), L,
+                                                       S, H, T, stream):
+            raise RuntimeError(self._lib.cohere_last_error().decode())
 
     def dec_gather_kv_q4(self, slot_of, frame_of, ck, cv, cks, cvs, kv):
         """What 4-bit caches hold of (slot, position) pairs, as bf16 rows laid out as dec_scatter_kv_q4 takes them (to
         move a slot to a decoder with other caches, or to look at it); zeros for slots or positions out of range."""
-        L, S, H, T = self._kv_q4_checks("dec_gather_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
-        if kv.shape[0] == 0:
-            return
-        _here("dec_gather_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
-        self._call("cohere_dec_gather_kv_q4", _ptr(slot_of), _ptr(frame_of), kv.shape[0], _ptr(ck), _ptr(cv), _ptr(cks),
-                   _ptr(cvs), L, S, H, T, _ptr(kv), kv.stride(0), _stream())
+        rows, ld, L, S, H, T, stream = self._kv_q4("dec_gather_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
+        if rows and self._lib.cohere_dec_gather_kv_q4(slot_of.data_ptr(), frame_of.data_ptr(), rows, ck.data_ptr(),
+                                                      cv.data_ptr(), cks.data_ptr(), cvs.data_ptr(), L, S, H, T,
+                                                      kv.data_ptr(), ld, stream):
+            raise RuntimeError(self._lib.cohere_last_error().decode())
 
     def dec_logits(self, logits, y, active, pos, tokens=None, first=None, plen=None, penalties=None, bias=None,
                    bias_of=None, mask=None, classes=None, trans=None, start=None, state=None):
@@ -719,39 +742,49 @@ class _Ext:
         lacks: mask int32 (M, ceil(V / 32)), start int32 (slots), and with classes int32 (V), trans int32 (M, C) and
         state int32 (slots, 2) the state moves with every token behind the prompt (plen). Absent rules are None; index
         values out of range switch a rule off for a slot."""
-        _check(logits.dim() == 2 and logits.shape == y.shape and logits.dtype == y.dtype == torch.bfloat16 and
-               logits.stride(1) == y.stride(1) == 1 and logits.shape[1] % 8 == 0 and logits.shape[1] > 0,
-               "dec_logits: bf16 logits and y (rows, V), unit column stride, V % 8 == 0")
-        rows, V = logits.shape
+        rows, V = logits.shape if logits.dim() == 2 else (0, 0)
+        if not (V > 0 and V % 8 == 0 and y.shape == (rows, V) and logits.dtype is _BF and y.dtype is _BF and
+                logits.stride(1) == 1 and y.stride(1) == 1):
+            raise RuntimeError("dec_logits: bf16 logits and y (rows, V), unit column stride, V % 8 == 0")
         S = pos.numel()
-        _check(_i32(active, rows) and _i32(pos, 1) and (first is None or _i32(first, S)) and
-               (plen is None or _i32(plen, S)), "dec_logits: int32 active per row, pos, first, plen per slot")
-        _check(tokens is None or (tokens.dtype == torch.int64 and tokens.dim() == 2 and tokens.shape[0] >= S and
-                                  tokens.shape[1] > 0 and tokens.is_contiguous()),
-               "dec_logits: contiguous int64 tokens (slots, positions)")
-        _check(penalties is None or (penalties.dtype == torch.float32 and penalties.shape == (S, 3) and
-                                     penalties.is_contiguous() and tokens is not None and first is not None),
-               "dec_logits: penalties fp32 (slots, 3) need tokens and first")
-        _check(bias is None or (bias.dtype == torch.bfloat16 and bias.dim() == 2 and bias.shape[0] > 0 and
-                                bias.shape[1] == V and bias.is_contiguous() and bias_of is not None and
-                                _i32(bias_of, S)), "dec_logits: bias bf16 (B, V) needs int32 bias_of per slot")
-        _check(mask is None or (mask.dim() == 2 and mask.shape[0] > 0 and mask.shape[1] == (V + 31) // 32 and
-                                _i32(mask, 1) and start is not None and _i32(start, S)),
-               "dec_logits: mask int32 (M, ceil(V / 32)) needs int32 start per slot")
-        _check((classes is None) == (trans is None) and (classes is None or (
-            mask is not None and classes.numel() == V and _i32(classes, V) and trans.dim() == 2 and
-            trans.shape[0] == mask.shape[0] and trans.shape[1] > 0 and _i32(trans, 1) and state is not None and
-            state.shape == (S, 2) and _i32(state, 1) and tokens is not None and plen is not None)),
-            "dec_logits: a grammar needs mask, classes (V), trans (M, C), state (slots, 2), tokens and plen")
+        if not (_index(active, rows) and _index(pos, 1) and (first is None or _index(first, S)) and
+                (plen is None or _index(plen, S))):
+            raise RuntimeError("dec_logits: int32 active per row, pos, first, plen per slot")
+        OUT, B, M, C = 1, 0, 0, 0
+        if tokens is not None:
+            if not (tokens.dim() == 2 and tokens.dtype is _I64 and tokens.is_contiguous()):
+                raise RuntimeError("dec_logits: contiguous int64 tokens (slots, positions)")
+            t_rows, OUT = tokens.shape
+            if t_rows < S or OUT == 0:
+                raise RuntimeError("dec_logits: contiguous int64 tokens (slots, positions)")
+        if penalties is not None and not (penalties.shape == (S, 3) and penalties.dtype is _F32 and
+                                          penalties.is_contiguous() and tokens is not None and first is not None):
+            raise RuntimeError("dec_logits: penalties fp32 (slots, 3) need tokens and first")
+        if bias is not None:
+            B = bias.shape[0]
+            if not (bias.shape == (B, V) and B > 0 and bias.dtype is _BF and bias.is_contiguous() and
+                    bias_of is not None and _index(bias_of, S)):
+                raise RuntimeError("dec_logits: bias bf16 (B, V) needs int32 bias_of per slot")
+        if mask is not None:
+            M = mask.shape[0]
+            if not (mask.shape == (M, (V + 31) // 32) and _index(mask, 1) and start is not None and _index(start, S)):
+                raise RuntimeError("dec_logits: mask int32 (M, ceil(V / 32)) needs int32 start per slot")
+        if classes is not None or trans is not None:
+            C = trans.shape[-1] if trans is not None else 0
+            if not (classes is not None and trans is not None and M > 0 and classes.numel() == V and _index(classes, V) and
+                    trans.shape == (M, C) and _index(trans, 1) and state is not None and state.shape == (S, 2) and
+                    _index(state, 1) and tokens is not None and plen is not None):
+                raise RuntimeError("dec_logits: a grammar needs mask, classes (V), trans (M, C), state (slots, 2), tokens "
+                                   "and plen")
         if rows == 0:
             return
-        _here("dec_logits", logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask, classes, trans,
-              start, state)
-        self._call("cohere_dec_logits", _ptr(logits), logits.stride(0), _ptr(y), y.stride(0), rows, V, _ptr(active),
-                   _ptr(pos), S, _ptr(tokens), tokens.shape[1] if tokens is not None else 1, _ptr(first), _ptr(plen),
-                   _ptr(penalties), _ptr(bias), bias.shape[0] if bias is not None else 0, _ptr(bias_of), _ptr(mask),
-                   mask.shape[0] if mask is not None else 0, _ptr(classes), _ptr(trans),
-                   trans.shape[1] if trans is not None else 0, _ptr(start), _ptr(state), _stream())
+        stream = _stream_of("dec_logits", logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask,
+                            classes, trans, start, state)
+        if self._lib.cohere_dec_logits(logits.data_ptr(), logits.stride(0), y.data_ptr(), y.stride(0), rows, V,
+                                       active.data_ptr(), pos.data_ptr(), S, _ptr(tokens), OUT, _ptr(first), _ptr(plen),
+                                       _ptr(penalties), _ptr(bias), B, _ptr(bias_of), _ptr(mask), M, _ptr(classes),
+                                       _ptr(trans), C, _ptr(start), _ptr(state), stream):
+            raise RuntimeError(self._lib.cohere_last_error().decode())
 
 
 _lib = load_library()
