@@ -19,17 +19,22 @@ using namespace cohere_q4;
 // ---- attention of one new token per row ---------------------------------------------------------------------------
 // scores and weights are in powers of two: s = q.k scale log2(e), p = 2^(s - m).
 //
-// A workgroup takes one row, one key head, G of its query heads and one part of the keys. Four lanes hold a key, each
-// lane one group of 32 dimensions (16 bytes of codes and its maximum), so a wave's load is 16 keys of 64 bytes, one
-// after the other. A pass is U keys per quad of lanes, all loads issued before any use.
-//   q.k: the query's group as 16-bit fixed point (a power of two of the group's own, so that values down to 2^-6 of the
-//   group's largest are exact and the rest within 2^-15 of it: far below the codes' step), split into four signed 4-bit
-//   digits that v_dot8_i32_i4 multiplies with the codes as they are: four instructions per eight products, no unpacking,
-//   exact sums. One conversion and one multiplication per group and key apply m and the scale.
-//   p v: the codes unpacked (3 instructions per 8, then a sign-extending conversion each) and one fma per value in fp32;
-//   the value's m goes into the weight.
-// Each quad keeps a running maximum, its lanes each a part of the sum (lane i the pass's key i) and 32 outputs; quads
-// meet at the end.
+// A workgroup takes one row, one key head, G of its query heads and one part of the keys; a wave takes 64 keys at a
+// time. Both products run on v_mfma_i32_16x16x64_i8, so that the codes need no conversion (three instructions turn a
+// word's eight codes into bytes 16 c) and the sums are exact:
+//   q k^T: A holds the queries as 16-bit fixed point (a power of two of each group of 32 dimensions, so that values down
+//   to 2^-7 of the group's largest are exact and the rest within 2^-16 of it) in two digits of 8 bits, rows 4 g + t: group
+//   g, t the head and digit (two heads fill the 16 rows), with zeros outside the row's group; B is 16 keys, lane (key,
+//   group g) holding the group's 16 bytes as loaded. Lane (key, g) of the result holds group g's sums, whose maximum it
+//   loaded with the codes: one conversion and one multiplication each, and the four groups meet by lane swaps that leave
+//   key l of the wave's 64 in lane l.
+//   softmax: one key a lane; the running maximum is the wave's.
+//   p v: A holds p m_g (m_g the value's maximum in group g) as 15-bit fixed point of the wave's largest, rows as above, B
+//   the codes of 64 keys and 16 dimensions 8 n + j (n the lane's column, j the product): lane (n, i) loads one word (8
+//   dimensions) of each of the keys 16 i .. 16 i + 15, and byte permutations put four keys' bytes into one word. Of the
+//   result, lanes of row group g = n / 4 hold what counts.
+// The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
+// read of them and they weigh nothing.
 struct Q4Args {
   const int32_t* active;
   const uint16_t* q;  // (rows, ldq): H query heads, then (self) KV keys, KV values of the new token
@@ -44,18 +49,46 @@ struct Q4Args {
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float UNIT = 112.f;  // outputs are summed in units of 1 / (7 * 16)
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+DEVI float nan_f() { return __uint_as_float(0x7fc00000u); }
+
+// the four rows of lanes' values of a, b, c, d reduced over the rows: row i gets the i-th operand's
+template <class Op>
+DEVI uint32_t rows4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, Op op) {
+  const auto x = __builtin_amdgcn_permlane32_swap(a, c, false, false);
+  const auto y = __builtin_amdgcn_permlane32_swap(b, d, false, false);
+  const auto z = __builtin_amdgcn_permlane16_swap(op(x[0], x[1]), op(y[0], y[1]), false, false);
+  return op(z[0], z[1]);
+}
+
+// four words as the words of their bytes 0, 1, 2, 3
+DEVI void bytes4(const uint32_t (&v)[4], uint32_t (&x)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), b = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u), d = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+  x[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  x[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  x[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  x[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+constexpr uint32_t HI4 = 0xf0f0f0f0u;
+DEVI int even4(uint32_t w) { return (int)((w << 4) & HI4); }  // the low nibbles as bytes 16 c
+DEVI int odd4(uint32_t w) { return (int)(w & HI4); }
 
 template <bool SELF, int G, int W>
 __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p) {
-  constexpr int QUADS = W * 16, U = 4;
-  __shared__ __attribute__((aligned(16))) uint32_t sq[G][NG][4][4];  // [head][group][digit][word]
+  constexpr int SETS = (G + 1) / 2, PARTS = W + (SELF ? 1 : 0);  // A operands; partial results, the new token's last
+  __shared__ __attribute__((aligned(16))) uint8_t sq[G][NG][2][GRP];
   __shared__ float sqs[G][NG];
-  __shared__ __attribute__((aligned(16))) float so[G][W][HD];
-  __shared__ float sm[G][W], sl[G][W];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), c = lane & 3, quad = tid >> 2;
+  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][SETS][16 * 64];
+  __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
+  __shared__ float sm[G][PARTS], sl[G][PARTS];
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, rowg = lane >> 4;
   const int r = blockIdx.x, kvh = blockIdx.y / p.chunks, ch = blockIdx.y % p.chunks, sp = blockIdx.z, nsp = gridDim.z;
-  // the chunk's query heads h0 .. h0 + G - 1, the last ones repeated where the chunk has fewer
+  // the chunk's query heads h0 .. h0 + G - 1, the last one repeated where the chunk has fewer
   const int h0 = kvh * p.ratio + ch * G, hlast = kvh * p.ratio + p.ratio - 1;
   int s = p.active[r];
   const bool slot_ok = (unsigned)s < (unsigned)p.S;
@@ -64,36 +97,38 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
   const bool row_ok = slot_ok && n >= 0 && (!SELF || n < p.T);
   n = row_ok ? (n < p.T ? n : p.T) : 0;
   const int64_t vec0 = ((int64_t)s * p.KV + kvh) * p.T;
-  const char* kb = reinterpret_cast<const char*>(p.k4) + vec0 * VB;
-  const char* vb = reinterpret_cast<const char*>(p.v4) + vec0 * VB;
-  const char* ksb = reinterpret_cast<const char*>(p.ks) + vec0 * (2 * NG);
-  const char* vsb = reinterpret_cast<const char*>(p.vs) + vec0 * (2 * NG);
   const int chunk = (n + nsp - 1) / nsp, start = min(n, sp * chunk), end = min(n, start + chunk);
+  const auto krs = __builtin_amdgcn_make_buffer_rsrc(p.k4 + vec0 * VB, 0, end * VB, 0x00027000);
+  const auto vrs = __builtin_amdgcn_make_buffer_rsrc(p.v4 + vec0 * VB, 0, end * VB, 0x00027000);
+  const auto kms = __builtin_amdgcn_make_buffer_rsrc(p.ks + vec0 * NG, 0, end * (2 * NG), 0x00027000);
+  const auto vms = __builtin_amdgcn_make_buffer_rsrc(p.vs + vec0 * NG, 0, end * (2 * NG), 0x00027000);
 
-  uint4 kr[U], vr[U];
-  uint32_t km[U], vm[U];
-  auto load_pass = [&](int j0) {
+  v4u kr[4];
+  uint32_t km[4], vr[16];
+  v2u vm;
+  auto load_k = [&](int j0) {
+    const uint32_t off = (uint32_t)(j0 + col) * VB + rowg * 16, moff = (uint32_t)(j0 + col) * (2 * NG) + rowg * 2;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * QUADS;
-      const uint32_t jj = j < end ? j : 0;
-      kr[u] = *reinterpret_cast<const uint4*>(kb + (jj * VB + c * 16));
-      km[u] = *reinterpret_cast<const uint16_t*>(ksb + (jj * (2 * NG) + c * 2));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * QUADS;
-      const uint32_t jj = j < end ? j : 0;
-      vr[u] = *reinterpret_cast<const uint4*>(vb + (jj * VB + c * 16));
-      vm[u] = *reinterpret_cast<const uint16_t*>(vsb + (jj * (2 * NG) + c * 2));
+    for (int t = 0; t < 4; ++t) {
+      kr[t] = __builtin_amdgcn_raw_buffer_load_b128(krs, off + t * 16 * VB, 0, 0);
+      km[t] = __builtin_amdgcn_raw_buffer_load_b16(kms, moff + t * 16 * (2 * NG), 0, 0);
     }
   };
-  int j0 = start + quad;
-  load_pass(j0);
+  auto load_v = [&](int j0) {
+    const uint32_t off = (uint32_t)(j0 + rowg * 16) * VB + col * 4;
+    vm = __builtin_amdgcn_raw_buffer_load_b64(vms, (uint32_t)(j0 + lane) * (2 * NG), 0, 0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b32(vrs, off + i * VB, 0, 0);
+  };
+  int j0 = start + wave * 64;
+  if (j0 < end) {
+    load_k(j0);
+    load_v(j0);
+  }
 
-  // the query's digits, a dimension per thread
+  // the queries' digits, a dimension per thread; byte 8 (d / 8) + 4 (d % 2) + d % 8 / 2 of its group, as the codes'
   for (int i = tid; i < G * HD; i += W * 64) {
-    const int g = i >> 7, d = i & (HD - 1);
+    const int g = i >> 7, d = i & (HD - 1), at = d & 31;
     const uint32_t bits = (uint32_t)p.q[(int64_t)r * p.ldq + min(h0 + g, hlast) * HD + d] << 16;
     uint32_t mb = bits & 0x7fffffffu;
     mb = max_u(mb, dpp_u<DPP_XOR1>(mb));
@@ -104,178 +139,177 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
     mb = max_u(sw[0], sw[1]);
     const bool ok = mb < 0x7f800000u;
     const float m = __uint_as_float(ok ? mb : 0u);
-    // m 2^e in (15291, 30583]: the largest number of four digits -8..7 is 30583
-    const int ex = 15 - __builtin_amdgcn_frexp_expf(m), e = ldexpf(m, ex) <= 30583.f ? ex : ex - 1;
-    const int t = ok ? (int)rintf(ldexpf(__uint_as_float(bits), e)) : 0;
-    const uint32_t u = (uint32_t)(t + 0x8888) ^ 0x8888u;  // digit k + 8 in nibble k, then k in two's complement
-    const int at = d & 7;
-    uint32_t mine = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t w = ((u >> (4 * k)) & 15u) << (4 * at);
-      w |= dpp_u<DPP_XOR1>(w);
-      w |= dpp_u<DPP_XOR2>(w);
-      w |= dpp_u<DPP_HALF_MIRROR>(w);
-      if (at == k) mine = w;
-    }
-    if (at < 4) sq[g][d >> 5][at][(d >> 3) & 3] = mine;
-    if ((d & 31) == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * LOG2E / 7.f, -e) : __uint_as_float(0x7fc00000u);
+    // m 2^e in (16319, 32639]: digits 127, 127 are 32639
+    const int ex = 15 - __builtin_amdgcn_frexp_expf(m), e = ldexpf(m, ex) <= 32639.f ? ex : ex - 1;
+    const int t = (ok ? (int)rintf(ldexpf(__uint_as_float(bits), e)) : 0) + 128;
+    uint8_t* dst = &sq[g][d >> 5][0][(at >> 3) * 8 + (at & 1) * 4 + ((at & 7) >> 1)];
+    dst[0] = (uint8_t)(t >> 8);
+    dst[GRP] = (uint8_t)(t ^ 128);
+    if (at == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / UNIT), -e) : nan_f();
   }
+  if constexpr (SELF) {
+    const bool fresh = row_ok && sp == 0;
+    const uint16_t* row = p.q + (int64_t)r * p.ldq;
+    const uint16_t* knew = row + (p.H + kvh) * HD;
+    // the new token: a partial result of its own per head, as computed
+    for (int g = wave; g < G; g += W) {
+      float dot = 0.f;
+      if (fresh) {
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(row + min(h0 + g, hlast) * HD + lane * 2);
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(knew + lane * 2);
+        const uint32_t c = *reinterpret_cast<const uint32_t*>(knew + p.KV * HD + lane * 2);
+        dot = __uint_as_float(a << 16) * __uint_as_float(b << 16);
+        dot = __builtin_fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), dot);
+        dot = wave_sum64(dot) * (p.scale * LOG2E);
+        so[g][W][lane * 2] = UNIT * __uint_as_float(c << 16);
+        so[g][W][lane * 2 + 1] = UNIT * __uint_as_float(c & 0xffff0000u);
+      }
+      if (lane == 0) {
+        sm[g][W] = fresh ? dot : -INFINITY;
+        sl[g][W] = fresh ? (dot == dot ? 1.f : dot) : 0.f;  // maxima pass over a NaN score, the sum keeps it
+      }
+    }
+    // and into the cache: 16 lanes a vector, 8 values each
+    if (fresh && ch == 0 && wave == W - 1 && lane < 32) {
+      float x[8];
+      const uint32_t mx = quad_max_u(unpack8(*reinterpret_cast<const uint4*>(knew + rowg * p.KV * HD + col * 8), x));
+      const Group g = group_of(mx);
+      const int64_t vec = vec0 + n;
+      *reinterpret_cast<uint32_t*>((rowg ? p.v4 : p.k4) + vec * VB + col * 4) = pack8(g, x);
+      if ((col & 3) == 0) (rowg ? p.vs : p.ks)[vec * NG + (col >> 2)] = g.store;
+    }
+  }
+  __syncthreads();
+  // A of the first product: row 4 g + t of set s is group g of head 2 s + t / 2, digit t % 2
+  v4i aq[SETS][2];
+  float qs[G];
+#pragma unroll
+  for (int st = 0; st < SETS; ++st) {
+    const int head = 2 * st + ((col & 3) >> 1);
+    const bool mine = (col >> 2) == rowg && head < G;
+    const v4i* src = reinterpret_cast<const v4i*>(&sq[head < G ? head : 0][rowg][col & 1][0]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const v4i t = src[i];
+      aq[st][i] = mine ? t : v4i{0, 0, 0, 0};
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g) qs[g] = sqs[g][rowg];
 
-  float m[G], l[G], acc[G][32];
+  float m[G], l[G], acc[G][8];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     m[g] = -INFINITY;
     l[g] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) acc[g][k] = 0.f;
+    for (int k = 0; k < 8; ++k) acc[g][k] = 0.f;
   }
-  // self-attention: the first quad of the first part takes the new token, as computed; the cache gets its 4 bits
-  if (SELF && row_ok && sp == 0 && quad == 0) {
-    const uint16_t* row = p.q + (int64_t)r * p.ldq;
-    const uint16_t* kp = row + (p.H + kvh) * HD + c * 32;
-    const uint16_t* vp = kp + p.KV * HD;
-    float x[4][8];
-    uint32_t mx = 0;
+  while (j0 < end) {
+    // scores of key j0 + lane
+    float sc[G];
+    {
+      float x[G][4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mx = max_u(mx, unpack8(*reinterpret_cast<const uint4*>(kp + w * 8), x[w]));
+      for (int t = 0; t < 4; ++t) {
+        const v4i b0 = {even4(kr[t].x), odd4(kr[t].x), even4(kr[t].y), odd4(kr[t].y)};
+        const v4i b1 = {even4(kr[t].z), odd4(kr[t].z), even4(kr[t].w), odd4(kr[t].w)};
+        const float mk = __uint_as_float(km[t] << 16);
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const uint16_t* qp = row + min(h0 + g, hlast) * HD + c * 32;
-      float dot = 0.f;
+        for (int st = 0; st < SETS; ++st) {
+          v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st][0], b0, v4i{0, 0, 0, 0}, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st][1], b1, d, 0, 0, 0);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float qf[8];
-        unpack8(*reinterpret_cast<const uint4*>(qp + w * 8), qf);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) dot = __builtin_fmaf(qf[k], x[w][k], dot);
+          for (int i = 0; i < 2; ++i)
+            if (2 * st + i < G) x[2 * st + i][t] = (float)(d[2 * i] * 256 + d[2 * i + 1]) * (mk * qs[2 * st + i]);
+        }
       }
-      dot += dpp_mov<DPP_XOR1>(dot);
-      dot += dpp_mov<DPP_XOR2>(dot);
-      m[g] = dot * (p.scale * LOG2E);
-      l[g] = c == 0 ? (m[g] == m[g] ? 1.f : m[g]) : 0.f;  // the maxima pass over a NaN score, the sum keeps it
-    }
-    const int64_t vec = vec0 + n;
-    if (ch == 0) {
-      const Group gk = group_of(mx);
-      *reinterpret_cast<uint4*>(p.k4 + vec * VB + c * 16) =
-          make_uint4(pack8(gk, x[0]), pack8(gk, x[1]), pack8(gk, x[2]), pack8(gk, x[3]));
-      p.ks[vec * NG + c] = gk.store;
-    }
-    mx = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      mx = max_u(mx, unpack8(*reinterpret_cast<const uint4*>(vp + w * 8), x[w]));
+      const auto add = [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
 #pragma unroll
       for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[g][w * 8 + k] = 7.f * x[w][k];  // outputs are summed in units of a seventh
+        sc[g] = __uint_as_float(rows4(__float_as_uint(x[g][0]), __float_as_uint(x[g][1]), __float_as_uint(x[g][2]),
+                                      __float_as_uint(x[g][3]), add));
     }
-    if (ch == 0) {
-      const Group gv = group_of(mx);
-      *reinterpret_cast<uint4*>(p.v4 + vec * VB + c * 16) =
-          make_uint4(pack8(gv, x[0]), pack8(gv, x[1]), pack8(gv, x[2]), pack8(gv, x[3]));
-      p.vs[vec * NG + c] = gv.store;
-    }
-  }
-  __syncthreads();
-  uint32_t qd[G][4][4];
-  float qs[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint4 t = *reinterpret_cast<const uint4*>(sq[g][c][k]);
-      qd[g][k][0] = t.x; qd[g][k][1] = t.y; qd[g][k][2] = t.z; qd[g][k][3] = t.w;
-    }
-    qs[g] = sqs[g][c];
-  }
-
-  while (j0 - quad < end) {  // the same for the whole workgroup
-    // scores of the pass's U keys, in every lane of the quad; keys past the end: -inf
-    float pw[G][U];
+    const bool live = j0 + lane < end;
+    const int jn = j0 + W * 64;
+    if (jn < end) load_k(jn);
+    // weights; p m_g in fixed point into A's rows
+    float inv[G];
+    const float vmx[NG] = {__uint_as_float(vm.x << 16), __uint_as_float(vm.x & 0xffff0000u),
+                           __uint_as_float(vm.y << 16), __uint_as_float(vm.y & 0xffff0000u)};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t w[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
-        int dg[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dg[k] = __builtin_amdgcn_sdot8((int)w[i], (int)qd[g][k][i], dg[k], false);
-        const int dot = (((dg[3] * 16 + dg[2]) * 16 + dg[1]) * 16) + dg[0];  // below 2^24: exact in fp32
-        float t = (float)dot * (__uint_as_float(km[u] << 16) * qs[g]);
-        t += dpp_mov<DPP_XOR1>(t);
-        t += dpp_mov<DPP_XOR2>(t);
-        pw[g][u] = j0 + u * QUADS < end ? t : -INFINITY;
-      }
-      float mx = m[g];
-#pragma unroll
-      for (int u = 0; u < U; ++u) mx = fmaxf(mx, pw[g][u]);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      // lane i of the quad raises key i's weight; the others take it from there
-      const float mine = c == 0 ? pw[g][0] : c == 1 ? pw[g][1] : c == 2 ? pw[g][2] : pw[g][3];
-      const float e = exp2_hw(mine - base), a = exp2_hw(m[g] - base);
-      pw[g][0] = dpp_mov<0x00>(e);
-      pw[g][1] = dpp_mov<0x55>(e);
-      pw[g][2] = dpp_mov<0xAA>(e);
-      pw[g][3] = dpp_mov<0xFF>(e);
+      const float sg = live ? sc[g] : -INFINITY;
+      const float mn = fmaxf(m[g], wave_max64(sg)), base = mn == -INFINITY ? 0.f : mn;
+      const float a = exp2_hw(m[g] - base), e = exp2_hw(sg - base);
       l[g] = __builtin_fmaf(l[g], a, e);
-      if (__any(a != 1.f)) {
+      m[g] = mn;
+      if (__builtin_amdgcn_readfirstlane(__float_as_int(a)) != 0x3f800000) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) acc[g][k] *= a;
+        for (int k = 0; k < 8; ++k) acc[g][k] *= a;
       }
-      m[g] = mx;
+      float w[NG];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) w[i] = e * vmx[i];
+      // the wave's largest of each group, in row i of lanes group i's (a NaN's bits are larger than any number's)
+      uint32_t y = rows4(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]), max_u);
+      y = max_u(y, dpp_u<DPP_XOR1>(y));
+      y = max_u(y, dpp_u<DPP_XOR2>(y));
+      y = max_u(y, dpp_u<DPP_ROR4>(y));
+      y = max_u(y, dpp_u<DPP_ROR8>(y));
+      // times 2^k at most 32639: k from the exponent of the next power of two but 0.4 % (0x10200 of a mantissa)
+      const int k = 141 - (int)((y + 0x10200u) >> 23);
+      inv[g] = y < 0x7f800000u ? ldexpf(1.f, -k) : nan_f();
+      uint8_t* dst = &sp8[wave][g >> 1][(g & 1) * 128 + col];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const uint32_t t =
+            __float_as_uint(ldexpf(w[i], __builtin_amdgcn_readlane(k, 16 * i)) + (12582912.f + 128.f)) ^ 128u;
+        dst[i * 256 + ((rowg ^ i) << 4)] = (uint8_t)(t >> 8);
+        dst[i * 256 + 64 + ((rowg ^ i) << 4)] = (uint8_t)t;
+      }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
+    v4i ap[SETS];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool live = j0 + u * QUADS < end;
-      float wt[G];
+    for (int st = 0; st < SETS; ++st)
+      ap[st] = *reinterpret_cast<const v4i*>(&sp8[wave][st][col * 64 + ((rowg ^ (col >> 2)) << 4)]);
+    uint32_t x[4][4];  // [four keys][bytes 0 .. 3 of their words]
 #pragma unroll
-      for (int g = 0; g < G; ++g) wt[g] = live ? pw[g][u] * __uint_as_float(vm[u] << 16) : 0.f;
-      const uint32_t w[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float v = (float)code(w[i], k);
-#pragma unroll
-          for (int g = 0; g < G; ++g) acc[g][i * 8 + k] = __builtin_fmaf(wt[g], v, acc[g][i * 8 + k]);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v[4] = {vr[4 * i], vr[4 * i + 1], vr[4 * i + 2], vr[4 * i + 3]};
+      bytes4(v, x[i]);
     }
-    j0 += U * QUADS;
-    if (j0 - quad < end) load_pass(j0);
+    if (jn < end) load_v(jn);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int b = j >> 1;
+      const v4i bv = j & 1 ? v4i{odd4(x[0][b]), odd4(x[1][b]), odd4(x[2][b]), odd4(x[3][b])}
+                           : v4i{even4(x[0][b]), even4(x[1][b]), even4(x[2][b]), even4(x[3][b])};
+#pragma unroll
+      for (int st = 0; st < SETS; ++st) {
+        const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap[st], bv, v4i{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (2 * st + i < G)
+            acc[2 * st + i][j] =
+                __builtin_fmaf((float)(d[2 * i] * 256 + d[2 * i + 1]), inv[2 * st + i], acc[2 * st + i][j]);
+      }
+    }
+    asm volatile("" ::: "memory");  // the next pass's weights are written after these are read
+    j0 = jn;
   }
 
-  // a wave's quads: maximum, sum and outputs. The outputs of the 16 quads meet by lane swaps (32 values over the four
-  // rows of lanes: two swaps leave row i with dimensions 8 i .. 8 i + 7 of the group), then within the rows.
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    const float M = wave_max64(m[g]), f = M == -INFINITY ? 0.f : exp2_hw(m[g] - M);
-    const float L = wave_sum64(l[g] * f);
-    float o[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float h[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[g][k + 8 * b] * f),
-                                                        __float_as_uint(acc[g][k + 8 * b + 16] * f), false, false);
-        h[b] = __uint_as_float(t[0]) + __uint_as_float(t[1]);
-      }
-      const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[0]), __float_as_uint(h[1]), false, false);
-      o[k] = __uint_as_float(t[0]) + __uint_as_float(t[1]);
-      o[k] += dpp_mov<DPP_ROR4>(o[k]);
-      o[k] += dpp_mov<DPP_ROR8>(o[k]);
-    }
-    if ((lane & 12) == 0) {
-      float* dst = &so[g][wave][c * 32 + (lane >> 4) * 8];
-      *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    const float L = wave_sum64(l[g]);
+    if (rowg == col >> 2) {
+      float* dst = &so[g][wave][col * 8];
+      *reinterpret_cast<float4*>(dst) = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[g][4], acc[g][5], acc[g][6], acc[g][7]);
     }
     if (lane == 0) {
-      sm[g][wave] = M;
+      sm[g][wave] = m[g];
       sl[g][wave] = L;
     }
   }
@@ -285,16 +319,17 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
     if (ch * G + g >= p.ratio) continue;
     float M = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[g][w]);
+    for (int w = 0; w < PARTS; ++w) M = fmaxf(M, sm[g][w]);
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float f = sm[g][w] == -INFINITY ? 0.f : exp2_hw(sm[g][w] - M);
+    for (int w = 0; w < PARTS; ++w) {
+      const float f = exp2_hw(sm[g][w] - (M == -INFINITY ? 0.f : M));
       L = __builtin_fmaf(f, sl[g][w], L);
-      O = __builtin_fmaf(f, so[g][w][d], O);
+      // a part without keys (weight 0) may be unwritten; a score that is no number counts (its sum is NaN)
+      if (f != 0.f) O = __builtin_fmaf(f, so[g][w][d], O);
     }
     const int64_t head = (int64_t)r * p.H + h0 + g;
     if (nsp == 1) {
-      p.out[head * HD + d] = f2bf(L == 0.f ? 0.f : O / (7.f * L));
+      p.out[head * HD + d] = f2bf(L == 0.f ? 0.f : O / (UNIT * L));
     } else {
       float* part = p.part + (head * nsp + sp) * (HD + 2);
       part[d] = O;
@@ -319,7 +354,7 @@ __global__ void __launch_bounds__(HD) dec_combine_q4_kernel(const float* __restr
     L = __builtin_fmaf(w, q[HD + 1], L);
     O = __builtin_fmaf(w, q[d], O);
   }
-  out[head * HD + d] = f2bf(L == 0.f ? 0.f : O / (7.f * L));
+  out[head * HD + d] = f2bf(L == 0.f ? 0.f : O / (UNIT * L));
 }
 
 // ---- filling and reading back -----------------------------------------------------------------------------------------
@@ -404,20 +439,27 @@ int kv_entry(bool gather, const KvArgs& p, int64_t rows, int64_t L, int64_t S, i
   return cohere::check_launch(name);
 }
 
-// query heads a workgroup takes (at most 4: 128 fp32 outputs a lane) and workgroups a key head
+// query heads a workgroup takes (at most 8) and workgroups a key head
 struct HeadPlan { int g, chunks; };
 HeadPlan head_plan(int64_t ratio) {
-  const int chunks = (int)((ratio + 3) / 4);
-  return {(int)((ratio + chunks - 1) / chunks), chunks};
+  const int chunks = (int)((ratio + 7) / 8), g = (int)((ratio + chunks - 1) / chunks);
+  return {g <= 4 ? g : g <= 6 ? 6 : 8, chunks};
 }
+
+#ifndef COHERE_Q4_WAVES
+#define COHERE_Q4_WAVES 8
+#endif
+constexpr int WAVES = COHERE_Q4_WAVES;  // a workgroup's
 
 template <bool SELF>
 void launch_attention(int g, const Q4Args& p, dim3 grid, hipStream_t s) {
   switch (g) {
-    case 1: dec_attention_q4_kernel<SELF, 1, 8><<<grid, 512, 0, s>>>(p); break;
-    case 2: dec_attention_q4_kernel<SELF, 2, 4><<<grid, 256, 0, s>>>(p); break;
-    case 3: dec_attention_q4_kernel<SELF, 3, 4><<<grid, 256, 0, s>>>(p); break;
-    default: dec_attention_q4_kernel<SELF, 4, 4><<<grid, 256, 0, s>>>(p); break;
+    case 1: dec_attention_q4_kernel<SELF, 1, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
+    case 2: dec_attention_q4_kernel<SELF, 2, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
+    case 3: dec_attention_q4_kernel<SELF, 3, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
+    case 4: dec_attention_q4_kernel<SELF, 4, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
+    case 6: dec_attention_q4_kernel<SELF, 6, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
+    default: dec_attention_q4_kernel<SELF, 8, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
   }
 }
 
@@ -427,7 +469,7 @@ extern "C" int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, i
   if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || T <= 0) return 1;
   const HeadPlan hp = head_plan(heads / kv_heads);
   // enough workgroups for two waves of the chip's 256 CUs, each with two passes of keys at least
-  const int64_t wgs = rows * kv_heads * hp.chunks, pass = hp.g == 1 ? 512 : 256;
+  const int64_t wgs = rows * kv_heads * hp.chunks, pass = WAVES * 64;
   const int64_t want = (1024 + wgs - 1) / wgs, most = (T + 2 * pass - 1) / (2 * pass);
   const int64_t n = want < most ? want : most;
   return n < 1 ? 1 : n > 64 ? 64 : n;
@@ -441,7 +483,7 @@ extern "C" int cohere_dec_attention_q4(int32_t self, const int32_t* active, int6
   COHERE_REQUIRE(rows >= 0 && rows <= 0x7fffffff && slots > 0 && slots <= 0x7fffffff && heads > 0 && kv_heads > 0 &&
                      heads % kv_heads == 0 && heads <= 65535 && splits >= 1 && splits <= 64,
                  "dec_attention_q4: bad sizes (heads a multiple of the key heads, 1 to 64 splits)");
-  COHERE_REQUIRE(T > 0 && T < (1 << 26), "dec_attention_q4: caches of 1 to 2^26 - 1 positions");  // 64 T in 32 bits
+  COHERE_REQUIRE(T > 0 && T < (1 << 25), "dec_attention_q4: caches of 1 to 2^25 - 1 positions");  // 64 T in 31 bits
   COHERE_REQUIRE(active && q && n && out && al(q, 16) && ldq % 8 == 0 && al(out, 2) &&
                      ldq >= (heads + (self ? 2 * kv_heads : 0)) * HD,
                  "dec_attention_q4: bad pointer or row stride");

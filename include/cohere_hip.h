@@ -267,7 +267,7 @@ int cohere_gemm_kv_q8(const uint16_t* a, int64_t lda, const uint16_t* w, const u
  * self == 0: keys 0 .. min(n[s], T) - 1. A row gets zeros if it has no keys, if its slot is out of range, if n[s] < 0 and
  * (self) if n[s] >= T; nothing is appended then. Two rows of one slot in a self-attention call each get their own
  * result; the cache holds either's token. splits (1 .. 64) divides each row's keys over workgroups and needs part with
- * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums. T < 2^26. */
+ * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums. T < 2^25. */
 int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
                             uint8_t* k4, uint8_t* v4, uint16_t* ks, uint16_t* vs, const int32_t* n, int64_t slots,
                             int64_t heads, int64_t kv_heads, int64_t T, float scale, int64_t splits, float* part,

@@ -38,12 +38,15 @@ def filled(g, slots, kv, T, std=1.0):
 def attention64(self_attn, active, q, k4, v4, ks, vs, n, scale, heads):
     """(out, bound): the attention in 64 bits (all on the CPU) and how far a right kernel may be off, elementwise.
 
-    Bound. The kernel holds a query group of 32 in 16-bit fixed point, off by at most half a step of 1 / 15291 of the
-    group's largest magnitude, so a score is off by at most sum_g m_g / 30582 * sum |k| * scale, and by the fp32 roundings
-    of about 16 operations on terms of sum |q k| scale (2^-24 each, and 2^-22 for the hardware's exponential with its
-    argument). A weight changed by a factor within exp(+-d) changes the output by at most (exp(2 d) - 1) sum p |v|. The
-    sums of n weights and outputs in fp32 add n / 512 + 64 roundings (a lane adds n / 128, then they meet) of 2^-24 of
-    sum p |v|; the result's own rounding is 2^-8 of it."""
+    Bound. The kernel holds a query group of 32 in fixed point, its largest magnitude above 16319 steps, so a score is off
+    by at most sum_g m_g / 32638 * sum |k| * scale, and by the fp32 roundings of about 16 operations on terms of sum |q k|
+    scale (2^-24 each, and 2^-22 for the hardware's exponential with its argument). A weight changed by a factor within
+    exp(+-d) changes the output by at most (exp(2 d) - 1) sum p |v|. The weights times the value's maximum m_g are held in
+    fixed point too, the largest of 64 keys above 16319 steps: each is off by at most half a step of the largest of all,
+    Y / 32638, and by no more than itself (below half a step it becomes 0), which moves the output by that times |c| / 7.
+    The sums of n weights and outputs in fp32 add n / 512 + 64 roundings (a lane adds n / 512 products, then they meet) of
+    2^-24 of sum p |v|; the result's own rounding is 2^-8 of it. The new token's weight and value are not in fixed
+    point."""
     rows, KV = q.shape[0], k4.shape[1]
     S, T = k4.shape[0], k4.shape[2]
     out = torch.zeros(rows, heads, 128, dtype=torch.float64)
@@ -65,12 +68,18 @@ def attention64(self_attn, active, q, k4, v4, ks, vs, n, scale, heads):
         p = torch.softmax(sc, -1)
         mg = qh.abs().reshape(*qh.shape[:2], 4, 32).amax(-1).repeat_interleave(32, -1)
         kt = k.abs().transpose(1, 2).contiguous()
-        d = (torch.matmul(mg, kt) / 30582 + torch.matmul(qh.abs(), kt) * 16 * 2.0 ** -24 + sc.abs() * 2.0 ** -22) * abs(scale)
+        d = (torch.matmul(mg, kt) / 32638 + torch.matmul(qh.abs(), kt) * 16 * 2.0 ** -24 + sc.abs() * 2.0 ** -22) * abs(scale)
         d = d.amax(-1, keepdim=True) + 2.0 ** -22
         spread = torch.matmul(p, v.abs())
         o = torch.matmul(p, v)
         out[r] = o.reshape(heads, 128)
         b = (torch.expm1(2 * d) + (k.shape[1] / 512 + 64) * 2.0 ** -24) * spread
+        if t:
+            vm = vs[s, :, :t].double()  # (KV, t, 4)
+            w = p[..., :t, None] * vm[:, None]  # (KV, ratio, t, 4)
+            w = torch.minimum(w.amax(2, keepdim=True) / 32638, w).repeat_interleave(32, -1)
+            share = (v[:, :t].abs() / vm.repeat_interleave(32, -1).clamp_min(1e-300))[:, None]  # |c| / 7
+            b = b + (w * share).sum(2)
         bound[r] = (b * (1 + 2.0 ** -8) + 2.0 ** -8 * o.abs() + 2.0 ** -134).reshape(heads, 128)
     return out.reshape(rows, -1), bound.reshape(rows, -1)
 

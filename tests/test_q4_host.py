@@ -117,7 +117,7 @@ def test_c_abi_refuses_without_launching():
         return lib.cohere_last_error().decode()
 
     ok = [0, fake, 2, fake, 512, fake, fake, fake, fake, fake, 3, 4, 2, 5, 1.0, 1, None, 0, fake, None]
-    for at, value in ((1, None), (4, 511), (4, 504), (5, fake + 8), (7, fake + 4), (10, 0), (11, 5), (13, 0), (13, 1 << 26),
+    for at, value in ((1, None), (4, 511), (4, 504), (5, fake + 8), (7, fake + 4), (10, 0), (11, 5), (13, 0), (13, 1 << 25),
                       (15, 0), (15, 65), (15, 2), (18, None)):
         args = list(ok)
         args[at] = value
