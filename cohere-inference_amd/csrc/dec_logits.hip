@@ -86,9 +86,14 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
       *reinterpret_cast<uint4*>(&cnt[(j * NT + tid) * 4]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const int64_t* t = a.tokens + (int64_t)s * a.OUT;
-    for (int i = lo + tid; i <= hi; i += NT) {
-      const int64_t d = t[i] - v0;
-      if (d >= 0 && d < SPAN) atomicAdd(&cnt[d], 1u);
+    // eight tokens a thread in flight
+    for (int i0 = lo + tid; i0 <= hi; i0 += NT * 8) {
+      int64_t d[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = hi - i0 >= k * NT ? t[i0 + k * NT] - v0 : -1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (d[k] >= 0 && d[k] < SPAN) atomicAdd(&cnt[d[k]], 1u);
     }
     __syncthreads();
   }
@@ -157,7 +162,8 @@ extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, in
                     reinterpret_cast<const uint8_t*>(mask), classes, trans, start, state, (int)slots, (int)V, (int)OUT,
                     (int)B, (int)M, (int)C};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  constexpr int J = 2;
-  dec_logits_kernel<J><<<dim3((unsigned)((V + J * 2048 - 1) / (J * 2048)), (unsigned)rows), NT, 0, s>>>(a);
+  const auto wgs = [&](int j) { return (unsigned)((V + j * 2048 - 1) / (j * 2048)); };
+  if (rows * wgs(4) >= 512) dec_logits_kernel<4><<<dim3(wgs(4), (unsigned)rows), NT, 0, s>>>(a);
+  else dec_logits_kernel<1><<<dim3(wgs(1), (unsigned)rows), NT, 0, s>>>(a);
   return cohere::check_launch("dec_logits");
 }

@@ -55,13 +55,23 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 DEVI float nan_f() { return __uint_as_float(0x7fc00000u); }
 
-// the four rows of lanes' values of a, b, c, d reduced over the rows: row i gets the i-th operand's
-template <class Op>
-DEVI uint32_t rows4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, Op op) {
+// of a and b: a summed over the two halves of the wave in its lower half, b in the upper; of two such, each summed over
+// the rows of 16 lanes of a half. Of a, b, c, d, quarter_sum(half_sum(a, c), half_sum(b, d)) has the sum of the i-th over
+// the four rows in row i.
+DEVI float half_sum(float a, float b) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+DEVI float quarter_sum(float a, float b) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+// the same with the maxima of four as unsigned numbers
+DEVI uint32_t rows_max(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const auto x = __builtin_amdgcn_permlane32_swap(a, c, false, false);
   const auto y = __builtin_amdgcn_permlane32_swap(b, d, false, false);
-  const auto z = __builtin_amdgcn_permlane16_swap(op(x[0], x[1]), op(y[0], y[1]), false, false);
-  return op(z[0], z[1]);
+  const auto z = __builtin_amdgcn_permlane16_swap(max_u(x[0], x[1]), max_u(y[0], y[1]), false, false);
+  return max_u(z[0], z[1]);
 }
 
 // four words as the words of their bytes 0, 1, 2, 3
@@ -74,14 +84,37 @@ DEVI void bytes4(const uint32_t (&v)[4], uint32_t (&x)[4]) {
   x[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
+// a score below every finite one that counts, so that differences of scores need no care for two infinities
+constexpr float BOTTOM = -3e38f, RISE = 8.f;
+
+// the largest value of the wave, in every lane: as unsigned numbers of the same order, whose maxima take the lane moves
+// as operands
+DEVI float wave_top(float v) {
+  const uint32_t b = __float_as_uint(v);
+  uint32_t u = b ^ (uint32_t)((int)b >> 31 | (int)0x80000000u);
+  u = max_u(u, dpp_u<DPP_XOR1>(u));
+  u = max_u(u, dpp_u<DPP_XOR2>(u));
+  u = max_u(u, dpp_u<DPP_ROR4>(u));
+  u = max_u(u, dpp_u<DPP_ROR8>(u));
+  const auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = max_u(x[0], x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  u = max_u(y[0], y[1]);
+  return __uint_as_float((int)u < 0 ? u & 0x7fffffffu : ~u);
+}
+
 constexpr uint32_t HI4 = 0xf0f0f0f0u;
 DEVI int even4(uint32_t w) { return (int)((w << 4) & HI4); }  // the low nibbles as bytes 16 c
 DEVI int odd4(uint32_t w) { return (int)(w & HI4); }
 
+// Registers: four waves a SIMD up to 4 heads (at 4 heads 3 waves give 88 us where 4 give 79: 16 rows of up to 32768
+// keys, 8 x 4 heads), two beyond.
 template <bool SELF, int G, int W>
-__global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p) {
+__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(G <= 4 ? 4 : 2)))
+dec_attention_q4_kernel(const Q4Args p) {
   constexpr int SETS = (G + 1) / 2, PARTS = W + (SELF ? 1 : 0);  // A operands; partial results, the new token's last
-  __shared__ __attribute__((aligned(16))) uint8_t sq[G][NG][2][GRP];
+  // the queries' digits [head][group][high, low][32], then 16 zeros
+  __shared__ __attribute__((aligned(16))) uint8_t sq[G * HD * 2 + 16];
   __shared__ float sqs[G][NG];
   __shared__ __attribute__((aligned(16))) uint8_t sp8[W][SETS][16 * 64];
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
@@ -121,10 +154,8 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
     for (int i = 0; i < 16; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b32(vrs, off + i * VB, 0, 0);
   };
   int j0 = start + wave * 64;
-  if (j0 < end) {
-    load_k(j0);
-    load_v(j0);
-  }
+  load_k(j0);
+  load_v(j0);
 
   // the queries' digits, a dimension per thread; byte 8 (d / 8) + 4 (d % 2) + d % 8 / 2 of its group, as the codes'
   for (int i = tid; i < G * HD; i += W * 64) {
@@ -142,11 +173,12 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
     // m 2^e in (16319, 32639]: digits 127, 127 are 32639
     const int ex = 15 - __builtin_amdgcn_frexp_expf(m), e = ldexpf(m, ex) <= 32639.f ? ex : ex - 1;
     const int t = (ok ? (int)rintf(ldexpf(__uint_as_float(bits), e)) : 0) + 128;
-    uint8_t* dst = &sq[g][d >> 5][0][(at >> 3) * 8 + (at & 1) * 4 + ((at & 7) >> 1)];
+    uint8_t* dst = &sq[(g * HD + (d & ~31)) * 2 + (at >> 3) * 8 + (at & 1) * 4 + ((at & 7) >> 1)];
     dst[0] = (uint8_t)(t >> 8);
     dst[GRP] = (uint8_t)(t ^ 128);
     if (at == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / UNIT), -e) : nan_f();
   }
+  if (tid < 4) *reinterpret_cast<uint32_t*>(&sq[G * HD * 2 + tid * 4]) = 0;
   if constexpr (SELF) {
     const bool fresh = row_ok && sp == 0;
     const uint16_t* row = p.q + (int64_t)r * p.ldq;
@@ -180,27 +212,21 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
     }
   }
   __syncthreads();
-  // A of the first product: row 4 g + t of set s is group g of head 2 s + t / 2, digit t % 2
-  v4i aq[SETS][2];
-  float qs[G];
-#pragma unroll
-  for (int st = 0; st < SETS; ++st) {
+  // A of the first product: row 4 g + t of set s is group g of head 2 s + t / 2, digit t % 2 (its halves 16 bytes apart),
+  // zeros outside the group
+  auto a_of = [&](int st, int half) {
     const int head = 2 * st + ((col & 3) >> 1);
     const bool mine = (col >> 2) == rowg && head < G;
-    const v4i* src = reinterpret_cast<const v4i*>(&sq[head < G ? head : 0][rowg][col & 1][0]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const v4i t = src[i];
-      aq[st][i] = mine ? t : v4i{0, 0, 0, 0};
-    }
-  }
+    return *reinterpret_cast<const v4i*>(&sq[mine ? (head * NG + rowg) * 64 + (col & 1) * 32 + half * 16 : G * HD * 2]);
+  };
+  float qs[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) qs[g] = sqs[g][rowg];
 
   float m[G], l[G], acc[G][8];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    m[g] = -INFINITY;
+    m[g] = BOTTOM;
     l[g] = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[g][k] = 0.f;
@@ -209,9 +235,14 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
     // scores of key j0 + lane
     float sc[G];
     {
-      float x[G][4];
+      v4i aq[SETS][2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int st = 0; st < SETS; ++st) aq[st][0] = a_of(st, 0), aq[st][1] = a_of(st, 1);
+      // tiles of 16 keys in the order 0, 2, 1, 3: what two of them give meets at once
+      float x[G], z[G];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = i == 1 ? 2 : i == 2 ? 1 : i;
         const v4i b0 = {even4(kr[t].x), odd4(kr[t].x), even4(kr[t].y), odd4(kr[t].y)};
         const v4i b1 = {even4(kr[t].z), odd4(kr[t].z), even4(kr[t].w), odd4(kr[t].w)};
         const float mk = __uint_as_float(km[t] << 16);
@@ -220,19 +251,20 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
           v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st][0], b0, v4i{0, 0, 0, 0}, 0, 0, 0);
           d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st][1], b1, d, 0, 0, 0);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (2 * st + i < G) x[2 * st + i][t] = (float)(d[2 * i] * 256 + d[2 * i + 1]) * (mk * qs[2 * st + i]);
+          for (int h = 0; h < 2; ++h) {
+            const int g = 2 * st + h;
+            if (g >= G) continue;
+            const float v = (float)(d[2 * h] * 256 + d[2 * h + 1]) * (mk * qs[g]);
+            if (i == 0 || i == 2) x[g] = v;
+            else if (i == 1) z[g] = half_sum(x[g], v);
+            else sc[g] = quarter_sum(z[g], half_sum(x[g], v));
+          }
         }
       }
-      const auto add = [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        sc[g] = __uint_as_float(rows4(__float_as_uint(x[g][0]), __float_as_uint(x[g][1]), __float_as_uint(x[g][2]),
-                                      __float_as_uint(x[g][3]), add));
     }
     const bool live = j0 + lane < end;
     const int jn = j0 + W * 64;
-    if (jn < end) load_k(jn);
+    load_k(jn);
     // weights; p m_g in fixed point into A's rows
     float inv[G];
     const float vmx[NG] = {__uint_as_float(vm.x << 16), __uint_as_float(vm.x & 0xffff0000u),
@@ -240,19 +272,22 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float sg = live ? sc[g] : -INFINITY;
-      const float mn = fmaxf(m[g], wave_max64(sg)), base = mn == -INFINITY ? 0.f : mn;
-      const float a = exp2_hw(m[g] - base), e = exp2_hw(sg - base);
-      l[g] = __builtin_fmaf(l[g], a, e);
-      m[g] = mn;
-      if (__builtin_amdgcn_readfirstlane(__float_as_int(a)) != 0x3f800000) {
+      // the base of the weights moves only when a score is above it by more than RISE (weights up to 2^RISE: the fixed
+      // point below is relative to them): rarely after the first keys, and otherwise one comparison
+      if (__any(sg > m[g] + RISE)) {
+        const float mn = wave_top(sg), a = exp2_hw(m[g] - mn);
+        l[g] *= a;
+        m[g] = mn;
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[g][k] *= a;
       }
+      const float e = exp2_hw(sg - m[g]);
+      l[g] += e;
       float w[NG];
 #pragma unroll
       for (int i = 0; i < NG; ++i) w[i] = e * vmx[i];
       // the wave's largest of each group, in row i of lanes group i's (a NaN's bits are larger than any number's)
-      uint32_t y = rows4(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]), max_u);
+      uint32_t y = rows_max(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
       y = max_u(y, dpp_u<DPP_XOR1>(y));
       y = max_u(y, dpp_u<DPP_XOR2>(y));
       y = max_u(y, dpp_u<DPP_ROR4>(y));
@@ -280,7 +315,6 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
       const uint32_t v[4] = {vr[4 * i], vr[4 * i + 1], vr[4 * i + 2], vr[4 * i + 3]};
       bytes4(v, x[i]);
     }
-    if (jn < end) load_v(jn);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int b = j >> 1;
@@ -296,6 +330,7 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
                 __builtin_fmaf((float)(d[2 * i] * 256 + d[2 * i + 1]), inv[2 * st + i], acc[2 * st + i][j]);
       }
     }
+    load_v(jn);  // here, not before the products: the words would live beside the bytes (16 registers)
     asm volatile("" ::: "memory");  // the next pass's weights are written after these are read
     j0 = jn;
   }
@@ -317,14 +352,14 @@ __global__ void __launch_bounds__(W * 64) dec_attention_q4_kernel(const Q4Args p
   for (int i = tid; i < G * HD; i += W * 64) {
     const int g = i >> 7, d = i & (HD - 1);
     if (ch * G + g >= p.ratio) continue;
-    float M = -INFINITY, L = 0.f, O = 0.f;
+    float M = BOTTOM, L = 0.f, O = 0.f;
 #pragma unroll
     for (int w = 0; w < PARTS; ++w) M = fmaxf(M, sm[g][w]);
 #pragma unroll
     for (int w = 0; w < PARTS; ++w) {
-      const float f = exp2_hw(sm[g][w] - (M == -INFINITY ? 0.f : M));
+      const float f = exp2_hw(sm[g][w] - M);
       L = __builtin_fmaf(f, sl[g][w], L);
-      // a part without keys (weight 0) may be unwritten; a score that is no number counts (its sum is NaN)
+      // the new token's outputs are unwritten where it does not count
       if (f != 0.f) O = __builtin_fmaf(f, so[g][w][d], O);
     }
     const int64_t head = (int64_t)r * p.H + h0 + g;
@@ -358,7 +393,7 @@ __global__ void __launch_bounds__(CG * HD) dec_combine_q4_kernel(const float* __
     const int s = grp + CG * i;
     v[i] = s < nsp ? base[s * (HD + 2) + d] : 0.f;
   }
-  const float M = wave_max64(ms), w = exp2_hw(ms - (M == -INFINITY ? 0.f : M)), L = wave_sum64(w * ls);
+  const float M = wave_max64(ms), w = exp2_hw(ms - M), L = wave_sum64(w * ls);
   float o = 0.f;
 #pragma unroll
   for (int i = 0; i < MAXSPLITS / CG; ++i) o = __builtin_fmaf(lane_value(w, grp + CG * i), v[i], o);
@@ -372,79 +407,115 @@ __global__ void __launch_bounds__(CG * HD) dec_combine_q4_kernel(const float* __
 
 // ---- filling and reading back -----------------------------------------------------------------------------------------
 // kv (rows, L * 2 * KV * 128): per layer KV keys then KV values; row i is position frame_of[i] of slot slot_of[i];
-// caches (L, S, KV, T). 16 lanes per vector, 8 values (one word of codes) each; a quad of lanes holds a group.
+// caches (L, S, KV, T). 16 lanes per vector, 8 values (one word of codes) each; a quad of lanes holds a group. A
+// workgroup takes 16 vectors of a row, in ROWS rows (fewer vectors to a row: more rows), so that a lane has ROWS loads in
+// flight and finds its vector's place once. Bound by the memory: see each kernel.
 struct KvArgs {
   uint16_t* kv;
   const int32_t *slot_of, *frame_of;
   uint8_t *k4, *v4;
   uint16_t *ks, *vs;
   int64_t ldkv;
-  int rows, L, S, H, T;
+  int rows, S, H, T, vecs, blocks, side;  // vectors a row, workgroups a row, rows side by side in a workgroup
 };
+constexpr int ROWS = 4;
 
+// a lane's place: its vector of a row and its rows row, row + side, ..
 struct KvPlace {
-  bool live, in;  // a row of the call; a position of the caches
-  int row, d8, kvi;
-  int64_t col, vec;
+  int d8, kvi, row, step;
+  int64_t col, head;  // head: the vector's (layer, slot 0, head) as a number of heads; slots are H heads apart
+  bool in;
 };
-
 DEVI KvPlace kv_place(const KvArgs& p) {
-  const int chunks = p.L * 2 * p.H * (HD / 8);
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int b = blockIdx.x, vslot = threadIdx.x >> 4;
+  int v, at = 0;
+  if (p.side == 1) {
+    v = b % p.blocks * 16 + vslot;
+  } else {
+    at = vslot / p.vecs;
+    v = vslot - at * p.vecs;
+  }
   KvPlace k;
-  k.live = idx < (int64_t)p.rows * chunks;
-  k.row = k.live ? (int)(idx / chunks) : 0;
-  const int c = k.live ? (int)(idx % chunks) : 0;
-  k.col = (int64_t)c * 8;
-  k.d8 = c % (HD / 8);
-  const int v = c / (HD / 8), h = v % p.H, l = v / (2 * p.H);
-  k.kvi = v / p.H % 2;
-  const int s = p.slot_of[k.row], t = p.frame_of[k.row];
-  k.in = (unsigned)s < (unsigned)p.S && (unsigned)t < (unsigned)p.T;
-  k.vec = k.in ? (((int64_t)l * p.S + s) * p.H + h) * p.T + t : 0;
+  k.in = v < p.vecs && at < p.side;
+  k.d8 = threadIdx.x & 15;
+  k.row = b / p.blocks * (ROWS * p.side) + at;
+  k.step = p.side;
+  const int lk = v / p.H, l = lk >> 1;
+  k.kvi = lk & 1;
+  k.col = (int64_t)v * HD + k.d8 * 8;
+  k.head = (int64_t)l * p.S * p.H + (v - lk * p.H);
   return k;
+}
+// the vector of row r in the caches, or -1
+DEVI int64_t kv_vec(const KvArgs& p, const KvPlace& k, int r) {
+  const int s = p.slot_of[r], t = p.frame_of[r];
+  if ((unsigned)s >= (unsigned)p.S || (unsigned)t >= (unsigned)p.T) return -1;
+  return (k.head + (int64_t)s * p.H) * p.T + t;
 }
 
 __global__ void __launch_bounds__(256) dec_scatter_kv_q4_kernel(const KvArgs p) {
   const KvPlace k = kv_place(p);
-  float x[8];
-  uint32_t mx = unpack8(*reinterpret_cast<const uint4*>(p.kv + (int64_t)k.row * p.ldkv + k.col), x);
-  mx = quad_max_u(mx);
-  if (!k.live || !k.in) return;
-  const Group g = group_of(mx);
-  *reinterpret_cast<uint32_t*>((k.kvi ? p.v4 : p.k4) + k.vec * VB + k.d8 * 4) = pack8(g, x);
-  if ((k.d8 & 3) == 0) (k.kvi ? p.vs : p.ks)[k.vec * NG + (k.d8 >> 2)] = g.store;
+  uint4 u[ROWS];
+  int64_t vec[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = k.row + i * k.step;
+    const bool live = k.in && r < p.rows;
+    u[i] = live ? *reinterpret_cast<const uint4*>(p.kv + (int64_t)r * p.ldkv + k.col) : make_uint4(0, 0, 0, 0);
+    vec[i] = live ? kv_vec(p, k, r) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    float x[8];
+    const Group g = group_of(quad_max_u(unpack8(u[i], x)));
+    const uint32_t w = pack8(g, x);
+    if (vec[i] < 0) continue;
+    *reinterpret_cast<uint32_t*>((k.kvi ? p.v4 : p.k4) + vec[i] * VB + k.d8 * 4) = w;
+    if ((k.d8 & 3) == 0) (k.kvi ? p.vs : p.ks)[vec[i] * NG + (k.d8 >> 2)] = g.store;
+  }
 }
 
 __global__ void __launch_bounds__(256) dec_gather_kv_q4_kernel(const KvArgs p) {
   const KvPlace k = kv_place(p);
-  if (!k.live) return;
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (k.in) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>((k.kvi ? p.v4 : p.k4) + k.vec * VB + k.d8 * 4);
-    const Step m = step_of(bf2f((k.kvi ? p.vs : p.ks)[k.vec * NG + (k.d8 >> 2)]));
+  uint32_t w[ROWS], m[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = k.row + i * k.step;
+    const int64_t vec = k.in && r < p.rows ? kv_vec(p, k, r) : -1;
+    w[i] = vec < 0 ? 0u : *reinterpret_cast<const uint32_t*>((k.kvi ? p.v4 : p.k4) + vec * VB + k.d8 * 4);
+    m[i] = vec < 0 ? 0u : (k.kvi ? p.vs : p.ks)[vec * NG + (k.d8 >> 2)];
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = k.row + i * k.step;
+    const Step st = step_of(__uint_as_float(m[i] << 16));
     float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = held(code(w, i), m);
-    o = make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
+    for (int j = 0; j < 8; ++j) f[j] = held(code(w[i], j), st);
+    if (k.in && r < p.rows)
+      *reinterpret_cast<uint4*>(p.kv + (int64_t)r * p.ldkv + k.col) =
+          make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
   }
-  *reinterpret_cast<uint4*>(p.kv + (int64_t)k.row * p.ldkv + k.col) = o;
 }
 
 bool al(const void* q, int n) { return (reinterpret_cast<uintptr_t>(q) & (n - 1)) == 0; }
 
-int kv_entry(bool gather, const KvArgs& p, int64_t rows, int64_t L, int64_t S, int64_t H, int64_t T, void* stream,
+int kv_entry(bool gather, KvArgs p, int64_t rows, int64_t L, int64_t S, int64_t H, int64_t T, void* stream,
              const char* name) {
   const std::string nm(name);
   const int64_t top = 0x7fffffff;
-  COHERE_REQUIRE(rows >= 0 && rows <= top && L > 0 && S > 0 && S <= top && H > 0 && T > 0 && T <= top &&
-                     L <= top / (2 * HD) / H && p.ldkv >= L * 2 * H * HD && p.ldkv % 8 == 0,
+  COHERE_REQUIRE(rows >= 0 && rows <= (1 << 30) && L > 0 && S > 0 && S <= top && H > 0 && T > 0 && T <= top &&
+                     H <= top / (2 * HD) / L && p.ldkv >= L * 2 * H * HD && p.ldkv % 8 == 0,
                  nm + ": bad sizes");
   COHERE_REQUIRE(p.kv && p.slot_of && p.frame_of && al(p.kv, 16), nm + ": bad pointer");
   COHERE_REQUIRE(p.k4 && p.v4 && p.ks && p.vs && al(p.k4, 16) && al(p.v4, 16) && al(p.ks, 8) && al(p.vs, 8),
                  nm + ": bad cache pointer");
   if (rows == 0) return 0;
-  const int64_t n = rows * L * 2 * H * (HD / 8), grid = (n + 255) / 256;
+  p.rows = (int)rows; p.S = (int)S; p.H = (int)H; p.T = (int)T;
+  p.vecs = (int)(L * 2 * H);
+  p.blocks = (p.vecs + 15) / 16;
+  p.side = p.vecs < 16 ? 16 / p.vecs : 1;
+  const int64_t grid = (rows + ROWS * p.side - 1) / (ROWS * p.side) * p.blocks;
   COHERE_REQUIRE(grid <= top, nm + ": too many rows for one call");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (gather) dec_gather_kv_q4_kernel<<<(unsigned)grid, 256, 0, s>>>(p);
@@ -459,20 +530,19 @@ HeadPlan head_plan(int64_t ratio) {
   return {g <= 4 ? g : g <= 6 ? 6 : 8, chunks};
 }
 
-#ifndef COHERE_Q4_WAVES
-#define COHERE_Q4_WAVES 8
-#endif
-constexpr int WAVES = COHERE_Q4_WAVES;  // a workgroup's
+// waves of a workgroup: 4 for one head (64 rows x 8 heads, up to 448 keys: 7.0 us, with 8 7.5 us), else 8 (37 rows x 4 x 3
+// heads, up to 1026 keys: 9.8 us, with 4 12.9 us)
+constexpr int waves_of(int g) { return g == 1 ? 4 : 8; }
 
 template <bool SELF>
 void launch_attention(int g, const Q4Args& p, dim3 grid, hipStream_t s) {
   switch (g) {
-    case 1: dec_attention_q4_kernel<SELF, 1, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
-    case 2: dec_attention_q4_kernel<SELF, 2, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
-    case 3: dec_attention_q4_kernel<SELF, 3, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
-    case 4: dec_attention_q4_kernel<SELF, 4, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
-    case 6: dec_attention_q4_kernel<SELF, 6, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
-    default: dec_attention_q4_kernel<SELF, 8, WAVES><<<grid, WAVES * 64, 0, s>>>(p); break;
+    case 1: dec_attention_q4_kernel<SELF, 1, waves_of(1)><<<grid, waves_of(1) * 64, 0, s>>>(p); break;
+    case 2: dec_attention_q4_kernel<SELF, 2, waves_of(2)><<<grid, waves_of(2) * 64, 0, s>>>(p); break;
+    case 3: dec_attention_q4_kernel<SELF, 3, waves_of(3)><<<grid, waves_of(3) * 64, 0, s>>>(p); break;
+    case 4: dec_attention_q4_kernel<SELF, 4, waves_of(4)><<<grid, waves_of(4) * 64, 0, s>>>(p); break;
+    case 6: dec_attention_q4_kernel<SELF, 6, waves_of(6)><<<grid, waves_of(6) * 64, 0, s>>>(p); break;
+    default: dec_attention_q4_kernel<SELF, 8, waves_of(8)><<<grid, waves_of(8) * 64, 0, s>>>(p); break;
   }
 }
 
@@ -481,11 +551,22 @@ void launch_attention(int g, const Q4Args& p, dim3 grid, hipStream_t s) {
 extern "C" int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, int64_t kv_heads, int64_t T) {
   if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || T <= 0) return 1;
   const HeadPlan hp = head_plan(heads / kv_heads);
-  // enough workgroups for two waves of the chip's 256 CUs, each with two passes of keys at least
-  const int64_t wgs = rows * kv_heads * hp.chunks, pass = WAVES * 64;
-  const int64_t want = (1024 + wgs - 1) / wgs, most = (T + 2 * pass - 1) / (2 * pass);
-  const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : n > 64 ? 64 : n;
+  // The time by a model, in passes of a workgroup (64 keys a wave): the keys of a part in passes, at least half of one
+  // (the loads' latency), times the rounds that the workgroups take, and what the parts' meeting costs. A round is 256
+  // workgroups (512 of one head, which take half the registers); where two share a CU their waits overlap. Fitted to
+  // sweeps over 1 .. 64 parts of 15 shapes (1 .. 128 rows, 1 .. 64 K keys, 1 .. 8 heads a key head): its choice is within
+  // 10 % of the best of each. Powers of two: 48 parts of 16384 keys (no whole rounds) take 8.7 us, 32 or 64 7.7.
+  const int64_t wgs = rows * kv_heads * hp.chunks;
+  const double pass = 64. * waves_of(hp.g), us = hp.g == 1 ? 1.15 : 0.2 + 0.5 * hp.g, slots = hp.g == 1 ? 512. : 256.;
+  int64_t best = 1;
+  double least = 0.;
+  for (int64_t n = 1; n <= 64 && (n == 1 || T / n >= 128); n *= 2) {
+    const double keys = (double)T / n / pass, rounds = wgs * n / slots;
+    double t = (keys > 0.5 ? keys : 0.5) * us * (rounds > 1. ? rounds : 1.) + (n > 1 ? 2.5 + 0.03 * n : 0.);
+    if (hp.g > 1 && hp.g <= 4 && rounds >= 2.) t *= 0.9;
+    if (n == 1 || t < least * 0.999) best = n, least = t;
+  }
+  return best;
 }
 
 extern "C" int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
@@ -521,8 +602,7 @@ extern "C" int cohere_dec_scatter_kv_q4(const uint16_t* kv, int64_t ldkv, int64_
                                         const int32_t* frame_of, uint8_t* ck, uint8_t* cv, uint16_t* cks, uint16_t* cvs,
                                         int64_t L, int64_t S, int64_t H, int64_t T, void* stream) {
   cohere::clear_error();
-  const KvArgs p{const_cast<uint16_t*>(kv), slot_of, frame_of, ck, cv, cks, cvs, ldkv, (int)rows, (int)L, (int)S,
-                 (int)H, (int)T};
+  const KvArgs p{const_cast<uint16_t*>(kv), slot_of, frame_of, ck, cv, cks, cvs, ldkv, 0, 0, 0, 0, 0, 0, 0};
   return kv_entry(false, p, rows, L, S, H, T, stream, "dec_scatter_kv_q4");
 }
 
@@ -531,6 +611,6 @@ extern "C" int cohere_dec_gather_kv_q4(const int32_t* slot_of, const int32_t* fr
                                        int64_t H, int64_t T, uint16_t* kv, int64_t ldkv, void* stream) {
   cohere::clear_error();
   const KvArgs p{kv, slot_of, frame_of, const_cast<uint8_t*>(ck), const_cast<uint8_t*>(cv), const_cast<uint16_t*>(cks),
-                 const_cast<uint16_t*>(cvs), ldkv, (int)rows, (int)L, (int)S, (int)H, (int)T};
+                 const_cast<uint16_t*>(cvs), ldkv, 0, 0, 0, 0, 0, 0, 0};
   return kv_entry(true, p, rows, L, S, H, T, stream, "dec_gather_kv_q4");
 }
