@@ -38,11 +38,12 @@ struct LogitArgs {
 
 constexpr int NT = 256;
 
-// J chunks of 8 logits a thread: a workgroup takes J * 2048 logits
-template <int J>
+// J chunks of 8 logits a thread: a workgroup takes J * 2048 logits; counts of BITS bits (16: of at most 65535 tokens)
+template <int J, int BITS>
 __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
   constexpr int SPAN = J * NT * 8;
-  __shared__ __attribute__((aligned(16))) uint32_t cnt[SPAN];
+  constexpr int PER = 32 / BITS;  // counts a word
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[SPAN / PER];
   const int r = blockIdx.y, tid = threadIdx.x, v0 = blockIdx.x * SPAN;
   const uint16_t* xr = a.x + (int64_t)r * a.ldx;
   uint16_t* yr = a.y + (int64_t)r * a.ldy;
@@ -55,45 +56,54 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
   const int s = a.active[r];
   const bool known = (unsigned)s < (unsigned)a.S;  // a row of no slot is copied
   float rep = 1.f, presence = 0.f, freq = 0.f;
-  int p = 0, state = -1, b = -1;
+  int p = 0, state = -1, b = -1, lo = 0, hi = -1;
   bool penal = false;
+  const int64_t* tokens = a.tokens + (known ? (int64_t)s * a.OUT : 0);
+  int64_t t[8];  // tokens lo + tid + k NT of this thread: on their way while the rest is looked up and the counts cleared
   if (known) {
     p = a.pos[s];
     if (a.pen) {
+      lo = a.first[s] > 0 ? a.first[s] : 0;
+      hi = p < a.OUT ? p : a.OUT - 1;
       rep = a.pen[s * (int64_t)3];
       presence = a.pen[s * (int64_t)3 + 1];
       freq = a.pen[s * (int64_t)3 + 2];
-      penal = rep != 1.f || presence != 0.f || freq != 0.f;
+      penal = lo <= hi;
+      if (penal) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = tokens[min(lo + tid + k * NT, hi)];
+      }
+      penal = penal && (rep != 1.f || presence != 0.f || freq != 0.f);
     }
     if (a.bias) b = a.bias_of[s];
     if (a.mask) {
       state = a.start[s];
       if (a.trans && p >= a.plen[s]) {
         state = a.state[s * (int64_t)2 + ((p + 1) & 1)];
-        const int64_t t = p >= 0 && p < a.OUT ? a.tokens[(int64_t)s * a.OUT + p] : -1;
-        const int cls = t >= 0 && t < a.V ? a.classes[t] : -1;
+        const int64_t v = p >= 0 && p < a.OUT ? tokens[p] : -1;
+        const int cls = v >= 0 && v < a.V ? a.classes[v] : -1;
         state = (unsigned)state < (unsigned)a.M && (unsigned)cls < (unsigned)a.C
                     ? a.trans[(int64_t)state * a.C + cls] : -1;
       }
       if (a.trans && blockIdx.x == 0 && tid == 0) a.state[s * (int64_t)2 + (p & 1)] = state;
     }
   }
-  const int lo = known && penal ? (a.first[s] > 0 ? a.first[s] : 0) : 0, hi = p < a.OUT ? p : a.OUT - 1;
-  penal = penal && lo <= hi;
+  const float inv = 1.f / rep;
   if (penal) {
 #pragma unroll
-    for (int j = 0; j < 2 * J; ++j)
+    for (int j = 0; j < 2 * J / PER; ++j)
       *reinterpret_cast<uint4*>(&cnt[(j * NT + tid) * 4]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const int64_t* t = a.tokens + (int64_t)s * a.OUT;
-    // eight tokens a thread in flight
-    for (int i0 = lo + tid; i0 <= hi; i0 += NT * 8) {
-      int64_t d[8];
+    for (int i0 = lo + tid; i0 <= hi;) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = hi - i0 >= k * NT ? t[i0 + k * NT] - v0 : -1;
+      for (int k = 0; k < 8; ++k) {
+        const int64_t d = t[k] - v0;
+        if (hi - i0 >= k * NT && d >= 0 && d < SPAN)
+          atomicAdd(&cnt[(uint32_t)d / PER], 1u << ((uint32_t)d % PER * (BITS % 32)));
+      }
+      i0 += NT * 8;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (d[k] >= 0 && d[k] < SPAN) atomicAdd(&cnt[d[k]], 1u);
+      for (int k = 0; k < 8; ++k) t[k] = tokens[min(hi, i0 + k * NT)];
     }
     __syncthreads();
   }
@@ -109,14 +119,22 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
     if (penal) {
-      const uint4 c0 = *reinterpret_cast<const uint4*>(&cnt[at]), c1 = *reinterpret_cast<const uint4*>(&cnt[at + 4]);
-      const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      uint32_t w8[8 / PER], c[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c[k]) {
-          f[k] = f[k] > 0.f ? f[k] / rep : f[k] * rep;
-          f[k] -= (float)c[k] * freq + presence;
+      for (int i = 0; i < 2 / PER; ++i)
+        *reinterpret_cast<uint4*>(&w8[4 * i]) = *reinterpret_cast<const uint4*>(&cnt[at / PER + 4 * i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) c[k] = PER == 1 ? w8[k] : k & 1 ? w8[k / 2] >> 16 : w8[k / 2] & 0xffffu;
+      // the quotient l / rep from the reciprocal, corrected once by the exact remainder (rounded right; the fixup is for
+      // infinities): 4 instructions where the division takes 11
+      if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float t = f[k] * inv, q = __builtin_fmaf(__builtin_fmaf(-t, rep, f[k]), inv, t);
+          const float l = f[k] > 0.f ? __builtin_amdgcn_div_fixupf(q, rep, f[k]) : f[k] * rep;
+          f[k] = c[k] ? l - ((float)c[k] * freq + presence) : f[k];
         }
+      }
     }
     if (br) {
       const uint4 t = *reinterpret_cast<const uint4*>(br + v);
@@ -148,7 +166,7 @@ extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, in
   cohere::clear_error();
   const int64_t top = 0x7fffffff;
   COHERE_REQUIRE(rows >= 0 && rows <= 65535 && V > 0 && V % 8 == 0 && V < (int64_t(1) << 30) && slots > 0 &&
-                     slots <= top && OUT > 0 && OUT <= top,
+                     slots <= top && OUT > 0 && OUT <= (1 << 30),
                  "dec_logits: bad sizes (the vocabulary a multiple of 8)");
   COHERE_REQUIRE(x && y && al(x, 16) && al(y, 16) && ldx >= V && ldy >= V && ldx % 8 == 0 && ldy % 8 == 0,
                  "dec_logits: logits rows must be 16-byte aligned");
@@ -163,7 +181,10 @@ extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, in
                     (int)B, (int)M, (int)C};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const auto wgs = [&](int j) { return (unsigned)((V + j * 2048 - 1) / (j * 2048)); };
-  if (rows * wgs(4) >= 512) dec_logits_kernel<4><<<dim3(wgs(4), (unsigned)rows), NT, 0, s>>>(a);
-  else dec_logits_kernel<1><<<dim3(wgs(1), (unsigned)rows), NT, 0, s>>>(a);
+  // 4096 logits a workgroup where that leaves four workgroups a CU (128 rows x 32000: 7.5 us, with 8192 8.1), else 2048
+  const dim3 wide(wgs(2), (unsigned)rows);
+  if (OUT > 65535) dec_logits_kernel<2, 32><<<wide, NT, 0, s>>>(a);
+  else if (rows * wgs(2) >= 1024) dec_logits_kernel<2, 16><<<wide, NT, 0, s>>>(a);
+  else dec_logits_kernel<1, 16><<<dim3(wgs(1), (unsigned)rows), NT, 0, s>>>(a);
   return cohere::check_launch("dec_logits");
 }

@@ -418,82 +418,93 @@ struct KvArgs {
   int64_t ldkv;
   int rows, S, H, T, vecs, blocks, side;  // vectors a row, workgroups a row, rows side by side in a workgroup
 };
-constexpr int ROWS = 4;
 
-// a lane's place: its vector of a row and its rows row, row + side, ..
+// a lane's place: its vector of a row and its rows row, row + side, .. A lane without a place (or a row) looks at the
+// last one and writes nothing: a load that only some lanes make is a branch, and the loads behind it would wait.
 struct KvPlace {
-  int d8, kvi, row, step;
+  int d8, kvi, row;
   int64_t col, head;  // head: the vector's (layer, slot 0, head) as a number of heads; slots are H heads apart
   bool in;
 };
+template <int ROWS>
 DEVI KvPlace kv_place(const KvArgs& p) {
-  const int b = blockIdx.x, vslot = threadIdx.x >> 4;
-  int v, at = 0;
-  if (p.side == 1) {
-    v = b % p.blocks * 16 + vslot;
-  } else {
+  const int rb = blockIdx.x / p.blocks, vslot = threadIdx.x >> 4;
+  int v = (blockIdx.x - rb * p.blocks) * 16 + vslot, at = 0;
+  if (p.side > 1) {
     at = vslot / p.vecs;
     v = vslot - at * p.vecs;
   }
   KvPlace k;
   k.in = v < p.vecs && at < p.side;
+  v = min(v, p.vecs - 1);
   k.d8 = threadIdx.x & 15;
-  k.row = b / p.blocks * (ROWS * p.side) + at;
-  k.step = p.side;
+  k.row = rb * (ROWS * p.side) + at;
   const int lk = v / p.H, l = lk >> 1;
   k.kvi = lk & 1;
   k.col = (int64_t)v * HD + k.d8 * 8;
   k.head = (int64_t)l * p.S * p.H + (v - lk * p.H);
   return k;
 }
-// the vector of row r in the caches, or -1
-DEVI int64_t kv_vec(const KvArgs& p, const KvPlace& k, int r) {
-  const int s = p.slot_of[r], t = p.frame_of[r];
-  if ((unsigned)s >= (unsigned)p.S || (unsigned)t >= (unsigned)p.T) return -1;
-  return (k.head + (int64_t)s * p.H) * p.T + t;
+
+// row i of a lane: its number, whether it is the lane's, and its vector in the caches (-1: none)
+struct KvRow {
+  int r;
+  bool live;
+  int64_t vec;
+};
+DEVI KvRow kv_row(const KvArgs& p, const KvPlace& k, int i) {
+  KvRow w;
+  w.r = k.row + i * p.side;
+  w.live = k.in && w.r < p.rows;
+  w.r = min(w.r, p.rows - 1);
+  const int s = p.slot_of[w.r], t = p.frame_of[w.r];
+  w.vec = (unsigned)s < (unsigned)p.S && (unsigned)t < (unsigned)p.T ? (k.head + (int64_t)s * p.H) * p.T + t : -1;
+  return w;
 }
 
+template <int ROWS>
 __global__ void __launch_bounds__(256) dec_scatter_kv_q4_kernel(const KvArgs p) {
-  const KvPlace k = kv_place(p);
+  const KvPlace k = kv_place<ROWS>(p);
   uint4 u[ROWS];
-  int64_t vec[ROWS];
+  KvRow w[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = k.row + i * k.step;
-    const bool live = k.in && r < p.rows;
-    u[i] = live ? *reinterpret_cast<const uint4*>(p.kv + (int64_t)r * p.ldkv + k.col) : make_uint4(0, 0, 0, 0);
-    vec[i] = live ? kv_vec(p, k, r) : -1;
+    w[i] = kv_row(p, k, i);
+    u[i] = *reinterpret_cast<const uint4*>(p.kv + (int64_t)w[i].r * p.ldkv + k.col);
   }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     float x[8];
     const Group g = group_of(quad_max_u(unpack8(u[i], x)));
-    const uint32_t w = pack8(g, x);
-    if (vec[i] < 0) continue;
-    *reinterpret_cast<uint32_t*>((k.kvi ? p.v4 : p.k4) + vec[i] * VB + k.d8 * 4) = w;
-    if ((k.d8 & 3) == 0) (k.kvi ? p.vs : p.ks)[vec[i] * NG + (k.d8 >> 2)] = g.store;
+    const uint32_t c = pack8(g, x);
+    if (!w[i].live || w[i].vec < 0) continue;
+    *reinterpret_cast<uint32_t*>((k.kvi ? p.v4 : p.k4) + w[i].vec * VB + k.d8 * 4) = c;
+    if ((k.d8 & 3) == 0) (k.kvi ? p.vs : p.ks)[w[i].vec * NG + (k.d8 >> 2)] = g.store;
   }
 }
 
+template <int ROWS>
 __global__ void __launch_bounds__(256) dec_gather_kv_q4_kernel(const KvArgs p) {
-  const KvPlace k = kv_place(p);
-  uint32_t w[ROWS], m[ROWS];
+  const KvPlace k = kv_place<ROWS>(p);
+  const uint8_t* codes = k.kvi ? p.v4 : p.k4;
+  const uint16_t* maxima = k.kvi ? p.vs : p.ks;
+  KvRow w[ROWS];
+  uint32_t c[ROWS], m[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = k.row + i * k.step;
-    const int64_t vec = k.in && r < p.rows ? kv_vec(p, k, r) : -1;
-    w[i] = vec < 0 ? 0u : *reinterpret_cast<const uint32_t*>((k.kvi ? p.v4 : p.k4) + vec * VB + k.d8 * 4);
-    m[i] = vec < 0 ? 0u : (k.kvi ? p.vs : p.ks)[vec * NG + (k.d8 >> 2)];
+    w[i] = kv_row(p, k, i);
+    const int64_t vec = w[i].vec < 0 ? 0 : w[i].vec;
+    c[i] = *reinterpret_cast<const uint32_t*>(codes + vec * VB + k.d8 * 4);
+    m[i] = maxima[vec * NG + (k.d8 >> 2)];
   }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = k.row + i * k.step;
-    const Step st = step_of(__uint_as_float(m[i] << 16));
+    const Step st = step_of(__uint_as_float(w[i].vec < 0 ? 0u : m[i] << 16));
     float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = held(code(w[i], j), st);
-    if (k.in && r < p.rows)
-      *reinterpret_cast<uint4*>(p.kv + (int64_t)r * p.ldkv + k.col) =
+    for (int j = 0; j < 8; ++j) f[j] = w[i].vec < 0 ? 0.f : held(code(c[i], j), st);
+    if (w[i].live)
+      *reinterpret_cast<uint4*>(p.kv + (int64_t)w[i].r * p.ldkv + k.col) =
           make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
   }
 }
@@ -515,11 +526,17 @@ int kv_entry(bool gather, KvArgs p, int64_t rows, int64_t L, int64_t S, int64_t 
   p.vecs = (int)(L * 2 * H);
   p.blocks = (p.vecs + 15) / 16;
   p.side = p.vecs < 16 ? 16 / p.vecs : 1;
-  const int64_t grid = (rows + ROWS * p.side - 1) / (ROWS * p.side) * p.blocks;
+  const auto wgs = [&](int n) { return (rows + n * p.side - 1) / (n * p.side) * p.blocks; };
+  // four rows a lane where that leaves two workgroups a CU (3000 rows x 8 layers x 8 heads: gather 23.2 us, with one row
+  // 30.8; 128 rows: one row 3.6 us, four 4.1)
+  const bool many = wgs(4) >= 512;
+  const int64_t grid = wgs(many ? 4 : 1);
   COHERE_REQUIRE(grid <= top, nm + ": too many rows for one call");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (gather) dec_gather_kv_q4_kernel<<<(unsigned)grid, 256, 0, s>>>(p);
-  else dec_scatter_kv_q4_kernel<<<(unsigned)grid, 256, 0, s>>>(p);
+  if (gather && many) dec_gather_kv_q4_kernel<4><<<(unsigned)grid, 256, 0, s>>>(p);
+  else if (gather) dec_gather_kv_q4_kernel<1><<<(unsigned)grid, 256, 0, s>>>(p);
+  else if (many) dec_scatter_kv_q4_kernel<4><<<(unsigned)grid, 256, 0, s>>>(p);
+  else dec_scatter_kv_q4_kernel<1><<<(unsigned)grid, 256, 0, s>>>(p);
   return cohere::check_launch(name);
 }
 
