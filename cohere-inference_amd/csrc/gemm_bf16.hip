@@ -46,6 +46,7 @@ bool launch_gemm_bf16(int tile, int epi, const GemmArgs& p, hipStream_t s) {
     case EPI_CONV_RELU: return tiles_bf16<EPI_CONV_RELU>(tile, p, s);
     case EPI_KV: return tiles_kv<EPI_KV>(tile, p, s);
     case EPI_KV8: return tiles_kv<EPI_KV8>(tile, p, s);
+    case EPI_KV4: return tiles_kv<EPI_KV4>(tile, p, s);
     default: return false;
   }
 }

@@ -38,6 +38,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "q4.h"
 
 namespace cohere_gemm {
 
@@ -46,8 +47,8 @@ namespace cohere_gemm {
 enum { EPI_BIAS = 0, EPI_SILU = 1, EPI_RELU = 2, EPI_RESID = 3, EPI_GLU = 4, EPI_SILU_Q8 = 5, EPI_CONV_RELU = 6,
        EPI_I32 = 7,
        // internal, bf16 operands: BIAS whose rows go straight into the decoder's cross-attention caches, as
-       // dec_scatter_kv (_q8: int8 with a scale per 128 columns) stores them
-       EPI_KV = 8, EPI_KV8 = 9 };
+       // dec_scatter_kv (_q8: int8 with a scale per 128 columns; _q4: 4 bits with a maximum per 32) stores them
+       EPI_KV = 8, EPI_KV8 = 9, EPI_KV4 = 10 };
 
 struct GemmArgs {
   const int8_t* X;       // tokens [M, K], row stride ldx
@@ -69,8 +70,9 @@ struct GemmArgs {
                          // one part each per XCD (set by launch_tile); 0: contiguous tile ranges per XCD
   int tiled;             // 2:4 only: W holds the stage-tiled layout of the kept values and selectors (E unused)
   // (last: the other epilogues' arguments stay in the cache lines they had)
-  // EPI_KV, EPI_KV8: column block c of 128 is layer c / 2H, key (even) or value (odd) c / H % 2, head c % H; caches
-  // (layers, S, H, T, 128) with scales (layers, S, H, T); output row m goes to slot slot_of[m], position frame_of[m]
+  // EPI_KV, EPI_KV8, EPI_KV4: column block c of 128 is layer c / 2H, key (even) or value (odd) c / H % 2, head c % H; caches
+  // (layers, S, H, T, 128) with scales (layers, S, H, T), in 4 bits (.., 64) with bf16 maxima (.., 4); output row m goes
+  // to slot slot_of[m], position frame_of[m] (in 4 bits: nowhere if that is out of range)
   void *kc, *vc;
   float *ks, *vs;
   const int32_t *slot_of, *frame_of;
@@ -180,7 +182,7 @@ DEVI int sw64(int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
 template <int BM, int BN, int WM, int WN, int ST, int MS, int EPI, bool GROUPED, bool SPARSE, int GS = 0,
           bool BF = false>
 __global__ void __launch_bounds__(WM* WN * 64) gemm_q8_kernel(const GemmArgs p) {
-  constexpr bool KV = EPI == EPI_KV || EPI == EPI_KV8;
+  constexpr bool KV = EPI == EPI_KV || EPI == EPI_KV8 || EPI == EPI_KV4;
   static_assert(!BF || (!SPARSE && !GROUPED && EPI != EPI_SILU_Q8 && EPI != EPI_I32), "bf16 operands");
   static_assert(!KV || (BF && BN % 128 == 0), "cache epilogue");
   static_assert(BF || (EPI != EPI_RELU && EPI != EPI_CONV_RELU), "bf16-only epilogue");
@@ -679,8 +681,18 @@ __global__ void __launch_bounds__(WM* WN * 64) gemm_q8_kernel(const GemmArgs p) 
           // product; writing the caches here saves the product's write and read (98 MB each at 3000 rows of 16384):
           // the whole fill of 8 x 375 frames 177 -> 147 us (123 with the slots and positions written by a kernel)
           const int cb = (oc0 >> 7) + (cc >> 4), d8 = cc & 15, hd = cb % p.H, kvi = cb / p.H % 2, l = cb / p.H / 2;
-          const int64_t vec = (((int64_t)l * p.S + p.slot_of[m]) * p.H + hd) * p.T + p.frame_of[m];
-          if constexpr (EPI == EPI_KV) {
+          const int slot_m = p.slot_of[m], frame_m = p.frame_of[m];
+          const int64_t vec = (((int64_t)l * p.S + slot_m) * p.H + hd) * p.T + frame_m;
+          if constexpr (EPI == EPI_KV4) {
+            // a quad of lanes holds a group of 32
+            float f[8];
+            const cohere_q4::Group grp = cohere_q4::group_of(cohere_q4::quad_max_u(cohere_q4::unpack8(o, f)));
+            const uint32_t codes = cohere_q4::pack8(grp, f);
+            if ((unsigned)slot_m < (unsigned)p.S && (unsigned)frame_m < (unsigned)p.T) {
+              *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kvi ? p.vc : p.kc) + vec * 64 + d8 * 4) = codes;
+              if ((d8 & 3) == 0) reinterpret_cast<uint16_t*>(kvi ? p.vs : p.ks)[vec * 4 + (d8 >> 2)] = grp.store;
+            }
+          } else if constexpr (EPI == EPI_KV) {
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(kvi ? p.vc : p.kc) + vec * 128 + d8 * 8) = o;
           } else {
             const uint32_t ov[4] = {o.x, o.y, o.z, o.w};
@@ -892,7 +904,7 @@ int ref_config_group(int cfg);
 constexpr bool bf16_tile(int tile) {
   return tile == 0 || tile == 3 || tile == 6 || tile == 7 || tile == 8 || tile == 9 || tile == 15 || tile == 17;
 }
-// those of them with the cache epilogues (EPI_KV, EPI_KV8): whole 128-column vectors
+// those of them with the cache epilogues (EPI_KV, EPI_KV8, EPI_KV4): whole 128-column vectors
 constexpr bool kv_tile(int tile) { return tile == 3 || tile == 6 || tile == 9 || tile == 15 || tile == 17; }
 bool launch_gemm_bf16(int tile, int epi, const GemmArgs& p, hipStream_t s);
 

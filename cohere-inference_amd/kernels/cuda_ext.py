@@ -41,7 +41,7 @@ EXPORTS = ("cohere_gemm_i8", "cohere_gemm_sp", "cohere_quantize_rows", "cohere_l
            "cohere_gemm_sp_tiled", "cohere_pack_24_tiled_bytes", "cohere_pack_24_tiled", "cohere_sub_conv0_dw_pw",
            "cohere_sub_dw_pw", "cohere_gemm_kv", "cohere_gemm_kv_q8", "cohere_gemm_tile",
            "cohere_piece_rows", "cohere_dec_attention_q4", "cohere_dec_attention_q4_splits", "cohere_dec_scatter_kv_q4",
-           "cohere_dec_gather_kv_q4", "cohere_dec_logits")
+           "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4", "cohere_dec_logits")
 
 
 def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
@@ -90,6 +90,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "cohere_sub_dw_pw": [P, P, P, P, I64, P, P, P, P, P, P],
         "cohere_piece_rows": [P, P, I64, P, P, I64, P],
         "cohere_gemm_kv": [P, I64, P, P, I64, I64, P, P, P, P, I64, I64, I64, I64, P],
+        "cohere_gemm_kv_q4": [P, I64, P, P, I64, I64, P, P, P, P, P, P, I64, I64, I64, I64, P],
         "cohere_gemm_kv_q8": [P, I64, P, P, I64, I64, P, P, P, P, P, P, I64, I64, I64, I64, P],
         "cohere_encoder_layers": [P, I64, P, I64, P, P, I64, P, P, I64, I64, I64, ctypes.c_double, I32, I32, I32, P,
                                   I64, P, I64, P],
@@ -732,6 +733,25 @@ class _Ext:
         if rows and self._lib.cohere_dec_gather_kv_q4(slot_of.data_ptr(), frame_of.data_ptr(), rows, ck.data_ptr(),
                                                       cv.data_ptr(), cks.data_ptr(), cvs.data_ptr(), L, S, H, T,
                                                       kv.data_ptr(), ld, stream):
+            raise RuntimeError(self._lib.cohere_last_error().decode())
+
+    def gemm_kv_q4(self, a, w, bias, slot_of, frame_of, ck, cv, cks, cvs):
+        """gemm_kv into 4-bit caches (L, S, H, T, 64) with maxima (L, S, H, T, 4): gemm with EPI_BIAS, then
+        dec_scatter_kv_q4, in one launch; the same bytes."""
+        L, S, H, T = self._q4_caches("gemm_kv_q4", ck, cv, cks, cvs, 4)
+        if not (a.dim() == 2 and w.dim() == 2 and a.dtype is _BF and w.dtype is _BF and a.stride(1) == 1 and
+                w.is_contiguous() and w.shape == (L * 2 * H * 128, a.shape[1]) and a.shape[1] % 32 == 0 and
+                (bias is None or (bias.dtype is _BF and bias.numel() == w.shape[0] and bias.is_contiguous()))):
+            raise RuntimeError("gemm_kv_q4: bf16 a (rows, K), w (L * 2 * H * 128, K), bias, K % 32 == 0")
+        rows = a.shape[0]
+        if not (_index(slot_of, rows) and _index(frame_of, rows)):
+            raise RuntimeError("gemm_kv_q4: int32 slot and position per row")
+        if rows == 0:
+            return
+        stream = _stream_of("gemm_kv_q4", a, w, bias, slot_of, frame_of, ck, cv, cks, cvs)
+        if self._lib.cohere_gemm_kv_q4(a.data_ptr(), a.stride(0), w.data_ptr(), _ptr(bias), rows, a.shape[1],
+                                       slot_of.data_ptr(), frame_of.data_ptr(), ck.data_ptr(), cv.data_ptr(),
+                                       cks.data_ptr(), cvs.data_ptr(), L, S, H, T, stream):
             raise RuntimeError(self._lib.cohere_last_error().decode())
 
     def dec_logits(self, logits, y, active, pos, tokens=None, first=None, plen=None, penalties=None, bias=None,

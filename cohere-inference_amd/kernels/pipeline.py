@@ -35,7 +35,7 @@ import torch
 
 from kernels.fast_encoder import FastEncoder
 from kernels.features import Features, dither
-from kernels.stream_decoder import StreamDecoder
+from kernels.stream_decoder import Grammar, Rules, StreamDecoder
 
 
 class _Request:
@@ -60,8 +60,8 @@ class _Request:
 class _Piece:
     """A piece waiting for (or in) the pipeline: its samples (on the GPU once `ready` has fired), prompt and limit."""
 
-    def __init__(self, samples, prompt, max_new, request=None, k=0, ready=None):
-        self.samples, self.prompt, self.max_new = samples, prompt, max_new
+    def __init__(self, samples, prompt, max_new, request=None, k=0, ready=None, rules=None):
+        self.samples, self.prompt, self.max_new, self.rules = samples, prompt, max_new, rules
         self.request, self.k, self.ready = request, k, ready
         self.n = len(samples)
         self.arrived = time.perf_counter()
@@ -91,7 +91,8 @@ class _Decoding:
 
     def admit(self, slots: list[int], pieces: list[_Piece], lengths: list[int]) -> None:
         dec = self.dec
-        dec.admit(slots, [p.prompt for p in pieces], lengths, [p.max_new or dec.max_new_tokens for p in pieces])
+        dec.admit(slots, [p.prompt for p in pieces], lengths, [p.max_new or dec.max_new_tokens for p in pieces],
+                  [p.rules for p in pieces])
         for s, p in zip(slots, pieces):
             self.holder[s] = p
             self.first_step[s] = self.steps
@@ -160,7 +161,9 @@ class Pipeline:
     """Features, encoder and decoder of a transformers CohereAsrForConditionalGeneration on one GPU (reference
     kernels/pipeline.py:60-250, same constructor arguments and defaults; `extractor` may be None for the
     CohereAsrFeatureExtractor settings). Keyword-only extras: frames (encoder frames per decoder slot), buckets
-    (decoder row buckets), chunk_frames (encoder frames per encoder call), sparse_w1 (both feed-forward linears 2:4)."""
+    (decoder row buckets), chunk_frames (encoder frames per encoder call), sparse_w1 (both feed-forward linears 2:4),
+    kv_bits (bits of a cached value of the decoder: 16, 8 or 4), and what lets requests have Rules: penalties, bias (a
+    table of rows over the vocabulary), grammar (kernels.stream_decoder.Grammar)."""
 
     CHUNK_FRAMES = 3000  # encoder frames per encoder call (reference pipeline.py:61)
     LAG = 1  # steps between a step's launch and the host reading its end flags (reference pipeline.py:64)
@@ -171,13 +174,14 @@ class Pipeline:
 
     def __init__(self, model, extractor=None, slots: int = 128, max_new_tokens: int = 448, int8: bool = False,
                  sparse: str | bool | None = None, *, frames: int | None = None, buckets=None,
-                 chunk_frames: int | None = None, sparse_w1: bool = False):
+                 chunk_frames: int | None = None, sparse_w1: bool = False, kv_bits: int | None = None,
+                 penalties: bool = False, bias: torch.Tensor | None = None, grammar: Grammar | None = None):
         dev = model.proj_out.weight.device
         self.device = dev
         self.features = Features(extractor, device=dev)
         self.encoder = FastEncoder(model.model.encoder, int8=int8, sparse=sparse, sparse_w1=sparse_w1)
         self.decoder = StreamDecoder(model, slots=slots, max_new_tokens=max_new_tokens, int8=int8, frames=frames,
-                                     buckets=buckets)
+                                     buckets=buckets, kv_bits=kv_bits, penalties=penalties, bias=bias, grammar=grammar)
         if chunk_frames is not None:
             self.CHUNK_FRAMES = chunk_frames
         self.stats = {"steps": 0, "chunks": 0, "frames": 0}
@@ -221,13 +225,15 @@ class Pipeline:
     # ---- in the caller's thread -----------------------------------------------------------------------------------
 
     @torch.no_grad()
-    def transcribe(self, pieces: list, prompt: torch.Tensor, max_new: list[int] | None = None) -> list[np.ndarray]:
+    def transcribe(self, pieces: list, prompt: torch.Tensor, max_new: list[int] | None = None,
+                   rules: Rules | None = None) -> list[np.ndarray]:
         """Token ids (prompt + generated, up to and including the end token) of each dithered piece (numpy fp32
-        samples or fp32 tensors on the GPU), greedy, in the caller's thread."""
+        samples or fp32 tensors on the GPU), greedy under the rules (None: none), in the caller's thread."""
         if self._threads:
             raise RuntimeError("Pipeline: transcribe() cannot run beside the submit() threads")
         dec = self.decoder
-        queue = [_Piece(x, prompt, max_new[i] if max_new else None, k=i) for i, x in enumerate(pieces)]
+        dec.check_rules(rules)
+        queue = [_Piece(x, prompt, max_new[i] if max_new else None, k=i, rules=rules) for i, x in enumerate(pieces)]
         result: list = [None] * len(queue)
         run, free = _Decoding(dec, self.LAG), list(range(dec.slots))[::-1]
         while queue or run.active:
@@ -251,11 +257,14 @@ class Pipeline:
 
     # ---- the service ----------------------------------------------------------------------------------------------
 
-    def submit(self, pieces: list[np.ndarray], prompt: torch.Tensor, max_new: list[int] | None = None) -> Future:
+    def submit(self, pieces: list[np.ndarray], prompt: torch.Tensor, max_new: list[int] | None = None,
+               rules: Rules | None = None) -> Future:
         """Decode dithered pieces (prepare()) with this prompt; the future's result is one int64 array per piece,
-        prompt + generated ids. max_new: tokens to generate at most per piece (default the decoder's max_new_tokens).
-        The samples are copied to the GPU here, on a stream of their own."""
+        prompt + generated ids. max_new: tokens to generate at most per piece (default the decoder's max_new_tokens);
+        rules: what its tokens are chosen under (kernels.stream_decoder.Rules; None: none). The samples are copied to
+        the GPU here, on a stream of their own."""
         self._validate(pieces, prompt)
+        self.decoder.check_rules(rules)
         req = _Request(len(pieces))
         if not pieces:
             req.future.set_result([])
@@ -270,7 +279,7 @@ class Pipeline:
             if self._closed:
                 raise RuntimeError("Pipeline: closed")
             for k, x in enumerate(gpu):
-                self._waiting.append(_Piece(x, prompt, max_new[k] if max_new else None, req, k, ready))
+                self._waiting.append(_Piece(x, prompt, max_new[k] if max_new else None, req, k, ready, rules))
             self._cv.notify_all()
         return req.future
 

@@ -15,6 +15,9 @@ as a fixed list of launches over preallocated buffers and captured into one HIP 
 
 from __future__ import annotations
 
+import dataclasses
+import math
+
 import torch
 
 from kernels.cuda_ext import DEC_EP_NONE, DEC_EP_RELU, DEC_EP_RESID, ext
@@ -111,6 +114,45 @@ def dequantize_q4(codes: torch.Tensor, maxima: torch.Tensor) -> torch.Tensor:
     return (c * maxima.double().unsqueeze(-1) / 7).float().reshape(*codes.shape[:-1], 128)
 
 
+# ---- rules on the choice of tokens ------------------------------------------------------------------------------------
+
+class Grammar:
+    """A deterministic automaton over token classes: classes (V) gives each token's class 0..C-1, transitions (M, C) the
+    state that a class leads to from each of M states, -1 where it is not allowed. `mask` has a bit per state and token
+    that is allowed (int32 (M, ceil(V / 32)), bit v % 32 of word v / 32)."""
+
+    def __init__(self, classes, transitions):
+        c, t = torch.as_tensor(classes).cpu().long(), torch.as_tensor(transitions).cpu().long()
+        if c.dim() != 1 or t.dim() != 2 or c.numel() == 0 or t.numel() == 0:
+            raise ValueError("Grammar: classes (V) and transitions (M, C)")
+        if c.min() < 0 or c.max() >= t.shape[1] or t.min() < -1 or t.max() >= t.shape[0]:
+            raise ValueError("Grammar: a class outside the transitions' columns, or a state outside their rows")
+        self.classes, self.transitions = c.to(torch.int32), t.to(torch.int32)
+        allowed = torch.zeros(t.shape[0], (c.numel() + 31) // 32 * 32, dtype=torch.int64)
+        allowed[:, :c.numel()] = (t >= 0)[:, c]
+        words = (allowed.reshape(t.shape[0], -1, 32) << torch.arange(32)).sum(-1)
+        self.mask = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+    @property
+    def states(self) -> int:
+        return self.transitions.shape[0]
+
+
+@dataclasses.dataclass(frozen=True)
+class Rules:
+    """What one request asks of its tokens (StreamDecoder.admit, Pipeline.submit): penalties for tokens that it has made
+    already (repetition divides a positive logit and multiplies a negative one, frequency counts, presence does not;
+    with `prompt`, the prompt's tokens too), the row of the decoder's bias table, and the grammar's state behind the
+    prompt (-1: none)."""
+
+    repetition: float = 1.0
+    presence: float = 0.0
+    frequency: float = 0.0
+    prompt: bool = False
+    bias: int = -1
+    start: int = -1
+
+
 # ---- the decoder and its captured step ------------------------------------------------------------------------------
 
 class _Projection:
@@ -172,15 +214,23 @@ class StreamDecoder:
     per active row. The step is a fixed list of launches over buffers allocated once (no allocation inside a step),
     built per bucket of row counts and captured into one HIP graph per bucket, so a step is one graph replay whatever
     the rows' positions and audio lengths. The model is a transformers CohereAsrForConditionalGeneration (or anything
-    with its decoder attributes); `frames` may be given instead of asking the encoder for its subsampled length."""
+    with its decoder attributes); `frames` may be given instead of asking the encoder for its subsampled length.
+
+    kv_bits: 16, 8 or 4 bits a cached value (default: 8 with int8, else 16; 4: quantize_q4's form, 72 bytes a vector of
+    128 where 8 bits take 132). penalties, bias (B, vocabulary) and grammar (a Grammar) let requests have Rules; any of
+    them puts one launch (ext.dec_logits) between the head and the pick of every step."""
 
     BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 112, 128)
 
     def __init__(self, model, slots: int = 128, max_new_tokens: int = 448, max_prompt: int = 16,
                  max_audio_s: float = 36.0, buckets=None, int8: bool = False, frames: int | None = None,
-                 capture: bool = True, fused: bool | None = None, chunk: int = 4):
+                 capture: bool = True, fused: bool | None = None, chunk: int = 4, kv_bits: int | None = None,
+                 penalties: bool = False, bias: torch.Tensor | None = None, grammar: Grammar | None = None):
         dec, cfg = model.model.decoder, model.config
         self.model, self.int8 = model, int8
+        self.kv_bits = kv_bits if kv_bits is not None else (8 if int8 else 16)
+        if self.kv_bits not in (4, 8, 16):
+            raise ValueError(f"StreamDecoder: caches of 16, 8 or 4 bits (got {kv_bits})")
         self.buckets = tuple(sorted(b for b in (buckets or self.BUCKETS) if b <= slots))
         if not self.buckets:
             raise ValueError("StreamDecoder: no bucket fits the slots")
@@ -216,15 +266,19 @@ class StreamDecoder:
         kv_b = [b for layer in dec.layers for b in (layer.encoder_attn.k_proj.bias, layer.encoder_attn.v_proj.bias)]
         self.cross_w, self.cross_b = torch.cat(kv_w).contiguous(), torch.cat(kv_b).contiguous()
 
-        # caches: (layer, slot, head, position, 128), int8 with one fp32 scale per 128-vector when int8
+        # caches: (layer, slot, head, position, 128), in 8 bits int8 with one fp32 scale per 128-vector, in 4 bits 64
+        # bytes of codes with four bf16 maxima
         L, S1 = len(self.blocks), slots + 1
-        kv_dtype = torch.int8 if int8 else self.embed.dtype
+        kv_dtype, kv_width = {16: (self.embed.dtype, self.d), 8: (torch.int8, self.d),
+                              4: (torch.uint8, self.d // 2)}[self.kv_bits]
 
         def cache(t):
-            return torch.zeros(L, S1, self.h, t, self.d, device=dev, dtype=kv_dtype)
+            return torch.zeros(L, S1, self.h, t, kv_width, device=dev, dtype=kv_dtype)
 
         def scales(t):
-            return torch.ones(L, S1, self.h, t, device=dev, dtype=torch.float32) if int8 else None
+            if self.kv_bits == 4:
+                return torch.zeros(L, S1, self.h, t, 4, device=dev, dtype=torch.bfloat16)
+            return torch.ones(L, S1, self.h, t, device=dev, dtype=torch.float32) if self.kv_bits == 8 else None
 
         self.self_k, self.self_v, self.self_ks, self.self_vs = cache(self.seq), cache(self.seq), scales(self.seq), \
             scales(self.seq)
@@ -242,6 +296,23 @@ class StreamDecoder:
         self.forced = torch.full((S1, max_prompt), self.pad, **i64)
         self.out = torch.full((S1, self.seq + 1), self.pad, **i64)
         self.flags = torch.ones(S1, dtype=torch.uint8).pin_memory()  # `finished`, copied out by every step
+
+        # rules on the choice (kernel arguments of ext.dec_logits; None: absent)
+        self.grammar, self.rules_on = grammar, penalties or bias is not None or grammar is not None
+        if bias is not None and (bias.dim() != 2 or bias.shape[0] == 0 or bias.shape[1] != self.head.n):
+            raise ValueError(f"StreamDecoder: a bias table (rows, {self.head.n})")
+        if grammar is not None and grammar.classes.numel() != self.head.n:
+            raise ValueError(f"StreamDecoder: a grammar over {self.head.n} tokens (got {grammar.classes.numel()})")
+        self.bias = None if bias is None else bias.to(device=dev, dtype=torch.bfloat16).contiguous()
+        self.bias_of = None if bias is None else torch.full((S1,), -1, **i32)
+        self.first = self.pen = self.mask = self.classes = self.trans = self.start = self.gstate = None
+        if penalties:
+            self.first = torch.zeros(S1, **i32)
+            self.pen = torch.tensor([1.0, 0.0, 0.0], device=dev).repeat(S1, 1)
+        if grammar is not None:
+            self.mask, self.classes, self.trans = (t.to(dev) for t in (grammar.mask, grammar.classes,
+                                                                       grammar.transitions))
+            self.start, self.gstate = torch.full((S1,), -1, **i32), torch.full((S1, 2), -1, **i32)
 
         # step buffers, sized for the largest bucket
         bm, bf = self.buckets[-1], dict(device=dev, dtype=self.embed.dtype)
@@ -281,7 +352,10 @@ class StreamDecoder:
             k, v, ks, vs, n = self.self_k[i], self.self_v[i], self.self_ks, self.self_vs, self.pos
         else:
             k, v, ks, vs, n = self.cross_k[i], self.cross_v[i], self.cross_ks, self.cross_vs, self.cross_len
-        if self.int8:
+        if self.kv_bits == 4:
+            ks, vs = ks[i], vs[i]
+            return lambda: ext.dec_attention_q4(self_attn, act, q, k, v, ks, vs, n, self.scale, splits, self.part, out)
+        if self.kv_bits == 8:
             ks, vs = ks[i], vs[i]
             return lambda: ext.dec_attention_q8(self_attn, act, q, k, v, ks, vs, n, self.scale, splits, self.part,
                                                 out)
@@ -312,7 +386,7 @@ class StreamDecoder:
                         lambda blk=blk: blk.co.fused(att, x, DEC_EP_RESID),
                         lambda blk=blk: blk.fc1.fused(x, ffn, DEC_EP_RELU, ln=blk.norms[2]),
                         lambda blk=blk: blk.fc2.fused(ffn, x, DEC_EP_RESID)]
-            ops += [lambda: self.head.fused(x, logits, ln=self.final_ln),
+            ops += [lambda: self.head.fused(x, logits, ln=self.final_ln), *self._rules(act, logits),
                     lambda: ext.dec_pick_embed(logits, act, self.dummy, self.tok, self.pos, self.finished, self.forced,
                                                self.plen, self.limit, self.out, self.pad, self.eos, self.embed,
                                                self.pos_table, *self.emb_ln, *self.blocks[0].norms[0], x, hn,
@@ -332,11 +406,19 @@ class StreamDecoder:
                     lambda blk=blk: blk.fc1(hn, ffn, relu=True),
                     lambda blk=blk: blk.fc2(ffn, proj),
                     lambda ln=after_ffn: ext.dec_add_ln(x, proj, *ln, hn)]
-        ops += [lambda: self.head(hn, logits),
+        ops += [lambda: self.head(hn, logits), *self._rules(act, logits),
                 lambda: ext.dec_pick(logits, act, self.dummy, self.tok, self.pos, self.finished, self.forced,
                                      self.plen, self.limit, self.out, self.pad, self.eos),
                 lambda: self.flags.copy_(self.finished, non_blocking=True)]
         return ops
+
+    def _rules(self, act, logits) -> list:
+        """The requests' rules on the logits, in place (nothing where the decoder was built without any)."""
+        if not self.rules_on:
+            return []
+        return [lambda: ext.dec_logits(logits, logits, act, self.pos, self.out, self.first, self.plen, self.pen,
+                                       self.bias, self.bias_of, self.mask, self.classes, self.trans, self.start,
+                                       self.gstate)]
 
     def _embed(self, b: int) -> None:
         """The embedding and first LayerNorm of the first b active rows (x, hn), on the current stream."""
@@ -400,7 +482,8 @@ class StreamDecoder:
     def fill_cross(self, hidden: torch.Tensor, lengths: list[int], slots: list[int], projected: bool = False) -> None:
         """Cross-attention keys and values of packed encoder frames hidden (sum(lengths), width) into the given slots,
         on the current stream: the decoder's input projection (unless projected), every layer's key and value
-        projections in one bf16 GEMM whose epilogue writes the slots' caches (quantized per 128-vector with int8)."""
+        projections in one bf16 GEMM whose epilogue writes the slots' caches (quantized per 128-vector in 8 bits, per 32
+        values in 4)."""
         from kernels.cuda_ext import EPI_BIAS
 
         rows = hidden.shape[0]
@@ -413,16 +496,39 @@ class StreamDecoder:
             mem = out
         where = torch.empty(2, rows, device=hidden.device, dtype=torch.int32)
         ext.piece_rows(slots, lengths, where[0], where[1])
-        ext.gemm_kv(mem, self.cross_w, self.cross_b, where[0], where[1], self.cross_k, self.cross_v, self.cross_ks,
-                    self.cross_vs)
+        gemm_kv = ext.gemm_kv_q4 if self.kv_bits == 4 else ext.gemm_kv
+        gemm_kv(mem, self.cross_w, self.cross_b, where[0], where[1], self.cross_k, self.cross_v, self.cross_ks,
+                self.cross_vs)
+
+    def check_rules(self, rules: Rules | None) -> None:
+        """Raise ValueError for rules that this decoder was not built for, or whose numbers no slot can have."""
+        if rules is None:
+            return
+        numbers = (rules.repetition, rules.presence, rules.frequency)
+        if not all(math.isfinite(x) for x in numbers) or rules.repetition <= 0:
+            raise ValueError(f"StreamDecoder: penalties {numbers} (finite, the repetition penalty above 0)")
+        if numbers != (1.0, 0.0, 0.0) and self.pen is None:
+            raise ValueError("StreamDecoder: penalties need a decoder built with penalties=True")
+        if not -1 <= rules.bias < (0 if self.bias is None else self.bias.shape[0]):
+            raise ValueError(f"StreamDecoder: bias row {rules.bias} of a table of "
+                             f"{0 if self.bias is None else self.bias.shape[0]}")
+        if not -1 <= rules.start < (0 if self.grammar is None else self.grammar.states):
+            raise ValueError(f"StreamDecoder: state {rules.start} of a grammar of "
+                             f"{0 if self.grammar is None else self.grammar.states}")
 
     def admit(self, slots: list[int], prompts: list[torch.Tensor], frames: list[int],
-              max_new: list[int] | None = None) -> None:
+              max_new: list[int] | None = None, rules: list[Rules | None] | None = None) -> None:
         """Start decoding in the given slots (on the decoder stream): each slot's prompt is forced by the steps
-        themselves, `frames` encoder frames attended to, at most max_new (default max_new_tokens) tokens made."""
+        themselves, `frames` encoder frames attended to, at most max_new (default max_new_tokens) tokens made, each
+        under its rules (None: none)."""
         n = len(slots)
         if n == 0:
             return
+        rules = [None] * n if rules is None else list(rules)
+        if len(rules) != n:
+            raise ValueError(f"StreamDecoder: {len(rules)} rules for {n} slots")
+        for r in rules:
+            self.check_rules(r)
         forced = torch.full((n, self.max_prompt), self.pad, dtype=torch.long)
         nums = torch.empty(n, 3, dtype=torch.int32)  # prompt length, position limit, frames
         for i, p in enumerate(prompts):
@@ -447,8 +553,21 @@ class StreamDecoder:
             self.limit.index_copy_(0, idx, nums_d[:, 1].contiguous())
             self.cross_len.index_copy_(0, idx, nums_d[:, 2].contiguous())
             self.finished.index_fill_(0, idx, 0)
+            if self.rules_on:
+                self._admit_rules(idx, [r or Rules() for r in rules], nums[:, 0])
         self.flags[torch.tensor(slots, dtype=torch.long)] = 0
         self._embed_stale = True
+
+    def _admit_rules(self, idx: torch.Tensor, rules: list[Rules], plen: torch.Tensor) -> None:
+        """The slots' rules (the grammar's states need none: they follow from the start and the tokens)."""
+        def put(t, values, dtype):
+            if t is not None:
+                t.index_copy_(0, idx, self._to_device(torch.tensor(values, dtype=dtype)))
+
+        put(self.pen, [(r.repetition, r.presence, r.frequency) for r in rules], torch.float32)
+        put(self.first, [0 if r.prompt else int(p) for r, p in zip(rules, plen)], torch.int32)
+        put(self.bias_of, [r.bias for r in rules], torch.int32)
+        put(self.start, [r.start for r in rules], torch.int32)
 
     def set_active(self, slots: list[int]) -> int:
         """The active rows of the next steps (on the decoder stream), padded with the dummy slot; returns the
@@ -484,5 +603,5 @@ class StreamDecoder:
         return sum(p.nbytes for blk in self.blocks for p in blk.projections()) + self.head.nbytes
 
 
-__all__ = ["DEFAULT_CONFIG", "StreamDecoder", "W8_CONFIGS", "W8_PERM", "bf16_linear", "dequantize_q4", "prepare_w8",
+__all__ = ["DEFAULT_CONFIG", "Grammar", "Rules", "StreamDecoder", "W8_CONFIGS", "W8_PERM", "bf16_linear", "dequantize_q4", "prepare_w8",
            "quantize_q4", "unprepare_w8", "w8_config", "w8_linear"]

@@ -282,6 +282,11 @@ int cohere_dec_scatter_kv_q4(const uint16_t* kv, int64_t ldkv, int64_t rows, con
                              const int32_t* frame_of, uint8_t* ck, uint8_t* cv, uint16_t* cks, uint16_t* cvs, int64_t L,
                              int64_t S, int64_t H, int64_t T, void* stream);
 
+/* cohere_gemm_kv into such caches: the bytes that cohere_gemm_bf16 (BIAS) and cohere_dec_scatter_kv_q4 give. */
+int cohere_gemm_kv_q4(const uint16_t* a, int64_t lda, const uint16_t* w, const uint16_t* bias, int64_t M, int64_t K,
+                      const int32_t* slot_of, const int32_t* frame_of, uint8_t* ck, uint8_t* cv, uint16_t* cks,
+                      uint16_t* cvs, int64_t L, int64_t S, int64_t H, int64_t T, void* stream);
+
 /* What such caches hold of position frame_of[i] of slot slot_of[i], rounded to bf16, into row i of kv (laid out as
  * cohere_dec_scatter_kv_q4 takes it); zeros for a slot or position out of range. */
 int cohere_dec_gather_kv_q4(const int32_t* slot_of, const int32_t* frame_of, int64_t rows, const uint8_t* ck,

@@ -137,3 +137,36 @@ def test_c_abi_refuses_without_launching():
         args = list(ok)
         args[at] = value
         assert "dec_logits" in refused("cohere_dec_logits", *args), at
+
+
+def test_grammar():
+    from kernels.stream_decoder import Grammar
+
+    classes = [0, 1, 2] * 13 + [0]
+    trans = [[0, -1, 1], [-1, -1, -1]]
+    g = Grammar(classes, trans)
+    assert g.states == 2 and g.mask.shape == (2, 2) and g.mask.dtype == torch.int32
+    for s in range(2):
+        for v in range(40):
+            assert (int(g.mask[s, v // 32]) >> (v % 32)) & 1 == (trans[s][classes[v]] >= 0)
+        assert int(g.mask[s, 1]) & ~0xff == 0
+    for c, t in (([], trans), (classes, []), ([3], trans), ([-1], trans), ([0], [[1]]), ([0], [[-2]]), ([[0]], trans)):
+        with pytest.raises(ValueError):
+            Grammar(c, t)
+
+
+def test_check_rules():
+    from kernels.stream_decoder import Grammar, Rules, StreamDecoder
+
+    dec = object.__new__(StreamDecoder)
+    dec.pen = dec.bias = dec.grammar = None
+    dec.check_rules(None)
+    dec.check_rules(Rules())
+    for r in (Rules(frequency=0.1), Rules(bias=0), Rules(start=0), Rules(repetition=-1.0)):
+        with pytest.raises(ValueError):
+            dec.check_rules(r)
+    dec.pen, dec.bias, dec.grammar = torch.zeros(1, 3), torch.zeros(2, 8), Grammar([0] * 8, [[0]])
+    dec.check_rules(Rules(1.2, 0.1, -0.1, True, 1, 0))
+    for r in (Rules(bias=2), Rules(start=1), Rules(start=-2), Rules(presence=float("nan"))):
+        with pytest.raises(ValueError):
+            dec.check_rules(r)
