@@ -2,15 +2,19 @@
 
     python cohere-inference_amd/csrc/build.py          # -> cohere-inference_amd/lib/libcohere_hip.so
 
+and lib/cohere_calls.so, the calls of torch_calls.cpp as a Python module (g++, torch's headers).
+
 Flags: -O3; -ffp-contract=off so every fp32 multiply/add the kernels write stays one rounding (the epilogues call
 fmaf explicitly where the reference fuses); packed-fp32 instructions disabled; no fast-math.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
@@ -47,12 +51,29 @@ def _compile(src: str, obj_dir: str = OBJ_DIR, defines=()) -> str:
     return obj
 
 
+def build_calls(out: str = os.path.join(OUT_DIR, "cohere_calls.so")) -> str:
+    """The Python module of the calls with torch tensors; it finds torch's libraries where the process loaded them."""
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    inc = os.path.join(torch_dir, "include")
+    tmp = out + ".tmp"
+    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", f"-I{INCLUDE}",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{inc}", f"-I{os.path.join(inc, 'torch', 'csrc', 'api', 'include')}",
+           os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp, f"-L{os.path.join(torch_dir, 'lib')}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_calls.cpp:\n{r.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
 def build(verbose: bool = False, out: str = LIB, defines=()) -> str:
     """Compiles every source and links `out`; defines (NAME=VALUE strings) select build options."""
     obj_dir = OBJ_DIR if not defines else os.path.join(OBJ_DIR, "_".join(defines).replace("=", ""))
     os.makedirs(obj_dir, exist_ok=True)
     os.makedirs(os.path.dirname(out), exist_ok=True)
-    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 1)) as ex:
+        calls = ex.submit(build_calls) if out == LIB else None
         objs = list(ex.map(lambda src: _compile(src, obj_dir, defines), SOURCES))
     tmp = out + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
@@ -60,6 +81,8 @@ def build(verbose: bool = False, out: str = LIB, defines=()) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, out)
+    if calls is not None:
+        calls.result()
     if verbose:
         print("built", out)
     return out

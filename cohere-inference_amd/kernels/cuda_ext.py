@@ -16,6 +16,8 @@ module without it raises ImportError -- there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 import torch
@@ -125,25 +127,21 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-# The methods over 4-bit caches and on logits are called once per layer and step, so their checks are written out: one
-# look at each property, messages made only for a refusal (the checks take more host time than the launch).
-_BF, _U8, _I32, _I64, _F32 = torch.bfloat16, torch.uint8, torch.int32, torch.int64, torch.float32
+# the functions that csrc/torch_calls.cpp calls with torch tensors
+CALLS = ("cohere_dec_attention_q4", "cohere_dec_scatter_kv_q4", "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4",
+         "cohere_dec_logits", "cohere_last_error")
 
 
-def _stream_of(what: str, *tensors) -> int:
-    """The current stream of the tensors' GPU (None: absent), which has to be the current one."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            dev = -1
-    if dev < 0 or dev != torch._C._cuda_getDevice():
-        raise RuntimeError(f"{what}: tensors on the current GPU expected")
-    return torch._C._cuda_getCurrentRawStream(dev)
-
-
-def _index(t, n: int) -> bool:
-    """At least n int32 values one after the other."""
-    return t.dtype is _I32 and t.numel() >= n and t.is_contiguous()
+def load_calls(lib: ctypes.CDLL, path: str = os.path.join(_PKG, "lib", "cohere_calls.so")):
+    """The module of the calls checked in C++, bound to this library's functions."""
+    if not os.path.exists(path):
+        raise ImportError(f"cohere_calls.so not built ({path}); run __graft_entry__.build() or "
+                          "python cohere-inference_amd/csrc/build.py")
+    loader = importlib.machinery.ExtensionFileLoader("cohere_calls", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("cohere_calls", loader))
+    loader.exec_module(module)
+    module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in CALLS})
+    return module
 
 
 _EMPTY = torch.empty(0)  # an absent per-layer tensor
@@ -654,22 +652,7 @@ class _Ext:
             self._call("cohere_gemm_kv_q8", _ptr(a), a.stride(0), _ptr(w), _ptr(bias), a.shape[0], a.shape[1],
                        _ptr(slot_of), _ptr(frame_of), _ptr(ck), _ptr(cv), _ptr(cks), _ptr(cvs), L, S, H, T, _stream())
 
-    # ---- caches in 4 bits, rules on logits (no counterpart in the reference) -----------------------------------------
-
-    @staticmethod
-    def _q4_caches(what, k4, v4, ks, vs, dims):
-        """The caches' leading sizes: codes uint8 (..., 64) and maxima bf16 (..., 4), keys and values alike."""
-        shape = k4.shape
-        if not (len(shape) == dims + 1 and shape[-1] == 64 and v4.shape == shape and k4.dtype is _U8 and
-                v4.dtype is _U8 and k4.is_contiguous() and v4.is_contiguous()):
-            raise RuntimeError(f"{what}: contiguous uint8 caches of 64 bytes a vector")
-        lead = shape[:dims]
-        if not (ks.shape == (*lead, 4) and vs.shape == ks.shape and ks.dtype is _BF and vs.dtype is _BF and
-                ks.is_contiguous() and vs.is_contiguous()):
-            raise RuntimeError(f"{what}: contiguous bf16 maxima, 4 a vector")
-        if 0 in lead:
-            raise RuntimeError(f"{what}: empty caches")
-        return lead
+    # ---- caches in 4 bits, rules on logits (no counterpart in the reference; arguments checked in torch_calls.cpp) ----
 
     def dec_attention_q4_splits(self, rows, heads, kv_heads, T) -> int:
         """The `splits` that fill the GPU in a dec_attention_q4 call of these sizes."""
@@ -681,78 +664,22 @@ class _Ext:
         holds the new token's queries, keys and values, appended at position n[slot] and attended as computed. Rows
         without keys, of slots out of range or (self-attention) of positions beyond T get zeros. splits > 1 needs part
         (rows x H x splits x 130 floats). kernels.stream_decoder.quantize_q4 states the form."""
-        S, KV, T = self._q4_caches("dec_attention_q4", k4, v4, ks, vs, 3)
-        if not (q.dim() == 2 and out.dim() == 2 and q.dtype is _BF and out.dtype is _BF and q.stride(1) == 1 and
-                out.is_contiguous()):
-            raise RuntimeError("dec_attention_q4: bf16 q (rows, ...) with unit column stride, contiguous out")
-        rows, width = q.shape
-        o_rows, o_width = out.shape
-        H = o_width >> 7
-        if not (o_rows == rows and H > 0 and o_width == H << 7 and H % KV == 0 and
-                width >= (H + (2 * KV if self_attn else 0)) << 7):
-            raise RuntimeError("dec_attention_q4: out (rows, H * 128), H a multiple of the key heads, q as wide as its heads")
-        if not (_index(active, rows) and _index(n, S)):
-            raise RuntimeError("dec_attention_q4: int32 active per row, n per slot")
-        part_len = 0 if part is None else part.numel()
-        if not (1 <= splits <= 64 and (splits == 1 or (part_len >= rows * H * splits * 130 and part.dtype is _F32 and
-                                                       part.is_contiguous()))):
-            raise RuntimeError("dec_attention_q4: 1 to 64 splits, more than 1 need part")
-        if rows == 0:
-            return
-        stream = _stream_of("dec_attention_q4", q, active, k4, v4, ks, vs, n, part, out)
-        if self._lib.cohere_dec_attention_q4(1 if self_attn else 0, active.data_ptr(), rows, q.data_ptr(), q.stride(0),
-                                             k4.data_ptr(), v4.data_ptr(), ks.data_ptr(), vs.data_ptr(), n.data_ptr(), S,
-                                             H, KV, T, scale, splits, None if part is None else part.data_ptr(),
-                                             part_len, out.data_ptr(), stream):
-            raise RuntimeError(self._lib.cohere_last_error().decode())
-
-    def _kv_q4(self, what, kv, slot_of, frame_of, ck, cv, cks, cvs):
-        """(rows, their stride, the caches' sizes, the stream) of a scatter or gather; rows 0: nothing to do."""
-        L, S, H, T = self._q4_caches(what, ck, cv, cks, cvs, 4)
-        if not (kv.dim() == 2 and kv.dtype is _BF and kv.stride(1) == 1 and kv.shape[1] == L * 2 * H * 128):
-            raise RuntimeError(f"{what}: bf16 kv (rows, L * 2 * H * 128) with unit column stride")
-        rows = kv.shape[0]
-        if not (_index(slot_of, rows) and _index(frame_of, rows)):
-            raise RuntimeError(f"{what}: int32 slot and position per row")
-        stream = _stream_of(what, kv, slot_of, frame_of, ck, cv, cks, cvs) if rows else 0
-        return rows, kv.stride(0), L, S, H, T, stream
+        _calls.dec_attention_q4(self_attn, active, q, k4, v4, ks, vs, n, scale, splits, part, out)
 
     def dec_scatter_kv_q4(self, kv, slot_of, frame_of, ck, cv, cks, cvs):
         """dec_scatter_kv into 4-bit caches (L, S, H, T, 64) with maxima (L, S, H, T, 4); rows of slots or positions out
         of range go nowhere."""
-        rows, ld, L, S, H, T, stream = self._kv_q4("dec_scatter_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
-        if rows and self._lib.cohere_dec_scatter_kv_q4(kv.data_ptr(), ld, rows, slot_of.data_ptr(), frame_of.data_ptr(),
-                                                       ck.data_ptr(), cv.data_ptr(), cks.data_ptr(), cvs.data_ptr(), L,
-                                                       S, H, T, stream):
-            raise RuntimeError(self._lib.cohere_last_error().decode())
+        _calls.dec_scatter_kv_q4(kv, slot_of, frame_of, ck, cv, cks, cvs)
 
     def dec_gather_kv_q4(self, slot_of, frame_of, ck, cv, cks, cvs, kv):
         """What 4-bit caches hold of (slot, position) pairs, as bf16 rows laid out as dec_scatter_kv_q4 takes them (to
         move a slot to a decoder with other caches, or to look at it); zeros for slots or positions out of range."""
-        rows, ld, L, S, H, T, stream = self._kv_q4("dec_gather_kv_q4", kv, slot_of, frame_of, ck, cv, cks, cvs)
-        if rows and self._lib.cohere_dec_gather_kv_q4(slot_of.data_ptr(), frame_of.data_ptr(), rows, ck.data_ptr(),
-                                                      cv.data_ptr(), cks.data_ptr(), cvs.data_ptr(), L, S, H, T,
-                                                      kv.data_ptr(), ld, stream):
-            raise RuntimeError(self._lib.cohere_last_error().decode())
+        _calls.dec_gather_kv_q4(slot_of, frame_of, ck, cv, cks, cvs, kv)
 
     def gemm_kv_q4(self, a, w, bias, slot_of, frame_of, ck, cv, cks, cvs):
         """gemm_kv into 4-bit caches (L, S, H, T, 64) with maxima (L, S, H, T, 4): gemm with EPI_BIAS, then
         dec_scatter_kv_q4, in one launch; the same bytes."""
-        L, S, H, T = self._q4_caches("gemm_kv_q4", ck, cv, cks, cvs, 4)
-        if not (a.dim() == 2 and w.dim() == 2 and a.dtype is _BF and w.dtype is _BF and a.stride(1) == 1 and
-                w.is_contiguous() and w.shape == (L * 2 * H * 128, a.shape[1]) and a.shape[1] % 32 == 0 and
-                (bias is None or (bias.dtype is _BF and bias.numel() == w.shape[0] and bias.is_contiguous()))):
-            raise RuntimeError("gemm_kv_q4: bf16 a (rows, K), w (L * 2 * H * 128, K), bias, K % 32 == 0")
-        rows = a.shape[0]
-        if not (_index(slot_of, rows) and _index(frame_of, rows)):
-            raise RuntimeError("gemm_kv_q4: int32 slot and position per row")
-        if rows == 0:
-            return
-        stream = _stream_of("gemm_kv_q4", a, w, bias, slot_of, frame_of, ck, cv, cks, cvs)
-        if self._lib.cohere_gemm_kv_q4(a.data_ptr(), a.stride(0), w.data_ptr(), _ptr(bias), rows, a.shape[1],
-                                       slot_of.data_ptr(), frame_of.data_ptr(), ck.data_ptr(), cv.data_ptr(),
-                                       cks.data_ptr(), cvs.data_ptr(), L, S, H, T, stream):
-            raise RuntimeError(self._lib.cohere_last_error().decode())
+        _calls.gemm_kv_q4(a, w, bias, slot_of, frame_of, ck, cv, cks, cvs)
 
     def dec_logits(self, logits, y, active, pos, tokens=None, first=None, plen=None, penalties=None, bias=None,
                    bias_of=None, mask=None, classes=None, trans=None, start=None, state=None):
@@ -762,50 +689,10 @@ class _Ext:
         lacks: mask int32 (M, ceil(V / 32)), start int32 (slots), and with classes int32 (V), trans int32 (M, C) and
         state int32 (slots, 2) the state moves with every token behind the prompt (plen). Absent rules are None; index
         values out of range switch a rule off for a slot."""
-        rows, V = logits.shape if logits.dim() == 2 else (0, 0)
-        if not (V > 0 and V % 8 == 0 and y.shape == (rows, V) and logits.dtype is _BF and y.dtype is _BF and
-                logits.stride(1) == 1 and y.stride(1) == 1):
-            raise RuntimeError("dec_logits: bf16 logits and y (rows, V), unit column stride, V % 8 == 0")
-        S = pos.numel()
-        if not (_index(active, rows) and _index(pos, 1) and (first is None or _index(first, S)) and
-                (plen is None or _index(plen, S))):
-            raise RuntimeError("dec_logits: int32 active per row, pos, first, plen per slot")
-        OUT, B, M, C = 1, 0, 0, 0
-        if tokens is not None:
-            if not (tokens.dim() == 2 and tokens.dtype is _I64 and tokens.is_contiguous()):
-                raise RuntimeError("dec_logits: contiguous int64 tokens (slots, positions)")
-            t_rows, OUT = tokens.shape
-            if t_rows < S or OUT == 0:
-                raise RuntimeError("dec_logits: contiguous int64 tokens (slots, positions)")
-        if penalties is not None and not (penalties.shape == (S, 3) and penalties.dtype is _F32 and
-                                          penalties.is_contiguous() and tokens is not None and first is not None):
-            raise RuntimeError("dec_logits: penalties fp32 (slots, 3) need tokens and first")
-        if bias is not None:
-            B = bias.shape[0]
-            if not (bias.shape == (B, V) and B > 0 and bias.dtype is _BF and bias.is_contiguous() and
-                    bias_of is not None and _index(bias_of, S)):
-                raise RuntimeError("dec_logits: bias bf16 (B, V) needs int32 bias_of per slot")
-        if mask is not None:
-            M = mask.shape[0]
-            if not (mask.shape == (M, (V + 31) // 32) and _index(mask, 1) and start is not None and _index(start, S)):
-                raise RuntimeError("dec_logits: mask int32 (M, ceil(V / 32)) needs int32 start per slot")
-        if classes is not None or trans is not None:
-            C = trans.shape[-1] if trans is not None else 0
-            if not (classes is not None and trans is not None and M > 0 and classes.numel() == V and _index(classes, V) and
-                    trans.shape == (M, C) and _index(trans, 1) and state is not None and state.shape == (S, 2) and
-                    _index(state, 1) and tokens is not None and plen is not None):
-                raise RuntimeError("dec_logits: a grammar needs mask, classes (V), trans (M, C), state (slots, 2), tokens "
-                                   "and plen")
-        if rows == 0:
-            return
-        stream = _stream_of("dec_logits", logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask,
-                            classes, trans, start, state)
-        if self._lib.cohere_dec_logits(logits.data_ptr(), logits.stride(0), y.data_ptr(), y.stride(0), rows, V,
-                                       active.data_ptr(), pos.data_ptr(), S, _ptr(tokens), OUT, _ptr(first), _ptr(plen),
-                                       _ptr(penalties), _ptr(bias), B, _ptr(bias_of), _ptr(mask), M, _ptr(classes),
-                                       _ptr(trans), C, _ptr(start), _ptr(state), stream):
-            raise RuntimeError(self._lib.cohere_last_error().decode())
+        _calls.dec_logits(logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask, classes, trans,
+                          start, state)
 
 
 _lib = load_library()
+_calls = load_calls(_lib)
 ext = _Ext(_lib)
