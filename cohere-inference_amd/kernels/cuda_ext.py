@@ -662,13 +662,14 @@ class _Ext:
         """dec_attention over caches in 4 bits: codes k4, v4 uint8 (slots, KV, T, 64) and maxima ks, vs bf16 (slots, KV,
         T, 4), H = out.shape[1] / 128 query heads, H / KV of them to a key head. Self-attention: q (rows, (H + 2 KV) 128)
         holds the new token's queries, keys and values, appended at position n[slot] and attended as computed. Rows
-        without keys, of slots out of range or (self-attention) of positions beyond T get zeros. splits > 1 needs part
-        (rows x H x splits x 130 floats). kernels.stream_decoder.quantize_q4 states the form."""
+        without keys, of slots out of range or (self-attention) of positions beyond T get zeros. A slot belongs to one row
+        of a self-attention call (two get their results, but leave an undefined position). splits > 1 needs part (rows x
+        H x splits x 130 floats). kernels.stream_decoder.quantize_q4 states the form."""
         _calls.dec_attention_q4(self_attn, active, q, k4, v4, ks, vs, n, scale, splits, part, out)
 
     def dec_scatter_kv_q4(self, kv, slot_of, frame_of, ck, cv, cks, cvs):
         """dec_scatter_kv into 4-bit caches (L, S, H, T, 64) with maxima (L, S, H, T, 4); rows of slots or positions out
-        of range go nowhere."""
+        of range go nowhere; a position is named once (else what it holds is undefined)."""
         _calls.dec_scatter_kv_q4(kv, slot_of, frame_of, ck, cv, cks, cvs)
 
     def dec_gather_kv_q4(self, slot_of, frame_of, ck, cv, cks, cvs, kv):

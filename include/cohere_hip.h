@@ -266,7 +266,8 @@ int cohere_gemm_kv_q8(const uint16_t* a, int64_t lda, const uint16_t* w, const u
  * token, which goes into the caches at position n[s] and is attended as computed, with keys 0 .. n[s] - 1 of the cache;
  * self == 0: keys 0 .. min(n[s], T) - 1. A row gets zeros if it has no keys, if its slot is out of range, if n[s] < 0 and
  * (self) if n[s] >= T; nothing is appended then. Two rows of one slot in a self-attention call each get their own
- * result; the cache holds either's token. splits (1 .. 64) divides each row's keys over workgroups and needs part with
+ * result, but what the cache then holds at their position is undefined (codes of one, maxima of the other). out must not
+ * overlap q. splits (1 .. 64) divides each row's keys over workgroups and needs part with
  * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums. T < 2^25. */
 int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
                             uint8_t* k4, uint8_t* v4, uint16_t* ks, uint16_t* vs, const int32_t* n, int64_t slots,
@@ -277,7 +278,7 @@ int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, c
 int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, int64_t kv_heads, int64_t T);
 
 /* cohere_dec_scatter_kv into caches ck, cv (L, S, H, T, 64) with maxima (L, S, H, T, 4); kv rows ldkv apart. A row whose
- * slot or position is out of range goes nowhere; of two rows for one position either stays. */
+ * slot or position is out of range goes nowhere; what a position holds that two rows name is undefined. */
 int cohere_dec_scatter_kv_q4(const uint16_t* kv, int64_t ldkv, int64_t rows, const int32_t* slot_of,
                              const int32_t* frame_of, uint8_t* ck, uint8_t* cv, uint16_t* cks, uint16_t* cvs, int64_t L,
                              int64_t S, int64_t H, int64_t T, void* stream);
