@@ -17,38 +17,41 @@ namespace cohere_q4 {
 constexpr int HD = 128, GRP = 32, NG = HD / GRP, VB = HD / 2;  // head size, group, groups and code bytes a vector
 
 // a group's maximum (its bits as an unsigned number, whose order is the magnitudes': a NaN or an infinity exceeds every
-// finite value) as what its codes are computed with. Very small and very large maxima are scaled by a power of two with
-// the values, so that neither 1 / m nor 7 x leaves the normal range.
+// finite value) as what its codes are computed with: 7 / m as hi + lo, hi of 15 bits, so that x hi is exact (8 + 15 bits)
+// and fma(x, lo, x hi) is 7 x / m rounded once (lo has 24 bits more: a quotient that fp32 holds comes out as it is). Very
+// small and very large maxima are scaled by a power of two with the values, to keep lo in the normal range.
 struct Group {
-  float m, inv, mul;
+  float hi, lo, scale;
   bool any;  // finite and not zero
   uint16_t store;  // the maximum as held
 };
 
 DEVI Group group_of(uint32_t mb) {
   Group g;
-  const float m = __uint_as_float(mb);
   g.any = mb != 0 && mb < 0x7f800000u;
-  const float f = m < 0x1p-64f ? 0x1p64f : m > 0x1p64f ? 0x1p-64f : 1.f;
-  g.m = g.any ? m * f : 1.f;
-  g.inv = 1.f / g.m;
-  g.mul = 7.f * f;
+  const float m = __uint_as_float(g.any ? mb : 0x3f800000u);
+  g.scale = m < 0x1p-64f ? 0x1p64f : m > 0x1p64f ? 0x1p-64f : 1.f;
+  const float ms = m * g.scale, inv = 1.f / ms;
+  g.hi = __uint_as_float(__float_as_uint(7.f * inv) & 0xfffffe00u);
+  g.lo = __builtin_fmaf(-g.hi, ms, 7.f) * inv;  // the remainder is exact: 15 + 8 bits below 7
   g.store = mb < 0x7f800000u ? (uint16_t)(mb >> 16) : (uint16_t)0x7fc0;
   return g;
 }
 
-// eight values' codes, the first in the lowest nibble. t = n inv is within two ulps of n / m; one correction by the
-// exact remainder makes it n / m rounded (exact where n / m is a half). Adding 1.5 2^23 rounds to an integer k, half to
-// even, in the sum's low bits (0x4B400000 + k); the eight sums are added up 4 bits apart, and what their constants add
-// (0x3F400000 modulo 2^32) comes off with the bias of 8 a digit that makes every digit's borrow vanish.
+// eight values' codes, the first in the lowest nibble. Adding 1.5 2^23 rounds to an integer k, half to even, in the sum's
+// low bits (0x4B400000 + k); the eight sums are added up 4 bits apart, and what their constants add (0x3F400000 modulo
+// 2^32) comes off with the bias of 8 a digit that makes every digit's borrow vanish.
 DEVI uint32_t pack8(const Group& g, const float (&x)[8]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = x[i];
+  if (g.scale != 1.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= g.scale;
+  }
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float n = x[i] * g.mul, t = n * g.inv;
-    const float q = __builtin_fmaf(__builtin_fmaf(-t, g.m, n), g.inv, t);
-    w = (w << 4) + __float_as_uint(q + 12582912.f);
-  }
+  for (int i = 7; i >= 0; --i) w = (w << 4) + __float_as_uint(__builtin_fmaf(f[i], g.lo, f[i] * g.hi) + 12582912.f);
   return g.any ? (w + (0x88888888u - 0x3F400000u)) ^ 0x88888888u : 0u;
 }
 

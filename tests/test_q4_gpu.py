@@ -222,6 +222,31 @@ def test_scatter_and_gather(gpu, L, KV, T, rows):
     assert_rounded(dequantize_q4(codes, maxima).to(BF), value64(codes, maxima), torch.zeros_like(c) + 2.0 ** -140)
 
 
+@pytest.mark.parametrize("exponent", [0, -140, -100, -64, 64, 120])
+def test_scatter_every_significand(gpu, exponent):
+    """Codes for every pair of a maximum's and a value's significand, values down to 2^-6 of the maximum (every tie of a
+    code among them), at magnitudes from the smallest to the largest."""
+    from kernels.cuda_ext import ext
+
+    print(f"scatter_q4 significands, 2^{exponent}", flush=True)
+    g = torch.Generator().manual_seed(exponent + 200)
+    m = torch.arange(128, 256, dtype=torch.float64).repeat_interleave(7 * 5)  # (groups): 5 sets of 31 cover 128 and more
+    shift = torch.arange(7).repeat_interleave(5).repeat(128)
+    x = (128 + (torch.arange(31)[None, :] + 31 * (torch.arange(len(m)) % 5)[:, None]) % 128).double()
+    x = torch.minimum(x * 2.0 ** -shift[:, None], m[:, None]) * (1 - 2 * torch.randint(0, 2, x.shape, generator=g))
+    v = torch.cat((m[:, None], x), 1) * 2.0 ** (exponent - 7)
+    v = v.to(BF)[:len(m) // 8 * 8].reshape(-1, 2 * 128)
+    rows = v.shape[0]
+    dev = [torch.zeros(1, 1, 1, rows, w, dtype=t, device="cuda") for w, t in ((64, torch.uint8), (64, torch.uint8), (4, BF),
+                                                                             (4, BF))]
+    slot, frame = torch.zeros(rows, dtype=torch.int32), torch.arange(rows, dtype=torch.int32)
+    ext.dec_scatter_kv_q4(v.cuda(), slot.cuda(), frame.cuda(), *dev)
+    c, top = codes64(v.reshape(rows, 2, 128))
+    for which in range(2):
+        assert torch.equal(dev[which][0, 0, 0].cpu(), pack(c[:, which]))
+        assert torch.equal(dev[2 + which][0, 0, 0].cpu(), top[:, which].to(BF))
+
+
 def test_scatter_nonfinite(gpu):
     from kernels.cuda_ext import ext
     from kernels.stream_decoder import quantize_q4
