@@ -7,6 +7,9 @@
 //   l += bias[bias_of[s]][v];   l = -inf where the mask row of the grammar's state lacks v
 // in fp32, each operation rounded by itself, the result rounded once to bf16 (what the pick reads).
 //
+// Bound by the memory where no token is penalised (128 rows x 100008 logits: 12.1 us, 4.3 TB/s read and written); the
+// penalties add the counts' way through LDS and 13 operations for each of eight logits next to a penalised one (16.6 us).
+//
 // The counts are made anew from the slot's tokens in every call (a workgroup counts, in LDS, the tokens of its own part
 // of the vocabulary): no counts to keep per slot (4 bytes x vocabulary x slots), to clear when a slot is taken over or
 // to wind back. Integer additions: their order does not show.
@@ -36,10 +39,8 @@ struct LogitArgs {
   int S, V, OUT, B, M, C;
 };
 
-constexpr int NT = 256;
-
-// J chunks of 8 logits a thread: a workgroup takes J * 2048 logits; counts of BITS bits (16: of at most 65535 tokens)
-template <int J, int BITS>
+// J chunks of 8 logits a thread: a workgroup takes J * 8 * NT logits; counts of BITS bits (16: of at most 65535 tokens)
+template <int J, int BITS, int NT>
 __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
   constexpr int SPAN = J * NT * 8;
   constexpr int PER = 32 / BITS;  // counts a word
@@ -59,7 +60,10 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
   int p = 0, state = -1, b = -1, lo = 0, hi = -1;
   bool penal = false;
   const int64_t* tokens = a.tokens + (known ? (int64_t)s * a.OUT : 0);
-  int64_t t[8];  // tokens lo + tid + k NT of this thread: on their way while the rest is looked up and the counts cleared
+  constexpr int NK = 2048 / NT;
+  uint2 t[NK];  // tokens lo + tid + k NT of this thread (low and high words): on their way while the rest is looked up and the counts cleared
+  // byte offsets in 32 bits (at most 2^28 tokens a slot)
+  const auto at = [&](int i) { return *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(tokens) + (uint32_t)i * 8u); };
   if (known) {
     p = a.pos[s];
     if (a.pen) {
@@ -71,7 +75,7 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
       penal = lo <= hi;
       if (penal) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = tokens[min(lo + tid + k * NT, hi)];
+        for (int k = 0; k < NK; ++k) t[k] = at(min(lo + tid + k * NT, hi));
       }
       penal = penal && (rep != 1.f || presence != 0.f || freq != 0.f);
     }
@@ -96,14 +100,13 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
     __syncthreads();
     for (int i0 = lo + tid; i0 <= hi;) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int64_t d = t[k] - v0;
-        if (hi - i0 >= k * NT && d >= 0 && d < SPAN)
-          atomicAdd(&cnt[(uint32_t)d / PER], 1u << ((uint32_t)d % PER * (BITS % 32)));
+      for (int k = 0; k < NK; ++k) {
+        const uint32_t d = t[k].x - (uint32_t)v0;  // a token below v0 comes out far above SPAN
+        if (i0 + k * NT <= hi && t[k].y == 0 && d < (uint32_t)SPAN) atomicAdd(&cnt[d / PER], 1u << (d % PER * (BITS % 32)));
       }
-      i0 += NT * 8;
+      i0 += NT * NK;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) t[k] = tokens[min(hi, i0 + k * NT)];
+      for (int k = 0; k < NK; ++k) t[k] = at(min(hi, i0 + k * NT));
     }
     __syncthreads();
   }
@@ -112,22 +115,24 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
       (unsigned)state < (unsigned)a.M ? a.mask + (int64_t)state * ((a.V + 31) / 32 * 4) : nullptr;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const int at = (j * NT + tid) * 8, v = v0 + at;
+    const int place = (j * NT + tid) * 8, v = v0 + place;
     if (v >= a.V) continue;
     const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
     float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
     if (penal) {
-      uint32_t w8[8 / PER], c[8];
+      uint32_t w8[8 / PER], c[8], any = 0;
 #pragma unroll
       for (int i = 0; i < 2 / PER; ++i)
-        *reinterpret_cast<uint4*>(&w8[4 * i]) = *reinterpret_cast<const uint4*>(&cnt[at / PER + 4 * i]);
+        *reinterpret_cast<uint4*>(&w8[4 * i]) = *reinterpret_cast<const uint4*>(&cnt[place / PER + 4 * i]);
+#pragma unroll
+      for (int i = 0; i < 8 / PER; ++i) any |= w8[i];
 #pragma unroll
       for (int k = 0; k < 8; ++k) c[k] = PER == 1 ? w8[k] : k & 1 ? w8[k / 2] >> 16 : w8[k / 2] & 0xffffu;
       // the quotient l / rep from the reciprocal, corrected once by the exact remainder (rounded right; the fixup is for
       // infinities): 4 instructions where the division takes 11
-      if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
+      if (any) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float t = f[k] * inv, q = __builtin_fmaf(__builtin_fmaf(-t, rep, f[k]), inv, t);
@@ -145,8 +150,10 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
     if (mr) {
       const uint32_t bits = mr[v >> 3];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (!(bits >> k & 1)) f[k] = -INFINITY;
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t keep = (uint32_t)((int)(bits << (31 - k)) >> 31);
+        f[k] = __uint_as_float((keep & __float_as_uint(f[k])) | (~keep & 0xff800000u));
+      }
     }
     *reinterpret_cast<uint4*>(yr + v) =
         make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
@@ -166,7 +173,7 @@ extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, in
   cohere::clear_error();
   const int64_t top = 0x7fffffff;
   COHERE_REQUIRE(rows >= 0 && rows <= 65535 && V > 0 && V % 8 == 0 && V < (int64_t(1) << 30) && slots > 0 &&
-                     slots <= top && OUT > 0 && OUT <= (1 << 30),
+                     slots <= top && OUT > 0 && OUT <= (1 << 28),
                  "dec_logits: bad sizes (the vocabulary a multiple of 8)");
   COHERE_REQUIRE(x && y && al(x, 16) && al(y, 16) && ldx >= V && ldy >= V && ldx % 8 == 0 && ldy % 8 == 0,
                  "dec_logits: logits rows must be 16-byte aligned");
@@ -180,11 +187,11 @@ extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, in
                     reinterpret_cast<const uint8_t*>(mask), classes, trans, start, state, (int)slots, (int)V, (int)OUT,
                     (int)B, (int)M, (int)C};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const auto wgs = [&](int j) { return (unsigned)((V + j * 2048 - 1) / (j * 2048)); };
-  // 4096 logits a workgroup where that leaves four workgroups a CU (128 rows x 32000: 7.5 us, with 8192 8.1), else 2048
-  const dim3 wide(wgs(2), (unsigned)rows);
-  if (OUT > 65535) dec_logits_kernel<2, 32><<<wide, NT, 0, s>>>(a);
-  else if (rows * wgs(2) >= 1024) dec_logits_kernel<2, 16><<<wide, NT, 0, s>>>(a);
-  else dec_logits_kernel<1, 16><<<dim3(wgs(1), (unsigned)rows), NT, 0, s>>>(a);
+  // 8192 logits a workgroup of 512 where that leaves two a CU (128 rows x 100008, up to 4096 tokens each: 16.6 us; 4096 a
+  // workgroup of 256 18.3, of 512 17.2), else 2048: one row of 16384 then has 8 workgroups
+  const auto grid = [&](int span) { return dim3((unsigned)((V + span - 1) / span), (unsigned)rows); };
+  if (OUT > 65535) dec_logits_kernel<2, 32, 256><<<grid(4096), 256, 0, s>>>(a);
+  else if (rows * ((V + 8191) / 8192) >= 512) dec_logits_kernel<2, 16, 512><<<grid(8192), 512, 0, s>>>(a);
+  else dec_logits_kernel<1, 16, 256><<<grid(2048), 256, 0, s>>>(a);
   return cohere::check_launch("dec_logits");
 }
