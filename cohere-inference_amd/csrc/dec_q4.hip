@@ -33,6 +33,10 @@ using namespace cohere_q4;
 //   the codes of 64 keys and 16 dimensions 8 n + j (n the lane's column, j the product): lane (n, i) loads one word (8
 //   dimensions) of each of the keys 16 i .. 16 i + 15, and byte permutations put four keys' bytes into one word. Of the
 //   result, lanes of row group g = n / 4 hold what counts.
+// Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
+// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 250 a wave and 64 keys (530).
+// 64 rows x 8 heads, 0 .. 447 keys: 7.0 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 77 us, 4.1
+// TB/s, what a copy reaches; one row x 8 heads, 64 K keys: 13.8 us, 5.4 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
 struct Q4Args {
@@ -409,7 +413,8 @@ __global__ void __launch_bounds__(CG * HD) dec_combine_q4_kernel(const float* __
 // kv (rows, L * 2 * KV * 128): per layer KV keys then KV values; row i is position frame_of[i] of slot slot_of[i];
 // caches (L, S, KV, T). 16 lanes per vector, 8 values (one word of codes) each; a quad of lanes holds a group. A
 // workgroup takes 16 vectors of a row, in ROWS rows (fewer vectors to a row: more rows), so that a lane has ROWS loads in
-// flight and finds its vector's place once. Bound by the memory: see each kernel.
+// flight and finds its vector's place once. Bound by the memory: 3000 rows x 8 layers x 8 heads (126 MB) 23.2 us to fill,
+// 22.2 to read back, 5.4 TB/s.
 struct KvArgs {
   uint16_t* kv;
   const int32_t *slot_of, *frame_of;

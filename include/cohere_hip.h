@@ -268,7 +268,9 @@ int cohere_gemm_kv_q8(const uint16_t* a, int64_t lda, const uint16_t* w, const u
  * (self) if n[s] >= T; nothing is appended then. Two rows of one slot in a self-attention call each get their own
  * result, but what the cache then holds at their position is undefined (codes of one, maxima of the other). out must not
  * overlap q. splits (1 .. 64) divides each row's keys over workgroups and needs part with
- * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums. T < 2^25. */
+ * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums and in the
+ * weights' fixed point (2^-15 of the largest weight of 64 keys). Finite while 2^15 min(n, T) max |v| is below 2^128. T <
+ * 2^25. */
 int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
                             uint8_t* k4, uint8_t* v4, uint16_t* ks, uint16_t* vs, const int32_t* n, int64_t slots,
                             int64_t heads, int64_t kv_heads, int64_t T, float scale, int64_t splits, float* part,
@@ -305,7 +307,8 @@ int cohere_dec_gather_kv_q4(const int32_t* slot_of, const int32_t* frame_of, int
  * The state is start[s] (int32 [slots]). With classes (int32 [V]) and trans (int32 [M, C]) it is start[s] while
  * p < plen[s] and trans[the state at p - 1][classes[tokens[s][p]]] later (-1 where any of these is out of range); the
  * state at p is written to state[s][p % 2] and the one at p - 1 expected in the other place (state int32 [slots, 2]).
- * A row whose slot is out of range is copied. V % 8 == 0; 16-byte aligned rows of x, y and bias. Row r of y may be all
+ * A row whose slot is out of range is copied. V % 8 == 0, rows <= 65535, OUT <= 2^28; 16-byte aligned rows of x, y and
+ * bias. Row r of y may be all
  * -inf: cohere_dec_pick then ends the row. */
 int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int64_t V,
                       const int32_t* active, const int32_t* pos, int64_t slots, const int64_t* tokens, int64_t OUT,

@@ -122,6 +122,24 @@ def test_attention_magnitudes(gpu, q_std, scale):
     _close(out, want, bound)
 
 
+@pytest.mark.parametrize("ratio", [1, 4])
+@pytest.mark.parametrize("slope", [0.002, 0.02, 0.3, -0.02])
+def test_attention_scores_that_rise(gpu, slope, ratio):
+    """Scores that rise (or fall) key by key, slowly and fast: the softmax base moves seldom, often or at every step."""
+    print(f"attention_q4 slope={slope} ratio={ratio}", flush=True)
+    T = 900
+    active, q, k4, v4, ks, vs, n, H = _case(17, False, 3, 2, ratio, T, [900, 899, 130], poison=False)
+    g = torch.Generator().manual_seed(4)
+    u = torch.randn(128, generator=g)
+    k = 0.3 * torch.randn(4, 2, T, 128, generator=g) + (slope * torch.arange(T))[None, None, :, None] * u / 4
+    c, m = codes64(k.to(BF))
+    q = (u.repeat(3, H) * 2 + 0.1 * torch.randn(3, H * 128, generator=g)).to(BF)
+    a = (active, q, pack(c), v4, m.to(BF), vs, n, H)
+    want, bound = attention64(False, *a[:7], 128 ** -0.5, H)
+    for splits in (1, 3):
+        _close(_run(False, *a, splits=splits)[0], want, bound)
+
+
 def test_attention_nonfinite_stays_in_its_row(gpu):
     """A NaN or infinity in a row's query, key or value makes that row's heads NaN, and no other's."""
     active, q, k4, v4, ks, vs, n, H = _case(3, True, 5, 2, 1, 64, [10, 20, 30, 40, 50])
