@@ -111,10 +111,9 @@ constexpr uint32_t HI4 = 0xf0f0f0f0u;
 DEVI int even4(uint32_t w) { return (int)((w << 4) & HI4); }  // the low nibbles as bytes 16 c
 DEVI int odd4(uint32_t w) { return (int)(w & HI4); }
 
-// Registers: four waves a SIMD up to 4 heads (at 4 heads 3 waves give 88 us where 4 give 79: 16 rows of up to 32768
-// keys, 8 x 4 heads), two beyond.
+// Registers: four waves a SIMD (at 4 heads 3 waves give 88 us where 4 give 79: 16 rows of up to 32768 keys, 8 x 4 heads).
 template <bool SELF, int G, int W>
-__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(G <= 4 ? 4 : 2)))
+__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4)))
 dec_attention_q4_kernel(const Q4Args p) {
   constexpr int SETS = (G + 1) / 2, PARTS = W + (SELF ? 1 : 0);  // A operands; partial results, the new token's last
   // the queries' digits [head][group][high, low][32], then 16 zeros
@@ -545,11 +544,13 @@ int kv_entry(bool gather, KvArgs p, int64_t rows, int64_t L, int64_t S, int64_t 
   return cohere::check_launch(name);
 }
 
-// query heads a workgroup takes (at most 8) and workgroups a key head
+// Query heads a workgroup takes (at most 4) and workgroups a key head. With up to 8 heads a workgroup, which reads the keys
+// once for all of them, the registers leave two waves a SIMD: 8 heads a key head in two workgroups 11.3 us, in one 17.4
+// (32 rows x 4 key heads, up to 1026 keys); 44.7 and 46.6 (8 rows x 8 key heads, up to 16 K keys).
 struct HeadPlan { int g, chunks; };
 HeadPlan head_plan(int64_t ratio) {
-  const int chunks = (int)((ratio + 7) / 8), g = (int)((ratio + chunks - 1) / chunks);
-  return {g <= 4 ? g : g <= 6 ? 6 : 8, chunks};
+  const int chunks = (int)((ratio + 3) / 4);
+  return {(int)((ratio + chunks - 1) / chunks), chunks};
 }
 
 // waves of a workgroup: 4 for one head (64 rows x 8 heads, up to 448 keys: 7.0 us, with 8 7.5 us), else 8 (37 rows x 4 x 3
@@ -562,9 +563,7 @@ void launch_attention(int g, const Q4Args& p, dim3 grid, hipStream_t s) {
     case 1: dec_attention_q4_kernel<SELF, 1, waves_of(1)><<<grid, waves_of(1) * 64, 0, s>>>(p); break;
     case 2: dec_attention_q4_kernel<SELF, 2, waves_of(2)><<<grid, waves_of(2) * 64, 0, s>>>(p); break;
     case 3: dec_attention_q4_kernel<SELF, 3, waves_of(3)><<<grid, waves_of(3) * 64, 0, s>>>(p); break;
-    case 4: dec_attention_q4_kernel<SELF, 4, waves_of(4)><<<grid, waves_of(4) * 64, 0, s>>>(p); break;
-    case 6: dec_attention_q4_kernel<SELF, 6, waves_of(6)><<<grid, waves_of(6) * 64, 0, s>>>(p); break;
-    default: dec_attention_q4_kernel<SELF, 8, waves_of(8)><<<grid, waves_of(8) * 64, 0, s>>>(p); break;
+    default: dec_attention_q4_kernel<SELF, 4, waves_of(4)><<<grid, waves_of(4) * 64, 0, s>>>(p); break;
   }
 }
 
@@ -576,8 +575,8 @@ extern "C" int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, i
   // The time by a model, in passes of a workgroup (64 keys a wave): the keys of a part in passes, at least half of one
   // (the loads' latency), times the rounds that the workgroups take, and what the parts' meeting costs. A round is 256
   // workgroups (512 of one head, which take half the registers); where two share a CU their waits overlap. Fitted to
-  // sweeps over 1 .. 64 parts of 15 shapes (1 .. 128 rows, 1 .. 64 K keys, 1 .. 8 heads a key head): its choice is within
-  // 10 % of the best of each. Powers of two: 48 parts of 16384 keys (no whole rounds) take 8.7 us, 32 or 64 7.7.
+  // sweeps over 1 .. 64 parts of 26 shapes (1 .. 128 rows, 1 .. 64 K keys, 1 .. 16 heads a key head): its choice is within
+  // 12 % of the best of each. Powers of two: 48 parts of 16384 keys (no whole rounds) take 8.7 us, 32 or 64 7.7.
   const int64_t wgs = rows * kv_heads * hp.chunks;
   const double pass = 64. * waves_of(hp.g), us = hp.g == 1 ? 1.15 : 0.2 + 0.5 * hp.g, slots = hp.g == 1 ? 512. : 256.;
   int64_t best = 1;
@@ -585,7 +584,7 @@ extern "C" int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, i
   for (int64_t n = 1; n <= 64 && (n == 1 || T / n >= 128); n *= 2) {
     const double keys = (double)T / n / pass, rounds = wgs * n / slots;
     double t = (keys > 0.5 ? keys : 0.5) * us * (rounds > 1. ? rounds : 1.) + (n > 1 ? 2.5 + 0.03 * n : 0.);
-    if (hp.g > 1 && hp.g <= 4 && rounds >= 2.) t *= 0.9;
+    if (hp.g > 1 && rounds >= 2.) t *= 0.9;
     if (n == 1 || t < least * 0.999) best = n, least = t;
   }
   return best;
