@@ -18,6 +18,7 @@ from __future__ import annotations
 import dataclasses
 import math
 
+import numpy as np
 import torch
 
 from kernels.cuda_ext import DEC_EP_NONE, DEC_EP_RELU, DEC_EP_RESID, ext
@@ -128,10 +129,10 @@ class Grammar:
         if c.min() < 0 or c.max() >= t.shape[1] or t.min() < -1 or t.max() >= t.shape[0]:
             raise ValueError("Grammar: a class outside the transitions' columns, or a state outside their rows")
         self.classes, self.transitions = c.to(torch.int32), t.to(torch.int32)
-        allowed = torch.zeros(t.shape[0], (c.numel() + 31) // 32 * 32, dtype=torch.int64)
+        allowed = torch.zeros(t.shape[0], (c.numel() + 31) // 32 * 32, dtype=torch.bool)
         allowed[:, :c.numel()] = (t >= 0)[:, c]
-        words = (allowed.reshape(t.shape[0], -1, 32) << torch.arange(32)).sum(-1)
-        self.mask = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+        bits = np.packbits(allowed.numpy(), axis=1, bitorder="little")
+        self.mask = torch.from_numpy(bits.view("<i4").astype(np.int32))
 
     @property
     def states(self) -> int:
@@ -217,7 +218,7 @@ class StreamDecoder:
     with its decoder attributes); `frames` may be given instead of asking the encoder for its subsampled length.
 
     kv_bits: 16, 8 or 4 bits a cached value (default: 8 with int8, else 16; 4: quantize_q4's form, 72 bytes a vector of
-    128 where 8 bits take 132). penalties, bias (B, vocabulary) and grammar (a Grammar) let requests have Rules; any of
+    128 where 8 bits take 132). penalties, bias (B, vocabulary; held in bf16) and grammar (a Grammar) let requests have Rules; any of
     them puts one launch (ext.dec_logits) between the head and the pick of every step."""
 
     BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 112, 128)
@@ -603,5 +604,5 @@ class StreamDecoder:
         return sum(p.nbytes for blk in self.blocks for p in blk.projections()) + self.head.nbytes
 
 
-__all__ = ["DEFAULT_CONFIG", "Grammar", "Rules", "StreamDecoder", "W8_CONFIGS", "W8_PERM", "bf16_linear", "dequantize_q4", "prepare_w8",
-           "quantize_q4", "unprepare_w8", "w8_config", "w8_linear"]
+__all__ = ["DEFAULT_CONFIG", "Grammar", "Rules", "StreamDecoder", "W8_CONFIGS", "W8_PERM", "bf16_linear",
+           "dequantize_q4", "prepare_w8", "quantize_q4", "unprepare_w8", "w8_config", "w8_linear"]

@@ -359,6 +359,25 @@ def test_one_slot_twice(gpu):
     assert torch.equal(k, k4)
 
 
+def test_many_rows(gpu):
+    """More rows than a grid's second dimension holds: bit for bit the results of two calls of half the rows."""
+    from kernels.cuda_ext import ext
+
+    rows, T = 70001, 3
+    g = torch.Generator(device="cuda").manual_seed(2)
+    active = torch.randperm(rows, generator=g, device="cuda").to(torch.int32)
+    n = (torch.arange(rows, device="cuda") % (T + 1)).to(torch.int32)
+    k4, v4 = (torch.randint(0, 256, (rows, 1, T, 64), generator=g, device="cuda").to(torch.uint8) for _ in range(2))
+    ks, vs = (torch.rand(rows, 1, T, 4, generator=g, device="cuda").to(BF) for _ in range(2))
+    q = torch.randn(rows, 128, generator=g, device="cuda").to(BF)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    call = (lambda a, x, o: ext.dec_attention_q4(False, a, x, k4, v4, ks, vs, n, 0.1, 1, None, o))
+    call(active, q, out)
+    for part in (slice(0, 35000), slice(35000, None)):
+        call(active[part], q[part], want[part])
+    assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and not out[n[active.long()] == 0].float().any()
+
+
 def test_refusals_on_the_gpu(gpu):
     """Tensors of another device than the current GPU, no rows, and too short rows."""
     from kernels.cuda_ext import ext
