@@ -92,7 +92,9 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
       if (a.trans && blockIdx.x == 0 && tid == 0) a.state[s * (int64_t)2 + (p & 1)] = state;
     }
   }
-  const float inv = 1.f / rep;
+  // rep = m 2^e with m in [1, 2): the quotient by m neither overflows nor needs a denormal reciprocal
+  const int e = __builtin_amdgcn_frexp_expf(rep) - 1;
+  const float m = 2.f * __builtin_amdgcn_frexp_mantf(rep), inv = 1.f / m;
   if (penal) {
 #pragma unroll
     for (int j = 0; j < 2 * J / PER; ++j)
@@ -130,13 +132,13 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
       for (int i = 0; i < 8 / PER; ++i) any |= w8[i];
 #pragma unroll
       for (int k = 0; k < 8; ++k) c[k] = PER == 1 ? w8[k] : k & 1 ? w8[k / 2] >> 16 : w8[k / 2] & 0xffffu;
-      // the quotient l / rep from the reciprocal, corrected once by the exact remainder (rounded right; the fixup is for
-      // infinities): 4 instructions where the division takes 11
+      // the quotient l / m from the reciprocal, corrected once by the exact remainder (rounded right; the fixup is for
+      // infinities), times 2^-e: 5 instructions where the division takes 11
       if (any) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float t = f[k] * inv, q = __builtin_fmaf(__builtin_fmaf(-t, rep, f[k]), inv, t);
-          const float l = f[k] > 0.f ? __builtin_amdgcn_div_fixupf(q, rep, f[k]) : f[k] * rep;
+          const float t = f[k] * inv, q = __builtin_fmaf(__builtin_fmaf(-t, m, f[k]), inv, t);
+          const float l = f[k] > 0.f ? __builtin_amdgcn_div_fixupf(__builtin_amdgcn_ldexpf(q, -e), rep, f[k]) : f[k] * rep;
           f[k] = c[k] ? l - ((float)c[k] * freq + presence) : f[k];
         }
       }

@@ -118,6 +118,26 @@ def test_special_logits(gpu):
     assert (_run(a)[0] == float("-inf")).all()
 
 
+@pytest.mark.parametrize("rep", [0.5, 0.75, 1e-39, 2.0 ** -149, 2.0 ** -126, 1e-20, 1e20, 2.0 ** 126, 3e38])
+def test_quotients_at_the_ends_of_the_range(gpu, rep):
+    """A repetition penalty over the whole range of fp32, logits over bf16's: quotients beyond it are infinite (never
+    NaN), those below it zero."""
+    print(f"dec_logits rep={rep}", flush=True)
+    a = {**_rules(6, 1, 64, 64, B=0), **{k: None for k in ("mask", "classes", "trans", "start", "state", "plen")}}
+    big = torch.finfo(BF).max
+    a["logits"][0, :16] = torch.tensor([big, 1.0, 2.0 ** -20, 1e-30, 1e-38, 1e-40, 1e30, 3.0, -big, -1.0, -1e-30, -1e-40,
+                                        0.0, -0.0, float("inf"), float("-inf")], dtype=BF)
+    a["tokens"][:] = torch.arange(64)
+    a["first"][:], a["pos"][:] = 0, 63
+    a["pen"][:] = torch.tensor([rep, 0.0, 0.0])
+    want, slack, _ = logits64(**a)
+    # halfway from bf16's largest value to 2^128, and above it: infinite, in fp32 already or by the last rounding
+    over = want.abs() >= 2.0 ** 128 - 2.0 ** 119
+    want[over] = want[over].sign() * float("inf")
+    slack[over] = 0
+    assert_rounded(_run(a)[0], want, slack)
+
+
 def test_nan_stays_where_it_is(gpu):
     a = _rules(6, 1, 64, 8, B=0, M=1)
     a["logits"][0, 5], a["start"][:], a["plen"][:] = float("nan"), 5, 100
