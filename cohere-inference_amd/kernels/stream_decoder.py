@@ -506,8 +506,9 @@ class StreamDecoder:
         if rules is None:
             return
         numbers = (rules.repetition, rules.presence, rules.frequency)
-        if not all(math.isfinite(x) for x in numbers) or rules.repetition <= 0:
-            raise ValueError(f"StreamDecoder: penalties {numbers} (finite, the repetition penalty above 0)")
+        held = torch.tensor(numbers, dtype=torch.float32).tolist()  # what a slot holds of them
+        if not all(math.isfinite(x) for x in held) or held[0] <= 0:
+            raise ValueError(f"StreamDecoder: penalties {numbers} (finite in fp32, the repetition penalty above 0)")
         if numbers != (1.0, 0.0, 0.0) and self.pen is None:
             raise ValueError("StreamDecoder: penalties need a decoder built with penalties=True")
         if not -1 <= rules.bias < (0 if self.bias is None else self.bias.shape[0]):

@@ -170,3 +170,16 @@ def test_check_rules():
     for r in (Rules(bias=2), Rules(start=1), Rules(start=-2), Rules(presence=float("nan"))):
         with pytest.raises(ValueError):
             dec.check_rules(r)
+
+
+@pytest.mark.parametrize("numbers", [dict(repetition=1e-300), dict(repetition=1e300), dict(presence=-1e39),
+                                     dict(frequency=3.5e38)])
+def test_check_rules_in_fp32(numbers):
+    """Penalties that fp32 holds as 0 or infinite."""
+    from kernels.stream_decoder import Rules, StreamDecoder
+
+    dec = object.__new__(StreamDecoder)
+    dec.pen, dec.bias, dec.grammar = torch.zeros(1, 3), None, None
+    dec.check_rules(Rules(1e-40, -3e38, 3e38))
+    with pytest.raises(ValueError, match="penalties"):
+        dec.check_rules(Rules(**numbers))
