@@ -8,7 +8,8 @@
 // in fp32, each operation rounded by itself, the result rounded once to bf16 (what the pick reads).
 //
 // Bound by the memory where no token is penalised (128 rows x 100008 logits: 12.1 us, 4.3 TB/s read and written); the
-// penalties add the counts' way through LDS and 13 operations for each of eight logits next to a penalised one (16.6 us).
+// penalties add the counts' way through LDS and 14 operations for each of eight logits that some lane of the wave has
+// penalised (16.4 us; 128 rows x 32000, up to 300 tokens: 5.1 and 6.2; one row of 16384, 200 tokens: 2.9 and 3.8).
 //
 // The counts are made anew from the slot's tokens in every call (a workgroup counts, in LDS, the tokens of its own part
 // of the vocabulary): no counts to keep per slot (4 bytes x vocabulary x slots), to clear when a slot is taken over or
@@ -60,8 +61,11 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
   int p = 0, state = -1, b = -1, lo = 0, hi = -1;
   bool penal = false;
   const int64_t* tokens = a.tokens + (known ? (int64_t)s * a.OUT : 0);
-  constexpr int NK = 2048 / NT;
-  uint2 t[NK];  // tokens lo + tid + k NT of this thread (low and high words): on their way while the rest is looked up and the counts cleared
+  constexpr int NK = 1024 / NT;
+  // tokens lo + tid + k NT of this thread (low and high words): on their way while the rest is looked up and the counts
+  // cleared. 1024 a workgroup at a time: with 2048 the loads past a short history's end cost 0.3 us (one row of 16384),
+  // with 512 a long one's round trips 0.6 (128 rows x 100008, up to 4096 tokens)
+  uint2 t[NK];
   // byte offsets in 32 bits (at most 2^28 tokens a slot)
   const auto at = [&](int i) { return *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(tokens) + (uint32_t)i * 8u); };
   if (known) {
@@ -100,15 +104,16 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
     for (int j = 0; j < 2 * J / PER; ++j)
       *reinterpret_cast<uint4*>(&cnt[(j * NT + tid) * 4]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int i0 = lo + tid; i0 <= hi;) {
+    for (int i0 = lo;;) {
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
         const uint32_t d = t[k].x - (uint32_t)v0;  // a token below v0 comes out far above SPAN
-        if (i0 + k * NT <= hi && t[k].y == 0 && d < (uint32_t)SPAN) atomicAdd(&cnt[d / PER], 1u << (d % PER * (BITS % 32)));
+        if (i0 + tid + k * NT <= hi && t[k].y == 0 && d < (uint32_t)SPAN) atomicAdd(&cnt[d / PER], 1u << (d % PER * (BITS % 32)));
       }
       i0 += NT * NK;
+      if (i0 > hi) break;
 #pragma unroll
-      for (int k = 0; k < NK; ++k) t[k] = at(min(hi, i0 + k * NT));
+      for (int k = 0; k < NK; ++k) t[k] = at(min(hi, i0 + tid + k * NT));
     }
     __syncthreads();
   }
@@ -137,6 +142,7 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
       if (any) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
+          if (!__any(c[k])) continue;  // seldom all eight, with few tokens (128 rows x 32000: 6.6 us without this)
           const float t = f[k] * inv, q = __builtin_fmaf(__builtin_fmaf(-t, m, f[k]), inv, t);
           const float l = f[k] > 0.f ? __builtin_amdgcn_div_fixupf(__builtin_amdgcn_ldexpf(q, -e), rep, f[k]) : f[k] * rep;
           f[k] = c[k] ? l - ((float)c[k] * freq + presence) : f[k];
@@ -189,8 +195,8 @@ extern "C" int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, in
                     reinterpret_cast<const uint8_t*>(mask), classes, trans, start, state, (int)slots, (int)V, (int)OUT,
                     (int)B, (int)M, (int)C};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  // 8192 logits a workgroup of 512 where that leaves two a CU (128 rows x 100008, up to 4096 tokens each: 16.6 us; 4096 a
-  // workgroup of 256 18.3, of 512 17.2), else 2048: one row of 16384 then has 8 workgroups
+  // 8192 logits a workgroup of 512 where that leaves two a CU (128 rows x 100008, up to 4096 tokens each: 16.4 us; 4096 a
+  // workgroup of 256 18.3, of 512 17.2, 16384 17.2), else 2048: one row of 16384 then has 8 workgroups
   const auto grid = [&](int span) { return dim3((unsigned)((V + span - 1) / span), (unsigned)rows); };
   if (OUT > 65535) dec_logits_kernel<2, 32, 256><<<grid(4096), 256, 0, s>>>(a);
   else if (rows * ((V + 8191) / 8192) >= 512) dec_logits_kernel<2, 16, 512><<<grid(8192), 512, 0, s>>>(a);
