@@ -29,17 +29,20 @@ using namespace cohere_q4;
 //   loaded with the codes: one conversion and one multiplication each, and the four groups meet by lane swaps that leave
 //   key l of the wave's 64 in lane l.
 //   softmax: one key a lane; the running maximum is the wave's.
-//   p v: A holds p m_g (m_g the value's maximum in group g) as 15-bit fixed point of the wave's largest, rows as above, B
-//   the codes of 64 keys and 16 dimensions 8 n + j (n the lane's column, j the product): lane (n, i) loads one word (8
-//   dimensions) of each of the keys 16 i .. 16 i + 15, and byte permutations put four keys' bytes into one word. Of the
-//   result, lanes of row group g = n / 4 hold what counts.
-// The two fixed points are the only roundings below 32 bits before the result's: a score is off by at most sum_g m_g sum
-// |k| / 32638, a weight by at most 2^-16 of the largest of its 64 (less than itself), where the bf16 result keeps 8 bits;
-// over the sizes below the result's relative error against 64 bits is 0.0015 .. 0.0017, as with everything in fp32.
+//   p v: A holds p m_g (m_g the value's maximum in group g) as 31-bit fixed point of the wave's largest, in four digits of
+//   8 bits, row 4 g + t digit t of group g (one head fills the 16 rows), B the codes of 64 keys and 16 dimensions 8 n + j
+//   (n the lane's column, j the product): lane (n, i) loads one word (8 dimensions) of each of the keys 16 i .. 16 i + 15,
+//   and byte permutations put four keys' bytes into one word. Of the result, lanes of row group g = n / 4 hold what
+//   counts. A p m_g below 2^-18 of the largest would have fewer than 12 bits of its own, and where the larger ones' codes
+//   are zero it is all that an output has: those wait for another round of digits and products, with a fixed point of
+//   their largest, until what is left of the pass is below 2^-27 of every output it could add to (scores have to lie 12.5
+//   apart, within 64 keys, for a second round).
+// Roundings below 32 bits before the result's: a score is off by at most sum_g m_g sum |k| / 32638, a weight by at most
+// 2^-13 of itself (2^-32 of the largest of its 64), where the bf16 result keeps 8 bits.
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
-// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 250 a wave and 64 keys (530).
-// 64 rows x 8 heads, 0 .. 447 keys: 7.0 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 77 us, 4.1
-// TB/s, what a copy reaches; one row x 8 heads, 64 K keys: 13.8 us, 5.4 TB/s from the Infinity Cache.
+// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 310 a wave and 64 keys (890).
+// 64 rows x 8 heads, 0 .. 447 keys: 8.0 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 111 us, the
+// vector ALU where the long rows are; one row x 8 heads, 64 K keys: 14.5 us, 5.2 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
 struct Q4Args {
@@ -114,6 +117,87 @@ constexpr uint32_t HI4 = 0xf0f0f0f0u;
 DEVI int even4(uint32_t w) { return (int)((w << 4) & HI4); }  // the low nibbles as bytes 16 c
 DEVI int odd4(uint32_t w) { return (int)(w & HI4); }
 
+// B of the second product: of a lane's words of 16 keys the words x of the bytes 0 .. 3 of four keys each, and of those
+// the codes of dimension 8 n + j
+DEVI void words_of(const uint32_t (&vr)[16], uint32_t (&x)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v[4] = {vr[4 * i], vr[4 * i + 1], vr[4 * i + 2], vr[4 * i + 3]};
+    bytes4(v, x[i]);
+  }
+}
+DEVI v4i values_b(const uint32_t (&x)[4][4], int j) {
+  const int b = j >> 1;
+  return j & 1 ? v4i{odd4(x[0][b]), odd4(x[1][b]), odd4(x[2][b]), odd4(x[3][b])}
+               : v4i{even4(x[0][b]), even4(x[1][b]), even4(x[2][b]), even4(x[3][b])};
+}
+
+// nothing made of x before this is used after it
+DEVI void keep_apart(uint32_t (&x)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]), "+v"(x[i][2]), "+v"(x[i][3]));
+}
+
+// A of the second product, 16 rows (group and digit) of 64 keys' bytes in LDS: the wave's weights e (a key a lane) times
+// the values' maxima vm, in units of 2^-k, 2^-k in inv. SOME: only those below cap, as bits, group i's in row i of lanes.
+// Weights below next, 2^-18 of the largest, are left out; returned is whether this lane has such.
+template <bool SOME>
+DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint32_t& next) {
+  const int lane = lane_id(), col = lane & 15, rowg = lane >> 4;
+  float w[NG] = {e * __uint_as_float(vm.x << 16), e * __uint_as_float(vm.x & 0xffff0000u),
+                 e * __uint_as_float(vm.y << 16), e * __uint_as_float(vm.y & 0xffff0000u)};
+  if constexpr (SOME) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+      w[i] = __float_as_uint(w[i]) < (uint32_t)__builtin_amdgcn_readlane((int)cap, 16 * i) ? w[i] : 0.f;
+  }
+  // the wave's largest of each group, in row i of lanes group i's (a NaN's bits are larger than any number's)
+  uint32_t y = rows_max(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
+  y = max_u(y, dpp_u<DPP_XOR1>(y));
+  y = max_u(y, dpp_u<DPP_XOR2>(y));
+  y = max_u(y, dpp_u<DPP_ROR4>(y));
+  y = max_u(y, dpp_u<DPP_ROR8>(y));
+  // times 2^k at most 0x7f7f7f7f, four digits of 127: k from the exponent of the next power of two but 0.4 % (0x10200 of a
+  // mantissa); 2^-k is not below fp32's smallest number
+  const int k = min(157 - (int)((y + 0x10200u) >> 23), 149);
+  inv = y < 0x7f800000u ? ldexpf(1.f, -k) : nan_f();
+  next = y > (18u << 23) ? y - (18u << 23) : 1u;
+  bool rest = false;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)next, 16 * i);
+    const bool low = __float_as_uint(w[i]) - 1u < c - 1u;  // not 0, and below c
+    rest |= low;
+    const float f = ldexpf(low ? 0.f : w[i], __builtin_amdgcn_readlane(k, 16 * i));
+    const uint32_t t = ((uint32_t)(int)rintf(f) + 0x80808080u) ^ 0x80808080u;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) sp8[i * 256 + b * 64 + ((rowg ^ i) << 4) + col] = (uint8_t)(t >> (24 - 8 * b));
+  }
+  return rest;
+}
+DEVI v4i weights_a(const uint8_t* sp8) {
+  const int lane = lane_id(), col = lane & 15, rowg = lane >> 4;
+  return *reinterpret_cast<const v4i*>(&sp8[col * 64 + ((rowg ^ (col >> 2)) << 4)]);
+}
+
+// the sum of four digits' sums, each of the last two at most 2^28 with the digit above it
+DEVI float digits4(const v4i& d) {
+  return __builtin_fmaf((float)(d[0] * 256 + d[1]), 65536.f, (float)(d[2] * 256 + d[3]));
+}
+
+// a wave's outputs, 8 dimensions in each lane that has them, behind each other in LDS
+template <int G, int PARTS>
+DEVI void outputs_to(float (&so)[G][PARTS][HD], int wave, const float (&acc)[G][8]) {
+  const int lane = lane_id(), col = lane & 15;
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+    if (lane >> 4 == col >> 2) {
+      float* dst = &so[g][wave][col * 8];
+      *reinterpret_cast<float4*>(dst) = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[g][4], acc[g][5], acc[g][6], acc[g][7]);
+    }
+}
+
 // Registers: four waves a SIMD (at 4 heads 3 waves give 88 us where 4 give 79: 16 rows of up to 32768 keys, 8 x 4 heads).
 template <bool SELF, int G, int W>
 __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4)))
@@ -121,8 +205,8 @@ dec_attention_q4_kernel(const Q4Args p) {
   constexpr int SETS = (G + 1) / 2, PARTS = W + (SELF ? 1 : 0);  // A operands; partial results, the new token's last
   // the queries' digits [head][group][high, low][32], then 16 zeros
   __shared__ __attribute__((aligned(16))) uint8_t sq[G * HD * 2 + 16];
-  __shared__ float sqs[G][NG];
-  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][SETS][16 * 64];
+  __shared__ float sqs[G][NG], se[W][G][64];
+  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G][16 * 64];
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
   __shared__ float sm[G][PARTS], sl[G][PARTS];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, rowg = lane >> 4;
@@ -146,7 +230,8 @@ dec_attention_q4_kernel(const Q4Args p) {
   uint32_t km[4], vr[16];
   v2u vm;
   auto load_k = [&](int j0) {
-    const uint32_t off = (uint32_t)(j0 + col) * VB + rowg * 16, moff = (uint32_t)(j0 + col) * (2 * NG) + rowg * 2;
+    uint32_t off = (uint32_t)(j0 + col) * VB + rowg * 16, moff = (uint32_t)(j0 + col) * (2 * NG) + rowg * 2;
+    asm volatile("" : "+v"(off), "+v"(moff));  // one register with constant offsets, not one for each load
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       kr[t] = __builtin_amdgcn_raw_buffer_load_b128(krs, off + t * 16 * VB, 0, 0);
@@ -154,7 +239,8 @@ dec_attention_q4_kernel(const Q4Args p) {
     }
   };
   auto load_v = [&](int j0) {
-    const uint32_t off = (uint32_t)(j0 + rowg * 16) * VB + col * 4;
+    uint32_t off = (uint32_t)(j0 + rowg * 16) * VB + col * 4;
+    asm volatile("" : "+v"(off));
     vm = __builtin_amdgcn_raw_buffer_load_b64(vms, (uint32_t)(j0 + lane) * (2 * NG), 0, 0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b32(vrs, off + i * VB, 0, 0);
@@ -225,10 +311,6 @@ dec_attention_q4_kernel(const Q4Args p) {
     const bool mine = (col >> 2) == rowg && head < G;
     return *reinterpret_cast<const v4i*>(&sq[mine ? (head * NG + rowg) * 64 + (col & 1) * 32 + half * 16 : G * HD * 2]);
   };
-  float qs[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) qs[g] = sqs[g][rowg];
-
   float m[G], l[G], acc[G][8];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -245,7 +327,9 @@ dec_attention_q4_kernel(const Q4Args p) {
 #pragma unroll
       for (int st = 0; st < SETS; ++st) aq[st][0] = a_of(st, 0), aq[st][1] = a_of(st, 1);
       // tiles of 16 keys in the order 0, 2, 1, 3: what two of them give meets at once
-      float x[G], z[G];
+      float x[G], z[G], qs[G];  // qs: read again in every pass, not kept in registers
+#pragma unroll
+      for (int g = 0; g < G; ++g) qs[g] = sqs[g][rowg];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = i == 1 ? 2 : i == 2 ? 1 : i;
@@ -271,84 +355,102 @@ dec_attention_q4_kernel(const Q4Args p) {
     const bool live = j0 + lane < end;
     const int jn = j0 + W * 64;
     load_k(jn);
-    // weights; p m_g in fixed point into A's rows
-    float inv[G];
-    const float vmx[NG] = {__uint_as_float(vm.x << 16), __uint_as_float(vm.x & 0xffff0000u),
-                           __uint_as_float(vm.y << 16), __uint_as_float(vm.y & 0xffff0000u)};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float sg = live ? sc[g] : -INFINITY;
       // the base of the weights moves only when a score is above it by more than RISE (weights up to 2^RISE: the fixed
       // point below is relative to them): rarely after the first keys, and otherwise one comparison
       if (__any(sg > m[g] + RISE)) {
-        const float mn = wave_top(sg), a = exp2_hw(m[g] - mn);
+        const float mn = lane_value(wave_top(sg), 0), a = exp2_hw(m[g] - mn);
         l[g] *= a;
         m[g] = mn;
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[g][k] *= a;
       }
-      const float e = exp2_hw(sg - m[g]);
-      l[g] += e;
-      float w[NG];
-#pragma unroll
-      for (int i = 0; i < NG; ++i) w[i] = e * vmx[i];
-      // the wave's largest of each group, in row i of lanes group i's (a NaN's bits are larger than any number's)
-      uint32_t y = rows_max(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
-      y = max_u(y, dpp_u<DPP_XOR1>(y));
-      y = max_u(y, dpp_u<DPP_XOR2>(y));
-      y = max_u(y, dpp_u<DPP_ROR4>(y));
-      y = max_u(y, dpp_u<DPP_ROR8>(y));
-      // times 2^k at most 32639: k from the exponent of the next power of two but 0.4 % (0x10200 of a mantissa)
-      const int k = 141 - (int)((y + 0x10200u) >> 23);
-      inv[g] = y < 0x7f800000u ? ldexpf(1.f, -k) : nan_f();
-      uint8_t* dst = &sp8[wave][g >> 1][(g & 1) * 128 + col];
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const uint32_t t =
-            __float_as_uint(ldexpf(w[i], __builtin_amdgcn_readlane(k, 16 * i)) + (12582912.f + 128.f)) ^ 128u;
-        dst[i * 256 + ((rowg ^ i) << 4)] = (uint8_t)(t >> 8);
-        dst[i * 256 + 64 + ((rowg ^ i) << 4)] = (uint8_t)t;
-      }
+      sc[g] = exp2_hw(sg - m[g]);
+      l[g] += sc[g];
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
-    v4i ap[SETS];
+    uint32_t x[4][4];
+    words_of(vr, x);
+    // p m_g in fixed point into A's rows, and the products; two heads at a time, whose operands fit the registers of four
+    // waves a SIMD
+    int rest = 0;  // a bit per head
 #pragma unroll
-    for (int st = 0; st < SETS; ++st)
-      ap[st] = *reinterpret_cast<const v4i*>(&sp8[wave][st][col * 64 + ((rowg ^ (col >> 2)) << 4)]);
-    uint32_t x[4][4];  // [four keys][bytes 0 .. 3 of their words]
+    for (int g0 = 0; g0 < G; g0 += 2) {
+      float inv[2];
+      // the bytes are made from their words for each two heads, not kept for all
+      keep_apart(x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t v[4] = {vr[4 * i], vr[4 * i + 1], vr[4 * i + 2], vr[4 * i + 3]};
-      bytes4(v, x[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int b = j >> 1;
-      const v4i bv = j & 1 ? v4i{odd4(x[0][b]), odd4(x[1][b]), odd4(x[2][b]), odd4(x[3][b])}
-                           : v4i{even4(x[0][b]), even4(x[1][b]), even4(x[2][b]), even4(x[3][b])};
-#pragma unroll
-      for (int st = 0; st < SETS; ++st) {
-        const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap[st], bv, v4i{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (2 * st + i < G)
-            acc[2 * st + i][j] =
-                __builtin_fmaf((float)(d[2 * i] * 256 + d[2 * i + 1]), inv[2 * st + i], acc[2 * st + i][j]);
+      for (int h = 0; h < 2 && g0 + h < G; ++h) {
+        uint32_t cap;
+        if (__any(weights<false>(sc[g0 + h], vm, 0, sp8[wave][g0 + h], inv[h], cap))) {
+          rest |= 1 << (g0 + h);
+          se[wave][g0 + h][lane] = sc[g0 + h];
+        }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
+      v4i ap[2];
+#pragma unroll
+      for (int h = 0; h < 2 && g0 + h < G; ++h) ap[h] = weights_a(sp8[wave][g0 + h]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const v4i bv = values_b(x, j);
+#pragma unroll
+        for (int h = 0; h < 2 && g0 + h < G; ++h)
+          acc[g0 + h][j] = __builtin_fmaf(
+              digits4(__builtin_amdgcn_mfma_i32_16x16x64_i8(ap[h], bv, v4i{0, 0, 0, 0}, 0, 0, 0)), inv[h], acc[g0 + h][j]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2 && g0 + h < G; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[g0 + h][j]));  // here, not sunk behind the next branch
+    }
+    asm volatile("" ::: "memory");  // the next weights are written after these are read
+    if (rest) {
+      // the rounds of small weights: rare, so a head at a time with its outputs in LDS, and the values and the next keys
+      // loaded again, so that the ordinary pass keeps its registers
+      outputs_to(so, wave, acc);
+      load_v(j0);
+      words_of(vr, x);
+#pragma unroll 1
+      for (int g = 0; g < G; ++g) {
+        if (!(rest >> g & 1)) continue;
+        float e = se[wave][g][lane], inv;
+        uint32_t cap;
+        bool more = weights<false>(e, vm, 0, sp8[wave][g], inv, cap);
+        float* o = &so[g][wave][col * 8];
+        while (__any(more)) {
+          keep_apart(x);
+          asm volatile("" : "+v"(e), "+v"(vm));
+          more = weights<true>(e, vm, cap, sp8[wave][g], inv, cap);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          const v4i ap = weights_a(sp8[wave][g]);
+          bool small = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, values_b(x, j), v4i{0, 0, 0, 0}, 0, 0, 0);
+            const float v = __builtin_fmaf(digits4(d), inv, o[j]);
+            if (rowg == col >> 2) o[j] = v;
+            small |= fabsf(v) < __uint_as_float(cap) * 0x1p40f;
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (!__any(small && rowg == col >> 2)) break;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[g][j] = so[g][wave][col * 8 + j];
+      load_k(jn);
     }
     load_v(jn);  // here, not before the products: the words would live beside the bytes (16 registers)
-    asm volatile("" ::: "memory");  // the next pass's weights are written after these are read
     j0 = jn;
   }
 
+  outputs_to(so, wave, acc);
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const float L = wave_sum64(l[g]);
-    if (rowg == col >> 2) {
-      float* dst = &so[g][wave][col * 8];
-      *reinterpret_cast<float4*>(dst) = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
-      *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[g][4], acc[g][5], acc[g][6], acc[g][7]);
-    }
     if (lane == 0) {
       sm[g][wave] = m[g];
       sl[g][wave] = L;

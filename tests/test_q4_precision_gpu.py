@@ -1,0 +1,100 @@
+"""What attention over 4-bit caches keeps of small weights, against the definition in 64 bits and a bound that knows
+nothing of how the kernel holds its weights and queries."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from q4_helpers import BF, attention64, codes64, pack, value64
+
+pytestmark = pytest.mark.gpu
+SCALE = 128 ** -0.5
+
+
+def _close(out, active, q, k4, v4, ks, vs, n, H, self_attn=False, scale=SCALE):
+    """out against the 64-bit form. A score may be off by what fp32 makes of it: 16 roundings of 2^-24 of sum |q k| scale
+    and 2^-22 of itself (the hardware's exponential and its argument); weights off by exp(+-d) move an output by at most
+    (exp(2 d) - 1) sum p |v|. The sums of n weights and outputs add n / 256 + 64 roundings of 2^-24 of sum p |v|, a weight
+    as the kernel holds it may be off by 2^-10 of itself, the result's rounding is 2^-8 of it."""
+    want, _ = attention64(self_attn, active, q, k4, v4, ks, vs, n, scale, H)
+    rows, KV = q.shape[0], k4.shape[1]
+    bound = torch.zeros(rows, H, 128, dtype=torch.float64)
+    for r in range(rows):
+        s = int(active[r])
+        t = int(n[s])
+        k, v = value64(k4[s, :, :t], ks[s, :, :t]), value64(v4[s, :, :t], vs[s, :, :t])
+        qr = q[r].double()
+        if self_attn:
+            new = qr[H * 128:(H + 2 * KV) * 128].reshape(2, KV, 1, 128)
+            k, v = torch.cat((k, new[0]), 1), torch.cat((v, new[1]), 1)
+        qh = qr[:H * 128].reshape(KV, H // KV, 128)
+        kt = k.transpose(1, 2).contiguous()
+        sc = torch.matmul(qh, kt) * scale
+        d = torch.matmul(qh.abs(), kt.abs()) * scale * 16 * 2.0 ** -24 + sc.abs() * 2.0 ** -22
+        d = d.amax(-1, keepdim=True) + 2.0 ** -22
+        spread = torch.matmul(torch.softmax(sc, -1), v.abs())
+        bound[r] = ((torch.expm1(2 * d) + (k.shape[1] / 256 + 64) * 2.0 ** -24 + 2.0 ** -10) * spread).reshape(H, 128)
+    bound = bound.reshape(rows, -1) * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 2.0 ** -134
+    err = (out.cpu().double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, worst {float((err / bound)[bad].max()):.3f} x bound"
+
+
+def _run(self_attn, active, q, k4, v4, ks, vs, n, H, splits=1, scale=SCALE):
+    from kernels.cuda_ext import ext
+
+    out = torch.full((q.shape[0], H * 128), float("nan"), dtype=BF).cuda()
+    part = torch.full((q.shape[0] * H * splits * 130,), float("nan")).cuda() if splits > 1 else None
+    dev = [t.cuda() for t in (active, q, k4, v4, ks, vs, n)]
+    ext.dec_attention_q4(self_attn, *dev, scale, splits, part, out)
+    torch.cuda.synchronize()
+    return out.cpu()
+
+
+def _held(x):
+    c, m = codes64(x.to(BF))
+    return pack(c), m.to(BF)
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("ratio", [1, 2, 3, 4])
+@pytest.mark.parametrize("gap", [4.0, 11.1, 16.0, 30.0, 60.0])
+def test_small_weights_beside_a_large_one(gpu, gap, ratio, splits):
+    """One key far above the others, whose value is zero in all but one dimension of each group: elsewhere the others'
+    weights, exp(-gap) and less, are all there is."""
+    print(f"attention_q4 gap={gap} ratio={ratio} splits={splits}", flush=True)
+    T = 200
+    g = torch.Generator().manual_seed(int(10 * gap))
+    k, v = torch.zeros(3, 2, T, 128), torch.randn(3, 2, T, 128, generator=g)
+    k[..., 0] = -1.0 - torch.arange(T) / T / 7
+    top = torch.tensor([5, 70, T - 1])  # among the first 64 keys, the next, the last
+    for s in range(3):
+        k[s, :, top[s]], v[s, :, top[s]] = 0.0, 0.0
+        v[s, :, top[s], ::32] = 1.0
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    q = torch.zeros(3, 2 * ratio, 128)
+    q[..., 0] = gap / SCALE * (1 + torch.arange(2 * ratio) / 64)
+    a = (torch.arange(3, dtype=torch.int32), q.reshape(3, -1).to(BF), k4, v4, ks, vs,
+         torch.full((3,), T, dtype=torch.int32), 2 * ratio)
+    _close(_run(False, *a, splits=splits), *a)
+
+
+@pytest.mark.parametrize("self_attn", [False, True])
+@pytest.mark.parametrize("spread", [3.0, 12.0])
+def test_scores_far_apart(gpu, spread, self_attn):
+    """Scores spread over +-2 spread, values with whole dimensions that only some keys have."""
+    print(f"attention_q4 spread={spread} self={self_attn}", flush=True)
+    g = torch.Generator().manual_seed(int(spread))
+    KV, ratio, T, rows = 2, 3, 700, 3
+    k, v = torch.randn(rows, KV, T, 128, generator=g), torch.randn(rows, KV, T, 128, generator=g)
+    v *= torch.rand(rows, KV, T, 128, generator=g) < 0.01
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    H = KV * ratio
+    q = spread * torch.randn(rows, (H + (2 * KV if self_attn else 0)) * 128, generator=g)
+    if self_attn:
+        q[:, H * 128:] /= spread
+    a = (torch.arange(rows, dtype=torch.int32), q.to(BF), k4, v4, ks, vs, torch.tensor([699, 64, 300], dtype=torch.int32), H)
+    _close(_run(self_attn, *a), *a, self_attn=self_attn)
