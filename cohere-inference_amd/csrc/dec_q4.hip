@@ -22,12 +22,12 @@ using namespace cohere_q4;
 // A workgroup takes one row, one key head, G of its query heads and one part of the keys; a wave takes 64 keys at a
 // time. Both products run on v_mfma_i32_16x16x64_i8, so that the codes need no conversion (three instructions turn a
 // word's eight codes into bytes 16 c) and the sums are exact:
-//   q k^T: A holds the queries as 16-bit fixed point (a power of two of each group of 32 dimensions, so that values down
-//   to 2^-7 of the group's largest are exact and the rest within 2^-16 of it) in two digits of 8 bits, rows 4 g + t: group
-//   g, t the head and digit (two heads fill the 16 rows), with zeros outside the row's group; B is 16 keys, lane (key,
-//   group g) holding the group's 16 bytes as loaded. Lane (key, g) of the result holds group g's sums, whose maximum it
-//   loaded with the codes: one conversion and one multiplication each, and the four groups meet by lane swaps that leave
-//   key l of the wave's 64 in lane l.
+//   q k^T: A holds the queries as 31-bit fixed point (a power of two of each group of 32 dimensions) in four digits of 8
+//   bits, row 4 g + t digit t of group g (one head fills the 16 rows), with zeros outside the row's group; B is 16 keys,
+//   lane (key, group g) holding the group's 16 bytes as loaded. Values down to 2^-23 of the group's largest are exact so;
+//   where there are smaller ones, they are held 2^23 larger in digits of their own, multiplied by the same keys (LEVELS of
+//   these hold any bf16 values: the queries are exact). Lane (key, g) of the result holds group g's sums, whose maximum it
+//   loaded with the codes, and the four groups meet by lane swaps that leave key l of the wave's 64 in lane l.
 //   softmax: one key a lane; the running maximum is the wave's.
 //   p v: A holds p m_g (m_g the value's maximum in group g) as 31-bit fixed point of the wave's largest, in four digits of
 //   8 bits, row 4 g + t digit t of group g (one head fills the 16 rows), B the codes of 64 keys and 16 dimensions 8 n + j
@@ -37,12 +37,12 @@ using namespace cohere_q4;
 //   are zero it is all that an output has: those wait for another round of digits and products, with a fixed point of
 //   their largest, until what is left of the pass is below 2^-27 of every output it could add to (scores have to lie 12.5
 //   apart, within 64 keys, for a second round).
-// Roundings below 32 bits before the result's: a score is off by at most sum_g m_g sum |k| / 32638, a weight by at most
-// 2^-13 of itself (2^-32 of the largest of its 64), where the bf16 result keeps 8 bits.
+// Of fewer than 32 bits before the result, which keeps 8, is thus only what a weight may lose, 2^-13 of itself (2^-32 of
+// the largest of its 64).
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
-// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 310 a wave and 64 keys (890).
-// 64 rows x 8 heads, 0 .. 447 keys: 8.0 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 111 us, the
-// vector ALU where the long rows are; one row x 8 heads, 64 K keys: 14.5 us, 5.2 TB/s from the Infinity Cache.
+// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 330 a wave and 64 keys (950).
+// 64 rows x 8 heads, 0 .. 447 keys: 8.4 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 125 us, the
+// vector ALU where the long rows are; one row x 8 heads, 64 K keys: 14.3 us, 5.3 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
 struct Q4Args {
@@ -202,11 +202,13 @@ DEVI void outputs_to(float (&so)[G][PARTS][HD], int wave, const float (&acc)[G][
 template <bool SELF, int G, int W>
 __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4)))
 dec_attention_q4_kernel(const Q4Args p) {
-  constexpr int SETS = (G + 1) / 2, PARTS = W + (SELF ? 1 : 0);  // A operands; partial results, the new token's last
-  // the queries' digits [head][group][high, low][32], then 16 zeros
-  __shared__ __attribute__((aligned(16))) uint8_t sq[G * HD * 2 + 16];
+  constexpr int PARTS = W + (SELF ? 1 : 0);  // partial results, the new token's last
+  // the queries' digits [level][head][group][high .. low][32], behind each head's 32 zeros
+  constexpr int QHEAD = HD * 4 + 32, LEVELS = 12;
+  __shared__ __attribute__((aligned(16))) uint8_t sq[LEVELS][G][QHEAD];
   __shared__ float sqs[G][NG], se[W][G][64];
-  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G][16 * 64];
+  __shared__ int slevels[W];
+  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G < 2 ? 1 : 2][16 * 64];
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
   __shared__ float sm[G][PARTS], sl[G][PARTS];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, rowg = lane >> 4;
@@ -250,8 +252,20 @@ dec_attention_q4_kernel(const Q4Args p) {
   load_v(j0);
 
   // the queries' digits, a dimension per thread; byte 8 (d / 8) + 4 (d % 2) + d % 8 / 2 of its group, as the codes'
-  for (int i = tid; i < G * HD; i += W * 64) {
-    const int g = i >> 7, d = i & (HD - 1), at = d & 31;
+  static_assert(G * HD <= W * 64, "a thread per dimension");
+  int deep = 0, level = 0, qe = 0;  // of the wave, of the dimension; the dimension's exponent
+  float qv = 0.f;
+  const auto digits_to = [&](int lv) {
+    const int g = tid >> 7, d = tid & (HD - 1), at = d & 31;
+    const int v = lv == level ? (int)ldexpf(qv, qe + 23 * lv) : 0;
+    const uint32_t t = ((uint32_t)v + 0x80808080u) ^ 0x80808080u;
+    uint8_t* dst = &sq[lv][g][(d >> 5) * 128 + (at >> 3) * 8 + (at & 1) * 4 + ((at & 7) >> 1)];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) dst[b * 32] = (uint8_t)(t >> (24 - 8 * b));
+    if (d < 8) *reinterpret_cast<uint32_t*>(&sq[lv][g][HD * 4 + d * 4]) = 0;
+  };
+  if (tid < G * HD) {
+    const int g = tid >> 7, d = tid & (HD - 1);
     const uint32_t bits = (uint32_t)p.q[(int64_t)r * p.ldq + min(h0 + g, hlast) * HD + d] << 16;
     uint32_t mb = bits & 0x7fffffffu;
     mb = max_u(mb, dpp_u<DPP_XOR1>(mb));
@@ -262,15 +276,18 @@ dec_attention_q4_kernel(const Q4Args p) {
     mb = max_u(sw[0], sw[1]);
     const bool ok = mb < 0x7f800000u;
     const float m = __uint_as_float(ok ? mb : 0u);
-    // m 2^e in (16319, 32639]: digits 127, 127 are 32639
-    const int ex = 15 - __builtin_amdgcn_frexp_expf(m), e = ldexpf(m, ex) <= 32639.f ? ex : ex - 1;
-    const int t = (ok ? (int)rintf(ldexpf(__uint_as_float(bits), e)) : 0) + 128;
-    uint8_t* dst = &sq[(g * HD + (d & ~31)) * 2 + (at >> 3) * 8 + (at & 1) * 4 + ((at & 7) >> 1)];
-    dst[0] = (uint8_t)(t >> 8);
-    dst[GRP] = (uint8_t)(t ^ 128);
-    if (at == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / UNIT), -e) : nan_f();
+    // m 2^qe from 2^30 - 2^22 to 0x7f7f7f7f, four digits of 127 (m has 8 bits: only 255 2^23 would be above). A value, of 8
+    // bits too, is whole in level 0 if it is at least 2^7 there, else in the first level where it is, below 2^30
+    qe = 31 - __builtin_amdgcn_frexp_expf(m);
+    qe -= ldexpf(m, qe) > 2139062143.f;
+    qv = ok ? __uint_as_float(bits) : 0.f;
+    const int ex = qv != 0.f ? __builtin_amdgcn_frexp_expf(qv) + qe : 8;
+    level = ex < 8 ? (30 - ex) / 23 : 0;
+    while (__any(level > deep)) ++deep;
+    digits_to(0);
+    if ((d & 31) == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / UNIT), -qe) : nan_f();
   }
-  if (tid < 4) *reinterpret_cast<uint32_t*>(&sq[G * HD * 2 + tid * 4]) = 0;
+  if (lane == 0) slevels[wave] = deep;
   if constexpr (SELF) {
     const bool fresh = row_ok && sp == 0;
     const uint16_t* row = p.q + (int64_t)r * p.ldq;
@@ -304,13 +321,19 @@ dec_attention_q4_kernel(const Q4Args p) {
     }
   }
   __syncthreads();
-  // A of the first product: row 4 g + t of set s is group g of head 2 s + t / 2, digit t % 2 (its halves 16 bytes apart),
-  // zeros outside the group
-  auto a_of = [&](int st, int half) {
-    const int head = 2 * st + ((col & 3) >> 1);
-    const bool mine = (col >> 2) == rowg && head < G;
-    return *reinterpret_cast<const v4i*>(&sq[mine ? (head * NG + rowg) * 64 + (col & 1) * 32 + half * 16 : G * HD * 2]);
-  };
+  int levels = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) levels = max(levels, slevels[w]);
+  levels = __builtin_amdgcn_readfirstlane(levels) + 1;
+  if (levels > 1) {
+    if (tid < G * HD)
+#pragma unroll 1
+      for (int lv = 1; lv < levels; ++lv) digits_to(lv);
+    __syncthreads();
+  }
+  // A of the first product: row 4 g + t is digit t of group g, its halves 16 bytes apart, zeros outside the group
+  const int a_at = (col >> 2) == rowg ? rowg * 128 + (col & 3) * 32 : HD * 4;
+
   float m[G], l[G], acc[G][8];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -323,33 +346,40 @@ dec_attention_q4_kernel(const Q4Args p) {
     // scores of key j0 + lane
     float sc[G];
     {
-      v4i aq[SETS][2];
+      // two heads at a time, whose operands fit the registers of four waves a SIMD
 #pragma unroll
-      for (int st = 0; st < SETS; ++st) aq[st][0] = a_of(st, 0), aq[st][1] = a_of(st, 1);
-      // tiles of 16 keys in the order 0, 2, 1, 3: what two of them give meets at once
-      float x[G], z[G], qs[G];  // qs: read again in every pass, not kept in registers
+      for (int g0 = 0; g0 < G; g0 += 2) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) qs[g] = sqs[g][rowg];
+        for (int h = 0; h < 2 && g0 + h < G; ++h) sc[g0 + h] = 0.f;
+        int lv = 0;
+        do {
+          v4i aq[2][2];
+          float qs[2], x[2], z[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = i == 1 ? 2 : i == 2 ? 1 : i;
-        const v4i b0 = {even4(kr[t].x), odd4(kr[t].x), even4(kr[t].y), odd4(kr[t].y)};
-        const v4i b1 = {even4(kr[t].z), odd4(kr[t].z), even4(kr[t].w), odd4(kr[t].w)};
-        const float mk = __uint_as_float(km[t] << 16);
-#pragma unroll
-        for (int st = 0; st < SETS; ++st) {
-          v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st][0], b0, v4i{0, 0, 0, 0}, 0, 0, 0);
-          d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[st][1], b1, d, 0, 0, 0);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int g = 2 * st + h;
-            if (g >= G) continue;
-            const float v = (float)(d[2 * h] * 256 + d[2 * h + 1]) * (mk * qs[g]);
-            if (i == 0 || i == 2) x[g] = v;
-            else if (i == 1) z[g] = half_sum(x[g], v);
-            else sc[g] = quarter_sum(z[g], half_sum(x[g], v));
+          for (int h = 0; h < 2 && g0 + h < G; ++h) {
+            aq[h][0] = *reinterpret_cast<const v4i*>(&sq[lv][g0 + h][a_at]);
+            aq[h][1] = *reinterpret_cast<const v4i*>(&sq[lv][g0 + h][a_at + 16]);
+            qs[h] = ldexpf(sqs[g0 + h][rowg], -23 * lv);
           }
-        }
+          // tiles of 16 keys in the order 0, 2, 1, 3: what two of them give meets at once
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = i == 1 ? 2 : i == 2 ? 1 : i;
+            asm volatile("" : "+v"(kr[t]));  // its bytes are made here, not kept for the next heads or level
+            const v4i b0 = {even4(kr[t].x), odd4(kr[t].x), even4(kr[t].y), odd4(kr[t].y)};
+            const v4i b1 = {even4(kr[t].z), odd4(kr[t].z), even4(kr[t].w), odd4(kr[t].w)};
+            const float mk = __uint_as_float(km[t] << 16);
+#pragma unroll
+            for (int h = 0; h < 2 && g0 + h < G; ++h) {
+              v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[h][0], b0, v4i{0, 0, 0, 0}, 0, 0, 0);
+              d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[h][1], b1, d, 0, 0, 0);
+              const float v = digits4(d) * qs[h] * mk;
+              if (i == 0 || i == 2) x[h] = v;
+              else if (i == 1) z[h] = half_sum(x[h], v);
+              else sc[g0 + h] += quarter_sum(z[h], half_sum(x[h], v));
+            }
+          }
+        } while (++lv < levels);
       }
     }
     const bool live = j0 + lane < end;
@@ -383,7 +413,7 @@ dec_attention_q4_kernel(const Q4Args p) {
 #pragma unroll
       for (int h = 0; h < 2 && g0 + h < G; ++h) {
         uint32_t cap;
-        if (__any(weights<false>(sc[g0 + h], vm, 0, sp8[wave][g0 + h], inv[h], cap))) {
+        if (__any(weights<false>(sc[g0 + h], vm, 0, sp8[wave][h], inv[h], cap))) {
           rest |= 1 << (g0 + h);
           se[wave][g0 + h][lane] = sc[g0 + h];
         }
@@ -391,7 +421,7 @@ dec_attention_q4_kernel(const Q4Args p) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
       v4i ap[2];
 #pragma unroll
-      for (int h = 0; h < 2 && g0 + h < G; ++h) ap[h] = weights_a(sp8[wave][g0 + h]);
+      for (int h = 0; h < 2 && g0 + h < G; ++h) ap[h] = weights_a(sp8[wave][h]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const v4i bv = values_b(x, j);
@@ -404,8 +434,8 @@ dec_attention_q4_kernel(const Q4Args p) {
       for (int h = 0; h < 2 && g0 + h < G; ++h)
 #pragma unroll
         for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[g0 + h][j]));  // here, not sunk behind the next branch
+      asm volatile("" ::: "memory");  // the next weights are written after these are read
     }
-    asm volatile("" ::: "memory");  // the next weights are written after these are read
     if (rest) {
       // the rounds of small weights: rare, so a head at a time with its outputs in LDS, and the values and the next keys
       // loaded again, so that the ordinary pass keeps its registers
@@ -417,14 +447,14 @@ dec_attention_q4_kernel(const Q4Args p) {
         if (!(rest >> g & 1)) continue;
         float e = se[wave][g][lane], inv;
         uint32_t cap;
-        bool more = weights<false>(e, vm, 0, sp8[wave][g], inv, cap);
+        bool more = weights<false>(e, vm, 0, sp8[wave][0], inv, cap);
         float* o = &so[g][wave][col * 8];
         while (__any(more)) {
           keep_apart(x);
           asm volatile("" : "+v"(e), "+v"(vm));
-          more = weights<true>(e, vm, cap, sp8[wave][g], inv, cap);
+          more = weights<true>(e, vm, cap, sp8[wave][0], inv, cap);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          const v4i ap = weights_a(sp8[wave][g]);
+          const v4i ap = weights_a(sp8[wave][0]);
           bool small = false;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {

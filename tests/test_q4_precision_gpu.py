@@ -1,9 +1,7 @@
-"""What attention over 4-bit caches keeps of small weights, against the definition in 64 bits and a bound that knows
+"""What attention over 4-bit caches keeps of small weights and queries, against the definition in 64 bits and a bound that knows
 nothing of how the kernel holds its weights and queries."""
 
 from __future__ import annotations
-
-import math
 
 import pytest
 import torch
@@ -18,7 +16,8 @@ def _close(out, active, q, k4, v4, ks, vs, n, H, self_attn=False, scale=SCALE):
     """out against the 64-bit form. A score may be off by what fp32 makes of it: 16 roundings of 2^-24 of sum |q k| scale
     and 2^-22 of itself (the hardware's exponential and its argument); weights off by exp(+-d) move an output by at most
     (exp(2 d) - 1) sum p |v|. The sums of n weights and outputs add n / 256 + 64 roundings of 2^-24 of sum p |v|, a weight
-    as the kernel holds it may be off by 2^-10 of itself, the result's rounding is 2^-8 of it."""
+    as the kernel holds it may be off by 2^-10 of itself, the result's rounding is 2^-8 of it. Weights that are below 2^-117 of
+    the largest may be lost: 2^(s - m) ends at 2^-126, fp32's smallest normal number, and m may lie 8 above the largest s."""
     want, _ = attention64(self_attn, active, q, k4, v4, ks, vs, n, scale, H)
     rows, KV = q.shape[0], k4.shape[1]
     bound = torch.zeros(rows, H, 128, dtype=torch.float64)
@@ -35,8 +34,10 @@ def _close(out, active, q, k4, v4, ks, vs, n, H, self_attn=False, scale=SCALE):
         sc = torch.matmul(qh, kt) * scale
         d = torch.matmul(qh.abs(), kt.abs()) * scale * 16 * 2.0 ** -24 + sc.abs() * 2.0 ** -22
         d = d.amax(-1, keepdim=True) + 2.0 ** -22
-        spread = torch.matmul(torch.softmax(sc, -1), v.abs())
-        bound[r] = ((torch.expm1(2 * d) + (k.shape[1] / 256 + 64) * 2.0 ** -24 + 2.0 ** -10) * spread).reshape(H, 128)
+        p = torch.softmax(sc, -1)
+        spread = torch.matmul(p, v.abs())
+        lost = torch.matmul(torch.where(p < 2.0 ** -117 * p.amax(-1, keepdim=True), p, torch.zeros_like(p)), v.abs())
+        bound[r] = ((torch.expm1(2 * d) + (k.shape[1] / 256 + 64) * 2.0 ** -24 + 2.0 ** -10) * spread + lost).reshape(H, 128)
     bound = bound.reshape(rows, -1) * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 2.0 ** -134
     err = (out.cpu().double() - want).abs()
     bad = ~(err <= bound)
@@ -83,7 +84,7 @@ def test_small_weights_beside_a_large_one(gpu, gap, ratio, splits):
 
 
 @pytest.mark.parametrize("self_attn", [False, True])
-@pytest.mark.parametrize("spread", [3.0, 12.0])
+@pytest.mark.parametrize("spread", [3.0, 12.0, 40.0])
 def test_scores_far_apart(gpu, spread, self_attn):
     """Scores spread over +-2 spread, values with whole dimensions that only some keys have."""
     print(f"attention_q4 spread={spread} self={self_attn}", flush=True)
@@ -98,3 +99,43 @@ def test_scores_far_apart(gpu, spread, self_attn):
         q[:, H * 128:] /= spread
     a = (torch.arange(rows, dtype=torch.int32), q.to(BF), k4, v4, ks, vs, torch.tensor([699, 64, 300], dtype=torch.int32), H)
     _close(_run(self_attn, *a), *a, self_attn=self_attn)
+
+
+@pytest.mark.parametrize("ratio,self_attn,splits", [(1, False, 1), (1, True, 4), (2, False, 1), (3, True, 1), (4, False, 4)])
+@pytest.mark.parametrize("factor", [2.0 ** 8, 2.0 ** 9, 2.0 ** 16, 2.0 ** 24, 2.0 ** 50, 2.0 ** 120])
+def test_one_large_query_channel(gpu, factor, ratio, self_attn, splits):
+    """One channel of a query group far larger than the others, and zero in every key: the scores are the others'."""
+    print(f"attention_q4 factor={factor} ratio={ratio} self={self_attn} splits={splits}", flush=True)
+    g = torch.Generator().manual_seed(ratio)
+    KV, T, rows = 2, 2048, 2
+    H = KV * ratio
+    k, v = torch.randn(rows, KV, T, 128, generator=g), torch.randn(rows, KV, T, 128, generator=g)
+    q = 1.5 * torch.randn(rows, H + (2 * KV if self_attn else 0), 128, generator=g)
+    for i, d in enumerate((0, 37, 95, 96)):
+        k[..., d] = 0
+        q[:, H:H + KV, d] = 0
+        q[:, i % H, d] = 1.5 * factor * (-1) ** i
+        q[:, H - 1, d] = 1.25 * factor
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
+         torch.tensor([T - 1, 1000], dtype=torch.int32), H)
+    _close(_run(self_attn, *a, splits=splits), *a, self_attn=self_attn)
+
+
+@pytest.mark.parametrize("ratio", [1, 2, 4])
+@pytest.mark.parametrize("low,high", [(-20, 60), (-133, 127), (-60, 0)])
+def test_queries_of_all_magnitudes(gpu, low, high, ratio):
+    """Query values of every exponent in one group, keys that are zero where the queries are large."""
+    print(f"attention_q4 exponents {low} .. {high} ratio={ratio}", flush=True)
+    g = torch.Generator().manual_seed(high - low)
+    KV, T, rows = 1, 600, 3
+    H = KV * ratio
+    q = torch.ldexp(1 + torch.rand(rows, 1, 128, generator=g), torch.randint(low, high, (rows, 1, 128), generator=g))
+    q = torch.where(torch.rand(rows, H, 128, generator=g) < 0.5, -q, q)
+    q[..., ::4] = torch.randn(rows, H, 32, generator=g)
+    k, v = 2 * torch.randn(rows, KV, T, 128, generator=g), torch.randn(rows, KV, T, 128, generator=g)
+    k = torch.where((q.abs().amax(1) > 4)[:, None, None, :], torch.zeros_like(k), k)
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
+         torch.tensor([T, 1, 257], dtype=torch.int32), H)
+    _close(_run(False, *a), *a)
