@@ -41,7 +41,7 @@ using namespace cohere_q4;
 // the largest of its 64).
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
 // and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 330 a wave and 64 keys (950).
-// 64 rows x 8 heads, 0 .. 447 keys: 8.4 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 125 us, the
+// 64 rows x 8 heads, 0 .. 447 keys: 8.3 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 130 us, the
 // vector ALU where the long rows are; one row x 8 heads, 64 K keys: 14.3 us, 5.3 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
@@ -59,7 +59,8 @@ struct Q4Args {
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float UNIT = 112.f;  // outputs are summed in units of 1 / (7 * 16)
+constexpr float CODE = 112.f;   // a product with bytes 16 c is this many times one with c / 7
+constexpr float UNIT = 0.875f;  // outputs are summed in this unit, CODE / 128: no larger than they are
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -117,6 +118,14 @@ constexpr uint32_t HI4 = 0xf0f0f0f0u;
 DEVI int even4(uint32_t w) { return (int)((w << 4) & HI4); }  // the low nibbles as bytes 16 c
 DEVI int odd4(uint32_t w) { return (int)(w & HI4); }
 
+// the lane's number, what follows from which is computed where it is used: a few instructions, where a register held
+// through the loop for each of a dozen addresses would be spilled
+DEVI int lane_here() {
+  int v = lane_id();
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // B of the second product: of a lane's words of 16 keys the words x of the bytes 0 .. 3 of four keys each, and of those
 // the codes of dimension 8 n + j
 DEVI void words_of(const uint32_t (&vr)[16], uint32_t (&x)[4][4]) {
@@ -138,12 +147,13 @@ DEVI void keep_apart(uint32_t (&x)[4][4]) {
   for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]), "+v"(x[i][2]), "+v"(x[i][3]));
 }
 
+constexpr int ROW8 = 80;  // 16 rows' b128 reads meet no bank twice, and every write has the lane's one address
 // A of the second product, 16 rows (group and digit) of 64 keys' bytes in LDS: the wave's weights e (a key a lane) times
-// the values' maxima vm, in units of 2^-k, 2^-k in inv. SOME: only those below cap, as bits, group i's in row i of lanes.
+// the values' maxima vm, in units of 2^-k, 2^-7-k in inv. SOME: only those below cap, as bits, group i's in row i of lanes.
 // Weights below next, 2^-18 of the largest, are left out; returned is whether this lane has such.
 template <bool SOME>
 DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint32_t& next) {
-  const int lane = lane_id(), col = lane & 15, rowg = lane >> 4;
+  const int lane = lane_here();
   float w[NG] = {e * __uint_as_float(vm.x << 16), e * __uint_as_float(vm.x & 0xffff0000u),
                  e * __uint_as_float(vm.y << 16), e * __uint_as_float(vm.y & 0xffff0000u)};
   if constexpr (SOME) {
@@ -158,9 +168,9 @@ DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint3
   y = max_u(y, dpp_u<DPP_ROR4>(y));
   y = max_u(y, dpp_u<DPP_ROR8>(y));
   // times 2^k at most 0x7f7f7f7f, four digits of 127: k from the exponent of the next power of two but 0.4 % (0x10200 of a
-  // mantissa); 2^-k is not below fp32's smallest number
-  const int k = min(157 - (int)((y + 0x10200u) >> 23), 149);
-  inv = y < 0x7f800000u ? ldexpf(1.f, -k) : nan_f();
+  // mantissa); 2^-7-k, for sums in UNITs, is not below fp32's smallest number
+  const int k = min(157 - (int)((y + 0x10200u) >> 23), 142);
+  inv = y < 0x7f800000u ? ldexpf(1.f, -7 - k) : nan_f();
   next = y > (18u << 23) ? y - (18u << 23) : 1u;
   bool rest = false;
 #pragma unroll
@@ -171,13 +181,13 @@ DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint3
     const float f = ldexpf(low ? 0.f : w[i], __builtin_amdgcn_readlane(k, 16 * i));
     const uint32_t t = ((uint32_t)(int)rintf(f) + 0x80808080u) ^ 0x80808080u;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) sp8[i * 256 + b * 64 + ((rowg ^ i) << 4) + col] = (uint8_t)(t >> (24 - 8 * b));
+    for (int b = 0; b < 4; ++b) sp8[(4 * i + b) * ROW8 + lane] = (uint8_t)(t >> (24 - 8 * b));
   }
   return rest;
 }
 DEVI v4i weights_a(const uint8_t* sp8) {
-  const int lane = lane_id(), col = lane & 15, rowg = lane >> 4;
-  return *reinterpret_cast<const v4i*>(&sp8[col * 64 + ((rowg ^ (col >> 2)) << 4)]);
+  const int lane = lane_here(), col = lane & 15, rowg = lane >> 4;
+  return *reinterpret_cast<const v4i*>(&sp8[col * ROW8 + (rowg << 4)]);
 }
 
 // the sum of four digits' sums, each of the last two at most 2^28 with the digit above it
@@ -188,7 +198,7 @@ DEVI float digits4(const v4i& d) {
 // a wave's outputs, 8 dimensions in each lane that has them, behind each other in LDS
 template <int G, int PARTS>
 DEVI void outputs_to(float (&so)[G][PARTS][HD], int wave, const float (&acc)[G][8]) {
-  const int lane = lane_id(), col = lane & 15;
+  const int lane = lane_here(), col = lane & 15;
 #pragma unroll
   for (int g = 0; g < G; ++g)
     if (lane >> 4 == col >> 2) {
@@ -208,7 +218,7 @@ dec_attention_q4_kernel(const Q4Args p) {
   __shared__ __attribute__((aligned(16))) uint8_t sq[LEVELS][G][QHEAD];
   __shared__ float sqs[G][NG], se[W][G][64];
   __shared__ int slevels[W];
-  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G < 2 ? 1 : 2][16 * 64];
+  __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G < 2 ? 1 : 2][16 * ROW8];
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
   __shared__ float sm[G][PARTS], sl[G][PARTS];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, rowg = lane >> 4;
@@ -232,6 +242,7 @@ dec_attention_q4_kernel(const Q4Args p) {
   uint32_t km[4], vr[16];
   v2u vm;
   auto load_k = [&](int j0) {
+    const int ln = lane_here(), col = ln & 15, rowg = ln >> 4;
     uint32_t off = (uint32_t)(j0 + col) * VB + rowg * 16, moff = (uint32_t)(j0 + col) * (2 * NG) + rowg * 2;
     asm volatile("" : "+v"(off), "+v"(moff));  // one register with constant offsets, not one for each load
 #pragma unroll
@@ -241,6 +252,7 @@ dec_attention_q4_kernel(const Q4Args p) {
     }
   };
   auto load_v = [&](int j0) {
+    const int lane = lane_here(), col = lane & 15, rowg = lane >> 4;
     uint32_t off = (uint32_t)(j0 + rowg * 16) * VB + col * 4;
     asm volatile("" : "+v"(off));
     vm = __builtin_amdgcn_raw_buffer_load_b64(vms, (uint32_t)(j0 + lane) * (2 * NG), 0, 0);
@@ -285,7 +297,7 @@ dec_attention_q4_kernel(const Q4Args p) {
     level = ex < 8 ? (30 - ex) / 23 : 0;
     while (__any(level > deep)) ++deep;
     digits_to(0);
-    if ((d & 31) == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / UNIT), -qe) : nan_f();
+    if ((d & 31) == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / CODE), -qe) : nan_f();
   }
   if (lane == 0) slevels[wave] = deep;
   if constexpr (SELF) {
@@ -388,10 +400,10 @@ dec_attention_q4_kernel(const Q4Args p) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float sg = live ? sc[g] : -INFINITY;
-      // the base of the weights moves only when a score is above it by more than RISE (weights up to 2^RISE: the fixed
-      // point below is relative to them): rarely after the first keys, and otherwise one comparison
-      if (__any(sg > m[g] + RISE)) {
-        const float mn = lane_value(wave_top(sg), 0), a = exp2_hw(m[g] - mn);
+      // the base of the weights is set RISE above the highest score, and moves only when a score passes it: rarely after
+      // the first keys, and otherwise one comparison. The weights are at most 1
+      if (__any(sg > m[g])) {
+        const float mn = lane_value(wave_top(sg) + RISE, 0), a = exp2_hw(m[g] - mn);
         l[g] *= a;
         m[g] = mn;
 #pragma unroll
@@ -440,6 +452,7 @@ dec_attention_q4_kernel(const Q4Args p) {
       // the rounds of small weights: rare, so a head at a time with its outputs in LDS, and the values and the next keys
       // loaded again, so that the ordinary pass keeps its registers
       outputs_to(so, wave, acc);
+      const int lane = lane_here(), col = lane & 15, rowg = lane >> 4;
       load_v(j0);
       words_of(vr, x);
 #pragma unroll 1
@@ -461,7 +474,7 @@ dec_attention_q4_kernel(const Q4Args p) {
             const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, values_b(x, j), v4i{0, 0, 0, 0}, 0, 0, 0);
             const float v = __builtin_fmaf(digits4(d), inv, o[j]);
             if (rowg == col >> 2) o[j] = v;
-            small |= fabsf(v) < __uint_as_float(cap) * 0x1p40f;
+            small |= fabsf(v) < __uint_as_float(cap) * 0x1p33f;
           }
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           if (!__any(small && rowg == col >> 2)) break;

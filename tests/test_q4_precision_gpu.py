@@ -16,8 +16,12 @@ def _close(out, active, q, k4, v4, ks, vs, n, H, self_attn=False, scale=SCALE):
     """out against the 64-bit form. A score may be off by what fp32 makes of it: 16 roundings of 2^-24 of sum |q k| scale
     and 2^-22 of itself (the hardware's exponential and its argument); weights off by exp(+-d) move an output by at most
     (exp(2 d) - 1) sum p |v|. The sums of n weights and outputs add n / 256 + 64 roundings of 2^-24 of sum p |v|, a weight
-    as the kernel holds it may be off by 2^-10 of itself, the result's rounding is 2^-8 of it. Weights that are below 2^-117 of
-    the largest may be lost: 2^(s - m) ends at 2^-126, fp32's smallest normal number, and m may lie 8 above the largest s."""
+    as the kernel holds it may be off by 2^-10 of itself, the result's rounding is 2^-8 of it. Weights that are below
+    2^-117 of the largest may be lost: 2^(s - m) ends at 2^-126, fp32's smallest normal number, and m may lie 8 above the
+    largest s. For the same reason sums of values below 2^-118 lose bits at fp32's lower end: outputs are summed in steps
+    of 2^-7 times a weight's, so a weight times its value's maximum is held in steps of no less than 2^-142, off by
+    2^-143, which the division by the sum of weights, no less than 2^-8 over the largest p, makes 2^-135 times that p: for
+    each key."""
     want, _ = attention64(self_attn, active, q, k4, v4, ks, vs, n, scale, H)
     rows, KV = q.shape[0], k4.shape[1]
     bound = torch.zeros(rows, H, 128, dtype=torch.float64)
@@ -29,6 +33,8 @@ def _close(out, active, q, k4, v4, ks, vs, n, H, self_attn=False, scale=SCALE):
         if self_attn:
             new = qr[H * 128:(H + 2 * KV) * 128].reshape(2, KV, 1, 128)
             k, v = torch.cat((k, new[0]), 1), torch.cat((v, new[1]), 1)
+        if k.shape[1] == 0:
+            continue
         qh = qr[:H * 128].reshape(KV, H // KV, 128)
         kt = k.transpose(1, 2).contiguous()
         sc = torch.matmul(qh, kt) * scale
@@ -37,7 +43,8 @@ def _close(out, active, q, k4, v4, ks, vs, n, H, self_attn=False, scale=SCALE):
         p = torch.softmax(sc, -1)
         spread = torch.matmul(p, v.abs())
         lost = torch.matmul(torch.where(p < 2.0 ** -117 * p.amax(-1, keepdim=True), p, torch.zeros_like(p)), v.abs())
-        bound[r] = ((torch.expm1(2 * d) + (k.shape[1] / 256 + 64) * 2.0 ** -24 + 2.0 ** -10) * spread + lost).reshape(H, 128)
+        bound[r] = ((torch.expm1(2 * d) + (k.shape[1] / 256 + 64) * 2.0 ** -24 + 2.0 ** -10) * spread + lost +
+                    2.0 ** -135 * k.shape[1] * p.amax(-1, keepdim=True)).reshape(H, 128)
     bound = bound.reshape(rows, -1) * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs() + 2.0 ** -134
     err = (out.cpu().double() - want).abs()
     bad = ~(err <= bound)
@@ -139,3 +146,34 @@ def test_queries_of_all_magnitudes(gpu, low, high, ratio):
     a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
          torch.tensor([T, 1, 257], dtype=torch.int32), H)
     _close(_run(False, *a), *a)
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("ratio", [1, 3])
+@pytest.mark.parametrize("largest,lengths", [(torch.finfo(BF).max, [0, 1]), (2.0 ** 126, [0, 1, 2]), (2.0 ** 118, [700, 600, 3]),
+                                             (2.0 ** -100, [5, 0, 700]), (2.0 ** -126, [5, 0, 300])])
+@pytest.mark.parametrize("self_attn", [False, True])
+def test_values_at_the_ends_of_the_range(gpu, self_attn, largest, lengths, ratio, splits):
+    """Values whose sum over the keys fp32 holds, up to the type's largest and down to its smallest: finite, and a lone
+    value as it is."""
+    print(f"attention_q4 largest={largest} self={self_attn} ratio={ratio} splits={splits}", flush=True)
+    if largest == torch.finfo(BF).max and self_attn:
+        lengths = [0, 0]
+    g = torch.Generator().manual_seed(7)
+    KV, T, rows = 2, 701, len(lengths)
+    H = KV * ratio
+    k, v = torch.randn(rows, KV, T, 128, generator=g), largest * (2 * torch.rand(rows, KV, T, 128, generator=g) - 1)
+    v[..., ::32] = largest
+    q = torch.randn(rows, H + (2 * KV if self_attn else 0), 128, generator=g)
+    if self_attn:
+        q[:, H + KV:] = largest * (2 * torch.rand(rows, KV, 128, generator=g) - 1)
+        q[:, H + KV:, :4] = largest
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
+         torch.tensor(lengths, dtype=torch.int32), H)
+    out = _run(self_attn, *a, splits=splits)
+    _close(out, *a, self_attn=self_attn)
+    for r in range(rows):
+        if self_attn and lengths[r] == 0:
+            new = a[1][r, (H + KV) * 128:].reshape(KV, 1, 128)
+            assert torch.equal(out[r].reshape(KV, ratio, 128), new.expand(KV, ratio, 128))
