@@ -33,16 +33,16 @@ using namespace cohere_q4;
 //   8 bits, row 4 g + t digit t of group g (one head fills the 16 rows), B the codes of 64 keys and 16 dimensions 8 n + j
 //   (n the lane's column, j the product): lane (n, i) loads one word (8 dimensions) of each of the keys 16 i .. 16 i + 15,
 //   and byte permutations put four keys' bytes into one word. Of the result, lanes of row group g = n / 4 hold what
-//   counts. A p m_g below 2^-18 of the largest would have fewer than 12 bits of its own, and where the larger ones' codes
+//   counts. A p m_g below 2^-20 of the largest would have fewer than 10 bits of its own, and where the larger ones' codes
 //   are zero it is all that an output has: those wait for another round of digits and products, with a fixed point of
-//   their largest, until what is left of the pass is below 2^-27 of every output it could add to (scores have to lie 12.5
+//   their largest, until what is left of the pass is below 2^-27 of every output it could add to (scores have to lie 14
 //   apart, within 64 keys, for a second round).
-// Of fewer than 32 bits before the result, which keeps 8, is thus only what a weight may lose, 2^-13 of itself (2^-32 of
+// Of fewer than 32 bits before the result, which keeps 8, is thus only what a weight may lose, 2^-11 of itself (2^-32 of
 // the largest of its 64).
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
 // and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 330 a wave and 64 keys (950).
-// 64 rows x 8 heads, 0 .. 447 keys: 8.3 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 130 us, the
-// vector ALU where the long rows are; one row x 8 heads, 64 K keys: 14.3 us, 5.3 TB/s from the Infinity Cache.
+// 64 rows x 8 heads, 0 .. 447 keys: 8.2 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 102 us, the
+// vector ALU; one row x 8 heads, 64 K keys: 14.4 us, 5.2 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
 struct Q4Args {
@@ -52,7 +52,7 @@ struct Q4Args {
   uint8_t *k4, *v4;   // (S, KV, T, 64)
   uint16_t *ks, *vs;  // (S, KV, T, 4)
   const int32_t* n;   // per slot; self: position of the new token, cross: keys
-  int S, H, KV, T, ratio, chunks;
+  int S, H, KV, T, ratio, chunks, rows_y;  // rows_y: the rows are the grid's second dimension
   float scale;
   uint16_t* out;  // (rows, H * 128)
   float* part;    // (rows, H, splits, 130) when split: outputs, maximum (power of two), sum
@@ -150,7 +150,7 @@ DEVI void keep_apart(uint32_t (&x)[4][4]) {
 constexpr int ROW8 = 80;  // 16 rows' b128 reads meet no bank twice, and every write has the lane's one address
 // A of the second product, 16 rows (group and digit) of 64 keys' bytes in LDS: the wave's weights e (a key a lane) times
 // the values' maxima vm, in units of 2^-k, 2^-7-k in inv. SOME: only those below cap, as bits, group i's in row i of lanes.
-// Weights below next, 2^-18 of the largest, are left out; returned is whether this lane has such.
+// Weights below next, 2^-20 of the largest, are left out; returned is whether this lane has such.
 template <bool SOME>
 DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint32_t& next) {
   const int lane = lane_here();
@@ -171,7 +171,7 @@ DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint3
   // mantissa); 2^-7-k, for sums in UNITs, is not below fp32's smallest number
   const int k = min(157 - (int)((y + 0x10200u) >> 23), 142);
   inv = y < 0x7f800000u ? ldexpf(1.f, -7 - k) : nan_f();
-  next = y > (18u << 23) ? y - (18u << 23) : 1u;
+  next = y > (20u << 23) ? y - (20u << 23) : 1u;
   bool rest = false;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
@@ -222,7 +222,8 @@ dec_attention_q4_kernel(const Q4Args p) {
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
   __shared__ float sm[G][PARTS], sl[G][PARTS];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, rowg = lane >> 4;
-  const int r = blockIdx.x, kvh = blockIdx.y / p.chunks, ch = blockIdx.y % p.chunks, sp = blockIdx.z, nsp = gridDim.z;
+  const int r = p.rows_y ? blockIdx.y : blockIdx.x, hc = p.rows_y ? blockIdx.x : blockIdx.y;
+  const int kvh = hc / p.chunks, ch = hc % p.chunks, sp = blockIdx.z, nsp = gridDim.z;
   // the chunk's query heads h0 .. h0 + G - 1, the last one repeated where the chunk has fewer
   const int h0 = kvh * p.ratio + ch * G, hlast = kvh * p.ratio + p.ratio - 1;
   int s = p.active[r];
@@ -728,19 +729,20 @@ void launch_attention(int g, const Q4Args& p, dim3 grid, hipStream_t s) {
 extern "C" int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, int64_t kv_heads, int64_t T) {
   if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || T <= 0) return 1;
   const HeadPlan hp = head_plan(heads / kv_heads);
-  // The time by a model, in passes of a workgroup (64 keys a wave): the keys of a part in passes, at least half of one
-  // (the loads' latency), times the rounds that the workgroups take, and what the parts' meeting costs. A round is 256
-  // workgroups (512 of one head, which take half the registers); where two share a CU their waits overlap. Fitted to
-  // sweeps over 1 .. 64 parts of 26 shapes (1 .. 128 rows, 1 .. 64 K keys, 1 .. 16 heads a key head): its choice is within
-  // 12 % of the best of each. Powers of two: 48 parts of 16384 keys (no whole rounds) take 8.7 us, 32 or 64 7.7.
+  // The time by a model, in us: the keys of a part in passes of a workgroup (64 keys a wave), at least 3/4 of one (the
+  // loads' latency), times a pass and the rounds that the workgroups take, and what the parts' meeting costs (a launch, and
+  // 520 bytes a head and part written and read). Several rounds of more than one head even out rows of different lengths.
+  // Fitted to sweeps over 1 .. 64 parts of 28 shapes (1 .. 128 rows, 465 .. 64 K keys, 1 .. 16 heads a key head, the rows
+  // of one length and from a sixteenth of it): its choice is within 10 % of the best of each. Powers of two: 48 parts of
+  // 16384 keys (no whole rounds) take 8.7 us, 32 or 64 7.7.
   const int64_t wgs = rows * kv_heads * hp.chunks;
-  const double pass = 64. * waves_of(hp.g), us = hp.g == 1 ? 1.15 : 0.2 + 0.5 * hp.g, slots = hp.g == 1 ? 512. : 256.;
+  const double pass = 64. * waves_of(hp.g), us = hp.g == 1 ? 0.9 : 0.5 * hp.g, slots = hp.g == 1 ? 768. : 512.;
   int64_t best = 1;
   double least = 0.;
   for (int64_t n = 1; n <= 64 && (n == 1 || T / n >= 128); n *= 2) {
     const double keys = (double)T / n / pass, rounds = wgs * n / slots;
-    double t = (keys > 0.5 ? keys : 0.5) * us * (rounds > 1. ? rounds : 1.) + (n > 1 ? 2.5 + 0.03 * n : 0.);
-    if (hp.g > 1 && rounds >= 2.) t *= 0.9;
+    double t = (keys > 0.75 ? keys : 0.75) * us * (rounds > 1. ? rounds : 1.) + (n > 1 ? 2. + 0.0016 * rows * heads * n : 0.);
+    if (hp.g > 1 && rounds >= 2.) t *= 0.85;
     if (n == 1 || t < least * 0.999) best = n, least = t;
   }
   return best;
@@ -766,9 +768,12 @@ extern "C" int cohere_dec_attention_q4(int32_t self, const int32_t* active, int6
   const HeadPlan hp = head_plan(heads / kv_heads);
   COHERE_REQUIRE(kv_heads * hp.chunks <= 65535 && rows * heads <= 0x7fffffff, "dec_attention_q4: too many heads");
   Q4Args p{active, q, ldq, k4, v4, ks, vs, n, (int)slots, (int)heads, (int)kv_heads, (int)T, (int)(heads / kv_heads),
-           hp.chunks, scale, out, part};
+           hp.chunks, rows <= 65535, scale, out, part};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)rows, (unsigned)(kv_heads * hp.chunks), (unsigned)splits);
+  // Workgroups go to the eight XCDs in turn: with a row's heads behind each other every XCD has a share of the long rows
+  // (16 rows x 8 x 4 heads, 2 .. 32 K keys, 8 parts: 107 us, with the rows first 127; all of 32 K: 153 and 151)
+  const unsigned ny = (unsigned)(kv_heads * hp.chunks);
+  const dim3 grid = p.rows_y ? dim3(ny, (unsigned)rows, (unsigned)splits) : dim3((unsigned)rows, ny, (unsigned)splits);
   if (self) launch_attention<true>(hp.g, p, grid, s);
   else launch_attention<false>(hp.g, p, grid, s);
   // few parts: 128 threads a head (64 rows x 16 heads in 2 parts 21.0 -> 19.5 us in all, in 4 25.2 -> 23.7)

@@ -269,7 +269,7 @@ int cohere_gemm_kv_q8(const uint16_t* a, int64_t lda, const uint16_t* w, const u
  * result, but what the cache then holds at their position is undefined (codes of one, maxima of the other). out must not
  * overlap q. splits (1 .. 64) divides each row's keys over workgroups and needs part with
  * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums and in the weights' last
- * bits (a weight keeps 12 at least; below 2^-118 of the row's largest it may be 0). Finite while (min(n, T) + 1) max |v|
+ * bits (a weight keeps 10 at least; below 2^-118 of the row's largest it may be 0). Finite while (min(n, T) + 1) max |v|
  * is below 2^128. T < 2^25. */
 int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
                             uint8_t* k4, uint8_t* v4, uint16_t* ks, uint16_t* vs, const int32_t* n, int64_t slots,
