@@ -33,12 +33,12 @@ using namespace cohere_q4;
 //   8 bits, row 4 g + t digit t of group g (one head fills the 16 rows), B the codes of 64 keys and 16 dimensions 8 n + j
 //   (n the lane's column, j the product): lane (n, i) loads one word (8 dimensions) of each of the keys 16 i .. 16 i + 15,
 //   and byte permutations put four keys' bytes into one word. Of the result, lanes of row group g = n / 4 hold what
-//   counts. A p m_g below 2^-20 of the largest would have fewer than 10 bits of its own, and where the larger ones' codes
-//   are zero it is all that an output has: those wait for another round of digits and products, with a fixed point of
-//   their largest, until what is left of the pass is below 2^-27 of every output it could add to (scores have to lie 14
-//   apart, within 64 keys, for a second round).
-// Of fewer than 32 bits before the result, which keeps 8, is thus only what a weight may lose, 2^-11 of itself (2^-32 of
-// the largest of its 64).
+//   counts. A p m_g is so off by half a unit, 2^-31 of the largest of the 64: more than 2^-11 of itself where it is below
+//   2^-20 of that, and it may be all that an output has, where the larger ones' codes are zero. If there are such weights,
+//   and an output that the units could change by 2^-11 (too_small), what the units left of all 64 is added in units of its
+//   own largest, and so on.
+// Of fewer than 32 bits before the result, which keeps 8, are thus only these units: an output is off by at most 2^-11 of
+// sum p |v| for them.
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
 // and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 330 a wave and 64 keys (950).
 // 64 rows x 8 heads, 0 .. 447 keys: 8.2 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 102 us, the
@@ -126,6 +126,16 @@ DEVI int lane_here() {
   return v;
 }
 
+// whether one of the wave's outputs is smaller than err times the largest weight y (as bits, by groups as weights_to's)
+DEVI bool too_small(const float (&acc)[8], uint32_t y, float err) {
+  const float c = __uint_as_float(y) * err;
+  bool r = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r |= fabsf(acc[j]) < c;
+  const int lane = lane_here();
+  return __any(r && lane >> 4 == (lane & 15) >> 2);
+}
+
 // B of the second product: of a lane's words of 16 keys the words x of the bytes 0 .. 3 of four keys each, and of those
 // the codes of dimension 8 n + j
 DEVI void words_of(const uint32_t (&vr)[16], uint32_t (&x)[4][4]) {
@@ -148,21 +158,16 @@ DEVI void keep_apart(uint32_t (&x)[4][4]) {
 }
 
 constexpr int ROW8 = 80;  // 16 rows' b128 reads meet no bank twice, and every write has the lane's one address
-// A of the second product, 16 rows (group and digit) of 64 keys' bytes in LDS: the wave's weights e (a key a lane) times
-// the values' maxima vm, in units of 2^-k, 2^-7-k in inv. SOME: only those below cap, as bits, group i's in row i of lanes.
-// Weights below next, 2^-20 of the largest, are left out; returned is whether this lane has such.
-template <bool SOME>
-DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint32_t& next) {
+// A of the second product, 16 rows (group and digit) of 64 keys' bytes in LDS: w, a key a lane and a weight for each group,
+// in units of 2^-k, 2^-7-k in inv; what the units leave of them in w. Returns the wave's largest magnitude of each group
+// in row i of lanes group i's, as bits (a NaN's are larger than any number's).
+template <bool WRITE>
+DEVI uint32_t weights_to(float (&w)[NG], uint8_t* sp8, float& inv) {
   const int lane = lane_here();
-  float w[NG] = {e * __uint_as_float(vm.x << 16), e * __uint_as_float(vm.x & 0xffff0000u),
-                 e * __uint_as_float(vm.y << 16), e * __uint_as_float(vm.y & 0xffff0000u)};
-  if constexpr (SOME) {
+  uint32_t a[NG];
 #pragma unroll
-    for (int i = 0; i < NG; ++i)
-      w[i] = __float_as_uint(w[i]) < (uint32_t)__builtin_amdgcn_readlane((int)cap, 16 * i) ? w[i] : 0.f;
-  }
-  // the wave's largest of each group, in row i of lanes group i's (a NaN's bits are larger than any number's)
-  uint32_t y = rows_max(__float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
+  for (int i = 0; i < NG; ++i) a[i] = __float_as_uint(w[i]) & 0x7fffffffu;
+  uint32_t y = rows_max(a[0], a[1], a[2], a[3]);
   y = max_u(y, dpp_u<DPP_XOR1>(y));
   y = max_u(y, dpp_u<DPP_XOR2>(y));
   y = max_u(y, dpp_u<DPP_ROR4>(y));
@@ -171,19 +176,33 @@ DEVI bool weights(float e, v2u vm, uint32_t cap, uint8_t* sp8, float& inv, uint3
   // mantissa); 2^-7-k, for sums in UNITs, is not below fp32's smallest number
   const int k = min(157 - (int)((y + 0x10200u) >> 23), 142);
   inv = y < 0x7f800000u ? ldexpf(1.f, -7 - k) : nan_f();
-  next = y > (20u << 23) ? y - (20u << 23) : 1u;
-  bool rest = false;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)next, 16 * i);
-    const bool low = __float_as_uint(w[i]) - 1u < c - 1u;  // not 0, and below c
-    rest |= low;
-    const float f = ldexpf(low ? 0.f : w[i], __builtin_amdgcn_readlane(k, 16 * i));
-    const uint32_t t = ((uint32_t)(int)rintf(f) + 0x80808080u) ^ 0x80808080u;
+    const int ki = __builtin_amdgcn_readlane(k, 16 * i);
+    const float f = rintf(ldexpf(w[i], ki));
+    w[i] -= ldexpf(f, -ki);  // exact
+    if constexpr (WRITE) {
+      const uint32_t t = ((uint32_t)(int)f + 0x80808080u) ^ 0x80808080u;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) sp8[(4 * i + b) * ROW8 + lane] = (uint8_t)(t >> (24 - 8 * b));
+      for (int b = 0; b < 4; ++b) sp8[(4 * i + b) * ROW8 + lane] = (uint8_t)(t >> (24 - 8 * b));
+    }
   }
-  return rest;
+  return y;
+}
+// whether one of this lane's weights, not 0, is below 2^-20 of the largest y: its units left it fewer than 10 bits
+DEVI bool coarse(const float (&w)[NG], uint32_t y) {
+  const uint32_t c = y > (20u << 23) ? y - (20u << 23) : 1u;
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < NG; ++i)
+    r |= __float_as_uint(w[i]) - 1u < (uint32_t)__builtin_amdgcn_readlane((int)c, 16 * i) - 1u;
+  return r;
+}
+DEVI void weights_of(float e, v2u vm, float (&w)[NG]) {
+  w[0] = e * __uint_as_float(vm.x << 16);
+  w[1] = e * __uint_as_float(vm.x & 0xffff0000u);
+  w[2] = e * __uint_as_float(vm.y << 16);
+  w[3] = e * __uint_as_float(vm.y & 0xffff0000u);
 }
 DEVI v4i weights_a(const uint8_t* sp8) {
   const int lane = lane_here(), col = lane & 15, rowg = lane >> 4;
@@ -216,7 +235,7 @@ dec_attention_q4_kernel(const Q4Args p) {
   // the queries' digits [level][head][group][high .. low][32], behind each head's 32 zeros
   constexpr int QHEAD = HD * 4 + 32, LEVELS = 12;
   __shared__ __attribute__((aligned(16))) uint8_t sq[LEVELS][G][QHEAD];
-  __shared__ float sqs[G][NG], se[W][G][64];
+  __shared__ float sqs[G][NG];
   __shared__ int slevels[W];
   __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G < 2 ? 1 : 2][16 * ROW8];
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
@@ -338,7 +357,7 @@ dec_attention_q4_kernel(const Q4Args p) {
 #pragma unroll
   for (int w = 0; w < W; ++w) levels = max(levels, slevels[w]);
   levels = __builtin_amdgcn_readfirstlane(levels) + 1;
-  if (levels > 1) {
+  if (__builtin_expect(levels > 1, 0)) {
     if (tid < G * HD)
 #pragma unroll 1
       for (int lv = 1; lv < levels; ++lv) digits_to(lv);
@@ -355,6 +374,9 @@ dec_attention_q4_kernel(const Q4Args p) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[g][k] = 0.f;
   }
+  // The units of 64 weights are off by 2^-25 of the largest in all, the passes' by so much each: 2^-11 of an output that is
+  // not below err times the largest
+  const float err = ldexpf((float)((end - start + W * 64 - 1) / (W * 64)), -14);
   while (j0 < end) {
     // scores of key j0 + lane
     float sc[G];
@@ -417,19 +439,20 @@ dec_attention_q4_kernel(const Q4Args p) {
     words_of(vr, x);
     // p m_g in fixed point into A's rows, and the products; two heads at a time, whose operands fit the registers of four
     // waves a SIMD
-    int rest = 0;  // a bit per head
 #pragma unroll
     for (int g0 = 0; g0 < G; g0 += 2) {
       float inv[2];
-      // the bytes are made from their words for each two heads, not kept for all
+      uint32_t top[2];
+      bool rest[2];
       keep_apart(x);
 #pragma unroll
       for (int h = 0; h < 2 && g0 + h < G; ++h) {
-        uint32_t cap;
-        if (__any(weights<false>(sc[g0 + h], vm, 0, sp8[wave][h], inv[h], cap))) {
-          rest |= 1 << (g0 + h);
-          se[wave][g0 + h][lane] = sc[g0 + h];
-        }
+        float w[NG], left[NG];
+        weights_of(sc[g0 + h], vm, w);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) left[i] = w[i];
+        top[h] = weights_to<true>(left, sp8[wave][h], inv[h]);
+        rest[h] = coarse(w, top[h]);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
       v4i ap[2];
@@ -448,44 +471,31 @@ dec_attention_q4_kernel(const Q4Args p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[g0 + h][j]));  // here, not sunk behind the next branch
       asm volatile("" ::: "memory");  // the next weights are written after these are read
-    }
-    if (rest) {
-      // the rounds of small weights: rare, so a head at a time with its outputs in LDS, and the values and the next keys
-      // loaded again, so that the ordinary pass keeps its registers
-      outputs_to(so, wave, acc);
-      const int lane = lane_here(), col = lane & 15, rowg = lane >> 4;
-      load_v(j0);
-      words_of(vr, x);
-#pragma unroll 1
-      for (int g = 0; g < G; ++g) {
-        if (!(rest >> g & 1)) continue;
-        float e = se[wave][g][lane], inv;
-        uint32_t cap;
-        bool more = weights<false>(e, vm, 0, sp8[wave][0], inv, cap);
-        float* o = &so[g][wave][col * 8];
-        while (__any(more)) {
+#pragma unroll
+      for (int h = 0; h < 2 && g0 + h < G; ++h) {
+        if (__builtin_expect(!__any(rest[h]) || !too_small(acc[g0 + h], top[h], err), 1)) continue;
+        // what the units left, in units of its own largest
+        float w[NG], left[NG];
+        asm volatile("" : "+v"(sc[g0 + h]), "+v"(vm));
+        weights_of(sc[g0 + h], vm, w);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) left[i] = w[i];
+        float unit;
+        uint32_t y = weights_to<false>(left, sp8[wave][h], unit);
+        do {
           keep_apart(x);
-          asm volatile("" : "+v"(e), "+v"(vm));
-          more = weights<true>(e, vm, cap, sp8[wave][0], inv, cap);
+          y = weights_to<true>(left, sp8[wave][h], unit);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          const v4i ap = weights_a(sp8[wave][0]);
-          bool small = false;
+          const v4i a = weights_a(sp8[wave][h]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(ap, values_b(x, j), v4i{0, 0, 0, 0}, 0, 0, 0);
-            const float v = __builtin_fmaf(digits4(d), inv, o[j]);
-            if (rowg == col >> 2) o[j] = v;
-            small |= fabsf(v) < __uint_as_float(cap) * 0x1p33f;
+            const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, values_b(x, j), v4i{0, 0, 0, 0}, 0, 0, 0);
+            acc[g0 + h][j] = __builtin_fmaf(digits4(d), unit, acc[g0 + h][j]);
+            asm volatile("" : "+v"(acc[g0 + h][j]));
           }
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (!__any(small && rowg == col >> 2)) break;
-        }
+          asm volatile("" ::: "memory");
+        } while (__any(coarse(w, y)) && too_small(acc[g0 + h], y, err));
       }
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[g][j] = so[g][wave][col * 8 + j];
-      load_k(jn);
     }
     load_v(jn);  // here, not before the products: the words would live beside the bytes (16 registers)
     j0 = jn;

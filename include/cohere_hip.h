@@ -268,9 +268,9 @@ int cohere_gemm_kv_q8(const uint16_t* a, int64_t lda, const uint16_t* w, const u
  * (self) if n[s] >= T; nothing is appended then. Two rows of one slot in a self-attention call each get their own
  * result, but what the cache then holds at their position is undefined (codes of one, maxima of the other). out must not
  * overlap q. splits (1 .. 64) divides each row's keys over workgroups and needs part with
- * rows x heads x splits x 130 floats; the result depends on it only in the order of fp32 sums and in the weights' last
- * bits (a weight keeps 10 at least; below 2^-118 of the row's largest it may be 0). Finite while (min(n, T) + 1) max |v|
- * is below 2^128. T < 2^25. */
+ * rows x heads x splits x 130 floats, of one call at a time; the result depends on it only in the order of fp32 sums and
+ * in the units that the weights are held in (an output is off by at most 2^-11 of sum p |v| for them; weights below 2^-118
+ * of the row's largest may be 0). Finite while (min(n, T) + 1) max |v| is below 2^128. T < 2^25. */
 int cohere_dec_attention_q4(int32_t self, const int32_t* active, int64_t rows, const uint16_t* q, int64_t ldq,
                             uint8_t* k4, uint8_t* v4, uint16_t* ks, uint16_t* vs, const int32_t* n, int64_t slots,
                             int64_t heads, int64_t kv_heads, int64_t T, float scale, int64_t splits, float* part,
