@@ -177,3 +177,26 @@ def test_values_at_the_ends_of_the_range(gpu, self_attn, largest, lengths, ratio
         if self_attn and lengths[r] == 0:
             new = a[1][r, (H + KV) * 128:].reshape(KV, 1, 128)
             assert torch.equal(out[r].reshape(KV, ratio, 128), new.expand(KV, ratio, 128))
+
+
+@pytest.mark.parametrize("ratio,splits", [(1, 1), (1, 3), (2, 1), (4, 2)])
+@pytest.mark.parametrize("step", [0.02, 0.05, 0.3])
+def test_weights_that_fall_over_many_keys(gpu, step, ratio, splits):
+    """Scores that fall by `step` from key to key (and from the last key to the first), values that only every ninth key
+    has: outputs made of weights of any size beside larger ones, in every pass over the keys."""
+    print(f"attention_q4 step={step} ratio={ratio} splits={splits}", flush=True)
+    g = torch.Generator().manual_seed(int(100 * step))
+    KV, T, rows = 2, 1500, 2
+    H = KV * ratio
+    k, v = torch.zeros(rows, KV, T, 128), torch.randn(rows, KV, T, 128, generator=g)
+    at = torch.arange(T).float()
+    for i in range(4):  # a key's place in its four groups' maxima, which bf16 holds to 8 bits each
+        k[..., 32 * i] = (at if i < 2 else at.remainder(7)) / T
+    k[1] = k[1].flip(1)
+    v = torch.where(torch.arange(T)[:, None] % 9 == torch.arange(128)[None, :] % 9, v, torch.zeros_like(v))
+    q = torch.zeros(rows, H, 128)
+    q[..., ::32] = -step * T / SCALE / 2 * (1 + torch.arange(H)[:, None] / 100)
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
+         torch.tensor([T, T - 1], dtype=torch.int32), H)
+    _close(_run(False, *a, splits=splits), *a)
