@@ -9,7 +9,7 @@
 //
 // Bound by the memory where no token is penalised (128 rows x 100008 logits: 12.1 us, 4.3 TB/s read and written); the
 // penalties add the counts' way through LDS and 14 operations for each of eight logits that some lane of the wave has
-// penalised (16.4 us; 128 rows x 32000, up to 300 tokens: 5.1 and 6.2; one row of 16384, 200 tokens: 2.9 and 3.8).
+// penalised (16.0 us; 128 rows x 32000, up to 300 tokens: 5.1 and 6.2; one row of 16384, 200 tokens: 2.9 and 3.8).
 //
 // The counts are made anew from the slot's tokens in every call (a workgroup counts, in LDS, the tokens of its own part
 // of the vocabulary): no counts to keep per slot (4 bytes x vocabulary x slots), to clear when a slot is taken over or
@@ -67,7 +67,9 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
   // with 512 a long one's round trips 0.6 (128 rows x 100008, up to 4096 tokens)
   uint2 t[NK];
   // byte offsets in 32 bits (at most 2^28 tokens a slot)
-  const auto at = [&](int i) { return *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(tokens) + (uint32_t)i * 8u); };
+  const auto at = [&](int i) {
+    return *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(tokens) + (uint32_t)i * 8u);
+  };
   if (known) {
     p = a.pos[s];
     if (a.pen) {
@@ -108,7 +110,8 @@ __global__ void __launch_bounds__(NT) dec_logits_kernel(const LogitArgs a) {
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
         const uint32_t d = t[k].x - (uint32_t)v0;  // a token below v0 comes out far above SPAN
-        if (i0 + tid + k * NT <= hi && t[k].y == 0 && d < (uint32_t)SPAN) atomicAdd(&cnt[d / PER], 1u << (d % PER * (BITS % 32)));
+        if (i0 + tid + k * NT <= hi && t[k].y == 0 && d < (uint32_t)SPAN)
+          atomicAdd(&cnt[d / PER], 1u << (d % PER * (BITS % 32)));
       }
       i0 += NT * NK;
       if (i0 > hi) break;

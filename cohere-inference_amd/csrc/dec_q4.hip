@@ -40,9 +40,9 @@ using namespace cohere_q4;
 // Of fewer than 32 bits before the result, which keeps 8, are thus only these units: an output is off by at most 2^-11 of
 // sum p |v| for them.
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
-// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 330 a wave and 64 keys (950).
-// 64 rows x 8 heads, 0 .. 447 keys: 8.2 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys: 102 us, the
-// vector ALU; one row x 8 heads, 64 K keys: 14.4 us, 5.2 TB/s from the Infinity Cache.
+// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 325 a wave and 64 keys (1060).
+// 64 rows x 8 heads, 0 .. 447 keys: 8.1 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys, 8 parts: 111
+// us, the vector ALU (issuing 57 % of the time); one row x 8 heads, 64 K keys: 14.4 us, 5.2 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
 struct Q4Args {
@@ -227,7 +227,8 @@ DEVI void outputs_to(float (&so)[G][PARTS][HD], int wave, const float (&acc)[G][
     }
 }
 
-// Registers: four waves a SIMD (at 4 heads 3 waves give 88 us where 4 give 79: 16 rows of up to 32768 keys, 8 x 4 heads).
+// Registers: four waves a SIMD (at 4 heads 3 waves give 138 us where 4 give 110: 16 rows of up to 32768 keys, 8 x 4
+// heads).
 template <bool SELF, int G, int W>
 __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(4)))
 dec_attention_q4_kernel(const Q4Args p) {
@@ -540,8 +541,8 @@ dec_attention_q4_kernel(const Q4Args p) {
 
 // The parts of a (row, head): every wave finds the maximum, the parts' weights (lane s part s's) and the sum; CG groups of
 // 128 threads sum N parts each, all their loads in flight at once (a loop over the parts with its loads one after the
-// other took 30 us for 64 parts, this 4.5). Up to 4 parts: one group, no meeting in LDS (64 rows x 16 heads in 2 parts with
-// the attention 19.5 us, with 512 threads a head 21.0).
+// other took 30 us for 64 parts, this 4.5). Up to 4 parts: one group, no meeting in LDS (64 rows x 16 heads in 2 parts: 1.5
+// us less than with 512 threads a head).
 template <int CG, int N>
 __global__ void __launch_bounds__(CG * HD) dec_combine_q4_kernel(const float* __restrict__ part, int nsp, uint16_t* out) {
   const int64_t head = blockIdx.x;
@@ -711,17 +712,17 @@ int kv_entry(bool gather, KvArgs p, int64_t rows, int64_t L, int64_t S, int64_t 
   return cohere::check_launch(name);
 }
 
-// Query heads a workgroup takes (at most 4) and workgroups a key head. With up to 8 heads a workgroup, which reads the keys
-// once for all of them, the registers leave two waves a SIMD: 8 heads a key head in two workgroups 11.3 us, in one 17.4
-// (32 rows x 4 key heads, up to 1026 keys); 44.7 and 46.6 (8 rows x 8 key heads, up to 16 K keys).
+// Query heads a workgroup takes (at most 4) and workgroups a key head. A workgroup of 8 heads would read the keys once for
+// all of them, but their outputs alone take half of the registers of four waves a SIMD, and the vector ALU, not the
+// memory, bounds 4 heads already (32 rows x 4 x 8 heads, up to 1026 keys: 16.3 us; 8 rows x 8 x 8, up to 16 K keys: 64).
 struct HeadPlan { int g, chunks; };
 HeadPlan head_plan(int64_t ratio) {
   const int chunks = (int)((ratio + 3) / 4);
   return {(int)((ratio + chunks - 1) / chunks), chunks};
 }
 
-// waves of a workgroup: 4 for one head (64 rows x 8 heads, up to 448 keys: 7.0 us, with 8 7.5 us), else 8 (37 rows x 4 x 3
-// heads, up to 1026 keys: 9.8 us, with 4 12.9 us)
+// waves of a workgroup: 4 for one head (64 rows x 8 heads, up to 448 keys: 8.1 us, with 8 8.6 us), else 8 (64 rows x 8 x 2
+// heads, up to 2048 keys: 22.8 us, with 4 23.9 us; more heads need a thread a dimension of each)
 constexpr int waves_of(int g) { return g == 1 ? 4 : 8; }
 
 template <bool SELF>
@@ -743,15 +744,16 @@ extern "C" int64_t cohere_dec_attention_q4_splits(int64_t rows, int64_t heads, i
   // loads' latency), times a pass and the rounds that the workgroups take, and what the parts' meeting costs (a launch, and
   // 520 bytes a head and part written and read). Several rounds of more than one head even out rows of different lengths.
   // Fitted to sweeps over 1 .. 64 parts of 28 shapes (1 .. 128 rows, 465 .. 64 K keys, 1 .. 16 heads a key head, the rows
-  // of one length and from a sixteenth of it): its choice is within 10 % of the best of each. Powers of two: 48 parts of
-  // 16384 keys (no whole rounds) take 8.7 us, 32 or 64 7.7.
+  // of one length and from a sixteenth of it): its choice is within 12 % of the best of each. Powers of two: 48 parts of
+  // 16384 keys (no whole rounds) take 9.2 us, 32 or 64 8.1 and 7.9.
   const int64_t wgs = rows * kv_heads * hp.chunks;
   const double pass = 64. * waves_of(hp.g), us = hp.g == 1 ? 0.9 : 0.5 * hp.g, slots = hp.g == 1 ? 768. : 512.;
   int64_t best = 1;
   double least = 0.;
   for (int64_t n = 1; n <= 64 && (n == 1 || T / n >= 128); n *= 2) {
     const double keys = (double)T / n / pass, rounds = wgs * n / slots;
-    double t = (keys > 0.75 ? keys : 0.75) * us * (rounds > 1. ? rounds : 1.) + (n > 1 ? 2. + 0.0016 * rows * heads * n : 0.);
+    double t = (keys > 0.75 ? keys : 0.75) * us * (rounds > 1. ? rounds : 1.);
+    if (n > 1) t += 2. + 0.0016 * rows * heads * n;
     if (hp.g > 1 && rounds >= 2.) t *= 0.85;
     if (n == 1 || t < least * 0.999) best = n, least = t;
   }
@@ -786,7 +788,7 @@ extern "C" int cohere_dec_attention_q4(int32_t self, const int32_t* active, int6
   const dim3 grid = p.rows_y ? dim3(ny, (unsigned)rows, (unsigned)splits) : dim3((unsigned)rows, ny, (unsigned)splits);
   if (self) launch_attention<true>(hp.g, p, grid, s);
   else launch_attention<false>(hp.g, p, grid, s);
-  // few parts: 128 threads a head (64 rows x 16 heads in 2 parts 21.0 -> 19.5 us in all, in 4 25.2 -> 23.7)
+  // few parts: 128 threads a head (64 rows x 16 heads in 2 or in 4 parts 1.5 us less)
   const unsigned hs = (unsigned)(rows * heads);
   if (splits > 4) dec_combine_q4_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(part, (int)splits, out);
   else if (splits > 1) dec_combine_q4_kernel<1, 4><<<hs, HD, 0, s>>>(part, (int)splits, out);

@@ -5,8 +5,8 @@
 // and codes 0, so that what attends to it is NaN too.
 //
 // Why groups of 32 with a maximum each: a normal vector keeps 20.3 dB of signal over the rounding, with one maximum over
-// 128 values 18.6 (the maximum of 128 is a fifth larger than that of 32, and a step is m / 7), for 6 bytes of 72. Why the maximum and not the step m / 7: it needs
-// no rounding, so a code can be exact. 7 x is exact in fp32 (8 + 3 bits); 7 x / m is either k + 1/2 exactly or further
+// 128 values 18.6 (the maximum of 128 is a fifth larger than that of 32, and a step is m / 7), for 6 bytes of 72. Why the
+// maximum and not the step m / 7: it needs no rounding, so a code can be exact. 7 x is exact in fp32 (8 + 3 bits); 7 x / m is either k + 1/2 exactly or further
 // from it than 1e-4 of its value (the numerators are 11-bit, the denominators 8-bit), so a quotient that is exact where
 // it is representable gives the code of the exact quotient.
 #pragma once

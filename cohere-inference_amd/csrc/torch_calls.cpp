@@ -1,5 +1,5 @@
 // The entry points over 4-bit caches and on logits as Python functions of torch tensors: the argument checks in C++,
-// because in Python they take longer than the launch (a lone call 8.6 us of host time, 3.4 of them the launch; here 5)
+// because in Python they take longer than the launch (a lone call 8.6 us of host time; here 4, what a launch alone takes)
 // and these calls are made once per layer and step. Bound to the C ABI's functions by address (bind), so that the
 // library is the one that kernels/cuda_ext.py loaded. A refused call raises RuntimeError.
 #define PY_SSIZE_T_CLEAN
@@ -122,7 +122,8 @@ void launch(F f) {
 // codes uint8 (..., 64) and maxima bf16 (..., 4), keys and values alike, `dims` sizes before them
 struct Caches {
   const Tensor &k4, &v4, &ks, &vs;
-  Caches(const Call& c, int at, int dims) : k4(c.tensor(at)), v4(c.tensor(at + 1)), ks(c.tensor(at + 2)), vs(c.tensor(at + 3)) {
+  Caches(const Call& c, int at, int dims)
+      : k4(c.tensor(at)), v4(c.tensor(at + 1)), ks(c.tensor(at + 2)), vs(c.tensor(at + 3)) {
     c.need(k4.dim() == dims + 1 && k4.size(dims) == 64 && v4.sizes() == k4.sizes() && k4.scalar_type() == at::kByte &&
                v4.scalar_type() == at::kByte && k4.is_contiguous() && v4.is_contiguous(),
            "contiguous uint8 caches of 64 bytes a vector");

@@ -660,11 +660,12 @@ class _Ext:
 
     def dec_attention_q4(self, self_attn, active, q, k4, v4, ks, vs, n, scale, splits, part, out):
         """dec_attention over caches in 4 bits: codes k4, v4 uint8 (slots, KV, T, 64) and maxima ks, vs bf16 (slots, KV,
-        T, 4), H = out.shape[1] / 128 query heads, H / KV of them to a key head. Self-attention: q (rows, (H + 2 KV) 128)
-        holds the new token's queries, keys and values, appended at position n[slot] and attended as computed. Rows
-        without keys, of slots out of range or (self-attention) of positions beyond T get zeros. A slot belongs to one row
-        of a self-attention call (two get their results, but leave an undefined position). splits > 1 needs part (rows x
-        H x splits x 130 floats). kernels.stream_decoder.quantize_q4 states the form."""
+        T, 4), H = out.shape[1] / 128 query heads, H / KV of them to a key head. Self-attention: q (rows, (H + 2 KV)
+        128) holds the new token's queries, keys and values, appended at position n[slot] and attended as computed.
+        Rows without keys, of slots out of range or (self-attention) of positions beyond T get zeros. A slot belongs
+        to one row of a self-attention call (two get their results, but leave an undefined position). splits > 1
+        needs part (rows x H x splits x 130 floats, of one call at a time); out must not overlap q.
+        kernels.stream_decoder.quantize_q4 states the form."""
         _calls.dec_attention_q4(self_attn, active, q, k4, v4, ks, vs, n, scale, splits, part, out)
 
     def dec_scatter_kv_q4(self, kv, slot_of, frame_of, ck, cv, cks, cvs):
@@ -684,12 +685,12 @@ class _Ext:
 
     def dec_logits(self, logits, y, active, pos, tokens=None, first=None, plen=None, penalties=None, bias=None,
                    bias_of=None, mask=None, classes=None, trans=None, start=None, state=None):
-        """Rules on a step's logits (rows, V) into y (which may be logits), before dec_pick: of slot s = active[r] at
-        position pos[s], penalties fp32 (slots, 3) (repetition, presence, frequency) for the tokens tokens[s,
-        first[s]..pos[s]], bias row bias_of[s] of bias bf16 (B, V), and -inf for what the mask row of the grammar's state
-        lacks: mask int32 (M, ceil(V / 32)), start int32 (slots), and with classes int32 (V), trans int32 (M, C) and
-        state int32 (slots, 2) the state moves with every token behind the prompt (plen). Absent rules are None; index
-        values out of range switch a rule off for a slot."""
+        """Rules on a step's logits (rows, V) into y (which may be logits, and does not overlap them otherwise), before
+        dec_pick: of slot s = active[r] at position pos[s], penalties fp32 (slots, 3) (repetition, presence,
+        frequency) for the tokens tokens[s, first[s]..pos[s]], bias row bias_of[s] of bias bf16 (B, V), and -inf for
+        what the mask row of the grammar's state lacks: mask int32 (M, ceil(V / 32)), start int32 (slots), and with
+        classes int32 (V), trans int32 (M, C) and state int32 (slots, 2) the state moves with every token behind the
+        prompt (plen). Absent rules are None; index values out of range switch a rule off for a slot."""
         _calls.dec_logits(logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask, classes, trans,
                           start, state)
 

@@ -218,8 +218,8 @@ class StreamDecoder:
     with its decoder attributes); `frames` may be given instead of asking the encoder for its subsampled length.
 
     kv_bits: 16, 8 or 4 bits a cached value (default: 8 with int8, else 16; 4: quantize_q4's form, 72 bytes a vector of
-    128 where 8 bits take 132). penalties, bias (B, vocabulary; held in bf16) and grammar (a Grammar) let requests have Rules; any of
-    them puts one launch (ext.dec_logits) between the head and the pick of every step."""
+    128 where 8 bits take 132). penalties, bias (B, vocabulary; held in bf16) and grammar (a Grammar) let requests have
+    Rules; any of them puts one launch (ext.dec_logits) between the head and the pick of every step."""
 
     BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 112, 128)
 

@@ -296,10 +296,10 @@ int cohere_dec_gather_kv_q4(const int32_t* slot_of, const int32_t* frame_of, int
                             const uint8_t* cv, const uint16_t* cks, const uint16_t* cvs, int64_t L, int64_t S, int64_t H,
                             int64_t T, uint16_t* kv, int64_t ldkv, void* stream);
 
-/* Rules on logits x [rows, V] bf16 (ldx) into y (ldy; y may be x), before cohere_dec_pick. Row r is slot s = active[r]; p =
- * pos[s] is the position of its newest token, tokens int64 [slots, OUT] what it holds. With c the times that token v is
- * among tokens[s][max(first[s], 0) .. min(p, OUT - 1)] and (rep, presence, frequency) = pen[s] (fp32 [slots, 3], null:
- * none), in fp32, one rounding each:
+/* Rules on logits x [rows, V] bf16 (ldx) into y (ldy; y may be x, and does not overlap it otherwise), before
+ * cohere_dec_pick. Row r is slot s = active[r]; p = pos[s] is the position of its newest token, tokens int64 [slots,
+ * OUT] what it holds. With c the times that token v is among tokens[s][max(first[s], 0) .. min(p, OUT - 1)] and (rep,
+ * presence, frequency) = pen[s] (fp32 [slots, 3], null: none), in fp32, one rounding each:
  *   c > 0: l = l > 0 ? l / rep : l * rep; l = l - (c * frequency + presence)
  *   l = l + bias[bias_of[s]][v]        (bias bf16 [B, V], null: none; bias_of[s] outside 0 .. B - 1: none)
  *   l = -inf where mask[state] lacks v (mask int32 [M, ceil(V / 32)], bit v % 32 of word v / 32, null: none; a state
@@ -308,8 +308,7 @@ int cohere_dec_gather_kv_q4(const int32_t* slot_of, const int32_t* frame_of, int
  * p < plen[s] and trans[the state at p - 1][classes[tokens[s][p]]] later (-1 where any of these is out of range); the
  * state at p is written to state[s][p % 2] and the one at p - 1 expected in the other place (state int32 [slots, 2]).
  * A row whose slot is out of range is copied. V % 8 == 0, rows <= 65535, OUT <= 2^28; 16-byte aligned rows of x, y and
- * bias. Row r of y may be all
- * -inf: cohere_dec_pick then ends the row. */
+ * bias. Row r of y may be all -inf: cohere_dec_pick then ends the row. */
 int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int64_t V,
                       const int32_t* active, const int32_t* pos, int64_t slots, const int64_t* tokens, int64_t OUT,
                       const int32_t* first, const int32_t* plen, const float* pen, const uint16_t* bias, int64_t B,
