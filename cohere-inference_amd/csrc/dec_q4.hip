@@ -214,6 +214,17 @@ DEVI float digits4(const v4i& d) {
   return __builtin_fmaf((float)(d[0] * 256 + d[1]), 65536.f, (float)(d[2] * 256 + d[3]));
 }
 
+// what sums of query digits times codes are to be multiplied by, scale 2^unit, in two parts: sums times 2^up and the scale
+// stay within fp32's range for queries of any magnitude
+struct DigitScale {
+  float scale;
+  int up, unit;
+};
+DEVI DigitScale digit_scale(float scale, int unit) {
+  const int up = max(-100, min(unit, 60));
+  return {ldexpf(scale, unit - up), up, unit};
+}
+
 // a wave's outputs, 8 dimensions in each lane that has them, behind each other in LDS
 template <int G, int PARTS>
 DEVI void outputs_to(float (&so)[G][PARTS][HD], int wave, const float (&acc)[G][8]) {
@@ -236,7 +247,7 @@ dec_attention_q4_kernel(const Q4Args p) {
   // the queries' digits [level][head][group][high .. low][32], behind each head's 32 zeros
   constexpr int QHEAD = HD * 4 + 32, LEVELS = 12;
   __shared__ __attribute__((aligned(16))) uint8_t sq[LEVELS][G][QHEAD];
-  __shared__ float sqs[G][NG];
+  __shared__ DigitScale sqs[G][NG];
   __shared__ int slevels[W];
   __shared__ __attribute__((aligned(16))) uint8_t sp8[W][G < 2 ? 1 : 2][16 * ROW8];
   __shared__ __attribute__((aligned(16))) float so[G][PARTS][HD];
@@ -318,7 +329,7 @@ dec_attention_q4_kernel(const Q4Args p) {
     level = ex < 8 ? (30 - ex) / 23 : 0;
     while (__any(level > deep)) ++deep;
     digits_to(0);
-    if ((d & 31) == 0) sqs[g][d >> 5] = ok ? ldexpf(p.scale * (LOG2E / CODE), -qe) : nan_f();
+    if ((d & 31) == 0) sqs[g][d >> 5] = digit_scale(ok ? p.scale * (LOG2E / CODE) : nan_f(), -qe);
   }
   if (lane == 0) slevels[wave] = deep;
   if constexpr (SELF) {
@@ -390,12 +401,14 @@ dec_attention_q4_kernel(const Q4Args p) {
         int lv = 0;
         do {
           v4i aq[2][2];
-          float qs[2], x[2], z[2];
+          float x[2], z[2];
+          DigitScale qs[2];
 #pragma unroll
           for (int h = 0; h < 2 && g0 + h < G; ++h) {
             aq[h][0] = *reinterpret_cast<const v4i*>(&sq[lv][g0 + h][a_at]);
             aq[h][1] = *reinterpret_cast<const v4i*>(&sq[lv][g0 + h][a_at + 16]);
-            qs[h] = ldexpf(sqs[g0 + h][rowg], -23 * lv);
+            qs[h] = sqs[g0 + h][rowg];
+            if (__builtin_expect(lv > 0, 0)) qs[h] = digit_scale(p.scale * (LOG2E / CODE), qs[h].unit - 23 * lv);
           }
           // tiles of 16 keys in the order 0, 2, 1, 3: what two of them give meets at once
 #pragma unroll
@@ -409,7 +422,7 @@ dec_attention_q4_kernel(const Q4Args p) {
             for (int h = 0; h < 2 && g0 + h < G; ++h) {
               v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[h][0], b0, v4i{0, 0, 0, 0}, 0, 0, 0);
               d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[h][1], b1, d, 0, 0, 0);
-              const float v = digits4(d) * qs[h] * mk;
+              const float v = ldexpf(digits4(d), qs[h].up) * (qs[h].scale * mk);
               if (i == 0 || i == 2) x[h] = v;
               else if (i == 1) z[h] = half_sum(x[h], v);
               else sc[g0 + h] += quarter_sum(z[h], half_sum(x[h], v));

@@ -200,3 +200,21 @@ def test_weights_that_fall_over_many_keys(gpu, step, ratio, splits):
     a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
          torch.tensor([T, T - 1], dtype=torch.int32), H)
     _close(_run(False, *a, splits=splits), *a)
+
+
+@pytest.mark.parametrize("ratio,self_attn", [(1, False), (1, True), (3, False), (4, True)])
+@pytest.mark.parametrize("size", [2.0 ** -119, 2.0 ** -90, 2.0 ** -60, 2.0 ** 60, 2.0 ** 90, 2.0 ** 121])
+def test_queries_and_keys_of_opposite_magnitudes(gpu, size, ratio, self_attn):
+    """Queries as small (or large) as bf16 has them over keys as large (or small): ordinary scores."""
+    print(f"attention_q4 size={size} ratio={ratio} self={self_attn}", flush=True)
+    g = torch.Generator().manual_seed(13)
+    KV, T, rows = 2, 300, 2
+    H = KV * ratio
+    k, v = torch.randn(rows, KV, T, 128, generator=g) / size, torch.randn(rows, KV, T, 128, generator=g)
+    q = torch.randn(rows, H + (2 * KV if self_attn else 0), 128, generator=g)
+    q[:, :H] *= size
+    q[:, H:H + KV] /= size
+    (k4, ks), (v4, vs) = _held(k), _held(v)
+    a = (torch.arange(rows, dtype=torch.int32), q.reshape(rows, -1).to(BF), k4, v4, ks, vs,
+         torch.tensor([T - 1, 70], dtype=torch.int32), H)
+    _close(_run(self_attn, *a), *a, self_attn=self_attn)
