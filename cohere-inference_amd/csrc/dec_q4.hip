@@ -40,8 +40,8 @@ using namespace cohere_q4;
 // Of fewer than 32 bits before the result, which keeps 8, are thus only these units: an output is off by at most 2^-11 of
 // sum p |v| for them.
 // Why the matrix cores for one query: with v_dot8_i32_i4 and one fma a value the vector ALU took 110 instructions a wave
-// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 325 a wave and 64 keys (1060).
-// 64 rows x 8 heads, 0 .. 447 keys: 8.1 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys, 8 parts: 111
+// and 16 keys (340 at 4 heads), and every lane's outputs had to meet at the end; here about 330 a wave and 64 keys (1065).
+// 64 rows x 8 heads, 0 .. 447 keys: 8.2 us, launch and load latency; 16 rows x 8 x 4 heads, 2 .. 32 K keys, 8 parts: 110
 // us, the vector ALU (issuing 57 % of the time); one row x 8 heads, 64 K keys: 14.4 us, 5.2 TB/s from the Infinity Cache.
 // The codes, maxima and keys past the end come back as zeros from the buffer loads' own bounds check, so that nothing is
 // read of them and they weigh nothing.
@@ -734,7 +734,7 @@ HeadPlan head_plan(int64_t ratio) {
   return {(int)((ratio + chunks - 1) / chunks), chunks};
 }
 
-// waves of a workgroup: 4 for one head (64 rows x 8 heads, up to 448 keys: 8.1 us, with 8 8.6 us), else 8 (64 rows x 8 x 2
+// waves of a workgroup: 4 for one head (64 rows x 8 heads, up to 448 keys: 8.2 us, with 8 8.6 us), else 8 (64 rows x 8 x 2
 // heads, up to 2048 keys: 22.8 us, with 4 23.9 us; more heads need a thread a dimension of each)
 constexpr int waves_of(int g) { return g == 1 ? 4 : 8; }
 
