@@ -1,0 +1,576 @@
+// Beam search on a decoding step's logits, for gfx950. No counterpart in the reference, which decodes greedily
+// (kernels/csrc/decoder_ops.cu:106-159). A group is one request's B beams (1 .. 16): slots g B .. g B + B - 1, best first.
+//
+//   dec_beam_select   the B best continuations over the beams and the vocabulary
+//   dec_beam_reorder  every beam takes over its parent's history: table, tokens, states, the page in part filled
+//   dec_beam_advance  the chosen tokens go into the slots' state; the next step's embeddings
+//
+// Selection. total[b][v] = score[b] + l[v] - max l - log sum exp(l - max l). Whether a candidate is in or out must not hang
+// on roundings: the sums are in 64 bits, of exponentials that are right to 6e-11 of themselves, and candidates are compared
+// in 64 bits. Within a beam the order is that of the logits (then of the indexes), so the first launch needs no sums to
+// find a part's B best: it compares 16-bit numbers.
+#include "cohere_hip.h"
+#include "common.h"
+#include "rows.h"
+
+#include <string>
+#include <type_traits>
+
+namespace {
+
+using namespace cohere_rows;
+
+constexpr int MAXB = 16;
+constexpr double LOG2E64 = 1.4426950408889634074;
+
+// a bf16 logit as a number of the same order; NaN counts as -inf, inf as the largest finite number, -0 as 0
+DEVI uint32_t order_of(uint32_t h) {
+  if ((h & 0x7fffu) > 0x7f80u) h = 0xff80u;
+  if (h == 0x7f80u) h = 0x7f7fu;
+  if (h == 0x8000u) h = 0;
+  return h & 0x8000u ? h ^ 0xffffu : h | 0x8000u;
+}
+DEVI float logit_of(uint32_t o) { return __uint_as_float((o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu) << 16); }
+constexpr uint32_t LOWEST = 0x7f;  // order_of(-inf)
+
+// a part's result: maximum, sum of exp(l - maximum), then B keys order << 32 | ~index, best first (0: none)
+struct Part {
+  float m;
+  uint32_t unused;
+  double sum;
+};
+__host__ __device__ inline int64_t part_bytes(int B) { return (int64_t)sizeof(Part) + 8 * B; }
+
+DEVI uint32_t wave_max_u(uint32_t v) {
+  const auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  for (int o = 1; o < 64; o <<= 1) v = mx(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return v;
+}
+DEVI uint64_t wave_max_u64(uint64_t v) {
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t w = __shfl_xor(v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+DEVI double wave_sum_d(double v) {
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// of 64 keys, one a lane (0: none, the others different), the place of this lane's among them
+DEVI int rank_of(uint64_t key) {
+  int r = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) {
+    const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+    r += o > key;
+  }
+  return r;
+}
+
+// 2^y for y in -1000 .. 0 to 6e-11 of itself: 2^(y - round y) by the Chebyshev interpolant of 2^x on -1/2 .. 1/2 of degree
+// 7, times a power of two
+DEVI double exp2_64(double y) {
+  const double magic = 6755399441055744.0;  // 1.5 2^52: the sum's last bit is 1
+  const double t = y + magic, f = y - (t - magic);
+  double p = 1.5303699001378845e-05;
+  p = __builtin_fma(p, f, 0.00015469729140704658);
+  p = __builtin_fma(p, f, 0.0013333478480888061);
+  p = __builtin_fma(p, f, 0.009618025613598036);
+  p = __builtin_fma(p, f, 0.055504109063177154);
+  p = __builtin_fma(p, f, 0.24022651213495422);
+  p = __builtin_fma(p, f, 0.6931471805568341);
+  p = __builtin_fma(p, f, 0.9999999999595622);
+  return __builtin_amdgcn_ldexp(p, (int)__builtin_bit_cast(uint64_t, t));
+}
+
+struct SelectArgs {
+  const uint16_t* logits;
+  int64_t ld;
+  const int32_t* groups;
+  const float* score;
+  const uint8_t* finished;
+  const int32_t* made;  // null: no norm
+  const float* norm;
+  int32_t* parent;
+  int64_t* token;
+  float* total;
+  char* work;
+  int n, G, B, V, N, pad, parts;
+};
+
+// A workgroup takes J * 2048 logits of a row: their maximum, the sum, and the B best. A wave finds its B best among few:
+// T, the B-th largest of its lanes' maxima, is no larger than the B-th best, and hardly more than B logits reach it; these
+// are ranked by counting, one a lane. Where more than 64 do (many equal logits, a mask that leaves little), the B best are
+// taken one by one.
+template <int J>
+__global__ void __launch_bounds__(256) beam_parts_kernel(const SelectArgs a) {
+  __shared__ uint64_t cand[4][64], best[4][MAXB];
+  __shared__ uint32_t smax[4];
+  __shared__ double ssum[4];
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), B = a.B;
+  const int r = blockIdx.y, v0 = blockIdx.x * (J * 2048), i = r / B, g = a.groups[i];
+  const uint16_t* row = a.logits + (int64_t)r * a.ld;
+  uint4 u[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int v = v0 + (j * 256 + tid) * 8;
+    u[j] = *reinterpret_cast<const uint4*>(row + min(v, a.V - 8));
+  }
+  if ((unsigned)g >= (unsigned)a.G) return;
+  const int slot = g * B + (r - i * B);
+  if (a.finished[slot] || !(a.score[slot] > -INFINITY)) return;  // its candidates are known without the logits
+  uint32_t o[J * 8], top = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const bool in = v0 + (j * 256 + tid) * 8 < a.V;
+    const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      o[j * 8 + k] = in ? order_of(k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu) : 0;  // 0: none
+      top = o[j * 8 + k] > top ? o[j * 8 + k] : top;
+    }
+  }
+  const auto key_of = [&](int e) {
+    return (uint64_t)o[e] << 32 | ~(uint32_t)(v0 + ((e >> 3) * 256 + tid) * 8 + (e & 7));
+  };
+  // the B-th largest of the lanes' maxima
+  uint32_t t = top, T = 0;
+  for (int k = 0; k < B; ++k) {
+    T = wave_max_u(t);
+    if (k == 0 && lane == 0) smax[wave] = T;
+    const uint64_t who = __ballot(t == T);
+    if (lane == __ffsll((unsigned long long)who) - 1) t = 0;
+  }
+  T = T ? T : 1;
+  if (lane < MAXB) best[wave][lane] = 0;
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < J * 8; ++e) {
+    const uint64_t who = __ballot(o[e] >= T);
+    if (who) {
+      const int at = count + __popcll(who & ((1ull << lane) - 1));
+      if (o[e] >= T && at < 64) cand[wave][at] = key_of(e);
+      count += __popcll(who);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
+  if (__builtin_expect(count <= 64, 1)) {
+    const uint64_t key = lane < count ? cand[wave][lane] : 0;
+    const int place = rank_of(key);
+    if (key && place < B) best[wave][place] = key;
+  } else {
+    uint64_t last = ~0ull;
+    for (int k = 0; k < B; ++k) {
+      uint64_t mine = 0;
+#pragma unroll
+      for (int e = 0; e < J * 8; ++e) {
+        const uint64_t key = key_of(e);
+        if (o[e] && key < last && key > mine) mine = key;
+      }
+      last = wave_max_u64(mine);
+      if (lane == 0) best[wave][k] = last;
+      if (!last) break;
+    }
+  }
+  __syncthreads();
+  uint32_t M = smax[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) M = smax[w] > M ? smax[w] : M;
+  const float m = M ? logit_of(M) : -INFINITY;
+  double sum = 0.;
+  if (m > -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < J * 8; ++e) {
+      // the difference first: it is exact, or nearly so, at any magnitude
+      const double y = ((double)logit_of(o[e]) - (double)m) * LOG2E64;
+      sum += exp2_64(o[e] > LOWEST && y > -1000. ? y : -1000.);
+    }
+  }
+  sum = wave_sum_d(sum);
+  if (lane == 0) ssum[wave] = sum;
+  __syncthreads();
+  if (wave != 0) return;
+  Part* out = reinterpret_cast<Part*>(a.work + ((int64_t)r * a.parts + blockIdx.x) * part_bytes(B));
+  uint64_t* keys = reinterpret_cast<uint64_t*>(out + 1);
+  if (lane == 0) {
+    out->m = m;
+    out->sum = (ssum[0] + ssum[1]) + (ssum[2] + ssum[3]);
+  }
+  const uint64_t key = lane < 4 * B ? best[lane / B][lane % B] : 0;
+  const int place = rank_of(key), have = __popcll(__ballot(key != 0));
+  if (key && place < B) keys[place] = key;
+  if (lane < B && lane >= have) keys[lane] = 0;
+}
+
+// A workgroup takes a group: a wave a beam's parts (their sum, and of their B best each the beam's B best), then the B x B
+// candidates are ranked by counting, a thread each.
+__global__ void __launch_bounds__(256) beam_merge_kernel(const SelectArgs a) {
+  __shared__ double srank[MAXB * MAXB], stotal[MAXB * MAXB];
+  __shared__ int sv[MAXB * MAXB];
+  __shared__ uint64_t tmp[4][MAXB];
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), B = a.B;
+  const int i = blockIdx.x, g = a.groups[i];
+  if ((unsigned)g >= (unsigned)a.G) {
+    if (tid < B) {
+      a.parent[i * B + tid] = tid;
+      a.token[i * B + tid] = a.pad;
+      a.total[i * B + tid] = -INFINITY;
+    }
+    return;
+  }
+  for (int b = wave; b < B; b += 4) {
+    const bool ended = a.finished[g * B + b] != 0;
+    const double start = (double)a.score[g * B + b];
+    double total = -INFINITY;
+    int v = 0;
+    if (!(start > -INFINITY)) {  // nothing but candidates of -inf (NaN counts as it): by their indexes
+      v = lane;
+    } else if (ended) {
+      v = lane == 0 ? a.pad : lane - 1 + (lane - 1 >= a.pad);
+      total = lane == 0 ? start : -INFINITY;
+    } else {
+      const char* at = a.work + ((int64_t)i * B + b) * a.parts * part_bytes(B);
+      float M = -INFINITY;
+      for (int p = lane; p < a.parts; p += 64) M = fmaxf(M, reinterpret_cast<const Part*>(at + p * part_bytes(B))->m);
+      M = wave_max64(M);
+      double S = 0.;
+      for (int p = lane; p < a.parts; p += 64) {
+        const Part* q = reinterpret_cast<const Part*>(at + p * part_bytes(B));
+        const double y = ((double)q->m - (double)M) * LOG2E64;
+        S += q->m > -INFINITY ? q->sum * exp2_64(y > -1000. ? y : -1000.) : 0.;
+      }
+      S = wave_sum_d(S);
+      // the sorted keys so far in lanes 0 .. B - 1, the next 64 - B beside them
+      uint64_t cur = 0;
+      for (int k0 = 0; k0 < a.parts * B; k0 += 64 - B) {
+        const int k = k0 + lane - B, p = k / B;
+        uint64_t key = cur;
+        if (lane >= B)
+          key = k < a.parts * B ? reinterpret_cast<const uint64_t*>(at + p * part_bytes(B) + sizeof(Part))[k - p * B] : 0;
+        const int place = rank_of(key);
+        if (lane < B) tmp[wave][lane] = 0;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (key && place < B) tmp[wave][place] = key;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        cur = lane < B ? tmp[wave][lane] : 0;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      v = (int)~(uint32_t)cur;
+      const float l = logit_of((uint32_t)(cur >> 32));
+      if (M > -INFINITY) total = start + ((double)l - (double)M - log(S));  // else: no logit above -inf
+    }
+    double rank = total;
+    if (a.norm) {
+      const int len = a.made[g * B + b] + (ended ? 0 : 1);
+      rank = total * (double)a.norm[min(max(len, 0), a.N - 1)];
+    }
+    if (lane < B) {
+      stotal[b * B + lane] = total == total ? total : -INFINITY;
+      srank[b * B + lane] = rank == rank ? rank : -INFINITY;
+      sv[b * B + lane] = v;
+    }
+  }
+  __syncthreads();
+  if (tid >= B * B) return;
+  const double mine = srank[tid];
+  const int b = tid / B, v = sv[tid];
+  int place = 0;
+  for (int c = 0; c < B * B; ++c) {
+    const double other = srank[c];
+    const int cb = c / B;
+    place += other > mine || (other == mine && (cb < b || (cb == b && sv[c] < v)));
+  }
+  if (place < B) {
+    a.parent[i * B + place] = b;
+    a.token[i * B + place] = v;
+    a.total[i * B + place] = (float)stotal[tid];
+  }
+}
+
+int select_j(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) >= 512 ? 4 : 1; }
+int64_t select_parts(int64_t rows, int64_t V) {
+  const int64_t span = 2048 * select_j(rows, V);
+  return (V + span - 1) / span;
+}
+
+// ---- reordering --------------------------------------------------------------------------------------------------------
+struct ReorderArgs {
+  const int32_t *groups, *parent, *n;
+  const uint8_t* done;
+  int32_t* table;
+  int64_t* tokens;
+  int32_t* states;
+  char *k, *v;
+  float *ks, *vs;
+  int G, B, W, OUT, NS, L, pages, shift, KV, bytes;  // NS: states a row, bytes of a vector held
+  uint32_t chunks;                                   // of 16 bytes of a page in part filled, all layers, keys and values
+};
+
+// Block 0 of a group moves its rows of the tables, a thread a column of all B beams; the others move what the page in part
+// filled holds, a thread 16 bytes of all B beams: read before any is written, so that nothing has to wait for anything.
+template <int MB>
+__global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) {
+  const int i = blockIdx.y, g = a.groups[i], B = a.B, tid = threadIdx.x;
+  if ((unsigned)g >= (unsigned)a.G || (a.done && a.done[g])) return;
+  const int64_t slot0 = (int64_t)g * B;
+  const int n = max(a.n[slot0], 0);
+  int from[MB];
+  bool moved = false;
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    const int q = b < B ? a.parent[(int64_t)i * B + b] : b;
+    from[b] = (unsigned)q < (unsigned)B ? q : b;
+    moved |= from[b] != b;
+  }
+  if (!moved) return;
+  if (blockIdx.x == 0) {
+    const auto move = [&](auto* rows, int width, int count) {
+      using T = std::remove_reference_t<decltype(*rows)>;
+      for (int c = tid; c < count; c += 256) {
+        T x[MB];
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+          if (b < B) x[b] = rows[(slot0 + from[b]) * width + c];
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+          if (b < B && from[b] != b) rows[(slot0 + b) * width + c] = x[b];
+      }
+    };
+    if (a.table) move(a.table, a.W, min(n >> a.shift, a.W));
+    if (a.tokens) move(a.tokens, a.OUT, min(n, a.OUT));
+    if (a.states) move(a.states, a.NS, a.NS);
+    return;
+  }
+  const int filled = n & ((1 << a.shift) - 1), place = n >> a.shift;
+  if (filled == 0 || place >= a.W) return;
+  const uint32_t c = (blockIdx.x - 1) * 256 + tid;
+  if (c >= a.chunks) return;
+  const int part = (int)(c & (a.bytes / 16 - 1));  // 16 of bf16, 8 of int8
+  uint32_t rest = c >> (a.bytes == 256 ? 4 : 3);
+  const int off = (int)(rest & ((1 << a.shift) - 1));
+  if (off >= filled) return;
+  rest >>= a.shift;
+  const uint32_t q = rest / (uint32_t)a.KV;
+  const int h = (int)(rest - q * a.KV), kvi = (int)(q & 1), layer = (int)(q >> 1);
+  char* pages = kvi ? a.v : a.k;
+  float* scales = kvi ? a.vs : a.ks;
+  int page[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) page[b] = b < B ? a.table[(slot0 + b) * a.W + place] : -1;
+  const auto vec = [&](int pg) { return ((((int64_t)layer * a.pages + pg) * a.KV + h) << a.shift) + off; };
+  // bit b: beam b's own page and its parent's are there, and two pages. The loads are made for every beam (of page 0
+  // where the bit is 0), the stores by the bit.
+  uint32_t go = 0;
+  v4i x[MB];
+  float sc[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    int src = -1;
+#pragma unroll
+    for (int q = 0; q < MB; ++q) src = from[b] == q ? page[q] : src;
+    const bool ok = from[b] != b && (unsigned)src < (unsigned)a.pages && (unsigned)page[b] < (unsigned)a.pages;
+    go |= ok ? 1u << b : 0u;
+    const int64_t at = vec(ok ? src : 0);
+    x[b] = *reinterpret_cast<const v4i*>(pages + at * a.bytes + part * 16);
+    sc[b] = scales ? scales[at] : 0.f;
+  }
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    if (!(go >> b & 1)) continue;
+    const int64_t at = vec(page[b]);
+    *reinterpret_cast<v4i*>(pages + at * a.bytes + part * 16) = x[b];
+    if (scales && part == 0) scales[at] = sc[b];
+  }
+}
+
+// ---- the chosen tokens -------------------------------------------------------------------------------------------------
+struct AdvanceArgs {
+  const int32_t *groups, *parent;
+  const int64_t* token;
+  const float* total;
+  int64_t* tok;
+  int32_t* pos;
+  float* score;
+  uint8_t *finished, *done, *flags;
+  int32_t* made;
+  const int32_t* limit;
+  int64_t* out;
+  int64_t eos;
+  int G, B, OUT, dummy, by_length;
+  const uint16_t *emb, *ptab, *w0, *b0, *w1, *b1;
+  float eps0, eps1;
+  uint16_t *x, *h;
+  int width, tokens, positions;  // rows of emb and ptab
+};
+
+template <int VEC>
+__global__ void __launch_bounds__(256) beam_advance_kernel(const AdvanceArgs a) {
+  __shared__ int64_t stok[MAXB];
+  __shared__ int spos[MAXB];
+  const int i = blockIdx.x, lane = lane_id(), wave = wave_id(), B = a.B;
+  const int g = a.groups[i];
+  if ((unsigned)g >= (unsigned)a.G) return;
+  const int64_t slot0 = (int64_t)g * B;
+  if (wave == 0) {
+    const bool live = g != a.dummy && !a.done[g], mine = lane < B;
+    const int b = mine ? lane : 0;
+    int64_t t = a.tok[slot0 + b];
+    int p = a.pos[slot0 + b];
+    if (live) {
+      const int q = a.parent[(int64_t)i * B + b], from = (unsigned)q < (unsigned)B ? q : b;
+      const bool was = a.finished[slot0 + from] != 0;
+      const int made = a.made[slot0 + from] + (was ? 0 : 1);
+      const float total = a.total[(int64_t)i * B + b];
+      t = a.token[(int64_t)i * B + b];
+      p = a.pos[slot0 + b] + 1;
+      const bool fin = was || t == a.eos || !(total > -INFINITY);
+      // the best beam of a group without norm stays the best once it has ended: the others' scores only fall
+      const uint64_t all = __ballot(fin || !mine), first = __ballot(mine && lane == 0 && fin);
+      const bool end = all == ~0ull || (!a.by_length && first) || p >= a.limit[g];
+      // every lane's loads came before any lane's stores: one wave, in order
+      if (mine) {
+        a.finished[slot0 + b] = fin;
+        a.made[slot0 + b] = made;
+        a.score[slot0 + b] = total;
+        a.tok[slot0 + b] = t;
+        a.pos[slot0 + b] = p;
+        if (p < a.OUT) a.out[(slot0 + b) * a.OUT + p] = t;
+        if (lane == 0 && end) {
+          a.done[g] = 1;
+          if (a.flags) a.flags[g] = 1;
+        }
+      }
+    }
+    if (mine) {
+      stok[lane] = t;
+      spos[lane] = p;
+    }
+  }
+  __syncthreads();
+  for (int b = wave; b < B; b += 4) {
+    const int64_t t = stok[b];
+    const int p = spos[b];
+    const int64_t r = ((int64_t)i * B + b) * a.width;
+    embed_row<VEC>(t >= 0 && t < a.tokens ? t : 0, min(max(p, 0), a.positions - 1), a.emb, a.ptab, a.w0, a.b0, a.eps0, a.w1,
+                   a.b1, a.eps1, a.x + r, a.h + r, a.width, lane);
+  }
+}
+
+bool al(const void* q, int n) { return (reinterpret_cast<uintptr_t>(q) & (n - 1)) == 0; }
+constexpr int64_t TOP = 0x7fffffff;
+
+}  // namespace
+
+extern "C" int64_t cohere_dec_beam_select_work(int64_t rows, int64_t V, int64_t beams) {
+  if (rows <= 0 || V <= 0 || beams < 1 || beams > MAXB) return 0;
+  return rows * select_parts(rows, V) * part_bytes((int)beams);
+}
+
+extern "C" int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V,
+                                      const int32_t* groups, int64_t slots, const float* score, const uint8_t* finished,
+                                      const int32_t* made, const float* norm, int64_t norm_len, int64_t pad,
+                                      int32_t* parent, int64_t* token, float* total, void* work, int64_t work_bytes,
+                                      void* stream) {
+  cohere::clear_error();
+  COHERE_REQUIRE(n >= 0 && beams >= 1 && beams <= MAXB && n * beams <= 65535 && slots > 0 && slots * beams <= TOP,
+                 "dec_beam_select: 1 to 16 beams, at most 65535 rows");
+  COHERE_REQUIRE(V >= beams && V % 8 == 0 && V < (int64_t(1) << 30) && ld >= V && ld % 8 == 0 && pad >= 0 && pad < V,
+                 "dec_beam_select: a vocabulary of at least `beams`, a multiple of 8, rows 16 bytes aligned, pad in it");
+  COHERE_REQUIRE(logits && groups && score && finished && parent && token && total && al(logits, 16),
+                 "dec_beam_select: bad pointer");
+  COHERE_REQUIRE(!norm || (made && norm_len > 0 && norm_len <= TOP), "dec_beam_select: norm needs made");
+  if (n == 0) return 0;
+  COHERE_REQUIRE(work && al(work, 8) && work_bytes >= cohere_dec_beam_select_work(n * beams, V, beams),
+                 "dec_beam_select: work of dec_beam_select_work bytes");
+  const int64_t rows = n * beams;
+  const SelectArgs a{logits, ld, groups, score, finished, made, norm, parent, token, total, static_cast<char*>(work),
+                     (int)n, (int)slots, (int)beams, (int)V, (int)norm_len, (int)pad, (int)select_parts(rows, V)};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)a.parts, (unsigned)rows);
+  if (select_j(rows, V) == 4) beam_parts_kernel<4><<<grid, 256, 0, s>>>(a);
+  else beam_parts_kernel<1><<<grid, 256, 0, s>>>(a);
+  beam_merge_kernel<<<(unsigned)n, 256, 0, s>>>(a);
+  return cohere::check_launch("dec_beam_select");
+}
+
+extern "C" int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
+                                       const int32_t* n, const uint8_t* done, int64_t slots, int32_t* table, int64_t width,
+                                       int64_t* tokens, int64_t OUT, int32_t* states, int64_t n_states, void* k, void* v,
+                                       float* ks, float* vs, int64_t L, int64_t pages, int64_t kv_heads, int64_t P,
+                                       int32_t bits, void* stream) {
+  cohere::clear_error();
+  int shift = -1;
+  for (int i = 0; i <= 8; ++i)
+    if (P == (int64_t(1) << i)) shift = i;
+  COHERE_REQUIRE(n_groups >= 0 && n_groups <= 65535 && beams >= 1 && beams <= MAXB && slots > 0 && slots * beams <= TOP,
+                 "dec_beam_reorder: 1 to 16 beams, at most 65535 groups");
+  COHERE_REQUIRE(groups && parent && n, "dec_beam_reorder: bad pointer");
+  COHERE_REQUIRE((!tokens || (OUT > 0 && OUT <= TOP)) && (!states || (n_states > 0 && n_states <= TOP)),
+                 "dec_beam_reorder: bad sizes");
+  COHERE_REQUIRE(!table || (width > 0 && width <= TOP && shift >= 0),
+                 "dec_beam_reorder: pages of a power of two up to 256 positions");
+  COHERE_REQUIRE(!k == !v && (!k || (table && (bits == 16 || bits == 8) && L > 0 && pages > 0 && pages <= TOP &&
+                                     kv_heads > 0 && al(k, 16) && al(v, 16) && (bits == 16 || (ks && vs)))),
+                 "dec_beam_reorder: pages in 16 or 8 bits (with scales) need a table");
+  if (n_groups == 0) return 0;
+  const int bytes = bits == 16 ? 256 : 128;
+  // a page of one position is never in part filled
+  COHERE_REQUIRE(!k || kv_heads <= TOP / (2 * 256 * 16) / L, "dec_beam_reorder: too many layers and heads");
+  const int64_t chunks = k && shift > 0 ? L * 2 * kv_heads * P * (bytes / 16) : 0, blocks = 1 + (chunks + 255) / 256;
+  const ReorderArgs a{groups, parent, n, done, table, tokens, states, static_cast<char*>(k), static_cast<char*>(v),
+                      bits == 8 ? ks : nullptr, bits == 8 ? vs : nullptr, (int)slots, (int)beams, (int)width, (int)OUT,
+                      (int)n_states, (int)L, (int)pages, shift < 0 ? 0 : shift, (int)kv_heads, bytes,
+                      (uint32_t)chunks};
+  const dim3 grid((unsigned)blocks, (unsigned)n_groups);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (beams <= 4) beam_reorder_kernel<4><<<grid, 256, 0, s>>>(a);
+  else if (beams <= 8) beam_reorder_kernel<8><<<grid, 256, 0, s>>>(a);
+  else beam_reorder_kernel<16><<<grid, 256, 0, s>>>(a);
+  return cohere::check_launch("dec_beam_reorder");
+}
+
+extern "C" int cohere_dec_beam_advance(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
+                                       const int64_t* token, const float* total, int64_t slots, int64_t dummy, int64_t* tok,
+                                       int32_t* pos, float* score, uint8_t* finished, int32_t* made, uint8_t* done,
+                                       const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos, int32_t by_length,
+                                       const uint16_t* emb, int64_t vocabulary, const uint16_t* ptab, int64_t positions,
+                                       const uint16_t* w0, const uint16_t* b0, float eps0, const uint16_t* w1,
+                                       const uint16_t* b1, float eps1, uint16_t* x, uint16_t* h, int64_t width,
+                                       uint8_t* flags_host, void* stream) {
+  cohere::clear_error();
+  COHERE_REQUIRE(n_groups >= 0 && n_groups <= TOP && beams >= 1 && beams <= MAXB && slots > 0 && slots * beams <= TOP &&
+                     OUT > 0 && OUT <= TOP,
+                 "dec_beam_advance: bad sizes (1 to 16 beams)");
+  COHERE_REQUIRE(groups && parent && token && total && tok && pos && score && finished && made && done && limit && out,
+                 "dec_beam_advance: bad pointer");
+  COHERE_REQUIRE(width > 0 && width % 8 == 0 && width <= 2048 && vocabulary > 0 && vocabulary <= TOP && positions > 0 &&
+                     positions <= TOP,
+                 "dec_beam_advance: width must be a multiple of 8, at most 2048");
+  COHERE_REQUIRE(emb && ptab && w0 && b0 && w1 && b1 && x && h && al(emb, 16) && al(ptab, 16) && al(x, 16) && al(h, 16) &&
+                     al(w0, 16) && al(b0, 16) && al(w1, 16) && al(b1, 16),
+                 "dec_beam_advance: bad embedding pointer");
+  uint8_t* flags = nullptr;
+  if (flags_host) {
+    void* d = nullptr;
+    COHERE_REQUIRE(hipHostGetDevicePointer(&d, flags_host, 0) == hipSuccess && d,
+                   "dec_beam_advance: the end flags must be pinned host memory");
+    flags = static_cast<uint8_t*>(d);
+  }
+  if (n_groups == 0) return 0;
+  const AdvanceArgs a{groups, parent, token, total, tok, pos, score, finished, done, flags, made, limit, out, eos,
+                      (int)slots, (int)beams, (int)OUT, (int)dummy, by_length, emb, ptab, w0, b0, w1, b1, eps0, eps1, x, h,
+                      (int)width, (int)vocabulary, (int)positions};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define ADVANCE(V) beam_advance_kernel<V><<<(unsigned)n_groups, 256, 0, s>>>(a)
+  switch ((width + 511) / 512) {
+    case 1: ADVANCE(1); break;
+    case 2: ADVANCE(2); break;
+    case 3: ADVANCE(3); break;
+    default: ADVANCE(4); break;
+  }
+#undef ADVANCE
+  return cohere::check_launch("dec_beam_advance");
+}

@@ -27,26 +27,6 @@ constexpr int HD = 128;  // head size
 
 // ---- embedding and residual LayerNorms: one wave per row ------------------------------------------------------------
 
-// one row's embedding by one wave: x = LN0(bf16(emb[t] + ptab[p])), h = LN1(x)
-// FULL: width == VEC * 512 (the loads then need no per-lane guard)
-template <int VEC, bool FULL = false>
-DEVI void embed_row(int64_t t, int p, const uint16_t* emb, const uint16_t* ptab, const uint16_t* w0,
-                    const uint16_t* b0, float eps0, const uint16_t* w1, const uint16_t* b1, float eps1, uint16_t* xr,
-                    uint16_t* hr, int width, int lane) {
-  const LnParams<VEC> p0 = load_ln<VEC, FULL>(w0, b0, width, lane), p1 = load_ln<VEC, FULL>(w1, b1, width, lane);
-  Row<VEC> e, q;
-  load_row<VEC, FULL>(emb + t * width, width, lane, e);
-  load_row<VEC, FULL>(ptab + (int64_t)p * width, width, lane, q);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) e.v[i][k] = round_bf(e.v[i][k] + q.v[i][k]);
-  ln_row<VEC>(e, width, lane, p0, eps0);
-  store_row<VEC>(e, width, lane, xr);
-  ln_row<VEC>(e, width, lane, p1, eps1);
-  store_row<VEC>(e, width, lane, hr);
-}
-
 template <int VEC>
 __global__ void __launch_bounds__(256) dec_embed_kernel(const int32_t* __restrict__ active,
                                                         const int64_t* __restrict__ tok, const int32_t* __restrict__ pos,

@@ -1,0 +1,152 @@
+// Caches in pages, as the kernels over them share it (dec_paged.hip, dec_paged_chunk.hip).
+//
+// Pages (pages, KV, P, 128), P a power of two up to 256; position t of slot s is in page table[s][t / P] at t % P. A
+// table entry outside 0 .. pages - 1 is an absent page: its positions are neither read nor written. 16 bits: bf16. 8 bits:
+// int8 codes with an fp32 scale per vector (pages, KV, P): s = max(m / 127, 2^-126), m the vector's largest magnitude,
+// code round_half_even(x fp32(1 / s)); a vector with a NaN or an infinity has a scale that is not finite and reads back as
+// NaN throughout.
+#pragma once
+#include "common.h"
+
+#include <type_traits>
+
+namespace cohere_paged {
+
+constexpr int HD = 128;  // head size
+constexpr float LOG2E = 1.4426950408889634f;
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+struct PagedArgs {
+  const int32_t *active, *starts;  // starts null: sequence i is row i
+  const uint16_t* q;               // (rows, ldq): H query heads, then KV keys, KV values of the new tokens
+  int64_t ldq;
+  void *k, *v;     // bf16 or int8 pages
+  float *ks, *vs;  // int8: scales
+  const int32_t *table, *n;
+  int R, S, slots, W, pages, shift, H, KV, ratio;  // rows, sequences, table width, log2 P
+  float scale;  // times log2(e): scores are powers of two
+  uint16_t* out;  // (rows, H * 128)
+  float* part;    // (rows, H, parts, 130) when split: outputs, maximum (power of two), sum
+  int parts;
+};
+
+DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// One workgroup's sequence and tile of TM query rows (x = token * ratio + head of the key head's): sequence i has the
+// tiles base(i) .. , base(i) = floor(starts[i] ratio / TM) + i, which leaves each at least the tiles that it needs, so that
+// neither the host nor a prefix sum has to know the chunks. Tiles without rows end at once.
+struct Tile {
+  int first, c, slot, x0, rows;  // first row, tokens; -1: none
+  bool ok;                       // the slot is in range
+};
+template <int TM>
+DEVI Tile tile_of(const PagedArgs& p, int w) {
+  Tile t;
+  int i = w;
+  t.x0 = 0;
+  if (p.starts) {
+    const int lane = lane_id();
+    int count = 0;
+    for (int i0 = 0; i0 < p.S; i0 += 64) {
+      const int at = i0 + lane;
+      const int64_t a = at < p.S ? min(max(p.starts[at], 0), p.R) : 0;
+      count += __popcll(__ballot(at < p.S && a * p.ratio / TM + at <= w));
+    }
+    i = count - 1;
+    if (i < 0) {
+      t.rows = 0;
+      return t;
+    }
+    const int a = min(max(p.starts[i], 0), p.R), b = min(max(p.starts[i + 1], a), p.R);
+    t.first = a;
+    t.c = b - a;
+    t.x0 = (w - ((int)((int64_t)a * p.ratio / TM) + i)) * TM;
+  } else {
+    const int tiles = (p.ratio + TM - 1) / TM;
+    i = w / tiles;
+    t.x0 = (w - i * tiles) * TM;
+    t.first = i;
+    t.c = 1;
+  }
+  const int64_t left = (int64_t)t.c * p.ratio - t.x0;
+  t.rows = left < TM ? (left > 0 ? (int)left : 0) : TM;
+  t.slot = p.active[i];
+  t.ok = (unsigned)t.slot < (unsigned)p.slots;
+  t.slot = t.ok ? t.slot : 0;
+  return t;
+}
+
+// the number of tiles that a grid has to have (the kernel's own: R ratio / TM + S, one a sequence and TM heads without starts)
+inline int64_t tiles_for(int64_t R, int64_t S, int64_t ratio, int64_t TM, bool starts) {
+  return starts ? R * ratio / TM + S : S * ((ratio + TM - 1) / TM);
+}
+
+// the largest magnitude of the 16 lanes' values as bits (a NaN's are above any number's)
+DEVI uint32_t row16_max_bits(uint32_t m) {
+  const auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  const auto mv = [](uint32_t v, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+  };
+  m = mx(m, mv(m, std::integral_constant<int, DPP_XOR1>{}));
+  m = mx(m, mv(m, std::integral_constant<int, DPP_XOR2>{}));
+  m = mx(m, mv(m, std::integral_constant<int, DPP_ROR4>{}));
+  return mx(m, mv(m, std::integral_constant<int, DPP_ROR8>{}));
+}
+
+DEVI void unpack8(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[2 * k] = __uint_as_float(w[k] << 16);
+    f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
+}
+
+// a vector (16 lanes, 8 values each, u) as it is held, at vector `vec` of the pages; every lane takes part, `live` writes
+template <bool Q8>
+DEVI void store_vec(const uint4& u, void* pages, float* scales, int64_t vec, int d8, bool live) {
+  if constexpr (!Q8) {
+    if (live) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + vec * HD + d8 * 8) = u;
+  } else {
+    float f[8];
+    unpack8(u, f);
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t b = __float_as_uint(f[k]) & 0x7fffffffu;
+      m = b > m ? b : m;
+    }
+    // (the bits of the largest magnitude, not fmaxf, which passes over a NaN)
+    const float mx = __uint_as_float(row16_max_bits(m)), d = mx / 127.f;
+    const float s = d < 0x1p-126f ? 0x1p-126f : d, inv = 1.f / s;
+    if (!live) return;
+    *reinterpret_cast<uint2*>(static_cast<int8_t*>(pages) + vec * HD + d8 * 8) =
+        make_uint2(q8x4(f[0], f[1], f[2], f[3], inv), q8x4(f[4], f[5], f[6], f[7], inv));
+    // an infinity's scale would read back its vector's zeros as NaN and the others as infinite or NaN: all NaN
+    if (d8 == 0) scales[vec] = mx < __uint_as_float(0x7f800000u) ? s : __uint_as_float(0x7fc00000u);
+  }
+}
+
+// The keys and values of the tile's own tokens (those whose first query row is in the tile) into their pages, by W waves.
+// No workgroup reads them there in the same launch: a chunk attends to its own tokens as given.
+template <bool Q8, int W>
+DEVI void append(const PagedArgs& p, const Tile& t, int n, int kvh, int TMrows) {
+  const int lane = lane_id(), wave = wave_id(), d8 = lane & 15;
+  const int j0 = (t.x0 + p.ratio - 1) / p.ratio, j1 = min(t.c, (t.x0 + TMrows + p.ratio - 1) / p.ratio);
+  const int P = 1 << p.shift;
+  for (int i = wave * 4; i < (j1 - j0) * 2; i += W * 4) {
+    const int at = i + (lane >> 4), j = j0 + (at >> 1), kvi = at & 1;
+    bool live = j < j1;
+    const int64_t pos = (int64_t)n + j;
+    const int64_t col = pos >> p.shift;
+    live = live && col < p.W;
+    const int page = live ? p.table[(int64_t)t.slot * p.W + col] : -1;
+    live = live && (unsigned)page < (unsigned)p.pages;
+    const int64_t vec = live ? (((int64_t)page * p.KV + kvh) << p.shift) + (pos & (P - 1)) : 0;
+    const uint4 u = *reinterpret_cast<const uint4*>(p.q + (int64_t)(t.first + min(j, t.c - 1)) * p.ldq +
+                                                    (p.H + kvi * p.KV + kvh) * HD + d8 * 8);
+    store_vec<Q8>(u, kvi ? p.v : p.k, kvi ? p.vs : p.ks, vec, d8, live);
+  }
+}
+
+}  // namespace cohere_paged

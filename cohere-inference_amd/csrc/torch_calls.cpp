@@ -1,4 +1,4 @@
-// The entry points over 4-bit caches and on logits as Python functions of torch tensors: the argument checks in C++,
+// The entry points over 4-bit caches and pages, on logits and of beam search as Python functions of torch tensors: the argument checks in C++,
 // because in Python they take longer than the launch (a lone call 8.6 us of host time; here 4, what a launch alone takes)
 // and these calls are made once per layer and step. Bound to the C ABI's functions by address (bind), so that the
 // library is the one that kernels/cuda_ext.py loaded. A refused call raises RuntimeError.
@@ -20,6 +20,13 @@ decltype(&cohere_dec_scatter_kv_q4) f_scatter;
 decltype(&cohere_dec_gather_kv_q4) f_gather;
 decltype(&cohere_gemm_kv_q4) f_gemm_kv;
 decltype(&cohere_dec_logits) f_logits;
+decltype(&cohere_dec_attention_paged) f_paged;
+decltype(&cohere_dec_attention_paged_q8) f_paged_q8;
+decltype(&cohere_dec_gather_paged) f_gather_paged;
+decltype(&cohere_dec_gather_paged_q8) f_gather_paged_q8;
+decltype(&cohere_dec_beam_select) f_select;
+decltype(&cohere_dec_beam_reorder) f_reorder;
+decltype(&cohere_dec_beam_advance) f_advance;
 decltype(&cohere_last_error) f_error;
 PyObject *get_device, *get_stream;  // torch._C's
 
@@ -261,6 +268,198 @@ void logits(const Call& c) {
   });
 }
 
+// pages (.., pages, KV, P, 128) with `lead` sizes before them, in 8 bits with scales
+struct Pages {
+  const Tensor &k, &v;
+  const Tensor *ks = nullptr, *vs = nullptr;
+  int64_t L, pages, KV, P;
+  Pages(const Call& c, int at, int lead, bool q8) : k(c.tensor(at)), v(c.tensor(at + 1)) {
+    c.need(k.dim() == lead + 4 && k.size(lead + 3) == 128 && v.sizes() == k.sizes() && k.is_contiguous() &&
+               v.is_contiguous() && k.scalar_type() == (q8 ? at::kChar : at::kBFloat16) &&
+               v.scalar_type() == k.scalar_type(),
+           q8 ? "contiguous int8 pages (.., pages, KV, P, 128)" : "contiguous bf16 pages (.., pages, KV, P, 128)");
+    c.need(k.numel() > 0, "no pages");
+    L = lead ? k.size(0) : 1; pages = k.size(lead); KV = k.size(lead + 1); P = k.size(lead + 2);
+    if (q8) {
+      ks = &c.tensor(at + 2);
+      vs = &c.tensor(at + 3);
+      c.need(ks->sizes() == k.sizes().slice(0, lead + 3) && vs->sizes() == ks->sizes() &&
+                 ks->scalar_type() == at::kFloat && vs->scalar_type() == at::kFloat && ks->is_contiguous() &&
+                 vs->is_contiguous(),
+             "contiguous fp32 scales, one a vector");
+    }
+  }
+};
+
+bool table_ok(const Call& c, const Tensor& t) { return t.dim() == 2 && t.size(0) > 0 && t.size(1) > 0 && c.index(t, 1); }
+
+template <bool Q8>
+void attention_paged(const Call& c) {
+  constexpr int Z = Q8 ? 2 : 0;
+  const Tensor &active = c.tensor(0), &q = c.tensor(2), &table = c.tensor(5 + Z), &n = c.tensor(6 + Z),
+               &out = c.tensor(10 + Z);
+  const Tensor *starts = c.maybe(1), *part = c.maybe(9 + Z);
+  const Pages kv(c, 3, 0, Q8);
+  const double scale = c.number(7 + Z);
+  const int64_t splits = c.whole(8 + Z);
+  c.need(q.dim() == 2 && out.dim() == 2 && q.scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16 &&
+             q.stride(1) == 1 && out.is_contiguous(),
+         "bf16 q (rows, ...) with unit column stride, contiguous out");
+  const int64_t rows = q.size(0), H = out.size(1) / 128, seqs = active.numel();
+  c.need(out.size(0) == rows && H > 0 && out.size(1) % 128 == 0 && H % kv.KV == 0 && q.size(1) >= (H + 2 * kv.KV) * 128,
+         "out (rows, H * 128), H a multiple of the key heads, q as wide as its heads");
+  c.need(table_ok(c, table) && c.index(active, seqs) && c.index(n, table.size(0)),
+         "int32 table (slots, pages), active per sequence, n per slot");
+  c.need(starts ? c.index(*starts, seqs + 1) : rows == seqs, "int32 starts (sequences + 1), or a row per sequence");
+  c.need(splits >= 1 && splits <= 64 && (splits == 1 || (part && part->scalar_type() == at::kFloat &&
+                                                        part->is_contiguous() &&
+                                                        part->numel() / 130 / splits >= rows * H)),
+         "1 to 64 splits, more than 1 need part");
+  if (rows == 0 || seqs == 0) return;
+  void* st = c.stream(q, &active, starts, &kv.k, &kv.v, kv.ks, kv.vs, &table, &n, part, &out);
+  launch([&] {
+    if constexpr (Q8)
+      return f_paged_q8(ptr<int32_t>(active), ptr<int32_t>(starts), seqs, ptr<uint16_t>(q), q.stride(0), rows,
+                        ptr<int8_t>(kv.k), ptr<int8_t>(kv.v), ptr<float>(kv.ks), ptr<float>(kv.vs), kv.pages, kv.P,
+                        ptr<int32_t>(table), table.size(1), ptr<int32_t>(n), table.size(0), H, kv.KV, (float)scale,
+                        splits, ptr<float>(part), part ? part->numel() : 0, ptr<uint16_t>(out), st);
+    else
+      return f_paged(ptr<int32_t>(active), ptr<int32_t>(starts), seqs, ptr<uint16_t>(q), q.stride(0), rows,
+                     ptr<uint16_t>(kv.k), ptr<uint16_t>(kv.v), kv.pages, kv.P, ptr<int32_t>(table), table.size(1),
+                     ptr<int32_t>(n), table.size(0), H, kv.KV, (float)scale, splits, ptr<float>(part),
+                     part ? part->numel() : 0, ptr<uint16_t>(out), st);
+  });
+}
+
+template <bool Q8>
+void gather_paged(const Call& c) {
+  const Tensor &slot_of = c.tensor(0), &pos_of = c.tensor(1), &table = c.tensor(2), &kv = c.tensor(Q8 ? 7 : 5);
+  const Pages p(c, 3, 1, Q8);
+  c.need(kv.dim() == 2 && kv.scalar_type() == at::kBFloat16 && kv.size(1) == p.L * 2 * p.KV * 128 && kv.stride(1) == 1,
+         "bf16 kv (rows, L * 2 * KV * 128) with unit column stride");
+  const int64_t rows = kv.size(0);
+  c.need(table_ok(c, table) && c.index(slot_of, rows) && c.index(pos_of, rows),
+         "int32 table (slots, pages), slot and position per row");
+  if (rows == 0) return;
+  void* st = c.stream(kv, &slot_of, &pos_of, &table, &p.k, &p.v, p.ks, p.vs);
+  launch([&] {
+    if constexpr (Q8)
+      return f_gather_paged_q8(ptr<int32_t>(slot_of), ptr<int32_t>(pos_of), rows, ptr<int32_t>(table), table.size(0),
+                               table.size(1), ptr<int8_t>(p.k), ptr<int8_t>(p.v), ptr<float>(p.ks), ptr<float>(p.vs), p.L,
+                               p.pages, p.KV, p.P, ptr<uint16_t>(kv), kv.stride(0), st);
+    else
+      return f_gather_paged(ptr<int32_t>(slot_of), ptr<int32_t>(pos_of), rows, ptr<int32_t>(table), table.size(0),
+                            table.size(1), ptr<uint16_t>(p.k), ptr<uint16_t>(p.v), p.L, p.pages, p.KV, p.P,
+                            ptr<uint16_t>(kv), kv.stride(0), st);
+  });
+}
+
+// a contiguous matrix (or vector, w < 0) of at least `rows` rows of one type
+bool matrix(const Tensor& t, at::ScalarType type, int64_t rows, int64_t w) {
+  return t.scalar_type() == type && t.is_contiguous() &&
+         (w < 0 ? t.dim() == 1 && t.size(0) >= rows : t.dim() == 2 && t.size(0) >= rows && t.size(1) == w);
+}
+
+void beam_select(const Call& c) {
+  const Tensor &logits = c.tensor(0), &groups = c.tensor(1), &score = c.tensor(2), &finished = c.tensor(3),
+               &parent = c.tensor(7), &token = c.tensor(8), &total = c.tensor(9), &work = c.tensor(10);
+  const Tensor *made = c.maybe(4), *norm = c.maybe(5);
+  const int64_t pad = c.whole(6), n = groups.numel();
+  c.need(score.dim() == 2 && score.size(0) > 0 && score.size(1) >= 1 && score.size(1) <= 16, "score (groups, 1 to 16 beams)");
+  const int64_t G = score.size(0), B = score.size(1);
+  c.need(logits.dim() == 2 && logits.scalar_type() == at::kBFloat16 && logits.size(0) == n * B && logits.stride(1) == 1,
+         "bf16 logits (groups * beams, V) with unit column stride");
+  c.need(c.index(groups, n) && matrix(score, at::kFloat, G, B) && matrix(finished, at::kByte, G, B),
+         "int32 groups, contiguous fp32 score and uint8 finished (groups, beams)");
+  c.need(!norm || (made && matrix(*made, at::kInt, G, B) && matrix(*norm, at::kFloat, 1, -1)),
+         "fp32 norm needs int32 made (groups, beams)");
+  c.need(matrix(parent, at::kInt, n, B) && matrix(token, at::kLong, n, B) && matrix(total, at::kFloat, n, B),
+         "int32 parent, int64 token, fp32 total (groups, beams)");
+  c.need(work.scalar_type() == at::kByte && work.is_contiguous(), "contiguous uint8 work");
+  if (n == 0) return;
+  void* st = c.stream(logits, &groups, &score, &finished, made, norm, &parent, &token, &total, &work);
+  launch([&] {
+    return f_select(ptr<uint16_t>(logits), logits.stride(0), n, B, logits.size(1), ptr<int32_t>(groups), G,
+                    ptr<float>(score), ptr<uint8_t>(finished), ptr<int32_t>(made), ptr<float>(norm),
+                    norm ? norm->numel() : 0, pad, ptr<int32_t>(parent), ptr<int64_t>(token), ptr<float>(total),
+                    work.data_ptr(), work.numel(), st);
+  });
+}
+
+void beam_reorder(const Call& c) {
+  const Tensor &groups = c.tensor(0), &parent = c.tensor(1), &n = c.tensor(2);
+  const Tensor *done = c.maybe(3), *table = c.maybe(4), *tokens = c.maybe(5), *states = c.maybe(6), *k = c.maybe(7),
+               *ks = c.maybe(9);
+  const int64_t m = groups.numel();
+  c.need(parent.dim() == 2 && parent.size(1) >= 1 && parent.size(1) <= 16, "parent (groups, 1 to 16 beams)");
+  const int64_t B = parent.size(1), slots = n.numel(), G = slots / B;
+  c.need(c.index(groups, m) && matrix(parent, at::kInt, m, B) && c.index(n, 1) && slots % B == 0,
+         "int32 groups, parent (groups, beams), n per slot (groups * beams)");
+  c.need(!done || matrix(*done, at::kByte, G, -1), "uint8 done per group");
+  c.need(!table || (table_ok(c, *table) && table->size(0) >= slots), "int32 table (slots, pages)");
+  c.need(!tokens || (tokens->dim() == 2 && tokens->size(1) > 0 && matrix(*tokens, at::kLong, slots, tokens->size(1))),
+         "contiguous int64 tokens (slots, positions)");
+  c.need(!states || (states->dim() == 2 && states->size(1) > 0 && matrix(*states, at::kInt, slots, states->size(1))),
+         "contiguous int32 states (slots, ..)");
+  c.need(!k || table, "pages need a table");
+  const Tensor* v = c.maybe(8);
+  const Tensor* vs = c.maybe(10);
+  c.need(!k == !v && !ks == !vs && (k || !ks), "keys and values, or neither");
+  int64_t L = 0, pages = 0, KV = 0, P = 1;
+  if (k) {
+    const Pages p(c, 7, 1, ks != nullptr);
+    L = p.L; pages = p.pages; KV = p.KV; P = p.P;
+  }
+  if (m == 0) return;
+  void* st = c.stream(groups, &parent, &n, done, table, tokens, states, k, v, ks, vs);
+  launch([&] {
+    return f_reorder(ptr<int32_t>(groups), m, B, ptr<int32_t>(parent), ptr<int32_t>(n), ptr<uint8_t>(done), G,
+                     ptr<int32_t>(table), table ? table->size(1) : 0, ptr<int64_t>(tokens), tokens ? tokens->size(1) : 0,
+                     ptr<int32_t>(states), states ? states->size(1) : 0, k ? k->data_ptr() : nullptr,
+                     v ? v->data_ptr() : nullptr, ptr<float>(ks), ptr<float>(vs), L, pages, KV, P, ks ? 8 : 16, st);
+  });
+}
+
+void beam_advance(const Call& c) {
+  const Tensor &groups = c.tensor(0), &parent = c.tensor(1), &token = c.tensor(2), &total = c.tensor(3), &tok = c.tensor(5),
+               &pos = c.tensor(6), &score = c.tensor(7), &finished = c.tensor(8), &made = c.tensor(9), &done = c.tensor(10),
+               &limit = c.tensor(11), &out = c.tensor(12), &emb = c.tensor(15), &ptab = c.tensor(16), &w0 = c.tensor(17),
+               &b0 = c.tensor(18), &w1 = c.tensor(20), &b1 = c.tensor(21), &x = c.tensor(23), &h = c.tensor(24);
+  const Tensor* flags = c.maybe(25);
+  const int64_t dummy = c.whole(4), eos = c.whole(13), n = groups.numel();
+  const bool by_length = c.truth(14);
+  const double eps0 = c.number(19), eps1 = c.number(22);
+  c.need(score.dim() == 2 && score.size(0) > 0 && score.size(1) >= 1 && score.size(1) <= 16, "score (groups, 1 to 16 beams)");
+  const int64_t G = score.size(0), B = score.size(1);
+  c.need(c.index(groups, n) && matrix(parent, at::kInt, n, B) && matrix(token, at::kLong, n, B) &&
+             matrix(total, at::kFloat, n, B),
+         "int32 groups and parent, int64 token, fp32 total (groups, beams)");
+  c.need(matrix(tok, at::kLong, G * B, -1) && matrix(pos, at::kInt, G * B, -1) && matrix(score, at::kFloat, G, B) &&
+             matrix(finished, at::kByte, G, B) && matrix(made, at::kInt, G, B) && matrix(done, at::kByte, G, -1) &&
+             matrix(limit, at::kInt, G, -1) && out.dim() == 2 && out.size(1) > 0 &&
+             matrix(out, at::kLong, G * B, out.size(1)),
+         "the groups' state: tok, pos, out per slot, score, finished, made (groups, beams), done, limit per group");
+  c.need(emb.dim() == 2 && ptab.dim() == 2 && emb.size(1) == ptab.size(1) && emb.size(0) > 0 && ptab.size(0) > 0, "emb, ptab");
+  const int64_t w = emb.size(1);
+  c.need(matrix(emb, at::kBFloat16, 1, w) && matrix(ptab, at::kBFloat16, 1, w) && matrix(w0, at::kBFloat16, w, -1) &&
+             matrix(b0, at::kBFloat16, w, -1) && matrix(w1, at::kBFloat16, w, -1) && matrix(b1, at::kBFloat16, w, -1) &&
+             matrix(x, at::kBFloat16, n * B, w) && matrix(h, at::kBFloat16, n * B, w),
+         "contiguous bf16 emb, ptab, norms, x, h of one width");
+  c.need(!flags || (flags->scalar_type() == at::kByte && flags->is_contiguous() && flags->numel() >= G && flags->is_cpu()),
+         "flags: pinned uint8 per group");
+  if (n == 0) return;
+  void* st = c.stream(groups, &parent, &token, &total, &tok, &pos, &score, &finished, &made, &done, &limit, &out, &emb,
+                      &ptab, &w0, &b0, &w1, &b1, &x, &h);
+  launch([&] {
+    return f_advance(ptr<int32_t>(groups), n, B, ptr<int32_t>(parent), ptr<int64_t>(token), ptr<float>(total), G, dummy,
+                     ptr<int64_t>(tok), ptr<int32_t>(pos), ptr<float>(score), ptr<uint8_t>(finished), ptr<int32_t>(made),
+                     ptr<uint8_t>(done), ptr<int32_t>(limit), ptr<int64_t>(out), out.size(1), eos, by_length,
+                     ptr<uint16_t>(emb), emb.size(0), ptr<uint16_t>(ptab), ptab.size(0), ptr<uint16_t>(w0),
+                     ptr<uint16_t>(b0), (float)eps0, ptr<uint16_t>(w1), ptr<uint16_t>(b1), (float)eps1, ptr<uint16_t>(x),
+                     ptr<uint16_t>(h), w, ptr<uint8_t>(flags), st);
+  });
+}
+
 // no C++ exception leaves a function that Python calls
 template <void (*F)(const Call&), int N>
 PyObject* entry(const char* name, PyObject* const* args, Py_ssize_t n) {
@@ -286,6 +485,15 @@ ENTRY("dec_scatter_kv_q4", scatter, 7)
 ENTRY("dec_gather_kv_q4", gather, 7)
 ENTRY("gemm_kv_q4", gemm_kv, 9)
 ENTRY("dec_logits", logits, 15)
+constexpr auto paged = attention_paged<false>, paged_q8 = attention_paged<true>, gather_pages = gather_paged<false>,
+               gather_pages_q8 = gather_paged<true>;
+ENTRY("dec_attention_paged", paged, 11)
+ENTRY("dec_attention_paged_q8", paged_q8, 13)
+ENTRY("dec_gather_paged", gather_pages, 6)
+ENTRY("dec_gather_paged_q8", gather_pages_q8, 8)
+ENTRY("dec_beam_select", beam_select, 11)
+ENTRY("dec_beam_reorder", beam_reorder, 11)
+ENTRY("dec_beam_advance", beam_advance, 26)
 
 // bind(addresses): the C ABI's functions by name
 PyObject* bind(PyObject*, PyObject* addresses) {
@@ -302,6 +510,13 @@ PyObject* bind(PyObject*, PyObject* addresses) {
   at("cohere_dec_gather_kv_q4", f_gather);
   at("cohere_gemm_kv_q4", f_gemm_kv);
   at("cohere_dec_logits", f_logits);
+  at("cohere_dec_attention_paged", f_paged);
+  at("cohere_dec_attention_paged_q8", f_paged_q8);
+  at("cohere_dec_gather_paged", f_gather_paged);
+  at("cohere_dec_gather_paged_q8", f_gather_paged_q8);
+  at("cohere_dec_beam_select", f_select);
+  at("cohere_dec_beam_reorder", f_reorder);
+  at("cohere_dec_beam_advance", f_advance);
   PyObject* c = PyImport_ImportModule("torch._C");
   if (c) {
     get_device = PyObject_GetAttrString(c, "_cuda_getDevice");
@@ -320,6 +535,13 @@ PyMethodDef methods[] = {METHOD("dec_attention_q4", attention),
                          METHOD("dec_gather_kv_q4", gather),
                          METHOD("gemm_kv_q4", gemm_kv),
                          METHOD("dec_logits", logits),
+                         METHOD("dec_attention_paged", paged),
+                         METHOD("dec_attention_paged_q8", paged_q8),
+                         METHOD("dec_gather_paged", gather_pages),
+                         METHOD("dec_gather_paged_q8", gather_pages_q8),
+                         METHOD("dec_beam_select", beam_select),
+                         METHOD("dec_beam_reorder", beam_reorder),
+                         METHOD("dec_beam_advance", beam_advance),
                          {"bind", bind, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "cohere_calls", "Calls of the C ABI with torch tensors.", -1, methods};

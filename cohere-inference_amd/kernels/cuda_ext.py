@@ -43,7 +43,10 @@ EXPORTS = ("cohere_gemm_i8", "cohere_gemm_sp", "cohere_quantize_rows", "cohere_l
            "cohere_gemm_sp_tiled", "cohere_pack_24_tiled_bytes", "cohere_pack_24_tiled", "cohere_sub_conv0_dw_pw",
            "cohere_sub_dw_pw", "cohere_gemm_kv", "cohere_gemm_kv_q8", "cohere_gemm_tile",
            "cohere_piece_rows", "cohere_dec_attention_q4", "cohere_dec_attention_q4_splits", "cohere_dec_scatter_kv_q4",
-           "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4", "cohere_dec_logits")
+           "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4", "cohere_dec_logits", "cohere_dec_attention_paged",
+           "cohere_dec_attention_paged_q8", "cohere_dec_attention_paged_splits", "cohere_dec_gather_paged",
+           "cohere_dec_gather_paged_q8", "cohere_dec_beam_select", "cohere_dec_beam_select_work",
+           "cohere_dec_beam_reorder", "cohere_dec_beam_advance")
 
 
 def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
@@ -79,6 +82,17 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "cohere_dec_gather_kv_q4": [P, P, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
         "cohere_dec_logits": [P, I64, P, I64, I64, I64, P, P, I64, P, I64, P, P, P, P, I64, P, P, I64, P, P, I64, P, P,
                               P],
+        "cohere_dec_attention_paged": [P, P, I64, P, I64, I64, P, P, I64, I64, P, I64, P, I64, I64, I64, F, I64, P, I64, P,
+                                       P],
+        "cohere_dec_attention_paged_q8": [P, P, I64, P, I64, I64, P, P, P, P, I64, I64, P, I64, P, I64, I64, I64, F, I64,
+                                          P, I64, P, P],
+        "cohere_dec_gather_paged": [P, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, P],
+        "cohere_dec_gather_paged_q8": [P, P, I64, P, I64, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
+        "cohere_dec_beam_select": [P, I64, I64, I64, I64, P, I64, P, P, P, P, I64, I64, P, P, P, P, I64, P],
+        "cohere_dec_beam_reorder": [P, I64, I64, P, P, P, I64, P, I64, P, I64, P, I64, P, P, P, P, I64, I64, I64, I64, I32,
+                                    P],
+        "cohere_dec_beam_advance": [P, I64, I64, P, P, P, I64, I64, P, P, P, P, P, P, P, P, I64, I64, I32, P, I64, P, I64,
+                                    P, P, F, P, P, F, P, P, I64, P, P],
         "cohere_dec_pick": [P, I64, I64, P, I64, P, P, P, P, I64, P, P, P, I64, I64, I64, P],
         "cohere_dec_pick_embed": [P, I64, I64, P, I64, P, P, P, P, I64, P, P, P, I64, I64, I64, P, P, P, P, F, P, P, F,
                                   P, P, I64, P, P],
@@ -109,6 +123,10 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.cohere_encoder_branch_workspace_bytes.restype = I64
     lib.cohere_dec_attention_q4_splits.argtypes = [I64, I64, I64, I64]
     lib.cohere_dec_attention_q4_splits.restype = I64
+    lib.cohere_dec_attention_paged_splits.argtypes = [I64, I64, I64, I64, I64]
+    lib.cohere_dec_attention_paged_splits.restype = I64
+    lib.cohere_dec_beam_select_work.argtypes = [I64, I64, I64]
+    lib.cohere_dec_beam_select_work.restype = I64
     lib.cohere_logmel_workspace_bytes.argtypes = [I64]
     lib.cohere_logmel_workspace_bytes.restype = I64
     lib.cohere_last_error.restype = ctypes.c_char_p
@@ -129,7 +147,9 @@ def _ptr(t: torch.Tensor | None):
 
 # the functions that csrc/torch_calls.cpp calls with torch tensors
 CALLS = ("cohere_dec_attention_q4", "cohere_dec_scatter_kv_q4", "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4",
-         "cohere_dec_logits", "cohere_last_error")
+         "cohere_dec_logits", "cohere_dec_attention_paged", "cohere_dec_attention_paged_q8", "cohere_dec_gather_paged",
+         "cohere_dec_gather_paged_q8", "cohere_dec_beam_select", "cohere_dec_beam_reorder", "cohere_dec_beam_advance",
+         "cohere_last_error")
 
 
 def load_calls(lib: ctypes.CDLL, path: str = os.path.join(_PKG, "lib", "cohere_calls.so")):
@@ -693,6 +713,70 @@ class _Ext:
         prompt (plen). Absent rules are None; index values out of range switch a rule off for a slot."""
         _calls.dec_logits(logits, y, active, pos, tokens, first, plen, penalties, bias, bias_of, mask, classes, trans,
                           start, state)
+
+    # ---- caches in pages, beam search (no counterpart in the reference; arguments checked in torch_calls.cpp) ---------
+    #
+    # Pages (pages, KV, P, 128) of P positions (a power of two up to 256), bf16, or int8 with fp32 scales (pages, KV, P);
+    # position t of a slot is in page table[slot, t // P] (int32) at t % P; entries out of range (-1) are absent pages.
+
+    def dec_attention_paged_splits(self, rows, seqs, heads, kv_heads, T) -> int:
+        """The `splits` that fill the GPU in a dec_attention_paged call of these sizes over up to T positions a slot."""
+        return int(self._lib.cohere_dec_attention_paged_splits(int(rows), int(seqs), int(heads), int(kv_heads), int(T)))
+
+    def dec_attention_paged(self, active, starts, q, k, v, table, n, scale, splits, part, out):
+        """Attention of a chunk of new tokens per sequence over bf16 pages. Sequence i is slot active[i] with n[slot]
+        positions held; its rows are starts[i]..starts[i + 1] - 1 (int32; None: row i alone). q (rows, (H + 2 KV) 128)
+        holds the new tokens' queries, keys and values, out (rows, H 128) bf16, H / KV query heads to a key head. Row j
+        of a sequence attends to the positions held and to the chunk's rows 0..j as given; the chunk is appended at
+        positions n[slot].. (n is left to the caller). Slots out of range or with n < 0 get zeros; rows outside
+        starts[0]..starts[-1] - 1 are left as they were. A slot, and a page that is appended to, belong to one sequence
+        of the call. splits > 1 needs part (rows x H x splits x 130 floats, of one call at a time); out must not overlap
+        q."""
+        _calls.dec_attention_paged(active, starts, q, k, v, table, n, scale, splits, part, out)
+
+    def dec_attention_paged_q8(self, active, starts, q, k, v, ks, vs, table, n, scale, splits, part, out):
+        """dec_attention_paged over int8 pages with scales ks, vs: the positions held are read as code x scale, the
+        chunk is attended as given and appended with scale max(m / 127, 2^-126) of a vector's largest magnitude m."""
+        _calls.dec_attention_paged_q8(active, starts, q, k, v, ks, vs, table, n, scale, splits, part, out)
+
+    def dec_gather_paged(self, slot_of, pos_of, table, k, v, kv):
+        """What the pages of all layers (L, pages, KV, P, 128) hold of (slot, position) pairs, as bf16 rows (rows, L 2 KV
+        128) laid out as dec_scatter_kv takes them (to move a request out of its pages, or to look at it); zeros for
+        slots or positions out of range and for absent pages."""
+        _calls.dec_gather_paged(slot_of, pos_of, table, k, v, kv)
+
+    def dec_gather_paged_q8(self, slot_of, pos_of, table, k, v, ks, vs, kv):
+        """dec_gather_paged from int8 pages with scales ks, vs (L, pages, KV, P)."""
+        _calls.dec_gather_paged_q8(slot_of, pos_of, table, k, v, ks, vs, kv)
+
+    def dec_beam_select_work(self, rows, V, beams) -> int:
+        """Bytes of dec_beam_select's workspace."""
+        return int(self._lib.cohere_dec_beam_select_work(int(rows), int(V), int(beams)))
+
+    def dec_beam_select(self, logits, groups, score, finished, made, norm, pad, parent, token, total, work):
+        """The best continuations over a group's beams and the vocabulary: logits bf16 (n B, V), row i B + b beam b of
+        group groups[i]; score fp32, finished uint8 and made int32 (groups, B). Candidates (b, v) have score + log
+        softmax(l)[v]; a finished beam has pad alone, with its score. Ranked by total x norm[tokens made] (norm fp32; made
+        and norm None: by total), the lowest b V + v first where equal. parent int32, token int64, total fp32 (n, B): the
+        B best, best first. work: uint8 of dec_beam_select_work(n B, V, B) bytes, of one call at a time."""
+        _calls.dec_beam_select(logits, groups, score, finished, made, norm, pad, parent, token, total, work)
+
+    def dec_beam_reorder(self, groups, parent, n, done, table, tokens, states, k, v, ks, vs):
+        """Every beam takes over its parent's history in place (slots: group x B + beam): table entries of full pages,
+        tokens int64 (slots, OUT) 0..n - 1, states int32 (slots, NS), and the positions of the page in part filled, in all
+        layers (k, v (L, pages, KV, P, 128), scales (L, pages, KV, P) in 8 bits), copied into the beam's own page. n int32
+        (slots): positions held, the same for a group's beams. done uint8 (groups): left as they are. done, table, tokens,
+        states, pages (with table: of one position then) and scales may be None. A group is named once."""
+        _calls.dec_beam_reorder(groups, parent, n, done, table, tokens, states, k, v, ks, vs)
+
+    def dec_beam_advance(self, groups, parent, token, total, dummy, tok, pos, score, finished, made, done, limit, out, eos,
+                         by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags):
+        """The chosen tokens into the groups' state, behind dec_beam_reorder, and the next step's embeddings (as
+        dec_embed) into x, h (n B, width): tok int64, pos int32 (slots), score fp32, finished uint8, made int32 (groups, B),
+        out int64 (slots, OUT), done uint8 and limit int32 (groups); flags: pinned uint8 (groups) or None. A group is done
+        once all its beams have finished, once the best has (by_length False), or at pos >= limit."""
+        _calls.dec_beam_advance(groups, parent, token, total, dummy, tok, pos, score, finished, made, done, limit, out,
+                                eos, by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags)
 
 
 _lib = load_library()

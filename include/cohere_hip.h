@@ -315,6 +315,94 @@ int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, 
                       const int32_t* bias_of, const int32_t* mask, int64_t M, const int32_t* classes,
                       const int32_t* trans, int64_t C, const int32_t* start, int32_t* state, void* stream);
 
+/* ---- caches in pages, beam search (no counterpart in the reference) -------------------------------------------------
+ * Pages (pages, kv_heads, P, 128) of P positions, P a power of two up to 256; position t of slot s is in page
+ * table[s][t / P] (int32 [slots, width]) at t % P. An entry outside 0 .. pages - 1 is an absent page; a position in one,
+ * or at width * P or behind it, is neither read nor written. 16 bits: bf16. 8 bits: int8 codes with an fp32 scale per
+ * 128-vector (pages, kv_heads, P): with m its largest magnitude s = max(fp32(m / 127), 2^-126), code
+ * round_half_even(x * fp32(1 / s)), the value held code * s; a vector with a NaN or an infinity is NaN throughout.
+ * width * P <= 2^30; offsets into the pages are 64 bits wide. 16-byte aligned pages, rows and outputs. */
+
+/* Attention of a chunk of new tokens per sequence. Sequence i (0 .. seqs - 1) is slot s = active[i] with n[s] positions
+ * held; its rows of q and out are starts[i] .. starts[i + 1] - 1 (int32 [seqs + 1], ascending, within 0 .. rows; starts
+ * null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq] holds heads x 128 queries, then
+ * kv_heads x 128 keys, then the values; query head h reads key head h / (heads / kv_heads). Row j of a sequence, position
+ * n[s] + j, attends to positions 0 .. n[s] - 1 as the pages hold them and to rows 0 .. j of its sequence as given, whose
+ * keys and values are appended at positions n[s] ..: out = softmax(q k^T scale) v, bf16 [rows, heads * 128]. Rows of a
+ * slot out of range, or with n[s] < 0, get zeros, and nothing is appended. Rows in front of starts[0] or from
+ * starts[seqs] on are left as they were. A page that is appended to belongs to one sequence of the call, and so does its
+ * slot; full pages may be shared by any number. What a row does not attend to never shows in it, NaN and infinities
+ * included. out must not overlap q. splits (1 .. 64) divides the keys over workgroups and needs part with rows x heads x
+ * splits x 130 floats, of one call at a time. fp32 sums and weights; calls with many rows per sequence hold the weights
+ * in bf16 for the product with the values. */
+int cohere_dec_attention_paged(const int32_t* active, const int32_t* starts, int64_t seqs, const uint16_t* q, int64_t ldq,
+                               int64_t rows, uint16_t* k, uint16_t* v, int64_t pages, int64_t P, const int32_t* table,
+                               int64_t width, const int32_t* n, int64_t slots, int64_t heads, int64_t kv_heads,
+                               float scale, int64_t splits, float* part, int64_t part_len, uint16_t* out, void* stream);
+int cohere_dec_attention_paged_q8(const int32_t* active, const int32_t* starts, int64_t seqs, const uint16_t* q,
+                                  int64_t ldq, int64_t rows, int8_t* k, int8_t* v, float* ks, float* vs, int64_t pages,
+                                  int64_t P, const int32_t* table, int64_t width, const int32_t* n, int64_t slots,
+                                  int64_t heads, int64_t kv_heads, float scale, int64_t splits, float* part,
+                                  int64_t part_len, uint16_t* out, void* stream);
+
+/* The number of splits that fills the GPU for such a call over up to T positions (1 for sizes that it would refuse). */
+int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t T);
+
+/* What the pages of all layers, k, v (L, pages, kv_heads, P, 128) and scales (L, pages, kv_heads, P), hold of position
+ * pos_of[i] of slot slot_of[i], rounded to bf16, into row i of kv [rows, ldkv] (per layer kv_heads keys, then the values,
+ * as cohere_dec_scatter_kv takes it); zeros for a slot or position out of range and for absent pages. */
+int cohere_dec_gather_paged(const int32_t* slot_of, const int32_t* pos_of, int64_t rows, const int32_t* table,
+                            int64_t slots, int64_t width, const uint16_t* k, const uint16_t* v, int64_t L, int64_t pages,
+                            int64_t kv_heads, int64_t P, uint16_t* kv, int64_t ldkv, void* stream);
+int cohere_dec_gather_paged_q8(const int32_t* slot_of, const int32_t* pos_of, int64_t rows, const int32_t* table,
+                               int64_t slots, int64_t width, const int8_t* k, const int8_t* v, const float* ks,
+                               const float* vs, int64_t L, int64_t pages, int64_t kv_heads, int64_t P, uint16_t* kv,
+                               int64_t ldkv, void* stream);
+
+/* The best continuations of n groups of beams (1 .. 16) hypotheses. Group slot g = groups[i] has score fp32 [slots,
+ * beams] (-inf or finite), finished uint8 [slots, beams] and, for norm, made int32 [slots, beams]; row i * beams + b of
+ * logits bf16 [n * beams, ld] is its beam b. Candidates (b, v): total = score[g][b] + l[v] - max l - log sum exp(l -
+ * max l), NaN logits counted as -inf (a row of nothing else gives -inf), infinite ones as the largest finite number; a
+ * finished beam has total = score[g][b] for v = pad and -inf for the others. Ranked by total * norm[min(made[g][b] +
+ * (finished ? 0 : 1), norm_len - 1)] (norm fp32, positive; null: by total), in 64 bits, then by the lowest b * V + v; a
+ * NaN counts as -inf. The best `beams` of them, best first, into row i of parent int32, token int64 and total fp32 [n,
+ * beams]. A group out of range gets parents 0 .., tokens pad and totals -inf. V % 8 == 0, V >= beams, 0 <= pad < V, n *
+ * beams <= 65535. work: cohere_dec_beam_select_work(n * beams, V, beams) bytes, 8-byte aligned, of one call at a time. */
+int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V, const int32_t* groups,
+                           int64_t slots, const float* score, const uint8_t* finished, const int32_t* made,
+                           const float* norm, int64_t norm_len, int64_t pad, int32_t* parent, int64_t* token, float* total,
+                           void* work, int64_t work_bytes, void* stream);
+int64_t cohere_dec_beam_select_work(int64_t rows, int64_t V, int64_t beams);
+
+/* Every beam takes over its parent's history, in place: row b of group g = groups[i] (slot g * beams + b) gets of row
+ * parent[i][b] (as they were before the call; a parent outside 0 .. beams - 1 leaves its row as it is) the table entries
+ * of full pages, 0 .. n / P - 1, with n = n[g * beams] positions held by each of the group's rows, the tokens (int64
+ * [slots * beams, OUT]) 0 .. n - 1 and the states (int32 [slots * beams, n_states]); and in all layers the first n % P
+ * positions of page table[..][n / P] are copied into its own page there, whose entry stays. The pages in part filled
+ * belong to one row each. slots counts the groups. Groups out of range, and those with done[g] != 0 (uint8 [slots], null:
+ * none), are left as they are; a group is named once. table, tokens, states, k and v may be null (absent). bits: 16, or 8
+ * with scales ks, vs. */
+int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
+                            const int32_t* n, const uint8_t* done, int64_t slots, int32_t* table, int64_t width,
+                            int64_t* tokens, int64_t OUT, int32_t* states, int64_t n_states, void* k, void* v, float* ks,
+                            float* vs, int64_t L, int64_t pages, int64_t kv_heads, int64_t P, int32_t bits, void* stream);
+
+/* The chosen tokens into the groups' state (what cohere_dec_pick_embed does for the greedy choice): for beam b of group g
+ * = groups[i], slot r = g * beams + b, with q = parent[i][b], t = token[i][b]: finished[r] = finished[q's] or t == eos or
+ * total[i][b] is not above -inf; made[r] = made[q's] + (finished[q's] ? 0 : 1); score[r] = total[i][b]; pos[r] += 1;
+ * out[r][pos[r]] = tok[r] = t. done[g] = 1 (and flags_host[g], pinned host memory, may be null) once all beams have
+ * finished, once the best has and by_length is 0, and at pos >= limit[g]. The group dummy, and groups that are done, keep
+ * their state. Then x, h [n_groups * beams, width] get the embedding of tok at pos, as cohere_dec_embed (emb [vocabulary,
+ * width], ptab [positions, width]; indexes out of range are brought into it). A group is named once (the dummy any
+ * number of times). */
+int cohere_dec_beam_advance(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
+                            const int64_t* token, const float* total, int64_t slots, int64_t dummy, int64_t* tok,
+                            int32_t* pos, float* score, uint8_t* finished, int32_t* made, uint8_t* done,
+                            const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos, int32_t by_length,
+                            const uint16_t* emb, int64_t vocabulary, const uint16_t* ptab, int64_t positions,
+                            const uint16_t* w0, const uint16_t* b0, float eps0, const uint16_t* w1, const uint16_t* b1,
+                            float eps1, uint16_t* x, uint16_t* h, int64_t width, uint8_t* flags_host, void* stream);
+
 /* Number of per-layer tensors of cohere_encoder_layers: the reference's 53 (its enum F,
  * kernels/csrc/encoder_loop.cpp:34-44) followed by 4 of this library's own (the feed-forwards' first linears in 2:4
  * form: ff1 kept bytes, ff1 selectors, ff2 kept bytes, ff2 selectors; NULL keeps the dense first linear, as the
