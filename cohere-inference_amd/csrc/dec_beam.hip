@@ -392,7 +392,7 @@ struct AdvanceArgs {
   const int64_t* token;
   const float* total;
   int64_t* tok;
-  int32_t* pos;
+  int32_t *pos, *held;
   float* score;
   uint8_t *finished, *done, *flags;
   int32_t* made;
@@ -437,6 +437,7 @@ __global__ void __launch_bounds__(256) beam_advance_kernel(const AdvanceArgs a) 
         a.score[slot0 + b] = total;
         a.tok[slot0 + b] = t;
         a.pos[slot0 + b] = p;
+        if (a.held) a.held[slot0 + b] = p + 1;
         if (p < a.OUT) a.out[(slot0 + b) * a.OUT + p] = t;
         if (lane == 0 && end) {
           a.done[g] = 1;
@@ -534,8 +535,8 @@ extern "C" int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, 
 
 extern "C" int cohere_dec_beam_advance(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
                                        const int64_t* token, const float* total, int64_t slots, int64_t dummy, int64_t* tok,
-                                       int32_t* pos, float* score, uint8_t* finished, int32_t* made, uint8_t* done,
-                                       const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos, int32_t by_length,
+                                       int32_t* pos, int32_t* held, float* score, uint8_t* finished,
+                                       int32_t* made, uint8_t* done, const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos, int32_t by_length,
                                        const uint16_t* emb, int64_t vocabulary, const uint16_t* ptab, int64_t positions,
                                        const uint16_t* w0, const uint16_t* b0, float eps0, const uint16_t* w1,
                                        const uint16_t* b1, float eps1, uint16_t* x, uint16_t* h, int64_t width,
@@ -560,7 +561,7 @@ extern "C" int cohere_dec_beam_advance(const int32_t* groups, int64_t n_groups, 
     flags = static_cast<uint8_t*>(d);
   }
   if (n_groups == 0) return 0;
-  const AdvanceArgs a{groups, parent, token, total, tok, pos, score, finished, done, flags, made, limit, out, eos,
+  const AdvanceArgs a{groups, parent, token, total, tok, pos, held, score, finished, done, flags, made, limit, out, eos,
                       (int)slots, (int)beams, (int)OUT, (int)dummy, by_length, emb, ptab, w0, b0, w1, b1, eps0, eps1, x, h,
                       (int)width, (int)vocabulary, (int)positions};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -422,19 +422,20 @@ void beam_reorder(const Call& c) {
 
 void beam_advance(const Call& c) {
   const Tensor &groups = c.tensor(0), &parent = c.tensor(1), &token = c.tensor(2), &total = c.tensor(3), &tok = c.tensor(5),
-               &pos = c.tensor(6), &score = c.tensor(7), &finished = c.tensor(8), &made = c.tensor(9), &done = c.tensor(10),
-               &limit = c.tensor(11), &out = c.tensor(12), &emb = c.tensor(15), &ptab = c.tensor(16), &w0 = c.tensor(17),
-               &b0 = c.tensor(18), &w1 = c.tensor(20), &b1 = c.tensor(21), &x = c.tensor(23), &h = c.tensor(24);
-  const Tensor* flags = c.maybe(25);
-  const int64_t dummy = c.whole(4), eos = c.whole(13), n = groups.numel();
-  const bool by_length = c.truth(14);
-  const double eps0 = c.number(19), eps1 = c.number(22);
+               &pos = c.tensor(6), &score = c.tensor(8), &finished = c.tensor(9), &made = c.tensor(10), &done = c.tensor(11),
+               &limit = c.tensor(12), &out = c.tensor(13), &emb = c.tensor(16), &ptab = c.tensor(17), &w0 = c.tensor(18),
+               &b0 = c.tensor(19), &w1 = c.tensor(21), &b1 = c.tensor(22), &x = c.tensor(24), &h = c.tensor(25);
+  const Tensor *held = c.maybe(7), *flags = c.maybe(26);
+  const int64_t dummy = c.whole(4), eos = c.whole(14), n = groups.numel();
+  const bool by_length = c.truth(15);
+  const double eps0 = c.number(20), eps1 = c.number(23);
   c.need(score.dim() == 2 && score.size(0) > 0 && score.size(1) >= 1 && score.size(1) <= 16, "score (groups, 1 to 16 beams)");
   const int64_t G = score.size(0), B = score.size(1);
   c.need(c.index(groups, n) && matrix(parent, at::kInt, n, B) && matrix(token, at::kLong, n, B) &&
              matrix(total, at::kFloat, n, B),
          "int32 groups and parent, int64 token, fp32 total (groups, beams)");
-  c.need(matrix(tok, at::kLong, G * B, -1) && matrix(pos, at::kInt, G * B, -1) && matrix(score, at::kFloat, G, B) &&
+  c.need(matrix(tok, at::kLong, G * B, -1) && matrix(pos, at::kInt, G * B, -1) &&
+             (!held || matrix(*held, at::kInt, G * B, -1)) && matrix(score, at::kFloat, G, B) &&
              matrix(finished, at::kByte, G, B) && matrix(made, at::kInt, G, B) && matrix(done, at::kByte, G, -1) &&
              matrix(limit, at::kInt, G, -1) && out.dim() == 2 && out.size(1) > 0 &&
              matrix(out, at::kLong, G * B, out.size(1)),
@@ -448,11 +449,11 @@ void beam_advance(const Call& c) {
   c.need(!flags || (flags->scalar_type() == at::kByte && flags->is_contiguous() && flags->numel() >= G && flags->is_cpu()),
          "flags: pinned uint8 per group");
   if (n == 0) return;
-  void* st = c.stream(groups, &parent, &token, &total, &tok, &pos, &score, &finished, &made, &done, &limit, &out, &emb,
+  void* st = c.stream(groups, &parent, &token, &total, &tok, &pos, held, &score, &finished, &made, &done, &limit, &out, &emb,
                       &ptab, &w0, &b0, &w1, &b1, &x, &h);
   launch([&] {
     return f_advance(ptr<int32_t>(groups), n, B, ptr<int32_t>(parent), ptr<int64_t>(token), ptr<float>(total), G, dummy,
-                     ptr<int64_t>(tok), ptr<int32_t>(pos), ptr<float>(score), ptr<uint8_t>(finished), ptr<int32_t>(made),
+                     ptr<int64_t>(tok), ptr<int32_t>(pos), ptr<int32_t>(held), ptr<float>(score), ptr<uint8_t>(finished), ptr<int32_t>(made),
                      ptr<uint8_t>(done), ptr<int32_t>(limit), ptr<int64_t>(out), out.size(1), eos, by_length,
                      ptr<uint16_t>(emb), emb.size(0), ptr<uint16_t>(ptab), ptab.size(0), ptr<uint16_t>(w0),
                      ptr<uint16_t>(b0), (float)eps0, ptr<uint16_t>(w1), ptr<uint16_t>(b1), (float)eps1, ptr<uint16_t>(x),
@@ -493,7 +494,7 @@ ENTRY("dec_gather_paged", gather_pages, 6)
 ENTRY("dec_gather_paged_q8", gather_pages_q8, 8)
 ENTRY("dec_beam_select", beam_select, 11)
 ENTRY("dec_beam_reorder", beam_reorder, 11)
-ENTRY("dec_beam_advance", beam_advance, 26)
+ENTRY("dec_beam_advance", beam_advance, 27)
 
 // bind(addresses): the C ABI's functions by name
 PyObject* bind(PyObject*, PyObject* addresses) {

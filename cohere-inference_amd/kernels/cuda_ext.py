@@ -91,7 +91,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "cohere_dec_beam_select": [P, I64, I64, I64, I64, P, I64, P, P, P, P, I64, I64, P, P, P, P, I64, P],
         "cohere_dec_beam_reorder": [P, I64, I64, P, P, P, I64, P, I64, P, I64, P, I64, P, P, P, P, I64, I64, I64, I64, I32,
                                     P],
-        "cohere_dec_beam_advance": [P, I64, I64, P, P, P, I64, I64, P, P, P, P, P, P, P, P, I64, I64, I32, P, I64, P, I64,
+        "cohere_dec_beam_advance": [P, I64, I64, P, P, P, I64, I64, P, P, P, P, P, P, P, P, P, I64, I64, I32, P, I64, P, I64,
                                     P, P, F, P, P, F, P, P, I64, P, P],
         "cohere_dec_pick": [P, I64, I64, P, I64, P, P, P, P, I64, P, P, P, I64, I64, I64, P],
         "cohere_dec_pick_embed": [P, I64, I64, P, I64, P, P, P, P, I64, P, P, P, I64, I64, I64, P, P, P, P, F, P, P, F,
@@ -769,14 +769,14 @@ class _Ext:
         states, pages (with table: of one position then) and scales may be None. A group is named once."""
         _calls.dec_beam_reorder(groups, parent, n, done, table, tokens, states, k, v, ks, vs)
 
-    def dec_beam_advance(self, groups, parent, token, total, dummy, tok, pos, score, finished, made, done, limit, out, eos,
-                         by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags):
+    def dec_beam_advance(self, groups, parent, token, total, dummy, tok, pos, held, score, finished, made, done, limit, out,
+                         eos, by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags):
         """The chosen tokens into the groups' state, behind dec_beam_reorder, and the next step's embeddings (as
-        dec_embed) into x, h (n B, width): tok int64, pos int32 (slots), score fp32, finished uint8, made int32 (groups, B),
+        dec_embed) into x, h (n B, width): tok int64, pos, held int32 (slots; held None or pos + 1), score fp32, finished uint8, made int32 (groups, B),
         out int64 (slots, OUT), done uint8 and limit int32 (groups); flags: pinned uint8 (groups) or None. A group is done
         once all its beams have finished, once the best has (by_length False), or at pos >= limit."""
-        _calls.dec_beam_advance(groups, parent, token, total, dummy, tok, pos, score, finished, made, done, limit, out,
-                                eos, by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags)
+        _calls.dec_beam_advance(groups, parent, token, total, dummy, tok, pos, held, score, finished, made, done, limit,
+                                out, eos, by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags)
 
 
 _lib = load_library()

@@ -1,5 +1,6 @@
 """End-to-end transcription on gfx950: audio pieces -> log-mel features -> packed encoder -> cross-attention caches ->
-greedy decoding with continuous batching -> token ids (the call surface of the reference's kernels/pipeline.py).
+greedy decoding (or beam search) with continuous batching -> token ids (the call surface of the reference's
+kernels/pipeline.py).
 
 Two ways in, one decoding engine (_Decoding: the active slots, the pieces they hold, the steps in flight -- launched
 in chunks of the decoder's `chunk` steps while no piece waits, one graph replay each -- and the end flags read LAG
@@ -33,6 +34,7 @@ from concurrent.futures import Future
 import numpy as np
 import torch
 
+from kernels.beam_decoder import BeamDecoder
 from kernels.fast_encoder import FastEncoder
 from kernels.features import Features, dither
 from kernels.stream_decoder import Grammar, Rules, StreamDecoder
@@ -96,8 +98,8 @@ class _Decoding:
         for s, p in zip(slots, pieces):
             self.holder[s] = p
             self.first_step[s] = self.steps
-            # the pick ends a row at its step `plen - 1 + max_new` after admission, if no end token came first
-            self.limit[s] = len(p.prompt) - 1 + (p.max_new or dec.max_new_tokens)
+            # the step that ends the slot, if no end token comes first
+            self.limit[s] = dec.steps_to_limit(len(p.prompt), p.max_new or dec.max_new_tokens)
         self.active += slots
         self.stale = True
 
@@ -135,7 +137,7 @@ class _Decoding:
             self.stale = True
             with torch.cuda.stream(dec.stream):
                 for s in ended:
-                    self.rows_host[s].copy_(dec.out[s], non_blocking=True)
+                    self.rows_host[s].copy_(dec.tokens(s), non_blocking=True)
             dec.stream.synchronize()
             for s in ended:
                 p = self.holder.pop(s)
@@ -162,8 +164,9 @@ class Pipeline:
     kernels/pipeline.py:60-250, same constructor arguments and defaults; `extractor` may be None for the
     CohereAsrFeatureExtractor settings). Keyword-only extras: frames (encoder frames per decoder slot), buckets
     (decoder row buckets), chunk_frames (encoder frames per encoder call), sparse_w1 (both feed-forward linears 2:4),
-    kv_bits (bits of a cached value of the decoder: 16, 8 or 4), and what lets requests have Rules: penalties, bias (a
-    table of rows over the vocabulary), grammar (kernels.stream_decoder.Grammar)."""
+    kv_bits (bits of a cached value of the decoder: 16, 8 or 4), what lets requests have Rules: penalties, bias (a
+    table of rows over the vocabulary), grammar (kernels.stream_decoder.Grammar), and beams (above 1: beam search,
+    kernels.beam_decoder.BeamDecoder, with length_penalty and page; buckets then count pieces, kv_bits 16 or 8)."""
 
     CHUNK_FRAMES = 3000  # encoder frames per encoder call (reference pipeline.py:61)
     LAG = 1  # steps between a step's launch and the host reading its end flags (reference pipeline.py:64)
@@ -175,13 +178,18 @@ class Pipeline:
     def __init__(self, model, extractor=None, slots: int = 128, max_new_tokens: int = 448, int8: bool = False,
                  sparse: str | bool | None = None, *, frames: int | None = None, buckets=None,
                  chunk_frames: int | None = None, sparse_w1: bool = False, kv_bits: int | None = None,
-                 penalties: bool = False, bias: torch.Tensor | None = None, grammar: Grammar | None = None):
+                 penalties: bool = False, bias: torch.Tensor | None = None, grammar: Grammar | None = None,
+                 beams: int = 1, length_penalty: float = 0.0, page: int = 1):
         dev = model.proj_out.weight.device
         self.device = dev
         self.features = Features(extractor, device=dev)
         self.encoder = FastEncoder(model.model.encoder, int8=int8, sparse=sparse, sparse_w1=sparse_w1)
-        self.decoder = StreamDecoder(model, slots=slots, max_new_tokens=max_new_tokens, int8=int8, frames=frames,
-                                     buckets=buckets, kv_bits=kv_bits, penalties=penalties, bias=bias, grammar=grammar)
+        args = dict(slots=slots, max_new_tokens=max_new_tokens, int8=int8, frames=frames, buckets=buckets,
+                    kv_bits=kv_bits, penalties=penalties, bias=bias, grammar=grammar)
+        if beams == 1 and (length_penalty != 0.0 or page != 1):
+            raise ValueError("Pipeline: length_penalty and page need beams above 1")
+        self.decoder = StreamDecoder(model, **args) if beams == 1 else \
+            BeamDecoder(model, beams=beams, length_penalty=length_penalty, page=page, **args)
         if chunk_frames is not None:
             self.CHUNK_FRAMES = chunk_frames
         self.stats = {"steps": 0, "chunks": 0, "frames": 0}
@@ -228,7 +236,8 @@ class Pipeline:
     def transcribe(self, pieces: list, prompt: torch.Tensor, max_new: list[int] | None = None,
                    rules: Rules | None = None) -> list[np.ndarray]:
         """Token ids (prompt + generated, up to and including the end token) of each dithered piece (numpy fp32
-        samples or fp32 tensors on the GPU), greedy under the rules (None: none), in the caller's thread."""
+        samples or fp32 tensors on the GPU), greedy (or the best beam's) under the rules (None: none), in the caller's
+        thread."""
         if self._threads:
             raise RuntimeError("Pipeline: transcribe() cannot run beside the submit() threads")
         dec = self.decoder

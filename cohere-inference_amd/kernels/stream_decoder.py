@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import dataclasses
 import math
+import types
 
 import numpy as np
 import torch
@@ -222,6 +223,7 @@ class StreamDecoder:
     Rules; any of them puts one launch (ext.dec_logits) between the head and the pick of every step."""
 
     BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 112, 128)
+    beams = 1  # rows of a slot
 
     def __init__(self, model, slots: int = 128, max_new_tokens: int = 448, max_prompt: int = 16,
                  max_audio_s: float = 36.0, buckets=None, int8: bool = False, frames: int | None = None,
@@ -269,33 +271,22 @@ class StreamDecoder:
 
         # caches: (layer, slot, head, position, 128), in 8 bits int8 with one fp32 scale per 128-vector, in 4 bits 64
         # bytes of codes with four bf16 maxima
-        L, S1 = len(self.blocks), slots + 1
-        kv_dtype, kv_width = {16: (self.embed.dtype, self.d), 8: (torch.int8, self.d),
-                              4: (torch.uint8, self.d // 2)}[self.kv_bits]
+        S1, S1B = slots + 1, (slots + 1) * self.beams
+        self._self_caches()
+        self.cross_k, self.cross_ks = self._cache(S1, frames)
+        self.cross_v, self.cross_vs = self._cache(S1, frames)
 
-        def cache(t):
-            return torch.zeros(L, S1, self.h, t, kv_width, device=dev, dtype=kv_dtype)
-
-        def scales(t):
-            if self.kv_bits == 4:
-                return torch.zeros(L, S1, self.h, t, 4, device=dev, dtype=torch.bfloat16)
-            return torch.ones(L, S1, self.h, t, device=dev, dtype=torch.float32) if self.kv_bits == 8 else None
-
-        self.self_k, self.self_v, self.self_ks, self.self_vs = cache(self.seq), cache(self.seq), scales(self.seq), \
-            scales(self.seq)
-        self.cross_k, self.cross_v, self.cross_ks, self.cross_vs = cache(frames), cache(frames), scales(frames), \
-            scales(frames)
-
-        # slot state (row `slots` is the dummy, never advanced)
+        # slot state (row `slots` is the dummy, never advanced); with beams, what each of a slot's beams has of its own
+        # is held for slot * beams + beam
         i32, i64 = dict(device=dev, dtype=torch.int32), dict(device=dev, dtype=torch.long)
-        self.tok = torch.full((S1,), self.pad, **i64)
-        self.pos = torch.zeros(S1, **i32)
-        self.plen = torch.ones(S1, **i32)
+        self.tok = torch.full((S1B,), self.pad, **i64)
+        self.pos = torch.zeros(S1B, **i32)
+        self.plen = torch.ones(S1B, **i32)
         self.limit = torch.zeros(S1, **i32)
         self.cross_len = torch.ones(S1, **i32)
         self.finished = torch.ones(S1, device=dev, dtype=torch.uint8)
         self.forced = torch.full((S1, max_prompt), self.pad, **i64)
-        self.out = torch.full((S1, self.seq + 1), self.pad, **i64)
+        self.out = torch.full((S1B, self.seq + 1), self.pad, **i64)
         self.flags = torch.ones(S1, dtype=torch.uint8).pin_memory()  # `finished`, copied out by every step
 
         # rules on the choice (kernel arguments of ext.dec_logits; None: absent)
@@ -305,27 +296,27 @@ class StreamDecoder:
         if grammar is not None and grammar.classes.numel() != self.head.n:
             raise ValueError(f"StreamDecoder: a grammar over {self.head.n} tokens (got {grammar.classes.numel()})")
         self.bias = None if bias is None else bias.to(device=dev, dtype=torch.bfloat16).contiguous()
-        self.bias_of = None if bias is None else torch.full((S1,), -1, **i32)
+        self.bias_of = None if bias is None else torch.full((S1B,), -1, **i32)
         self.first = self.pen = self.mask = self.classes = self.trans = self.start = self.gstate = None
         if penalties:
-            self.first = torch.zeros(S1, **i32)
-            self.pen = torch.tensor([1.0, 0.0, 0.0], device=dev).repeat(S1, 1)
+            self.first = torch.zeros(S1B, **i32)
+            self.pen = torch.tensor([1.0, 0.0, 0.0], device=dev).repeat(S1B, 1)
         if grammar is not None:
             self.mask, self.classes, self.trans = (t.to(dev) for t in (grammar.mask, grammar.classes,
                                                                        grammar.transitions))
-            self.start, self.gstate = torch.full((S1,), -1, **i32), torch.full((S1, 2), -1, **i32)
+            self.start, self.gstate = torch.full((S1B,), -1, **i32), torch.full((S1B, 2), -1, **i32)
 
         # step buffers, sized for the largest bucket
-        bm, bf = self.buckets[-1], dict(device=dev, dtype=self.embed.dtype)
-        self.active = torch.full((bm,), self.dummy, **i32)
+        bm, bf = self.buckets[-1] * self.beams, dict(device=dev, dtype=self.embed.dtype)
+        self.active = self._idle_rows()
         self.x, self.hn, self.att = (torch.zeros(bm, self.width, **bf) for _ in range(3))
         self.qkv_out = torch.zeros(bm, 3 * self.width, **bf)
         self.q_out = torch.zeros(bm, self.width, **bf)
         self.proj_out = torch.zeros(bm, self.width, **bf)
         self.ffn_out = torch.zeros(bm, self.blocks[0].fc1.n, **bf)
         self.logits = torch.zeros(bm, self.head.n, **bf)
-        self.part = torch.empty(max(b * self.h * self._splits(b) * (self.d + 2) for b in self.buckets), device=dev,
-                                dtype=torch.float32)
+        self.part = torch.empty(max(b * self.beams * self.h * self._splits(b) * (self.d + 2) for b in self.buckets),
+                                device=dev, dtype=torch.float32)
 
         self.stream = torch.cuda.Stream(device=dev)
         self._embed_stale, self._embed_rows = True, 0
@@ -337,6 +328,24 @@ class StreamDecoder:
         self.chunk_graphs: dict[int, torch.cuda.CUDAGraph] = {}
         if capture:
             self._capture()
+
+    def _cache(self, slots: int, t: int):
+        """A cache of every layer and its scales (None in 16 bits): (layer, slot, head, position, ..), or pages."""
+        dims, dev = (len(self.blocks), slots, self.h, t), dict(device=self.device)
+        if self.kv_bits == 4:
+            return (torch.zeros(*dims, self.d // 2, dtype=torch.uint8, **dev),
+                    torch.zeros(*dims, 4, dtype=torch.bfloat16, **dev))
+        if self.kv_bits == 8:
+            return torch.zeros(*dims, self.d, dtype=torch.int8, **dev), torch.ones(*dims, dtype=torch.float32, **dev)
+        return torch.zeros(*dims, self.d, dtype=self.embed.dtype, **dev), None
+
+    def _self_caches(self) -> None:
+        self.self_k, self.self_ks = self._cache(self.slots + 1, self.seq)
+        self.self_v, self.self_vs = self._cache(self.slots + 1, self.seq)
+
+    def _idle_rows(self) -> torch.Tensor:
+        """The active rows of the largest bucket where no slot is active."""
+        return torch.full((self.buckets[-1],), self.dummy, device=self.device, dtype=torch.int32)
 
     @staticmethod
     def _splits(b: int) -> int:
@@ -367,51 +376,66 @@ class StreamDecoder:
         per layer self-attention (qkv, attention over the slot's cache, o, residual + LayerNorm), cross-attention (q,
         attention over the slot's frames, o, residual + LayerNorm) and feed-forward (fc1 + ReLU, fc2, residual + the
         next LayerNorm), then the head, the greedy pick and the end flags' copy to the host."""
-        act, x, hn, att = self.active[:b], self.x[:b], self.hn[:b], self.att[:b]
-        qkv, q, proj, ffn, logits = (t[:b] for t in (self.qkv_out, self.q_out, self.proj_out, self.ffn_out,
-                                                     self.logits))
+        act, bufs, logits = self.active[:b], self._buffers(b), self.logits[:b]
+        self_attn = [self._attention(i, True, act, bufs.qkv, 1, bufs.att) for i in range(len(self.blocks))]
+        cross = [self._attention(i, False, act, bufs.q, self._splits(b), bufs.att) for i in range(len(self.blocks))]
+        ops = self._layers(bufs, self_attn, cross) + self._head(bufs, logits) + self._rules(act, logits)
+        if self.fused:
+            # the pick computes the next step's embedding of its row and writes the end flags to the host itself. The
+            # same bits as the unfused step. The step's own embedding comes from the previous step's pick, or from
+            # step() when the rows changed.
+            return ops + [lambda: ext.dec_pick_embed(logits, act, self.dummy, self.tok, self.pos, self.finished,
+                                                     self.forced, self.plen, self.limit, self.out, self.pad, self.eos,
+                                                     self.embed, self.pos_table, *self.emb_ln, *self.blocks[0].norms[0],
+                                                     bufs.x, bufs.hn, self.flags)]
+        return [lambda: self._embed(b)] + ops + [
+            lambda: ext.dec_pick(logits, act, self.dummy, self.tok, self.pos, self.finished, self.forced, self.plen,
+                                 self.limit, self.out, self.pad, self.eos),
+            lambda: self.flags.copy_(self.finished, non_blocking=True)]
+
+    def _buffers(self, rows: int) -> types.SimpleNamespace:
+        """The step buffers of the first `rows` rows."""
+        return types.SimpleNamespace(x=self.x[:rows], hn=self.hn[:rows], att=self.att[:rows], qkv=self.qkv_out[:rows],
+                                     q=self.q_out[:rows], proj=self.proj_out[:rows], ffn=self.ffn_out[:rows])
+
+    def _layers(self, bufs, self_attn: list, cross: list) -> list:
+        """The layers' launches on rows whose embedding and first LayerNorm are in x, hn; self_attn and cross are each
+        layer's attention launches (qkv -> att, q -> att)."""
+        x, hn, att, qkv, q, proj, ffn = (bufs.x, bufs.hn, bufs.att, bufs.qkv, bufs.q, bufs.proj, bufs.ffn)
+        ops = []
         if self.fused:
             # the residual adds ride on o / cross-o / fc2's epilogues and the LayerNorms on the next projection's
-            # prologue (8 launches a layer instead of 11); the pick computes the next step's embedding of its row and
-            # writes the end flags to the host itself. The same bits as the unfused step. The step's own embedding
-            # comes from the previous step's pick, or from step() when the rows changed.
-            ops = []
+            # prologue (8 launches a layer instead of 11)
             for i, blk in enumerate(self.blocks):
-                first = i == 0
-                ops += [(lambda blk=blk: blk.qkv.fused(hn, qkv)) if first else
+                ops += [(lambda blk=blk: blk.qkv.fused(hn, qkv)) if i == 0 else
                         (lambda blk=blk: blk.qkv.fused(x, qkv, ln=blk.norms[0])),
-                        self._attention(i, True, act, qkv, 1, att),
+                        self_attn[i],
                         lambda blk=blk: blk.o.fused(att, x, DEC_EP_RESID),
                         lambda blk=blk: blk.cq.fused(x, q, ln=blk.norms[1]),
-                        self._attention(i, False, act, q, self._splits(b), att),
+                        cross[i],
                         lambda blk=blk: blk.co.fused(att, x, DEC_EP_RESID),
                         lambda blk=blk: blk.fc1.fused(x, ffn, DEC_EP_RELU, ln=blk.norms[2]),
                         lambda blk=blk: blk.fc2.fused(ffn, x, DEC_EP_RESID)]
-            ops += [lambda: self.head.fused(x, logits, ln=self.final_ln), *self._rules(act, logits),
-                    lambda: ext.dec_pick_embed(logits, act, self.dummy, self.tok, self.pos, self.finished, self.forced,
-                                               self.plen, self.limit, self.out, self.pad, self.eos, self.embed,
-                                               self.pos_table, *self.emb_ln, *self.blocks[0].norms[0], x, hn,
-                                               self.flags)]
             return ops
-        ops = [lambda: self._embed(b)]
         for i, blk in enumerate(self.blocks):
             after_ffn = self.blocks[i + 1].norms[0] if i + 1 < len(self.blocks) else self.final_ln
             ops += [lambda blk=blk: blk.qkv(hn, qkv),
-                    self._attention(i, True, act, qkv, 1, att),
+                    self_attn[i],
                     lambda blk=blk: blk.o(att, proj),
                     lambda blk=blk: ext.dec_add_ln(x, proj, *blk.norms[1], hn),
                     lambda blk=blk: blk.cq(hn, q),
-                    self._attention(i, False, act, q, self._splits(b), att),
+                    cross[i],
                     lambda blk=blk: blk.co(att, proj),
                     lambda blk=blk: ext.dec_add_ln(x, proj, *blk.norms[2], hn),
                     lambda blk=blk: blk.fc1(hn, ffn, relu=True),
                     lambda blk=blk: blk.fc2(ffn, proj),
                     lambda ln=after_ffn: ext.dec_add_ln(x, proj, *ln, hn)]
-        ops += [lambda: self.head(hn, logits), *self._rules(act, logits),
-                lambda: ext.dec_pick(logits, act, self.dummy, self.tok, self.pos, self.finished, self.forced,
-                                     self.plen, self.limit, self.out, self.pad, self.eos),
-                lambda: self.flags.copy_(self.finished, non_blocking=True)]
         return ops
+
+    def _head(self, bufs, logits) -> list:
+        if self.fused:
+            return [lambda: self.head.fused(bufs.x, logits, ln=self.final_ln)]
+        return [lambda: self.head(bufs.hn, logits)]
 
     def _rules(self, act, logits) -> list:
         """The requests' rules on the logits, in place (nothing where the decoder was built without any)."""
@@ -422,12 +446,18 @@ class StreamDecoder:
                                        self.gstate)]
 
     def _embed(self, b: int) -> None:
-        """The embedding and first LayerNorm of the first b active rows (x, hn), on the current stream."""
-        ext.dec_embed(self.active[:b], self.tok, self.pos, self.embed, self.pos_table, *self.emb_ln,
-                      *self.blocks[0].norms[0], self.x[:b], self.hn[:b])
+        """The embedding and first LayerNorm of the bucket's active rows (x, hn), on the current stream."""
+        rows = b * self.beams
+        ext.dec_embed(self.active[:rows], self.tok, self.pos, self.embed, self.pos_table, *self.emb_ln,
+                      *self.blocks[0].norms[0], self.x[:rows], self.hn[:rows])
+
+    @property
+    def _embeds_ahead(self) -> bool:
+        """Whether a step leaves the next step's embeddings (the program then begins behind them)."""
+        return self.fused
 
     def _run(self, b: int) -> None:
-        if self.fused:
+        if self._embeds_ahead:
             self._embed(b)
         for op in self.programs[b]:
             op()
@@ -531,17 +561,7 @@ class StreamDecoder:
             raise ValueError(f"StreamDecoder: {len(rules)} rules for {n} slots")
         for r in rules:
             self.check_rules(r)
-        forced = torch.full((n, self.max_prompt), self.pad, dtype=torch.long)
-        nums = torch.empty(n, 3, dtype=torch.int32)  # prompt length, position limit, frames
-        for i, p in enumerate(prompts):
-            p = torch.as_tensor(p, dtype=torch.long).flatten()
-            if not 1 <= len(p) <= self.max_prompt:
-                raise ValueError(f"StreamDecoder: a prompt of {len(p)} tokens (1..{self.max_prompt})")
-            if not 1 <= frames[i] <= self.frames:
-                raise ValueError(f"StreamDecoder: {frames[i]} encoder frames (1..{self.frames})")
-            forced[i, :len(p)] = p
-            nums[i] = torch.tensor([len(p), len(p) - 1 + (max_new[i] if max_new else self.max_new_tokens),
-                                    frames[i]])
+        forced, nums = self._requests(prompts, frames, max_new)
         out_rows = torch.full((n, self.seq + 1), self.pad, dtype=torch.long)
         out_rows[:, :self.max_prompt] = forced
         with torch.cuda.stream(self.stream):
@@ -559,6 +579,22 @@ class StreamDecoder:
                 self._admit_rules(idx, [r or Rules() for r in rules], nums[:, 0])
         self.flags[torch.tensor(slots, dtype=torch.long)] = 0
         self._embed_stale = True
+
+    def _requests(self, prompts, frames, max_new) -> tuple[torch.Tensor, torch.Tensor]:
+        """Host tensors of requests: their prompts (n, max_prompt), padded, and (prompt length, position limit, frames)."""
+        n = len(prompts)
+        forced = torch.full((n, self.max_prompt), self.pad, dtype=torch.long)
+        nums = torch.empty(n, 3, dtype=torch.int32)
+        for i, p in enumerate(prompts):
+            p = torch.as_tensor(p, dtype=torch.long).flatten()
+            if not 1 <= len(p) <= self.max_prompt:
+                raise ValueError(f"StreamDecoder: a prompt of {len(p)} tokens (1..{self.max_prompt})")
+            if not 1 <= frames[i] <= self.frames:
+                raise ValueError(f"StreamDecoder: {frames[i]} encoder frames (1..{self.frames})")
+            forced[i, :len(p)] = p
+            nums[i] = torch.tensor([len(p), len(p) - 1 + (max_new[i] if max_new else self.max_new_tokens),
+                                    frames[i]])
+        return forced, nums
 
     def _admit_rules(self, idx: torch.Tensor, rules: list[Rules], plen: torch.Tensor) -> None:
         """The slots' rules (the grammar's states need none: they follow from the start and the tokens)."""
@@ -588,7 +624,7 @@ class StreamDecoder:
         pick; after admit / set_active / reset, or on a different bucket, they are computed first."""
         with torch.cuda.stream(self.stream):
             if bucket in self.graphs:
-                if self.fused and (self._embed_stale or bucket != self._embed_rows):
+                if self._embeds_ahead and (self._embed_stale or bucket != self._embed_rows):
                     self._embed(bucket)
                 if n > 1 and n == self.chunk and bucket in self.chunk_graphs:
                     self.chunk_graphs[bucket].replay()
@@ -599,6 +635,15 @@ class StreamDecoder:
                 for _ in range(n):
                     self._run(bucket)
             self._embed_stale, self._embed_rows = False, bucket
+
+    def tokens(self, slot: int) -> torch.Tensor:
+        """The slot's tokens by position, on the GPU."""
+        return self.out[slot]
+
+    @staticmethod
+    def steps_to_limit(prompt: int, max_new: int) -> int:
+        """The steps from admission to the one that ends a slot by its token limit."""
+        return prompt - 1 + max_new
 
     def weight_bytes(self) -> int:
         """Bytes of projection weights one step reads."""

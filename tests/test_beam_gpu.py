@@ -255,10 +255,11 @@ def test_advance(gpu, B, width, by_length):
     w0, b0, w1, b1 = (torch.randn(width, generator=g).to(BF) for _ in range(4))
     dev = [t.cuda() for t in (groups, parent, token, total)]
     state = [t.cuda() for t in (tok, pos, score, finished, made, done, limit, out)]
+    held = torch.full_like(state[1], -3) if B != 4 else None
     x, h = (torch.empty(n * B, width, dtype=BF).cuda() for _ in range(2))
     flags = torch.zeros(G, dtype=torch.uint8).pin_memory()
     norms = [t.cuda() for t in (w0, b0, w1, b1)]
-    ext.dec_beam_advance(*dev, dummy, *state, eos, by_length, emb.cuda(), ptab.cuda(), norms[0], norms[1], 1e-5, norms[2],
+    ext.dec_beam_advance(*dev, dummy, *state[:2], held, *state[2:], eos, by_length, emb.cuda(), ptab.cuda(), norms[0], norms[1], 1e-5, norms[2],
                          norms[3], 1e-6, x, h, flags)
     torch.cuda.synchronize()
     w = [t.clone() for t in (tok, pos, score, finished, made, done, out)]
@@ -276,6 +277,9 @@ def test_advance(gpu, B, width, by_length):
         w[5][gr] = all(ends) or (not by_length and ends[0]) or p >= int(limit[gr])
     for got, want in zip(state[:6] + state[7:], w):
         assert torch.equal(got.cpu(), want)
+    if held is not None:
+        moved = w[1] != pos
+        assert torch.equal(held.cpu(), torch.where(moved, w[1] + 1, torch.full_like(w[1], -3)))
     assert torch.equal(flags.bool(), w[5].bool() & ~done.bool())
     rows = (groups.long()[:, None] * B + torch.arange(B)).reshape(-1).int().cuda()
     x1, h1 = torch.empty_like(x), torch.empty_like(h)

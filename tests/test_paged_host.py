@@ -168,7 +168,7 @@ def test_advance_refuses():
     from kernels.cuda_ext import ext
 
     a = dict(groups=torch.zeros(2, **I32), parent=torch.zeros(2, 4, **I32), token=torch.zeros(2, 4, **I64),
-             total=torch.zeros(2, 4), dummy=2, tok=torch.zeros(12, **I64), pos=torch.zeros(12, **I32),
+             total=torch.zeros(2, 4), dummy=2, tok=torch.zeros(12, **I64), pos=torch.zeros(12, **I32), held=None,
              score=torch.zeros(3, 4), finished=torch.zeros(3, 4, **U8), made=torch.zeros(3, 4, **I32),
              done=torch.zeros(3, **U8), limit=torch.zeros(3, **I32), out=torch.zeros(12, 9, **I64), eos=1, by_length=False,
              emb=torch.zeros(64, 256, dtype=BF), ptab=torch.zeros(9, 256, dtype=BF), w0=torch.zeros(256, dtype=BF),
@@ -177,7 +177,7 @@ def test_advance_refuses():
     for change in (dict(tok=torch.zeros(11, **I64)), dict(pos=torch.zeros(12, **I64)), dict(made=torch.zeros(3, 3, **I32)),
                    dict(done=torch.zeros(2, **U8)), dict(out=torch.zeros(12, 0, **I64)),
                    dict(emb=torch.zeros(64, 128, dtype=BF)), dict(w0=torch.zeros(255, dtype=BF)),
-                   dict(x=torch.zeros(7, 256, dtype=BF)), dict(flags=torch.zeros(2, **U8)), dict(score=torch.zeros(3, 17)),
+                   dict(x=torch.zeros(7, 256, dtype=BF)), dict(flags=torch.zeros(2, **U8)), dict(held=torch.zeros(11, **I32)), dict(score=torch.zeros(3, 17)),
                    dict()):  # the last one only for its place
         with pytest.raises(RuntimeError, match="dec_beam_advance"):
             ext.dec_beam_advance(*{**a, **change}.values())
