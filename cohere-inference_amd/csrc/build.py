@@ -27,7 +27,7 @@ OBJ_DIR = os.path.join(ROOT, "_build")
 
 SOURCES = ["capi.cpp", "gemm_q8.hip", "gemm_q8_dense.hip", "gemm_q8_sparse.hip", "gemm_q8_rows.hip", "dec_w8.hip", "quant.hip",
            "encoder_ops.hip", "encoder_loop.cpp", "encoder_noalloc.hip", "decoder_ops.hip", "dec_q4.hip", "dec_logits.hip",
-           "dec_paged.hip", "dec_beam.hip",
+           "dec_paged.hip", "dec_paged_chunk.hip", "dec_beam.hip",
            "gemm_bf16.hip", "frontend.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

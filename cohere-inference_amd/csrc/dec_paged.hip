@@ -393,6 +393,9 @@ int log2_of(int64_t P) {
 
 constexpr int64_t TOP = 0x7fffffff;
 
+// whether a call goes to the kernel of 128 query rows a workgroup: more than 32 rows per sequence and key head on average
+bool many_rows(int64_t rows, int64_t seqs, int64_t ratio) { return rows * ratio > 32 * seqs; }
+
 template <bool Q8>
 int attention_entry(PagedArgs p, int64_t rows, int64_t seqs, int64_t slots, int64_t heads, int64_t kv_heads, int64_t width,
                     int64_t pages, int64_t P, int64_t splits, int64_t part_len, void* stream, const char* name) {
@@ -420,7 +423,8 @@ int attention_entry(PagedArgs p, int64_t rows, int64_t seqs, int64_t slots, int6
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)wgs, (unsigned)splits);
   constexpr int W = 4;
-  if (shift >= 4) paged_rows_kernel<Q8, true, W><<<grid, W * 64, 0, s>>>(p);
+  if (many_rows(rows, seqs, p.ratio) && p.scale != 0.f) launch_chunk(p, Q8, s);
+  else if (shift >= 4) paged_rows_kernel<Q8, true, W><<<grid, W * 64, 0, s>>>(p);
   else paged_rows_kernel<Q8, false, W><<<grid, W * 64, 0, s>>>(p);
   const unsigned hs = (unsigned)(rows * heads);
   if (splits > 4) paged_combine_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
@@ -457,7 +461,8 @@ int gather_entry(GatherArgs p, int64_t rows, int64_t slots, int64_t width, int64
 
 extern "C" int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t T) {
   if (rows <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || T <= 0) return 1;
-  const int64_t wgs = tiles_for(rows, seqs, heads / kv_heads, 16, rows != seqs) * kv_heads;
+  const int64_t ratio = heads / kv_heads, wgs =
+      tiles_for(rows, seqs, ratio, many_rows(rows, seqs, ratio) ? 128 : 16, rows != seqs) * kv_heads;
   int64_t n = 1;
   while (n < 64 && wgs * n < 512 && T / (2 * n) >= 128) n *= 2;
   return n;

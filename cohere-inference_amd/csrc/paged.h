@@ -149,4 +149,8 @@ DEVI void append(const PagedArgs& p, const Tile& t, int n, int kvh, int TMrows) 
   }
 }
 
+// the kernel for chunks of many query rows (dec_paged_chunk.hip)
+int64_t chunk_workgroups(const PagedArgs& p);
+void launch_chunk(const PagedArgs& p, bool q8, hipStream_t s);
+
 }  // namespace cohere_paged
