@@ -161,6 +161,7 @@ paged_chunk_kernel(const PagedArgs p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
   float base = -INFINITY, l = 0.f;
+  bool bad = false;  // some values of the chunk's own tokens are infinite or NaN
 
   int entry = 0;
   uint64_t live = 0, next = 0;
@@ -258,48 +259,7 @@ paged_chunk_kernel(const PagedArgs p) {
             const v4s d = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)(src + 8 * 256));
             vf[dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(a, d, 0, 1, 2, 3, 4, 5, 6, 7));
           }
-          if (causal) {
-            // infinities and NaN: 0 x them is NaN, where a query does not see the key. They leave the product, and come
-            // in key by key for the queries that see them.
-            bool bad = false;
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-              const v4i q = __builtin_bit_cast(v4i, vf[dt]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) bad |= (q[i] & 0x7f80) == 0x7f80 || (q[i] & 0x7f800000) == 0x7f800000;
-            }
-            if (__builtin_expect(__any(bad), 0)) {
-#pragma unroll
-              for (int dt = 0; dt < 4; ++dt) {
-                v4i q = __builtin_bit_cast(v4i, vf[dt]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  q[i] &= ((q[i] & 0x7f80) == 0x7f80 ? 0 : 0xffff) | ((q[i] & 0x7f800000) == 0x7f800000 ? 0 : (int)0xffff0000u);
-                vf[dt] = __builtin_bit_cast(v8bf, q);
-              }
-#pragma unroll 1
-              for (int kk = 0; kk < 16; ++kk) {
-                // the weight of the lane's query: element 4 (kk / 8) + kk % 4 of half kk / 4 % 2
-                const int e = (kk >> 3) * 4 + (kk & 3), wi = e >> 1;
-                const int two = wi == 0 ? w[0] : wi == 1 ? w[1] : wi == 2 ? w[2] : w[3];
-                const float own = __uint_as_float(e & 1 ? (uint32_t)two & 0xffff0000u : (uint32_t)two << 16);
-                const float pk = __shfl(own, (kk >> 2 & 1) * 32 + col, 64);
-                const bool sees = t0 + k0 + kk <= tok;
-                const char* src = vbuf[buf] + (k0 + kk) * 256 + half * 8;
-#pragma unroll
-                for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                  for (int g = 0; g < 4; ++g) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(src + (((dt * 4 + g) ^ ((kk & 3) << 2)) * 16));
-                    const float v[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u),
-                                        __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u)};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                      if (sees && !(fabsf(v[k]) < INFINITY)) acc[dt][4 * g + k] += pk * v[k];
-                  }
-              }
-            }
-          }
+          if (causal) bad |= leave_out(vf);
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[dt], pf, acc[dt], 0, 0, 0);
         }
@@ -309,6 +269,20 @@ paged_chunk_kernel(const PagedArgs p) {
   }
   l = xor32_sum(l);
   if (wave * 32 + col < t.rows) {
+    if (__builtin_expect(bad, 0)) {
+      // of the part's tiles of the chunk's tokens those that some row of the wave's does not see whole
+      const int from = max((tok0 + 1) / KT, max(start - np, 0)) * KT, to = min(tok + 1, (end - np) * KT);
+#pragma unroll 1
+      for (int j = from; j < to; ++j) {
+        const uint16_t* src = rowkv + (int64_t)j * p.ldq + p.KV * HD + half * 4;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[dt][4 * g + k] += not_finite(src[dt * 32 + g * 8 + k]);
+      }
+    }
     const int64_t at = (int64_t)(t.first + tok) * p.H + head;
     if (nsp == 1) {
       const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -102,6 +102,31 @@ DEVI void unpack8(const uint4& u, float (&f)[8]) {
   }
 }
 
+// Infinities and NaN among a chunk's own values: 0 x them is NaN, where a query does not see the key. They leave the product
+// (made zeros; whether there were any in the wave), and are added to the outputs of the rows that see them at the end.
+template <int N>
+DEVI bool leave_out(v8bf (&v)[N]) {
+  const auto marks = [](int w) { return ((uint32_t)w & 0x7f807f80u) + 0x00800080u; };  // bits 15, 31: exponent of all ones
+  uint32_t any = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= marks(__builtin_bit_cast(v4i, v[k])[i]);
+  const bool some = __any(any & 0x80008000u);
+  if (__builtin_expect(some, 0)) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v4i w = __builtin_bit_cast(v4i, v[k]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] &= (int)~((marks(w[i]) >> 15 & 0x00010001u) * 0xffffu);
+      v[k] = __builtin_bit_cast(v8bf, w);
+    }
+  }
+  return some;
+}
+// the value, if it is infinite or NaN
+DEVI float not_finite(uint32_t h) { return (h & 0x7f80u) == 0x7f80u ? __uint_as_float(h << 16) : 0.f; }
+
 // a vector (16 lanes, 8 values each, u) as it is held, at vector `vec` of the pages; every lane takes part, `live` writes
 template <bool Q8>
 DEVI void store_vec(const uint4& u, void* pages, float* scales, int64_t vec, int d8, bool live) {
@@ -127,11 +152,12 @@ DEVI void store_vec(const uint4& u, void* pages, float* scales, int64_t vec, int
   }
 }
 
-// The keys and values of the tile's own tokens (those whose first query row is in the tile) into their pages, by W waves.
+// The keys and values of the tile's own tokens (those whose first query row is in the tile) into their pages, by W waves,
+// the last one first (the first one has more to do where there are few keys).
 // No workgroup reads them there in the same launch: a chunk attends to its own tokens as given.
 template <bool Q8, int W>
 DEVI void append(const PagedArgs& p, const Tile& t, int n, int kvh, int TMrows) {
-  const int lane = lane_id(), wave = wave_id(), d8 = lane & 15;
+  const int lane = lane_id(), wave = W - 1 - wave_id(), d8 = lane & 15;
   const int j0 = (t.x0 + p.ratio - 1) / p.ratio, j1 = min(t.c, (t.x0 + TMrows + p.ratio - 1) / p.ratio);
   const int P = 1 << p.shift;
   for (int i = wave * 4; i < (j1 - j0) * 2; i += W * 4) {

@@ -30,8 +30,8 @@ def _check(c, splits=1, starts="own", **kw):
 def test_single_tokens(gpu, bits, ratio, page, held):
     print(f"paged single bits={bits} ratio={ratio} page={page}", flush=True)
     c = Paged(page * 100 + ratio, held, [1] * len(held), 2, ratio, page, bits, pad=8)
-    _check(c)
-    _check(c, starts=None)
+    _check(c, weights_bf16=ratio > 16)
+    _check(c, starts=None, weights_bf16=ratio > 16)
 
 
 @pytest.mark.parametrize("bits", [16, 8])
