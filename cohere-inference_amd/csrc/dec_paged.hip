@@ -58,8 +58,9 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
   const int last = p.starts ? (t.x0 + t.rows - 1) / p.ratio : 0, nr = last / KB + 1;
   int n = 0, nb = 0, start = 0, end = 0, b = wave;
   bool row_ok = false;
+  const int held = p.n[t.slot];  // on its way
   const auto bounds = [&]() {
-    n = t.ok ? p.n[t.slot] : -1;
+    n = t.ok ? held : -1;
     row_ok = n >= 0;
     n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
     nb = row_ok ? nr + (n + KB - 1) / KB : 0;
@@ -91,6 +92,19 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     const uint16_t* qp = p.q + (int64_t)(t.first + tok) * p.ldq + head * HD;
 #pragma unroll
     for (int s = 0; s < 4; ++s) qf[s] = *reinterpret_cast<const v8bf*>(qp + dims(s));
+  }
+
+  const uint16_t* rowkv = p.q + (int64_t)t.first * p.ldq + (p.H + kvh) * HD;
+  // A chunk of one token has one key of its own, which every row sees: its score is the first maximum and its value the
+  // first outputs, without a product; the loads are made here, and waited for behind the first block's.
+  const bool single = t.c == 1, first = single && b == 0;
+  v8bf k1[4];
+  uint2 v1[8];
+  if (first) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) k1[s] = *reinterpret_cast<const v8bf*>(rowkv + dims(s));
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) v1[dt] = *reinterpret_cast<const uint2*>(rowkv + p.KV * HD + dt * 16 + grp * 4);
   }
 
   v4f acc[8];  // dimensions 16 dt + 4 grp + i of query col in acc[dt][i]
@@ -152,8 +166,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
 
   // the chunk's own blocks, as given; bad: of the wave's some values are infinite or NaN
   bool bad = false;
-  const uint16_t* rowkv = p.q + (int64_t)t.first * p.ldq + (p.H + kvh) * HD;
-  for (; b < (SPLIT ? min(end, nr) : nr); b += W) {
+  for (; !single && b < (SPLIT ? min(end, nr) : nr); b += W) {
     const int j0 = b * KB;
     const auto own_row = [&](int j) { return rowkv + (int64_t)min(j, t.c - 1) * p.ldq; };
 #pragma unroll
@@ -275,6 +288,25 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     end = nb;
   }
   if (sp == 0 && row_ok) append<Q8, W>(p, t, n, kvh, 16);
+  if (first) {
+    float dot = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float a[8], c[8];
+      unpack8(__builtin_bit_cast(uint4, qf[s]), a);
+      unpack8(__builtin_bit_cast(uint4, k1[s]), c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(a[i], c[i], dot);
+    }
+    dot = xor32_sum(xor16_sum(dot)) * p.scale;
+    m = dot == dot ? dot : -INFINITY;  // maxima pass over a NaN, the sum keeps it
+    const float e = dot == -INFINITY ? 0.f : exp2_hw(dot - m);  // 1, but for scores that are not finite
+    l = grp == 0 ? e : 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt)
+      acc[dt] = e * v4f{__uint_as_float(v1[dt].x << 16), __uint_as_float(v1[dt].x & 0xffff0000u),
+                        __uint_as_float(v1[dt].y << 16), __uint_as_float(v1[dt].y & 0xffff0000u)};
+  }
 
   // Each block's loads are made under the products of the one before it.
   for (b = b0; b < end; b += W) {
@@ -379,34 +411,39 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     }
   }
   __syncthreads();
-  for (int i = tid; i < t.rows * HD; i += W * 64) {
-    const int r = i >> 7, dim = i & (HD - 1), xr = t.x0 + r, tk = p.starts ? xr / p.ratio : 0;
-    float MM = -INFINITY, L = 0.f, O = 0.f;
+  int left_out = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) left_out |= sbad[w];
+  const int dim = (tid & 31) * 4;  // 32 threads a row, 4 dimensions each
+  for (int r = tid >> 5; r < t.rows; r += W * 2) {
+    const int xr = t.x0 + r, tk = p.starts ? xr / p.ratio : 0;
+    float MM = -INFINITY, L = 0.f;
+    v4f O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < W; ++w) MM = fmaxf(MM, sm[w][r]);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float mw = sm[w][r];
       L += mw == -INFINITY ? sl[w][r] : exp2_hw(mw - MM) * sl[w][r];
-      O += reinterpret_cast<const float*>(region + w * REGION)[r * LD + dim];
+      O += *reinterpret_cast<const v4f*>(region + w * REGION + (r * LD + dim) * 4);
     }
-    int left_out = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) left_out |= sbad[w];
     if (__builtin_expect(left_out && row_ok, 0)) {  // the row sees what was left out up to its own token
       const int from = SPLIT ? start * KB : 0, to = min(tk + 1, SPLIT ? end * KB : t.c);
-      for (int j = from; j < to; ++j) O += not_finite(rowkv[(int64_t)j * p.ldq + p.KV * HD + dim]);
+      for (int j = from; j < to; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[i] += not_finite(rowkv[(int64_t)j * p.ldq + p.KV * HD + dim + i]);
     }
     const int64_t at = (int64_t)(t.first + tk) * p.H + kvh * p.ratio + (xr - tk * p.ratio);
     if (nsp == 1) {
-      p.out[at * HD + dim] = f2bf(L == 0.f ? 0.f : O / L);
+      float o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = L == 0.f ? 0.f : O[i] / L;
+      *reinterpret_cast<uint2*>(p.out + at * HD + dim) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
     } else {
-      float* part = p.part + (at * nsp + sp) * (HD + 2);
-      part[dim] = O;
-      if (dim == 0) {
-        part[HD] = MM;
-        part[HD + 1] = L;
-      }
+      float* part = p.part + (at * nsp + sp) * (HD + 2);  // parts are 520 bytes apart: 8-byte stores
+      *reinterpret_cast<float2*>(part + dim) = make_float2(O[0], O[1]);
+      *reinterpret_cast<float2*>(part + dim + 2) = make_float2(O[2], O[3]);
+      if (dim == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(MM, L);
     }
   }
 }
