@@ -20,20 +20,18 @@ namespace {
 
 using namespace cohere_rows;
 
-constexpr int MAXB = 16;
+constexpr int MAXB = 16, MK = 8;
 constexpr double LOG2E64 = 1.4426950408889634074;
 
-// a bf16 logit as a number of the same order; NaN counts as -inf, inf as the largest finite number, -0 as 0
+// a finite bf16 logit as a number of the same order, -0 as 0
 DEVI uint32_t order_of(uint32_t h) {
-  if ((h & 0x7fffu) > 0x7f80u) h = 0xff80u;
-  if (h == 0x7f80u) h = 0x7f7fu;
   if (h == 0x8000u) h = 0;
   return h & 0x8000u ? h ^ 0xffffu : h | 0x8000u;
 }
 DEVI float logit_of(uint32_t o) { return __uint_as_float((o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu) << 16); }
-constexpr uint32_t LOWEST = 0x7f;  // order_of(-inf)
 
-// a part's result: maximum, sum of exp(l - maximum), then B keys order << 32 | ~index, best first (0: none)
+// a part's result: maximum, sum of exp(l - maximum), then B keys order << 32 | ~index of logits above -inf, best first (0:
+// none). Where a beam has fewer than B of these, its other candidates, all of -inf, are the lowest indexes without a key.
 struct Part {
   float m;
   uint32_t unused;
@@ -41,11 +39,6 @@ struct Part {
 };
 __host__ __device__ inline int64_t part_bytes(int B) { return (int64_t)sizeof(Part) + 8 * B; }
 
-DEVI uint32_t wave_max_u(uint32_t v) {
-  const auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-  for (int o = 1; o < 64; o <<= 1) v = mx(v, (uint32_t)__shfl_xor((int)v, o, 64));
-  return v;
-}
 DEVI uint64_t wave_max_u64(uint64_t v) {
   for (int o = 1; o < 64; o <<= 1) {
     const uint64_t w = __shfl_xor(v, o, 64);
@@ -58,32 +51,46 @@ DEVI double wave_sum_d(double v) {
   return v;
 }
 
-// of 64 keys, one a lane (0: none, the others different), the place of this lane's among them
-DEVI int rank_of(uint64_t key) {
+// of the first n lanes' keys (0: none, the others different) the place of this lane's among them
+DEVI int rank_of(uint64_t key, int n) {
   int r = 0;
-#pragma unroll 8
-  for (int i = 0; i < 64; ++i) {
-    const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
-                       (uint32_t)__builtin_amdgcn_readlane((int)key, i);
-    r += o > key;
-  }
+  for (int i = 0; i < n; i += 4)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i + k) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)key, i + k);
+      r += o > key;
+    }
   return r;
 }
 
-// 2^y for y in -1000 .. 0 to 6e-11 of itself: 2^(y - round y) by the Chebyshev interpolant of 2^x on -1/2 .. 1/2 of degree
-// 7, times a power of two
-DEVI double exp2_64(double y) {
+// exp(d) for d <= 0 to 6e-11 of itself, d below -700 or NaN as -700: 2^(y - round y) by the Chebyshev interpolant of 2^x on
+// -1/2 .. 1/2 of degree 7, times a power of two, y = d log2 e. N at once, whose chains of products fill each other's waits.
+template <int N>
+DEVI void exp_64(double (&d)[N]) {
   const double magic = 6755399441055744.0;  // 1.5 2^52: the sum's last bit is 1
-  const double t = y + magic, f = y - (t - magic);
-  double p = 1.5303699001378845e-05;
-  p = __builtin_fma(p, f, 0.00015469729140704658);
-  p = __builtin_fma(p, f, 0.0013333478480888061);
-  p = __builtin_fma(p, f, 0.009618025613598036);
-  p = __builtin_fma(p, f, 0.055504109063177154);
-  p = __builtin_fma(p, f, 0.24022651213495422);
-  p = __builtin_fma(p, f, 0.6931471805568341);
-  p = __builtin_fma(p, f, 0.9999999999595622);
-  return __builtin_amdgcn_ldexp(p, (int)__builtin_bit_cast(uint64_t, t));
+  constexpr double C[7] = {0.00015469729140704658, 0.0013333478480888061, 0.009618025613598036, 0.055504109063177154,
+                           0.24022651213495422,    0.6931471805568341,    0.9999999999595622};
+  double t[N], f[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) d[e] = fmax(d[e], -700.);
+#pragma unroll
+  for (int e = 0; e < N; ++e) t[e] = __builtin_fma(d[e], LOG2E64, magic);
+#pragma unroll
+  for (int e = 0; e < N; ++e) f[e] = __builtin_fma(d[e], LOG2E64, magic - t[e]);
+#pragma unroll
+  for (int e = 0; e < N; ++e) d[e] = 1.5303699001378845e-05;
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] = __builtin_fma(d[e], f[e], C[i]);
+#pragma unroll
+  for (int e = 0; e < N; ++e) d[e] = __builtin_amdgcn_ldexp(d[e], (int)__builtin_bit_cast(uint64_t, t[e]));
+}
+DEVI double exp_64(double d) {
+  double x[1] = {d};
+  exp_64(x);
+  return x[0];
 }
 
 struct SelectArgs {
@@ -103,116 +110,217 @@ struct SelectArgs {
 
 // A workgroup takes J * 2048 logits of a row: their maximum, the sum, and the B best. A wave finds its B best among few:
 // T, the B-th largest of its lanes' maxima, is no larger than the B-th best, and hardly more than B logits reach it; these
-// are ranked by counting, one a lane. Where more than 64 do (many equal logits, a mask that leaves little), the B best are
-// taken one by one.
+// are ranked by counting, one a lane. Where more than 64 do (many equal logits, few lanes with a logit above -inf), the B
+// best are taken one by one. What bounds it is the vector unit: of 25 instructions a logit 15 are the exponential (205 rows
+// of 100008 in 27.8 us: 9.3 M instructions, which alone take 15.5; reading 41 MB takes 8).
 template <int J>
 __global__ void __launch_bounds__(256) beam_parts_kernel(const SelectArgs a) {
   __shared__ uint64_t cand[4][64], best[4][MAXB];
-  __shared__ uint32_t smax[4];
+  __shared__ float smax[4];
   __shared__ double ssum[4];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), B = a.B;
-  const int r = blockIdx.y, v0 = blockIdx.x * (J * 2048), i = r / B, g = a.groups[i];
+  const int lane = lane_id(), wave = wave_id(), B = a.B;
+  const int r = blockIdx.y, v0 = (blockIdx.x * 4 + wave) * (J * 512);
   const uint16_t* row = a.logits + (int64_t)r * a.ld;
-  uint4 u[J];
+  uint32_t w[J][4];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const int v = v0 + (j * 256 + tid) * 8;
-    u[j] = *reinterpret_cast<const uint4*>(row + min(v, a.V - 8));
+    const int v = v0 + (j * 64 + lane) * 8;
+    const uint4 u = *reinterpret_cast<const uint4*>(row + min(v, a.V - 8));
+    const bool in = v < a.V;
+    w[j][0] = in ? u.x : 0xff80ff80u;
+    w[j][1] = in ? u.y : 0xff80ff80u;
+    w[j][2] = in ? u.z : 0xff80ff80u;
+    w[j][3] = in ? u.w : 0xff80ff80u;
   }
-  if ((unsigned)g >= (unsigned)a.G) return;
-  const int slot = g * B + (r - i * B);
-  if (a.finished[slot] || !(a.score[slot] > -INFINITY)) return;  // its candidates are known without the logits
-  uint32_t o[J * 8], top = 0;
+  if constexpr (J > 1) {  // an ended beam's candidates are known without its logits; few logits are done before that is
+    const int i = r / B, g = a.groups[i];
+    if ((unsigned)g >= (unsigned)a.G) return;
+    const int slot = g * B + (r - i * B);
+    if (a.finished[slot] || !(a.score[slot] > -INFINITY)) return;
+  }
+  const auto logit = [&](int j, int k) { return __uint_as_float(k & 1 ? w[j][k >> 1] & 0xffff0000u : w[j][k >> 1] << 16); };
+  float of[J], top = -INFINITY;  // maxima, which pass over NaN
+  const auto maxima = [&]() {
+    top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const bool in = v0 + (j * 256 + tid) * 8 < a.V;
-    const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+    for (int j = 0; j < J; ++j) {
+      of[j] = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      o[j * 8 + k] = in ? order_of(k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu) : 0;  // 0: none
-      top = o[j * 8 + k] > top ? o[j * 8 + k] : top;
+      for (int k = 0; k < 8; ++k) of[j] = fmaxf(of[j], logit(j, k));
+      top = fmaxf(top, of[j]);
     }
+  };
+  maxima();
+  if (__builtin_expect(__any(top == INFINITY), 0)) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if ((w[j][k] & 0xffffu) == 0x7f80u) --w[j][k];
+        if (w[j][k] >> 16 == 0x7f80u) w[j][k] -= 0x10000u;
+      }
+    maxima();
   }
-  const auto key_of = [&](int e) {
-    return (uint64_t)o[e] << 32 | ~(uint32_t)(v0 + ((e >> 3) * 256 + tid) * 8 + (e & 7));
+  const auto key_of = [&](int j, int k) {
+    return (uint64_t)order_of(__float_as_uint(logit(j, k)) >> 16) << 32 | ~(uint32_t)(v0 + (j * 64 + lane) * 8 + k);
   };
   // the B-th largest of the lanes' maxima
-  uint32_t t = top, T = 0;
+  float t = top, T = -INFINITY, m = -INFINITY;
   for (int k = 0; k < B; ++k) {
-    T = wave_max_u(t);
-    if (k == 0 && lane == 0) smax[wave] = T;
+    T = wave_max64(t);
+    if (k == 0) m = T;
     const uint64_t who = __ballot(t == T);
-    if (lane == __ffsll((unsigned long long)who) - 1) t = 0;
+    if (lane == __ffsll((unsigned long long)who) - 1) t = -INFINITY;
   }
-  T = T ? T : 1;
+  T = fmaxf(T, -3.3895313892515355e38f);  // the lowest finite number
   if (lane < MAXB) best[wave][lane] = 0;
   int count = 0;
 #pragma unroll
-  for (int e = 0; e < J * 8; ++e) {
-    const uint64_t who = __ballot(o[e] >= T);
-    if (who) {
-      const int at = count + __popcll(who & ((1ull << lane) - 1));
-      if (o[e] >= T && at < 64) cand[wave][at] = key_of(e);
-      count += __popcll(who);
+  for (int j = 0; j < J; ++j) {
+    if (!__any(of[j] >= T)) continue;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool in = logit(j, k) >= T;
+      const uint64_t who = __ballot(in);
+      if (who) {
+        const int at = count + __popcll(who & ((1ull << lane) - 1));
+        if (in && at < 64) cand[wave][at] = key_of(j, k);
+        count += __popcll(who);
+      }
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
   if (__builtin_expect(count <= 64, 1)) {
     const uint64_t key = lane < count ? cand[wave][lane] : 0;
-    const int place = rank_of(key);
+    const int place = rank_of(key, count);
     if (key && place < B) best[wave][place] = key;
   } else {
     uint64_t last = ~0ull;
     for (int k = 0; k < B; ++k) {
       uint64_t mine = 0;
+#pragma unroll 1
+      for (int j = 0; j < J; ++j) {
+        uint32_t x[4] = {w[0][0], w[0][1], w[0][2], w[0][3]};
 #pragma unroll
-      for (int e = 0; e < J * 8; ++e) {
-        const uint64_t key = key_of(e);
-        if (o[e] && key < last && key > mine) mine = key;
+        for (int q = 1; q < J; ++q)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) x[y] = q == j ? w[q][y] : x[y];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const uint32_t h = y & 1 ? x[y >> 1] >> 16 : x[y >> 1] & 0xffffu;
+          const uint64_t key = (uint64_t)order_of(h) << 32 | ~(uint32_t)(v0 + (j * 64 + lane) * 8 + y);
+          if (__uint_as_float(h << 16) > -INFINITY && key < last && key > mine) mine = key;
+        }
       }
       last = wave_max_u64(mine);
       if (lane == 0) best[wave][k] = last;
       if (!last) break;
     }
   }
-  __syncthreads();
-  uint32_t M = smax[0];
-#pragma unroll
-  for (int w = 1; w < 4; ++w) M = smax[w] > M ? smax[w] : M;
-  const float m = M ? logit_of(M) : -INFINITY;
   double sum = 0.;
   if (m > -INFINITY) {
 #pragma unroll
-    for (int e = 0; e < J * 8; ++e) {
-      // the difference first: it is exact, or nearly so, at any magnitude
-      const double y = ((double)logit_of(o[e]) - (double)m) * LOG2E64;
-      sum += exp2_64(o[e] > LOWEST && y > -1000. ? y : -1000.);
-    }
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {
+        double d[2] = {(double)logit(j, k) - (double)m, (double)logit(j, k + 1) - (double)m};  // exact, or nearly so
+        exp_64(d);
+        sum += d[0];
+        sum += d[1];
+      }
+    sum = wave_sum_d(sum);
   }
-  sum = wave_sum_d(sum);
-  if (lane == 0) ssum[wave] = sum;
+  if (lane == 0) {
+    smax[wave] = m;
+    ssum[wave] = sum;
+  }
   __syncthreads();
   if (wave != 0) return;
   Part* out = reinterpret_cast<Part*>(a.work + ((int64_t)r * a.parts + blockIdx.x) * part_bytes(B));
   uint64_t* keys = reinterpret_cast<uint64_t*>(out + 1);
+  const float M = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3])), mw = smax[lane & 3];
+  sum = mw > -INFINITY ? ssum[lane & 3] * exp_64((double)mw - (double)M) : 0.;
+  sum += __shfl_xor(sum, 1, 64);
+  sum += __shfl_xor(sum, 2, 64);
   if (lane == 0) {
-    out->m = m;
-    out->sum = (ssum[0] + ssum[1]) + (ssum[2] + ssum[3]);
+    out->m = M;
+    out->sum = sum;
   }
   const uint64_t key = lane < 4 * B ? best[lane / B][lane % B] : 0;
-  const int place = rank_of(key), have = __popcll(__ballot(key != 0));
+  const int place = rank_of(key, 4 * B), have = __popcll(__ballot(key != 0));
   if (key && place < B) keys[place] = key;
   if (lane < B && lane >= have) keys[lane] = 0;
 }
 
+// Of a wave's keys, N a lane, the B best: the e-th best in lane e, lanes behind them 0. As above, by the logits' order alone
+// until few are left.
+template <int N>
+DEVI uint64_t best_of(const uint64_t (&key)[N], int B, uint64_t* cand, uint64_t* best) {
+  const int lane = lane_id();
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) top = fmaxf(top, (float)(uint32_t)(key[e] >> 32));  // 16 bits: exact
+  float t = top, T = 0.f;
+  for (int k = 0; k < B; ++k) {
+    T = wave_max64(t);
+    const uint64_t who = __ballot(t == T);
+    if (lane == __ffsll((unsigned long long)who) - 1) t = 0.f;
+  }
+  T = fmaxf(T, 1.f);
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const bool in = (float)(uint32_t)(key[e] >> 32) >= T;
+    const uint64_t who = __ballot(in);
+    const int at = count + __popcll(who & ((1ull << lane) - 1));
+    if (in && at < 64) cand[at] = key[e];
+    count += __popcll(who);
+  }
+  if (lane < MAXB) best[lane] = 0;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes, read back by its other lanes
+  if (__builtin_expect(count <= 64, 1)) {
+    const uint64_t mine = lane < count ? cand[lane] : 0;
+    const int place = rank_of(mine, count);
+    if (mine && place < B) best[place] = mine;
+  } else {
+    uint64_t last = ~0ull;
+    for (int k = 0; k < B; ++k) {
+      uint64_t mine = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (key[e] < last && key[e] > mine) mine = key[e];
+      last = wave_max_u64(mine);
+      if (lane == 0) best[k] = last;
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  const uint64_t mine = lane < B ? best[lane] : 0;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, before the next are written
+  return mine;
+}
+
 // A workgroup takes a group: a wave a beam's parts (their sum, and of their B best each the beam's B best), then the B x B
 // candidates are ranked by counting, a thread each.
-__global__ void __launch_bounds__(256) beam_merge_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(64 * MAXB) beam_merge_kernel(const SelectArgs a) {
   __shared__ double srank[MAXB * MAXB], stotal[MAXB * MAXB];
-  __shared__ int sv[MAXB * MAXB];
-  __shared__ uint64_t tmp[4][MAXB];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), B = a.B;
-  const int i = blockIdx.x, g = a.groups[i];
+  __shared__ int sv[MAXB * MAXB], splace[MAXB * MAXB];
+  __shared__ uint64_t cand[MAXB][64], best[MAXB][MAXB];
+  const int tid = threadIdx.x, lane = lane_id(), b = wave_id(), B = a.B, i = blockIdx.x;
+  const char* at = a.work + ((int64_t)i * B + b) * a.parts * part_bytes(B);
+  const auto key_at = [&](int k) {
+    const int p = k / B;
+    return k < a.parts * B ? reinterpret_cast<const uint64_t*>(at + p * part_bytes(B) + sizeof(Part))[k - p * B] : 0;
+  };
+  // on their way before it is known whether they count: what an ended beam's parts hold is not looked at
+  Part q = {-INFINITY, 0, 0.};
+  if (lane < a.parts) q = *reinterpret_cast<const Part*>(at + lane * part_bytes(B));
+  uint64_t next[MK];
+  const auto load = [&](int k0) {
+#pragma unroll
+    for (int e = 0; e < MK; ++e) next[e] = key_at(k0 + e * 64 + lane);
+  };
+  load(0);
+  const int g = a.groups[i];
   if ((unsigned)g >= (unsigned)a.G) {
     if (tid < B) {
       a.parent[i * B + tid] = tid;
@@ -221,76 +329,82 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(const SelectArgs a) {
     }
     return;
   }
-  for (int b = wave; b < B; b += 4) {
-    const bool ended = a.finished[g * B + b] != 0;
-    const double start = (double)a.score[g * B + b];
-    double total = -INFINITY;
-    int v = 0;
-    if (!(start > -INFINITY)) {  // nothing but candidates of -inf (NaN counts as it): by their indexes
-      v = lane;
-    } else if (ended) {
-      v = lane == 0 ? a.pad : lane - 1 + (lane - 1 >= a.pad);
-      total = lane == 0 ? start : -INFINITY;
-    } else {
-      const char* at = a.work + ((int64_t)i * B + b) * a.parts * part_bytes(B);
-      float M = -INFINITY;
-      for (int p = lane; p < a.parts; p += 64) M = fmaxf(M, reinterpret_cast<const Part*>(at + p * part_bytes(B))->m);
-      M = wave_max64(M);
-      double S = 0.;
-      for (int p = lane; p < a.parts; p += 64) {
-        const Part* q = reinterpret_cast<const Part*>(at + p * part_bytes(B));
-        const double y = ((double)q->m - (double)M) * LOG2E64;
-        S += q->m > -INFINITY ? q->sum * exp2_64(y > -1000. ? y : -1000.) : 0.;
-      }
-      S = wave_sum_d(S);
-      // the sorted keys so far in lanes 0 .. B - 1, the next 64 - B beside them
-      uint64_t cur = 0;
-      for (int k0 = 0; k0 < a.parts * B; k0 += 64 - B) {
-        const int k = k0 + lane - B, p = k / B;
-        uint64_t key = cur;
-        if (lane >= B)
-          key = k < a.parts * B ? reinterpret_cast<const uint64_t*>(at + p * part_bytes(B) + sizeof(Part))[k - p * B] : 0;
-        const int place = rank_of(key);
-        if (lane < B) tmp[wave][lane] = 0;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (key && place < B) tmp[wave][place] = key;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        cur = lane < B ? tmp[wave][lane] : 0;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
-      v = (int)~(uint32_t)cur;
-      const float l = logit_of((uint32_t)(cur >> 32));
-      if (M > -INFINITY) total = start + ((double)l - (double)M - log(S));  // else: no logit above -inf
+  const bool ended = a.finished[g * B + b] != 0;
+  const double start = (double)a.score[g * B + b];
+  double weight = 1.;
+  if (a.norm) weight = (double)a.norm[min(max(a.made[g * B + b] + (ended ? 0 : 1), 0), a.N - 1)];
+  double total = -INFINITY;
+  int v = 0;
+  if (!(start > -INFINITY)) {  // nothing but candidates of -inf (NaN counts as it): by their indexes
+    v = lane;
+  } else if (ended) {
+    v = lane == 0 ? a.pad : lane - 1 + (lane - 1 >= a.pad);
+    total = lane == 0 ? start : -INFINITY;
+  } else {
+    float M = q.m;
+    for (int p = lane + 64; p < a.parts; p += 64) M = fmaxf(M, reinterpret_cast<const Part*>(at + p * part_bytes(B))->m);
+    M = wave_max64(M);
+    double S = q.m > -INFINITY ? q.sum * exp_64((double)q.m - (double)M) : 0.;
+    for (int p = lane + 64; p < a.parts; p += 64) {
+      const Part* o = reinterpret_cast<const Part*>(at + p * part_bytes(B));
+      S += o->m > -INFINITY ? o->sum * exp_64((double)o->m - (double)M) : 0.;
     }
-    double rank = total;
-    if (a.norm) {
-      const int len = a.made[g * B + b] + (ended ? 0 : 1);
-      rank = total * (double)a.norm[min(max(len, 0), a.N - 1)];
+    S = wave_sum_d(S);
+    // the best so far in lanes 0 .. B - 1, best first, and MK keys a lane more in each round
+    uint64_t cur = 0;
+    for (int k0 = 0; k0 < a.parts * B; k0 += 64 * MK) {
+      uint64_t key[MK + 1];
+#pragma unroll
+      for (int e = 0; e < MK; ++e) key[e] = next[e];
+      key[MK] = cur;
+      if (k0 + 64 * MK < a.parts * B) load(k0 + 64 * MK);
+      cur = best_of(key, B, cand[b], best[b]);
     }
-    if (lane < B) {
-      stotal[b * B + lane] = total == total ? total : -INFINITY;
-      srank[b * B + lane] = rank == rank ? rank : -INFINITY;
-      sv[b * B + lane] = v;
+    const int have = __popcll(__ballot(cur != 0));
+    v = (int)~(uint32_t)cur;
+    if (cur) total = start + ((double)logit_of((uint32_t)(cur >> 32)) - (double)M - log(S));
+    if (have < B) {  // the lowest indexes that have no key
+      int free = 0;
+      for (int u = 0, to = have; to < B; ++u) {
+        if (__any(cur != 0 && v == u)) continue;
+        if (lane == to) free = u;
+        ++to;
+      }
+      if (lane >= have) v = free;
     }
   }
+  if (lane < B) {
+    const double rank = total * weight;
+    stotal[b * B + lane] = total == total ? total : -INFINITY;
+    srank[b * B + lane] = rank == rank ? rank : -INFINITY;
+    sv[b * B + lane] = v;
+  }
+  if (tid < B * B) splace[tid] = 0;
   __syncthreads();
-  if (tid >= B * B) return;
-  const double mine = srank[tid];
-  const int b = tid / B, v = sv[tid];
-  int place = 0;
-  for (int c = 0; c < B * B; ++c) {
-    const double other = srank[c];
-    const int cb = c / B;
-    place += other > mine || (other == mine && (cb < b || (cb == b && sv[c] < v)));
-  }
+  // a candidate's place: 64 / B threads, each counts the better ones of some beams
+  const int c = tid % (B * B), cb = c / B, share = tid / (B * B), shares = 64 / B;
+  const double mine = srank[c];
+  v = sv[c];
+  int better = 0;
+  for (int ob = share < shares ? share : B; ob < B; ob += shares)
+    for (int k = 0; k < B; ++k) {
+      const double other = srank[ob * B + k];
+      better += other > mine || (other == mine && (ob < cb || (ob == cb && sv[ob * B + k] < v)));
+    }
+  if (better) atomicAdd(&splace[c], better);
+  __syncthreads();
+  const int place = tid < B * B ? splace[tid] : B;
   if (place < B) {
-    a.parent[i * B + place] = b;
+    a.parent[i * B + place] = cb;
     a.token[i * B + place] = v;
-    a.total[i * B + place] = (float)stotal[tid];
+    a.total[i * B + place] = (float)stotal[c];
   }
 }
 
-int select_j(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) >= 512 ? 4 : 1; }
+// Logits a workgroup over 2048: 8 where that makes a workgroup a CU still, so that a wave's search for its B best is paid
+// for by more logits (4 x 16 beams, 64000 logits: 30 us, with 1 45; 64 x 4, 16384: 14.2 and 15.7). Below that 1, for the
+// wave's own length (1 x 4, 16384: 9.7 us, with 8 12.3; 16 x 4: 11.1 and 13.5).
+int select_j(int64_t rows, int64_t V) { return rows * ((V + 16383) / 16384) >= 256 ? 8 : 1; }
 int64_t select_parts(int64_t rows, int64_t V) {
   const int64_t span = 2048 * select_j(rows, V);
   return (V + span - 1) / span;
@@ -491,9 +605,9 @@ extern "C" int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_
                      (int)n, (int)slots, (int)beams, (int)V, (int)norm_len, (int)pad, (int)select_parts(rows, V)};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)a.parts, (unsigned)rows);
-  if (select_j(rows, V) == 4) beam_parts_kernel<4><<<grid, 256, 0, s>>>(a);
+  if (select_j(rows, V) == 8) beam_parts_kernel<8><<<grid, 256, 0, s>>>(a);
   else beam_parts_kernel<1><<<grid, 256, 0, s>>>(a);
-  beam_merge_kernel<<<(unsigned)n, 256, 0, s>>>(a);
+  beam_merge_kernel<<<(unsigned)n, (unsigned)beams * 64, 0, s>>>(a);
   return cohere::check_launch("dec_beam_select");
 }
 

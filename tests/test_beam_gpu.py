@@ -100,6 +100,27 @@ def test_select_masked_rows(gpu):
         _same(a, made=made, norm=torch.tensor([1.0, 0.5, 0.25]))
 
 
+def test_select_many_rows(gpu):
+    """As many rows as take long stretches a workgroup: masks, equal logits, NaN and infinities there too."""
+    for B in (3, 4, 13):
+        n = 300 // B
+        a, made = _inputs(B, n, B, 16400)
+        x = a[0].reshape(n, B, -1)
+        x[0] = -math.inf
+        x[1, :, 5:] = -math.inf
+        x[2, 0, :16380] = -math.inf
+        x[3, :, ::7] = float("nan")
+        x[4, 0, 100:104] = math.inf
+        x[5] = 0.25
+        x[6] = (torch.randint(0, 3, x[6].shape, generator=torch.Generator().manual_seed(1)) / 4).to(BF)
+        x[7, -1, 4096:] = float("nan")
+        x[8, :, :] = -math.inf
+        x[8, 0, 4096:4104] = 1.0  # one lane's
+        x[9, :, 512:1024] = 8.0
+        _same(a)
+        _same(a, made=made, norm=torch.tensor([1.0, 0.5, 0.25]))
+
+
 def test_select_ended_beams(gpu):
     """Groups whose beams have all ended keep them in order of their scores; pad at the ends of the vocabulary."""
     for pad in (0, 5, 63):
