@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     bounds();
     end = nb;
   }
-  if (sp == 0 && row_ok) append<Q8, W>(p, t, n, kvh, 16);
+  if (sp == 0 && row_ok) append<Q8, W, 2>(p, t, n, kvh, 16);
   if (first) {
     float dot = 0.f;
 #pragma unroll
@@ -487,6 +487,34 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
   }
 }
 
+// The same behind the kernel of many rows, whose rows have parts of their own number: a wave a (row, head), which reads those
+// parts alone that it has.
+__global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __restrict__ part, const int32_t* starts, int S,
+                                                                 int64_t count, int H, int nsp, uint16_t* out) {
+  const int lane = lane_id();
+  const int64_t head = (int64_t)blockIdx.x * 4 + wave_id();
+  if (head >= count) return;
+  const float* base = part + head * nsp * (HD + 2);
+  const float2 ml = *reinterpret_cast<const float2*>(base + min(lane, nsp - 1) * (HD + 2) + HD);
+  const int r = (int)(head / H);
+  if (r < starts[0] || r >= starts[S]) return;
+  if (lane_value(ml.y, 0) < 0.f) return;  // one part, which wrote the outputs
+  const bool in = lane < nsp && ml.x != -INFINITY;
+  const float M = wave_max64(in ? ml.x : -INFINITY), w = in ? exp2_hw(ml.x - M) : 0.f;
+  const float L = wave_sum64(lane < nsp ? (in ? w * ml.y : ml.y) : 0.f);
+  float o0 = 0.f, o1 = 0.f;
+  const uint64_t there = __ballot(in);
+  const int last = 64 - __clzll(there);
+#pragma unroll 4
+  for (int i = 0; i < last; ++i) {
+    const float2 v = *reinterpret_cast<const float2*>(base + i * (HD + 2) + lane * 2);
+    const float wi = lane_value(w, i);
+    o0 = there >> i & 1 ? __builtin_fmaf(wi, v.x, o0) : o0;  // nothing may have been written there
+    o1 = there >> i & 1 ? __builtin_fmaf(wi, v.y, o1) : o1;
+  }
+  *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(o0 / L, o1 / L);
+}
+
 // ---- reading back ------------------------------------------------------------------------------------------------------
 // kv (rows, L * 2 * KV * 128): per layer KV keys, then KV values, of position pos_of[i] of slot slot_of[i]; pages (L, pages,
 // KV, P, 128). 16 lanes a vector, 8 values each; a workgroup takes 16 vectors of a row, in ROWS rows.
@@ -598,10 +626,12 @@ int attention_entry(PagedArgs p, int64_t rows, int64_t seqs, int64_t slots, int6
   COHERE_REQUIRE(wgs <= TOP && rows * heads <= TOP, nm + ": too many rows and heads");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)wgs, (unsigned)splits);
-  if (many_rows(rows, seqs, p.ratio) && p.scale != 0.f) launch_chunk(p, Q8, s);
+  const bool many = many_rows(rows, seqs, p.ratio) && p.scale != 0.f;
+  if (many) launch_chunk(p, Q8, s);
   else launch_rows<Q8>(p, grid, s);
   const unsigned hs = (unsigned)(rows * heads);
-  if (splits > 4) paged_combine_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
+  if (splits > 1 && many) paged_combine_many_kernel<<<(hs + 3) / 4, 256, 0, s>>>(p.part, p.starts, p.S, hs, p.H, p.parts, p.out);
+  else if (splits > 4) paged_combine_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
   else if (splits > 1) paged_combine_kernel<1, 4><<<hs, HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
   return cohere::check_launch(name);
 }

@@ -13,6 +13,7 @@
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
 // need three products for one).
 #include "paged.h"
+#include <cstdlib>
 
 namespace {
 
@@ -32,6 +33,17 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 // used by nothing else in these kernels.
 DEVI void copy_to_lds(const void* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+// the same through a buffer: from `offset` behind its start, zeros behind its end. Five wait states lie between a vector
+// instruction's write of a scalar register and a memory instruction's read of it.
+DEVI void buffer_to_lds(v4i buffer, uint32_t offset, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(offset), "s"(buffer)
+               : "memory");
+}
+DEVI v4i buffer_of(const void* base, int64_t offset, uint32_t bytes) {
+  const uint64_t at = (uint64_t)base + offset;
+  const auto uniform = [](uint32_t x) { return (int)__builtin_amdgcn_readfirstlane((int)x); };
+  return v4i{uniform((uint32_t)at), uniform((uint32_t)(at >> 32) & 0xffffu), uniform(bytes), 0x00027000};
 }
 DEVI uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(LDS_AS const void*)p; }
 
@@ -65,12 +77,16 @@ paged_chunk_kernel(const PagedArgs p) {
   }
   const float scale = fabsf(p.scale);
   int n = t.ok ? p.n[t.slot] : -1;
+  const int32_t* row = p.table + (int64_t)t.slot * p.W;
+  const int entry0 = row[min(lane >> p.shift, p.W - 1)];  // of a first part's first tile, on its way beside n
   const bool row_ok = n >= 0;
   n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
   const int hi = row_ok ? (t.x0 + t.rows - 1) / p.ratio + 1 : 0;  // the chunk's tokens that the tile's last row sees
   const int np = (n + KT - 1) / KT, nb = np + (hi + KT - 1) / KT;
-  const int chunk = (nb + nsp - 1) / nsp, start = min(nb, sp * chunk), end = min(nb, start + chunk);
-  const int32_t* row = p.table + (int64_t)t.slot * p.W;
+  // as many parts as there are for `least` tiles each
+  const int parts = max(1, min(nsp, (nb + p.least - 1) / p.least));
+  if (sp >= parts) return;
+  const int chunk = (nb + parts - 1) / parts, start = min(nb, sp * chunk), end = min(nb, start + chunk);
   const int P1 = (1 << p.shift) - 1;
   const uint16_t* rowkv = p.q + (int64_t)t.first * p.ldq + (p.H + kvh) * HD;
 
@@ -81,20 +97,66 @@ paged_chunk_kernel(const PagedArgs p) {
     const int at = first_of(b) + lane;
     return (uint64_t)__ballot(b < np ? at < n && (unsigned)entry < (unsigned)p.pages : at < hi);
   };
-  // the vector of key kk of a page tile; every lane has to be active
+  // the vector of key kk of a tile of small pages; every lane has to be active
   const auto vec_of = [&](int t0, int entry, int kk) {
-    const int page = BIG ? __builtin_amdgcn_readlane(entry, wave * 16) : __shfl(entry, kk, 64);
-    return (((int64_t)page * p.KV + kvh) << p.shift) + ((t0 + kk) & P1);
+    return (((int64_t)__shfl(entry, kk, 64) * p.KV + kvh) << p.shift) + ((t0 + kk) & P1);
   };
-  // int8 pages: 16 keys a wave on their way through registers
+  // A wave brings 16 keys of a tile. In LDS the 16-byte pieces c of a key's 256 bytes lie at 16 (c ^ key % 16), of a value's at
+  // 16 (c ^ 4 (key % 4)); the i-th copy is of 4 keys, 16 lanes each. int8 pages come through registers.
   v4i kr[2], vr[2];
   float sr;
+  const int kk0 = wave * 16, k4 = lane >> 4;
+  const uint32_t piece_v = (uint32_t)((lane & 15) ^ (k4 << 2)) * 16;
+  const auto piece_k = [&](int i) { return (uint32_t)((lane & 15) ^ (i * 4 + k4)) * 16; };
   const auto issue = [&](int b, int entry, uint64_t live, int buf) {
     const int t0 = first_of(b);
-    if (Q8 && b < np) {
+    const uint32_t kdst = __builtin_amdgcn_readfirstlane(lds_address(kbuf[buf])) + kk0 * 256,
+                   vdst = __builtin_amdgcn_readfirstlane(lds_address(vbuf[buf])) + kk0 * 256;
+    if (b >= np) {  // of the chunk's tokens
+      const uint32_t stride = (uint32_t)p.ldq * 2, bytes = (uint32_t)max(min(hi - t0 - kk0, 16), 0) * stride;
+      const int64_t at = (int64_t)(t0 + kk0) * stride;
+      const v4i kb = buffer_of(rowkv, at, bytes), vb = buffer_of(rowkv + p.KV * HD, at, bytes);
+      uint32_t first = k4;
+      asm volatile("" : "+v"(first));  // the offsets are made here: kept over the tiles they would take 8 registers
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t offset = (i * 4 + first) * stride;
+        buffer_to_lds(kb, offset + piece_k(i), kdst + i * 1024);
+        buffer_to_lds(vb, offset + piece_v, vdst + i * 1024);
+      }
+      sr = 1.f;
+    } else if constexpr (BIG) {  // the wave's keys are one page's
+      const int page = __builtin_amdgcn_readlane(entry, kk0);
+      const bool ok = (unsigned)page < (unsigned)p.pages;
+      const int64_t vec = (((int64_t)(ok ? page : 0) * p.KV + kvh) << p.shift) + ((t0 + kk0) & P1);
+      const uint32_t keys = ok ? (uint32_t)max(min(n - t0 - kk0, 16), 0) : 0;
+      if constexpr (Q8) {
+        const auto from = [&](const void* pages, int size) {
+          return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(pages)) + vec * size, 0,
+                                                   keys * size, 0x00027000);
+        };
+        const auto kb = from(p.k, HD), vb = from(p.v, HD);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          kr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, lane * 16 + i * 1024, 0, 0));
+          vr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vb, lane * 16 + i * 1024, 0, 0));
+        }
+        const int at = (lane & 15) * 4;
+        const uint32_t ks = __builtin_amdgcn_raw_buffer_load_b32(from(p.ks, 4), at, 0, 0),
+                       vs = __builtin_amdgcn_raw_buffer_load_b32(from(p.vs, 4), at, 0, 0);
+        sr = __uint_as_float(lane < 16 ? ks : vs);
+      } else {
+        const v4i kb = buffer_of(p.k, vec * (2 * HD), keys * (2 * HD)), vb = buffer_of(p.v, vec * (2 * HD), keys * (2 * HD));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          buffer_to_lds(kb, (i * 4 + k4) * 256 + piece_k(i), kdst + i * 1024);
+          buffer_to_lds(vb, (i * 4 + k4) * 256 + piece_v, vdst + i * 1024);
+        }
+      }
+    } else if constexpr (Q8) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int kk = wave * 16 + i * 8 + (lane >> 3);
+        const int kk = kk0 + i * 8 + (lane >> 3);
         const int64_t vec = vec_of(t0, entry, kk);
         const bool there = live >> kk & 1;
         const int64_t at = (there ? vec : 0) * HD + (lane & 7) * 16;
@@ -102,29 +164,22 @@ paged_chunk_kernel(const PagedArgs p) {
         vr[i] = *reinterpret_cast<const v4i*>(static_cast<const int8_t*>(p.v) + at);
         if (!there) kr[i] = vr[i] = v4i{0, 0, 0, 0};
       }
-      const int kk = wave * 16 + (lane & 15);
+      const int kk = kk0 + (lane & 15);
       const int64_t vec = vec_of(t0, entry, kk);
       const bool there = live >> kk & 1;
       sr = (lane < 16 ? p.ks : p.vs)[there ? vec : 0];
       sr = there ? sr : 0.f;
-      return;
-    }
-    // one way for both kinds of tile: a branch would make the compiler wait for the loads in flight
-    const bool own = Q8 || b >= np;
-    const char* kb = own ? reinterpret_cast<const char*>(rowkv) : static_cast<const char*>(p.k);
-    const char* vb = own ? reinterpret_cast<const char*>(rowkv + p.KV * HD) : static_cast<const char*>(p.v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int kk = wave * 16 + i * 4 + (lane >> 4), ck = (lane & 15) ^ (kk & 15), cv = (lane & 15) ^ ((kk & 3) << 2);
-      const int64_t held = Q8 ? 0 : vec_of(t0, entry, kk) * (2 * HD), given = (int64_t)(t0 + kk) * p.ldq * 2;
-      const int64_t at = own ? given : held;
-      const bool there = live >> kk & 1;
-      const char* kp = there ? kb + at + ck * 16 : reinterpret_cast<const char*>(zero_row);
-      const char* vp = there ? vb + at + cv * 16 : reinterpret_cast<const char*>(zero_row);
-      copy_to_lds(kp, __builtin_amdgcn_readfirstlane(lds_address(kbuf[buf])) + (wave * 16 + i * 4) * 256);
-      copy_to_lds(vp, __builtin_amdgcn_readfirstlane(lds_address(vbuf[buf])) + (wave * 16 + i * 4) * 256);
+      for (int i = 0; i < 4; ++i) {
+        const int kk = kk0 + i * 4 + k4;
+        const int64_t at = vec_of(t0, entry, kk) * (2 * HD);
+        const bool there = live >> kk & 1;
+        const char* zero = reinterpret_cast<const char*>(zero_row);
+        copy_to_lds(there ? static_cast<const char*>(p.k) + at + piece_k(i) : zero, kdst + i * 1024);
+        copy_to_lds(there ? static_cast<const char*>(p.v) + at + piece_v : zero, vdst + i * 1024);
+      }
     }
-    sr = 1.f;
   };
   // int8: what is in the registers goes into LDS
   const auto convert = [&](int b, int buf) {
@@ -163,110 +218,155 @@ paged_chunk_kernel(const PagedArgs p) {
   float base = -INFINITY, l = 0.f;
   bool bad = false;  // some values of the chunk's own tokens are infinite or NaN
 
-  int entry = 0;
-  uint64_t live = 0, next = 0;
-  if (start < end) {
-    entry = entry_of(start);
-    next = live_of(start, entry);
-    issue(start, entry, next, 0);
-    convert(start, 0);
-    entry = start + 1 < end ? entry_of(start + 1) : 0;
-  }
-  for (int b = start; b < end; ++b) {
-    const int buf = (b - start) & 1;
-    asm volatile("" : "+v"(entry));  // waited for here, not behind the next tile's loads
-    tile_barrier();                  // this tile is in LDS, and no wave reads the other buffer any more
-    live = next;
-    if (b + 1 < end) {
-      next = live_of(b + 1, entry);
-      issue(b + 1, entry, next, buf ^ 1);
-      if (b + 2 < end) entry = entry_of(b + 2);
-    }
+  // a tile's products; OWN: of the chunk's tokens
+  const auto tile = [&](int b, int buf, uint64_t live, auto own) {
+    constexpr bool OWN = decltype(own)::value;
     const int t0 = first_of(b);
-    // rows of the chunk that no row of the wave's sees
-    if (!(idle || (b >= np && t0 > tok1))) {
-      const bool causal = b >= np && t0 + KT - 1 > tok0;
+    if (idle || (OWN && t0 > tok1)) return;  // no row of the wave's sees them
+    const bool causal = OWN && t0 + KT - 1 > tok0;
+    constexpr int AHEAD = Q8 ? 4 : 6;  // keys' pieces on their way from LDS
+    // The order of these steps is this source's, kept by the fences: vector work stands between the matrix products, which
+    // take 32 cycles each whatever else the wave does, and what is read from LDS is asked for some products ahead.
+    v16f s[2];  // scores, then weights, of 32 keys each
+    v8bf kf[AHEAD];
+    const auto read_k = [&](int j) {
+      kf[j % AHEAD] = *reinterpret_cast<const v8bf*>(kbuf[buf] + ((j >> 3) * 32 + col) * 256 +
+                                                     ((((j & 7) * 2 + half) ^ (col & 15)) * 16));
+    };
+    // keys 16 u + 4 half + (lane % 16) / 4 (and 8 on), dimensions 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) ..
+    v8bf vf[2][4];
+    const auto read_v = [&](int u) {
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {  // 32 keys
-        v16f s;
+      for (int dt = 0; dt < 4; ++dt) {
+        const int kk = half * 4 + ((lane & 15) >> 2), c = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+        const char* src = vbuf[buf] + (u * 16 + kk) * 256 + ((c ^ ((kk & 3) << 2)) * 16) + (lane & 1) * 8;
+        const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)src);
+        const v4s d = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)(src + 8 * 256));
+        vf[u & 1][dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(a, d, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    };
+    v4f ks[Q8 ? 4 : 1], vs[Q8 ? 2 : 1][2];  // scales of the lane's keys of 32, of 16
+    const auto read_ks = [&](int z) {
+      if constexpr (Q8)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-        const char* src = kbuf[buf] + (z * 32 + col) * 256;
+        for (int g = 0; g < 4; ++g) ks[g] = *reinterpret_cast<const v4f*>(&sscale[buf][0][z * 32 + g * 8 + half * 4]);
+    };
+    const auto read_vs = [&](int u) {
+      if constexpr (Q8)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const v8bf kf = *reinterpret_cast<const v8bf*>(src + (((c * 2 + half) ^ (col & 15)) * 16));
-          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c], s, 0, 0, 0);
-        }
-        if constexpr (Q8) {
+        for (int g = 0; g < 2; ++g) vs[u & 1][g] = *reinterpret_cast<const v4f*>(&sscale[buf][1][u * 16 + g * 8 + half * 4]);
+    };
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const v4f k4 = *reinterpret_cast<const v4f*>(&sscale[buf][0][z * 32 + g * 8 + half * 4]);
+    for (int j = 0; j < AHEAD; ++j) read_k(j);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[4 * g + k] *= k4[k];
-          }
-        }
-        if (causal || live != ~0ull) {
-          // bit r of seen: key z 32 + 8 (r / 4) + 4 half + r % 4 is there, and not behind the query's token
-          const uint32_t there = (uint32_t)(live >> (z * 32)) >> (half * 4);
-          const int upto = causal ? tok - t0 - z * 32 - half * 4 : 32;
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    float mx = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int kk = (r >> 2) * 8 + (r & 3);
-            s[r] = (there >> kk & 1) && kk <= upto ? s[r] : -INFINITY;
-          }
-        }
-        float mx = s[0];
+    for (int j = 0; j < 16; ++j) {
+      s[j >> 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD], qf[j & 7], s[j >> 3], 0, 0, 0);
+      if (j + AHEAD < 16) read_k(j + AHEAD);
+      if (j + AHEAD == 16) read_v(0);
+      if constexpr (Q8) {  // the first half's scales under the second half's products
+        if (j == 5) read_ks(0);
+        if (j >= 10 && j < 14)
 #pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx = xor32_max(mx) * scale;
-        if (__any(mx > base)) {
-          const float to = mx > base ? mx + RISE : base, a = to == -INFINITY ? 1.f : exp2_hw(base - to);
-          l *= a;
+          for (int k = 0; k < 4; ++k) s[0][4 * (j - 10) + k] *= ks[j - 10][k];
+        if (j == 14) read_ks(1);
+        if (j == 15) read_vs(0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (Q8)
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt)
+      for (int r = 0; r < 16; ++r) s[1][r] *= ks[r >> 2][r & 3];
+    if (causal || live != ~0ull) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
-          base = to;
-        }
-        const float off = base == -INFINITY ? 0.f : -base;
+      for (int z = 0; z < 2; ++z) {
+        // bit 8 (r / 4) + r % 4: key z 32 + 8 (r / 4) + 4 half + r % 4 is there, and not behind the query's token
+        const int upto = causal ? tok - t0 - z * 32 : 31;
+        const uint32_t seen = (uint32_t)(live >> (z * 32)) & (upto < 0 ? 0u : ~0u >> max(31 - upto, 0)), mine = seen >> (half * 4);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[r] = exp2_hw(__builtin_fmaf(s[r], scale, off));
-          l += s[r];
-        }
-        if constexpr (Q8) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const v4f v4 = *reinterpret_cast<const v4f*>(&sscale[buf][1][z * 32 + g * 8 + half * 4]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[4 * g + k] *= v4[k];
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {  // 16 keys a product
-          v4i w;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = (int)pack_bf2(s[u * 8 + 2 * k], s[u * 8 + 2 * k + 1]);
-          const v8bf pf = __builtin_bit_cast(v8bf, w);
-          const int k0 = z * 32 + u * 16;
-          v8bf vf[4];
-#pragma unroll
-          for (int dt = 0; dt < 4; ++dt) {
-            // keys k0 + 4 half + (lane % 16) / 4 (and 8 on), dimensions 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) ..
-            const int kk = half * 4 + ((lane & 15) >> 2), c = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-            const char* src = vbuf[buf] + (k0 + kk) * 256 + ((c ^ ((kk & 3) << 2)) * 16) + (lane & 1) * 8;
-            const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)src);
-            const v4s d = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)(src + 8 * 256));
-            vf[dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(a, d, 0, 1, 2, 3, 4, 5, 6, 7));
-          }
-          if (causal) bad |= leave_out(vf);
-#pragma unroll
-          for (int dt = 0; dt < 4; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[dt], pf, acc[dt], 0, 0, 0);
+          const int kk = (r >> 2) * 8 + (r & 3);
+          const uint32_t keep = (uint32_t)((int)(mine << (31 - kk)) >> 31);
+          s[z][r] = __uint_as_float((__float_as_uint(s[z][r]) & keep) | (0xff800000u & ~keep));
         }
       }
     }
-    if (b + 1 < end) convert(b + 1, buf ^ 1);
+#pragma unroll
+    for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+    mx = xor32_max(mx) * scale;
+    if (__any(mx > base)) {
+      const float to = mx > base ? mx + RISE : base, a = to == -INFINITY ? 1.f : exp2_hw(base - to);
+      l *= a;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
+      base = to;
+    }
+    const float off = base == -INFINITY ? 0.f : -base;
+    // 16 keys a product: weights of keys u 16 .. as the lane's scores s[u / 2][8 (u % 2) ..], a quarter of them at a time
+    v4i w[2];
+    const auto weigh = [&](int u, int k) {
+      float e[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        e[i] = exp2_hw(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + 2 * k + i], scale, off));
+        l += e[i];
+        if constexpr (Q8) e[i] *= vs[u & 1][k >> 1][(k & 1) * 2 + i];
+      }
+      w[u & 1][k] = (int)pack_bf2(e[0], e[1]);
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) weigh(0, k);
+    read_vs(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (u < 3) read_v(u + 1);
+      if constexpr (OWN)
+        if (causal) bad |= leave_out(vf[u & 1]);
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u & 1][dt], __builtin_bit_cast(v8bf, w[u & 1]), acc[dt], 0, 0, 0);
+        if (u < 3) weigh(u + 1, dt);
+        if (dt == 3 && u < 2) read_vs(u + 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  int entry = 0;
+  uint64_t next = 0;
+  if (start < end) {
+    entry = start == 0 ? entry0 : entry_of(start);
+    next = live_of(start, entry);
+    issue(start, entry, next, 0);
   }
+  if (sp == 0 && row_ok) append<Q8, W, 8>(p, t, n, kvh, TM);
+  if (start < end) {
+    convert(start, 0);
+    entry = start + 1 < end ? entry_of(start + 1) : 0;
+  }
+  const auto tiles = [&](int b, int to, auto own) {
+    for (; b < to; ++b) {
+      const int buf = (b - start) & 1;
+      asm volatile("" : "+v"(entry));  // waited for here, not behind the next tile's loads
+      tile_barrier();                  // this tile is in LDS, and no wave reads the other buffer any more
+      const uint64_t live = next;
+      if (b + 1 < end) {
+        next = live_of(b + 1, entry);
+        issue(b + 1, entry, next, buf ^ 1);
+        if (b + 2 < end) entry = entry_of(b + 2);
+      }
+      tile(b, buf, live, own);
+      if (b + 1 < end) convert(b + 1, buf ^ 1);
+    }
+  };
+  tiles(start, min(end, np), std::false_type{});
+  tiles(max(start, np), end, std::true_type{});
   l = xor32_sum(l);
   if (wave * 32 + col < t.rows) {
     if (__builtin_expect(bad, 0)) {
@@ -284,7 +384,7 @@ paged_chunk_kernel(const PagedArgs p) {
       }
     }
     const int64_t at = (int64_t)(t.first + tok) * p.H + head;
-    if (nsp == 1) {
+    if (parts == 1) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = p.out + at * HD + half * 4;
 #pragma unroll
@@ -308,8 +408,14 @@ paged_chunk_kernel(const PagedArgs p) {
                 make_float2(acc[dt][4 * g + k], acc[dt][4 * g + k + 1]);
       if (half == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(base, l);
     }
+    // for the joining: a negative sum, there is nothing to join; nothing in the parts that are not made
+    if (sp == 0 && half == 0) {
+      float* part = p.part + at * nsp * (HD + 2) + HD;
+      if (nsp > 1 && parts == 1) *reinterpret_cast<float2*>(part) = make_float2(0.f, -1.f);
+      for (int i = parts == 1 ? nsp : parts; i < nsp; ++i)
+        *reinterpret_cast<float2*>(part + i * (HD + 2)) = make_float2(-INFINITY, 0.f);
+    }
   }
-  if (sp == 0 && row_ok) append<Q8, W>(p, t, n, kvh, TM);
 }
 
 }  // namespace
@@ -320,7 +426,8 @@ int64_t chunk_workgroups(const PagedArgs& p) {
   return tiles_for(p.R, p.S, p.ratio, TM, p.starts != nullptr) * p.KV;
 }
 
-void launch_chunk(const PagedArgs& p, bool q8, hipStream_t s) {
+void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
+  p.least = getenv("LEAST") ? atoi(getenv("LEAST")) : 16;
   const dim3 grid((unsigned)chunk_workgroups(p), (unsigned)p.parts);
   if (q8 && p.shift >= 4) paged_chunk_kernel<true, true><<<grid, W * 64, 0, s>>>(p);
   else if (q8) paged_chunk_kernel<true, false><<<grid, W * 64, 0, s>>>(p);

@@ -27,7 +27,7 @@ struct PagedArgs {
   float scale;  // times log2(e): scores are powers of two
   uint16_t* out;  // (rows, H * 128)
   float* part;    // (rows, H, parts, 130) when split: outputs, maximum (power of two), sum
-  int parts;
+  int parts, least;  // least: tiles of a part, many rows
 };
 
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -153,30 +153,37 @@ DEVI void store_vec(const uint4& u, void* pages, float* scales, int64_t vec, int
 }
 
 // The keys and values of the tile's own tokens (those whose first query row is in the tile) into their pages, by W waves,
-// the last one first (the first one has more to do where there are few keys).
+// the last one first (the first one has more to do where there are few keys), N steps' loads on their way at once.
 // No workgroup reads them there in the same launch: a chunk attends to its own tokens as given.
-template <bool Q8, int W>
+template <bool Q8, int W, int N>
 DEVI void append(const PagedArgs& p, const Tile& t, int n, int kvh, int TMrows) {
   const int lane = lane_id(), wave = W - 1 - wave_id(), d8 = lane & 15;
   const int j0 = (t.x0 + p.ratio - 1) / p.ratio, j1 = min(t.c, (t.x0 + TMrows + p.ratio - 1) / p.ratio);
-  const int P = 1 << p.shift;
-  for (int i = wave * 4; i < (j1 - j0) * 2; i += W * 4) {
-    const int at = i + (lane >> 4), j = j0 + (at >> 1), kvi = at & 1;
-    bool live = j < j1;
-    const int64_t pos = (int64_t)n + j;
-    const int64_t col = pos >> p.shift;
-    live = live && col < p.W;
-    const int page = live ? p.table[(int64_t)t.slot * p.W + col] : -1;
-    live = live && (unsigned)page < (unsigned)p.pages;
-    const int64_t vec = live ? (((int64_t)page * p.KV + kvh) << p.shift) + (pos & (P - 1)) : 0;
-    const uint4 u = *reinterpret_cast<const uint4*>(p.q + (int64_t)(t.first + min(j, t.c - 1)) * p.ldq +
-                                                    (p.H + kvi * p.KV + kvh) * HD + d8 * 8);
-    store_vec<Q8>(u, kvi ? p.v : p.k, kvi ? p.vs : p.ks, vec, d8, live);
+  const int P = 1 << p.shift, kvi = (lane >> 4) & 1;
+  const uint16_t* src = p.q + (int64_t)t.first * p.ldq + (p.H + kvi * p.KV + kvh) * HD + d8 * 8;
+  for (int i = wave * 4; i < (j1 - j0) * 2; i += N * W * 4) {
+    v4i u[N];
+    int page[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = j0 + ((i + k * W * 4 + (lane >> 4)) >> 1);
+      const int64_t column = ((int64_t)n + j) >> p.shift;
+      page[k] = p.table[(int64_t)t.slot * p.W + min(column, (int64_t)p.W - 1)];
+      if (j >= j1 || column >= p.W) page[k] = -1;
+      u[k] = *reinterpret_cast<const v4i*>(src + (int64_t)min(j, t.c - 1) * p.ldq);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t pos = (int64_t)n + j0 + ((i + k * W * 4 + (lane >> 4)) >> 1);
+      const bool live = (unsigned)page[k] < (unsigned)p.pages;
+      const int64_t vec = live ? (((int64_t)page[k] * p.KV + kvh) << p.shift) + (pos & (P - 1)) : 0;
+      store_vec<Q8>(__builtin_bit_cast(uint4, u[k]), kvi ? p.v : p.k, kvi ? p.vs : p.ks, vec, d8, live);
+    }
   }
 }
 
 // the kernel for chunks of many query rows (dec_paged_chunk.hip)
 int64_t chunk_workgroups(const PagedArgs& p);
-void launch_chunk(const PagedArgs& p, bool q8, hipStream_t s);
+void launch_chunk(PagedArgs p, bool q8, hipStream_t s);
 
 }  // namespace cohere_paged
