@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
 }
 
 // The same behind the kernel of many rows, whose rows have parts of their own number: a wave a (row, head), which reads those
-// parts alone that it has.
+// parts alone that it has, N at a time.
+template <int N>
 __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __restrict__ part, const int32_t* starts, int S,
                                                                  int64_t count, int H, int nsp, uint16_t* out) {
   const int lane = lane_id();
@@ -505,12 +506,18 @@ __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __
   float o0 = 0.f, o1 = 0.f;
   const uint64_t there = __ballot(in);
   const int last = 64 - __clzll(there);
-#pragma unroll 4
-  for (int i = 0; i < last; ++i) {
-    const float2 v = *reinterpret_cast<const float2*>(base + i * (HD + 2) + lane * 2);
-    const float wi = lane_value(w, i);
-    o0 = there >> i & 1 ? __builtin_fmaf(wi, v.x, o0) : o0;  // nothing may have been written there
-    o1 = there >> i & 1 ? __builtin_fmaf(wi, v.y, o1) : o1;
+  for (int i0 = 0; i0 < last; i0 += N) {
+    float2 v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = *reinterpret_cast<const float2*>(base + min(i0 + i, last - 1) * (HD + 2) + lane * 2);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i0 + i < last && there >> (i0 + i) & 1) {  // in the others nothing has to have been written
+        const float wi = lane_value(w, i0 + i);
+        o0 = __builtin_fmaf(wi, v[i].x, o0);
+        o1 = __builtin_fmaf(wi, v[i].y, o1);
+      }
   }
   *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(o0 / L, o1 / L);
 }
@@ -630,7 +637,9 @@ int attention_entry(PagedArgs p, int64_t rows, int64_t seqs, int64_t slots, int6
   if (many) launch_chunk(p, Q8, s);
   else launch_rows<Q8>(p, grid, s);
   const unsigned hs = (unsigned)(rows * heads);
-  if (splits > 1 && many) paged_combine_many_kernel<<<(hs + 3) / 4, 256, 0, s>>>(p.part, p.starts, p.S, hs, p.H, p.parts, p.out);
+  const unsigned hs4 = (hs + 3) / 4;
+  if (many && splits > 4) paged_combine_many_kernel<16><<<hs4, 256, 0, s>>>(p.part, p.starts, p.S, hs, p.H, p.parts, p.out);
+  else if (many && splits > 1) paged_combine_many_kernel<4><<<hs4, 256, 0, s>>>(p.part, p.starts, p.S, hs, p.H, p.parts, p.out);
   else if (splits > 4) paged_combine_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
   else if (splits > 1) paged_combine_kernel<1, 4><<<hs, HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
   return cohere::check_launch(name);
@@ -665,14 +674,14 @@ int gather_entry(GatherArgs p, int64_t rows, int64_t slots, int64_t width, int64
 
 extern "C" int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t T) {
   if (rows <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || T <= 0) return 1;
-  // Parts until the GPU is full, and then, where they stay long, until long and short sequences even out: few-row kernel,
-  // of 256 CUs x 3 workgroups: 1 x 8 heads over 64 K positions in 1, 16 and 64 parts 564, 50 and 44 us; 32 x 8 (x 4) over 1
-  // .. 16 K, int8, 1, 2 and 8 parts 187, 152 and 127; 64 x 8 over up to 1 K 21, 2 parts 25. Kernel of 128 rows, x 2: 256
-  // tokens over 32 K 855, 16 parts 86, 32 70; 8 x 512 tokens over nothing 33, 2 parts 47.
+  // Parts until the GPU is full, and then, where they stay long, until long and short sequences even out. Few-row kernel,
+  // of 256 CUs x 2 workgroups: 1 x 8 heads over 64 K positions in 1, 16 and 64 parts 564, 50 and 44 us; 32 x 8 (x 4) over 1
+  // .. 16 K, int8, 1, 2 and 8 parts 187, 152 and 126; 64 x 8 over up to 1 K 21, 2 parts 25. Kernel of 128 rows: 256 tokens
+  // over 32 K 606, 16 parts 72, 32 63; 9 ragged sequences of up to 3 K 106, 2 parts 85; 8 x 512 tokens over nothing 26, 2 31.
   const int64_t ratio = heads / kv_heads;
   const bool many = many_rows(rows, seqs, ratio);
   const int64_t wgs = tiles_for(rows, seqs, ratio, many ? 128 : 16, rows != seqs) * kv_heads;
-  const int64_t full = many ? 256 : 512, most = many ? 1024 : 2048, least = many ? 256 : 192, longer = many ? 512 : 1024;
+  const int64_t full = many ? 256 : 512, most = many ? 1024 : 2048, least = 192, longer = many ? 768 : 1024;
   int64_t n = 1;
   while (n < 64 && wgs * 2 * n <= most && T / (2 * n) >= (wgs * n < full ? least : longer)) n *= 2;
   return n;

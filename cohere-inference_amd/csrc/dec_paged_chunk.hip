@@ -8,12 +8,14 @@
 //   S^T = K Q^T on v_mfma_f32_32x32x16_bf16: queries in registers, a lane's result is 16 keys of query l % 32.
 //   O^T = V^T P^T on the same instruction: the weights as they stand are its B operand (the order of the 16 keys of a
 //   product is free, and taken as the lanes hold them), V^T comes through the transposing LDS read.
+// What bounds it: a tile's 32 products keep a SIMD's matrix core 1024 cycles, its 200 vector instructions (32 exponentials)
+// take about as long, and two waves a SIMD overlap them only in part. 4 x 2048 tokens x 32 heads behind 6 to 8 K positions:
+// 1086 us, 1013 TFLOP/s (a large product of the library: 1188); the matrix cores are busy 36% of the time, LDS 18%.
 // Maximum, sum and outputs of a query stay in lanes l % 32 = query. The base of a query's weights is set 2^8 above its
 // largest score and moves only when a score passes it, so that rescaling is rare and weights are at most 1.
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
 // need three products for one).
 #include "paged.h"
-#include <cstdlib>
 
 namespace {
 
@@ -57,7 +59,8 @@ paged_chunk_kernel(const PagedArgs p) {
   __shared__ __attribute__((aligned(16))) float sscale[Q8 ? 2 : 1][2][Q8 ? KT : 1];  // of a tile's keys and values
   const int lane = lane_id(), wave = wave_id(), col = lane & 31, half = lane >> 5;
   const int kvh = blockIdx.x % p.KV, sp = blockIdx.y, nsp = p.parts;
-  const Tile t = tile_of<TM>(p, blockIdx.x / p.KV);
+  // a chunk's last tiles first: they see the most keys, and what starts last ends last
+  const Tile t = tile_of<TM>(p, gridDim.x / p.KV - 1 - blockIdx.x / p.KV);
   if (t.rows == 0) return;
   // the lane's query row (the tile's last one repeated), its token and head
   const int x = t.x0 + min(wave * 32 + col, t.rows - 1), tok = x / p.ratio, head = kvh * p.ratio + (x - tok * p.ratio);
@@ -427,7 +430,10 @@ int64_t chunk_workgroups(const PagedArgs& p) {
 }
 
 void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
-  p.least = getenv("LEAST") ? atoi(getenv("LEAST")) : 16;
+  // Tiles that a part has at least: few where there are few workgroups (4 x 24 tokens over 1 K, 8 parts asked for: 14.9 us,
+  // with 12 tiles 19.4), else enough that a part's start and the joining are small beside it (9 ragged sequences of up to
+  // 3 K, 4 asked for: 90 us, with 4 tiles 95; 2048 tokens over nothing, 2 asked for: 75, no parts 62).
+  p.least = chunk_workgroups(p) < 256 ? 4 : 12;
   const dim3 grid((unsigned)chunk_workgroups(p), (unsigned)p.parts);
   if (q8 && p.shift >= 4) paged_chunk_kernel<true, true><<<grid, W * 64, 0, s>>>(p);
   else if (q8) paged_chunk_kernel<true, false><<<grid, W * 64, 0, s>>>(p);
