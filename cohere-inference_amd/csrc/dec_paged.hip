@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     bounds();
     end = nb;
   }
-  if (sp == 0 && row_ok) append<Q8, W, 2>(p, t, n, kvh, 16);
+  Append<Q8, W, 2> own;  // 16 tokens at most: two steps
+  const bool writes = sp == 0 && row_ok && own.load(p, t, n, kvh, 16, 0);
   if (first) {
     float dot = 0.f;
 #pragma unroll
@@ -386,6 +387,8 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     m = -INFINITY;
     l = 0.f;
   }
+
+  if (writes) own.store(p, n, kvh);
 
   // the waves' results meet: each wave's outputs by its share of the largest maximum, summed by all threads
   l = xor32_sum(xor16_sum(l));

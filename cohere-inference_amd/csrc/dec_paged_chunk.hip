@@ -348,7 +348,10 @@ paged_chunk_kernel(const PagedArgs p) {
     next = live_of(start, entry);
     issue(start, entry, next, 0);
   }
-  if (sp == 0 && row_ok) append<Q8, W, 8>(p, t, n, kvh, TM);
+  if (sp == 0 && row_ok) {
+    Append<Q8, W, 8> own;
+    for (int i = 0; own.load(p, t, n, kvh, TM, i); i += 8) own.store(p, n, kvh);
+  }
   if (start < end) {
     convert(start, 0);
     entry = start + 1 < end ? entry_of(start + 1) : 0;

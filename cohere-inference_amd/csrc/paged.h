@@ -153,34 +153,42 @@ DEVI void store_vec(const uint4& u, void* pages, float* scales, int64_t vec, int
 }
 
 // The keys and values of the tile's own tokens (those whose first query row is in the tile) into their pages, by W waves,
-// the last one first (the first one has more to do where there are few keys), N steps' loads on their way at once.
+// the last one first (the first one has more to do where there are few keys), 4 vectors a wave and step: N steps from step
+// i on are loaded, and stored later.
 // No workgroup reads them there in the same launch: a chunk attends to its own tokens as given.
 template <bool Q8, int W, int N>
-DEVI void append(const PagedArgs& p, const Tile& t, int n, int kvh, int TMrows) {
-  const int lane = lane_id(), wave = W - 1 - wave_id(), d8 = lane & 15;
-  const int j0 = (t.x0 + p.ratio - 1) / p.ratio, j1 = min(t.c, (t.x0 + TMrows + p.ratio - 1) / p.ratio);
-  const int P = 1 << p.shift, kvi = (lane >> 4) & 1;
-  const uint16_t* src = p.q + (int64_t)t.first * p.ldq + (p.H + kvi * p.KV + kvh) * HD + d8 * 8;
-  for (int i = wave * 4; i < (j1 - j0) * 2; i += N * W * 4) {
-    v4i u[N];
-    int page[N];
+struct Append {
+  v4i u[N];
+  int page[N], first;
+
+  // whether there is something to do
+  DEVI bool load(const PagedArgs& p, const Tile& t, int n, int kvh, int TMrows, int i) {
+    const int lane = lane_id(), kvi = (lane >> 4) & 1;
+    const int j0 = (t.x0 + p.ratio - 1) / p.ratio, j1 = min(t.c, (t.x0 + TMrows + p.ratio - 1) / p.ratio);
+    first = j0 * 2 + (i * W + W - 1 - wave_id()) * 4 + (lane >> 4);
+    if (first - (lane >> 4) >= j1 * 2) return false;
+    const uint16_t* src = p.q + (int64_t)t.first * p.ldq + (p.H + kvi * p.KV + kvh) * HD + (lane & 15) * 8;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int j = j0 + ((i + k * W * 4 + (lane >> 4)) >> 1);
+      const int j = (first + k * W * 4) >> 1;
       const int64_t column = ((int64_t)n + j) >> p.shift;
       page[k] = p.table[(int64_t)t.slot * p.W + min(column, (int64_t)p.W - 1)];
       if (j >= j1 || column >= p.W) page[k] = -1;
       u[k] = *reinterpret_cast<const v4i*>(src + (int64_t)min(j, t.c - 1) * p.ldq);
     }
+    return true;
+  }
+  DEVI void store(const PagedArgs& p, int n, int kvh) const {
+    const int lane = lane_id(), kvi = (lane >> 4) & 1;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int64_t pos = (int64_t)n + j0 + ((i + k * W * 4 + (lane >> 4)) >> 1);
+      const int64_t pos = (int64_t)n + ((first + k * W * 4) >> 1);
       const bool live = (unsigned)page[k] < (unsigned)p.pages;
-      const int64_t vec = live ? (((int64_t)page[k] * p.KV + kvh) << p.shift) + (pos & (P - 1)) : 0;
-      store_vec<Q8>(__builtin_bit_cast(uint4, u[k]), kvi ? p.v : p.k, kvi ? p.vs : p.ks, vec, d8, live);
+      const int64_t vec = live ? (((int64_t)page[k] * p.KV + kvh) << p.shift) + (pos & ((1 << p.shift) - 1)) : 0;
+      store_vec<Q8>(__builtin_bit_cast(uint4, u[k]), kvi ? p.v : p.k, kvi ? p.vs : p.ks, vec, lane & 15, live);
     }
   }
-}
+};
 
 // the kernel for chunks of many query rows (dec_paged_chunk.hip)
 int64_t chunk_workgroups(const PagedArgs& p);
