@@ -255,3 +255,77 @@ def test_long_context(gpu):
     c = Paged(14, [9000], [2], 1, 4, 64, 16)
     _check(c, 32)
     _check(c, 1)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.07, 1e-30])
+def test_scales(gpu, scale):
+    """Scales that turn the order of the scores round, or leave nothing of it."""
+    for chunk, splits in (([1, 1], 1), ([1, 1], 3), ([90, 20], 1), ([90, 20], 4)):
+        c = Paged(15, [300, 0], chunk, 2, 2, 16, 16)
+        c.scale = scale
+        _check(c, splits, weights_bf16=True)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_parts_of_a_tiles_own_number(gpu, bits):
+    """So many sequences that parts have to be long: some have several, some one, some no row."""
+    c = Paged(16, [1700, 0, 90, 800] * 8, [18, 17, 0, 40] * 8, 8, 1, 16, bits)
+    for splits in (2, 5):
+        _check(c, splits, weights_bf16=True)
+
+
+def test_chunks_captured_while_positions_move(gpu):
+    """A captured chunk whose sequences have other numbers of parts in every replay, its workspace left as it was."""
+    from kernels.cuda_ext import ext
+
+    c = Paged(17, [900, 300, 0], [60, 30, 50], 2, 2, 16, 16)
+    starts, active, q, k, v, table, n = (t.cuda() for t in (c.starts, c.active, c.q.contiguous(), c.k.nan_to_num(),
+                                                            c.v.nan_to_num(), c.table, c.n))
+    out = torch.zeros(c.rows, c.H * D, dtype=BF, device="cuda")
+    part = torch.full((c.rows * c.H * 6 * 130,), float("nan"), device="cuda")
+
+    def call(splits=6):
+        ext.dec_attention_paged(active, starts, q, k, v, table, n, c.scale, splits, part, out)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    slots = c.active.long()
+    for held in ([900, 300, 0], [0, 0, 0], [10, 299, 0], [860, 0, 0], [900, 300, 0]):
+        now = c.n.clone()
+        now[slots] = torch.tensor(held, dtype=torch.int32)
+        n.copy_(now.cuda())
+        out.zero_()
+        part.fill_(float("nan"))
+        call()
+        want = out.clone()
+        part.fill_(-3.0)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        torch.randn(1000, device="cuda").sum()
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams, each with its own cache and workspace, beside each other."""
+    from kernels.cuda_ext import ext
+
+    runs, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i, chunk in enumerate(([1, 1, 1], [33, 80, 7])):
+        c = Paged(18 + i, [500, 40, 7], chunk, 4, 2, 16, 16)
+        t = [x.cuda() for x in (c.active, c.starts, c.q.contiguous(), c.k, c.v, c.table, c.n)]
+        out = torch.zeros(c.rows, c.H * D, dtype=BF, device="cuda")
+        part = torch.empty(c.rows * c.H * 4 * 130, device="cuda")
+        runs.append((c, t, part, out))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, (c, t, part, out) in zip(streams, runs):
+            with torch.cuda.stream(s):
+                ext.dec_attention_paged(*t, c.scale, 4, part, out)
+    torch.cuda.synchronize()
+    for c, _, _, out in runs:
+        want, bound, _ = c.attention64(weights_bf16=True)
+        close(out.cpu(), want, bound)
