@@ -8,9 +8,10 @@
 //   S^T = K Q^T on v_mfma_f32_32x32x16_bf16: queries in registers, a lane's result is 16 keys of query l % 32.
 //   O^T = V^T P^T on the same instruction: the weights as they stand are its B operand (the order of the 16 keys of a
 //   product is free, and taken as the lanes hold them), V^T comes through the transposing LDS read.
-// What bounds it: a tile's 32 products keep a SIMD's matrix core 1024 cycles, its 200 vector instructions (32 exponentials)
-// take about as long, and two waves a SIMD overlap them only in part. 4 x 2048 tokens x 32 heads behind 6 to 8 K positions:
-// 1086 us, 1013 TFLOP/s (a large product of the library: 1188); the matrix cores are busy 36% of the time, LDS 18%.
+// What bounds it: a tile's 32 products keep a SIMD's matrix core 1024 cycles and its 200 vector instructions (32 exponentials
+// at 8 cycles) about as long; a wave does one after the other, and two waves a SIMD, what the registers allow, overlap them
+// only in part. 4 x 2048 tokens x 32 heads behind 6 to 8 K positions: 1044 us, 1054 TFLOP/s (a large product of the library:
+// 1188); a tile alone on its CU takes 1.2 us, int8 1.9 (their conversion).
 // Maximum, sum and outputs of a query stay in lanes l % 32 = query. The base of a query's weights is set 2^8 above its
 // largest score and moves only when a score passes it, so that rescaling is rare and weights are at most 1.
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
@@ -222,20 +223,19 @@ paged_chunk_kernel(const PagedArgs p) {
   bool bad = false;  // some values of the chunk's own tokens are infinite or NaN
 
   // a tile's products; OWN: of the chunk's tokens
-  const auto tile = [&](int b, int buf, uint64_t live, auto own) {
+  constexpr int AHEAD = Q8 ? 4 : 6;  // keys' pieces on their way from LDS
+  const auto read_k = [&](v8bf (&kf)[AHEAD], int buf, int j) {
+    kf[j % AHEAD] = *reinterpret_cast<const v8bf*>(kbuf[buf] + ((j >> 3) * 32 + col) * 256 +
+                                                   ((((j & 7) * 2 + half) ^ (col & 15)) * 16));
+  };
+  const auto tile = [&](int b, int buf, uint64_t live, v8bf (&kf)[AHEAD], auto own) {
     constexpr bool OWN = decltype(own)::value;
     const int t0 = first_of(b);
     if (idle || (OWN && t0 > tok1)) return;  // no row of the wave's sees them
     const bool causal = OWN && t0 + KT - 1 > tok0;
-    constexpr int AHEAD = Q8 ? 4 : 6;  // keys' pieces on their way from LDS
-    // The order of these steps is this source's, kept by the fences: vector work stands between the matrix products, which
-    // take 32 cycles each whatever else the wave does, and what is read from LDS is asked for some products ahead.
+      // The order of these steps is this source's, kept by the fences: vector work stands between the matrix products, for the
+    // other wave's products to run under, and what is read from LDS is asked for some products ahead.
     v16f s[2];  // scores, then weights, of 32 keys each
-    v8bf kf[AHEAD];
-    const auto read_k = [&](int j) {
-      kf[j % AHEAD] = *reinterpret_cast<const v8bf*>(kbuf[buf] + ((j >> 3) * 32 + col) * 256 +
-                                                     ((((j & 7) * 2 + half) ^ (col & 15)) * 16));
-    };
     // keys 16 u + 4 half + (lane % 16) / 4 (and 8 on), dimensions 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) ..
     v8bf vf[2][4];
     const auto read_v = [&](int u) {
@@ -260,15 +260,16 @@ paged_chunk_kernel(const PagedArgs p) {
         for (int g = 0; g < 2; ++g) vs[u & 1][g] = *reinterpret_cast<const v4f*>(&sscale[buf][1][u * 16 + g * 8 + half * 4]);
     };
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) read_k(j);
-#pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
     float mx = -INFINITY;
+    // Within a wave nothing runs under a matrix product, another wave's vector work does: of the two waves of a SIMD the one
+    // with products alone to do goes first (4 x 2048 tokens 1068 -> 1050 us, int8 1457 -> 1348).
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       s[j >> 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD], qf[j & 7], s[j >> 3], 0, 0, 0);
-      if (j + AHEAD < 16) read_k(j + AHEAD);
+      if (j + AHEAD < 16) read_k(kf, buf, j + AHEAD);
       if (j + AHEAD == 16) read_v(0);
       if constexpr (Q8) {  // the first half's scales under the second half's products
         if (j == 5) read_ks(0);
@@ -310,6 +311,7 @@ paged_chunk_kernel(const PagedArgs p) {
       base = to;
     }
     const float off = base == -INFINITY ? 0.f : -base;
+    __builtin_amdgcn_s_setprio(0);
     // 16 keys a product: weights of keys u 16 .. as the lane's scores s[u / 2][8 (u % 2) ..], a quarter of them at a time
     v4i w[2];
     const auto weigh = [&](int u, int k) {
@@ -362,12 +364,15 @@ paged_chunk_kernel(const PagedArgs p) {
       asm volatile("" : "+v"(entry));  // waited for here, not behind the next tile's loads
       tile_barrier();                  // this tile is in LDS, and no wave reads the other buffer any more
       const uint64_t live = next;
+      v8bf kf[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) read_k(kf, buf, j);
       if (b + 1 < end) {
         next = live_of(b + 1, entry);
         issue(b + 1, entry, next, buf ^ 1);
         if (b + 2 < end) entry = entry_of(b + 2);
       }
-      tile(b, buf, live, own);
+      tile(b, buf, live, kf, own);
       if (b + 1 < end) convert(b + 1, buf ^ 1);
     }
   };
