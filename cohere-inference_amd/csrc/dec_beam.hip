@@ -303,15 +303,18 @@ DEVI uint64_t best_of(const uint64_t (&key)[N], int B, uint64_t* cand, uint64_t*
 // candidates are ranked by counting, a thread each.
 __global__ void __launch_bounds__(64 * MAXB) beam_merge_kernel(const SelectArgs a) {
   __shared__ double srank[MAXB * MAXB], stotal[MAXB * MAXB];
-  __shared__ int sv[MAXB * MAXB], splace[MAXB * MAXB];
+  __shared__ uint64_t sid[MAXB * MAXB];
+  __shared__ int splace[MAXB * MAXB];
   __shared__ uint64_t cand[MAXB][64], best[MAXB][MAXB];
   const int tid = threadIdx.x, lane = lane_id(), b = wave_id(), B = a.B, i = blockIdx.x;
   const char* at = a.work + ((int64_t)i * B + b) * a.parts * part_bytes(B);
+  const uint32_t inverse = 0xffffffffu / B + 1;
   const auto key_at = [&](int k) {
-    const int p = k / B;
+    const int p = B == 1 ? k : (int)__umulhi(k, inverse);  // k / B: k B < 2^32
     return k < a.parts * B ? reinterpret_cast<const uint64_t*>(at + p * part_bytes(B) + sizeof(Part))[k - p * B] : 0;
   };
-  // on their way before it is known whether they count: what an ended beam's parts hold is not looked at
+  // Read before it is known whether they count, and worked on while that is on its way: an ended beam's parts may hold
+  // anything, and nothing is taken from them.
   Part q = {-INFINITY, 0, 0.};
   if (lane < a.parts) q = *reinterpret_cast<const Part*>(at + lane * part_bytes(B));
   uint64_t next[MK];
@@ -331,8 +334,38 @@ __global__ void __launch_bounds__(64 * MAXB) beam_merge_kernel(const SelectArgs 
   }
   const bool ended = a.finished[g * B + b] != 0;
   const double start = (double)a.score[g * B + b];
-  double weight = 1.;
-  if (a.norm) weight = (double)a.norm[min(max(a.made[g * B + b] + (ended ? 0 : 1), 0), a.N - 1)];
+  const int made = a.norm ? a.made[g * B + b] : 0;
+  float M = q.m;
+  for (int p = lane + 64; p < a.parts; p += 64) M = fmaxf(M, reinterpret_cast<const Part*>(at + p * part_bytes(B))->m);
+  M = wave_max64(M);
+  double S = q.m > -INFINITY ? q.sum * exp_64((double)q.m - (double)M) : 0.;
+  for (int p = lane + 64; p < a.parts; p += 64) {
+    const Part* o = reinterpret_cast<const Part*>(at + p * part_bytes(B));
+    S += o->m > -INFINITY ? o->sum * exp_64((double)o->m - (double)M) : 0.;
+  }
+  S = wave_sum_d(S);
+  const float weight = a.norm ? a.norm[min(max(made + (ended ? 0 : 1), 0), a.N - 1)] : 1.f;
+  // the best so far in lanes 0 .. B - 1, best first, and MK keys a lane more in each round; 64 keys or fewer are ranked as
+  // they are
+  uint64_t cur = 0;
+  const int all_keys = a.parts * B;
+  if (all_keys <= 64) {
+    const int place = rank_of(next[0], all_keys);
+    if (lane < MAXB) best[b][lane] = 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next[0] && place < B) best[b][place] = next[0];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    cur = lane < B ? best[b][lane] : 0;
+  } else {
+    for (int k0 = 0; k0 < all_keys; k0 += 64 * MK) {
+      uint64_t key[MK + 1];
+#pragma unroll
+      for (int e = 0; e < MK; ++e) key[e] = next[e];
+      key[MK] = cur;
+      if (k0 + 64 * MK < all_keys) load(k0 + 64 * MK);
+      cur = best_of(key, B, cand[b], best[b]);
+    }
+  }
   double total = -INFINITY;
   int v = 0;
   if (!(start > -INFINITY)) {  // nothing but candidates of -inf (NaN counts as it): by their indexes
@@ -341,25 +374,6 @@ __global__ void __launch_bounds__(64 * MAXB) beam_merge_kernel(const SelectArgs 
     v = lane == 0 ? a.pad : lane - 1 + (lane - 1 >= a.pad);
     total = lane == 0 ? start : -INFINITY;
   } else {
-    float M = q.m;
-    for (int p = lane + 64; p < a.parts; p += 64) M = fmaxf(M, reinterpret_cast<const Part*>(at + p * part_bytes(B))->m);
-    M = wave_max64(M);
-    double S = q.m > -INFINITY ? q.sum * exp_64((double)q.m - (double)M) : 0.;
-    for (int p = lane + 64; p < a.parts; p += 64) {
-      const Part* o = reinterpret_cast<const Part*>(at + p * part_bytes(B));
-      S += o->m > -INFINITY ? o->sum * exp_64((double)o->m - (double)M) : 0.;
-    }
-    S = wave_sum_d(S);
-    // the best so far in lanes 0 .. B - 1, best first, and MK keys a lane more in each round
-    uint64_t cur = 0;
-    for (int k0 = 0; k0 < a.parts * B; k0 += 64 * MK) {
-      uint64_t key[MK + 1];
-#pragma unroll
-      for (int e = 0; e < MK; ++e) key[e] = next[e];
-      key[MK] = cur;
-      if (k0 + 64 * MK < a.parts * B) load(k0 + 64 * MK);
-      cur = best_of(key, B, cand[b], best[b]);
-    }
     const int have = __popcll(__ballot(cur != 0));
     v = (int)~(uint32_t)cur;
     if (cur) total = start + ((double)logit_of((uint32_t)(cur >> 32)) - (double)M - log(S));
@@ -374,29 +388,32 @@ __global__ void __launch_bounds__(64 * MAXB) beam_merge_kernel(const SelectArgs 
     }
   }
   if (lane < B) {
-    const double rank = total * weight;
+    const double rank = total * (double)weight;
     stotal[b * B + lane] = total == total ? total : -INFINITY;
     srank[b * B + lane] = rank == rank ? rank : -INFINITY;
-    sv[b * B + lane] = v;
+    sid[b * B + lane] = (uint64_t)b << 32 | (uint32_t)v;
   }
   if (tid < B * B) splace[tid] = 0;
   __syncthreads();
-  // a candidate's place: 64 / B threads, each counts the better ones of some beams
-  const int c = tid % (B * B), cb = c / B, share = tid / (B * B), shares = 64 / B;
+  // a candidate's place: 64 / B threads, each counts the better ones in a share of all
+  const int all = B * B, c = tid % all, shares = 64 / B, each = (all + shares - 1) / shares, first = tid / all * each;
   const double mine = srank[c];
-  v = sv[c];
+  const uint64_t id = sid[c];
   int better = 0;
-  for (int ob = share < shares ? share : B; ob < B; ob += shares)
-    for (int k = 0; k < B; ++k) {
-      const double other = srank[ob * B + k];
-      better += other > mine || (other == mine && (ob < cb || (ob == cb && sv[ob * B + k] < v)));
+  for (int j = 0; j < each; j += 8)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int at = min(first + j + k, all - 1);
+      const double other = srank[at];
+      const bool counts = j + k < each && first + j + k < all;
+      better += counts && (other > mine || (other == mine && sid[at] < id));
     }
   if (better) atomicAdd(&splace[c], better);
   __syncthreads();
   const int place = tid < B * B ? splace[tid] : B;
   if (place < B) {
-    a.parent[i * B + place] = cb;
-    a.token[i * B + place] = v;
+    a.parent[i * B + place] = (int)(id >> 32);
+    a.token[i * B + place] = (uint32_t)id;
     a.total[i * B + place] = (float)stotal[c];
   }
 }
