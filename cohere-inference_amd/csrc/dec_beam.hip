@@ -114,7 +114,7 @@ struct SelectArgs {
 // best are taken one by one. What bounds it is the vector unit: of 25 instructions a logit 15 are the exponential (205 rows
 // of 100008 in 27.8 us: 9.3 M instructions, which alone take 15.5; reading 41 MB takes 8).
 template <int J>
-__global__ void __launch_bounds__(256) beam_parts_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) beam_parts_kernel(const SelectArgs a) {
   __shared__ uint64_t cand[4][64], best[4][MAXB];
   __shared__ float smax[4];
   __shared__ double ssum[4];
