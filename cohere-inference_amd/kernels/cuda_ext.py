@@ -772,9 +772,10 @@ class _Ext:
     def dec_beam_advance(self, groups, parent, token, total, dummy, tok, pos, held, score, finished, made, done, limit, out,
                          eos, by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags):
         """The chosen tokens into the groups' state, behind dec_beam_reorder, and the next step's embeddings (as
-        dec_embed) into x, h (n B, width): tok int64, pos, held int32 (slots; held None or pos + 1), score fp32, finished uint8, made int32 (groups, B),
-        out int64 (slots, OUT), done uint8 and limit int32 (groups); flags: pinned uint8 (groups) or None. A group is done
-        once all its beams have finished, once the best has (by_length False), or at pos >= limit."""
+        dec_embed) into x, h (n B, width): tok int64, pos, held int32 (slots; held None or pos + 1), score fp32, finished
+        uint8, made int32 (groups, B), out int64 (slots, OUT), done uint8 and limit int32 (groups); flags: pinned uint8
+        (groups) or None. A group is done once all its beams have finished, once the best has (by_length False), or at
+        pos >= limit."""
         _calls.dec_beam_advance(groups, parent, token, total, dummy, tok, pos, held, score, finished, made, done, limit,
                                 out, eos, by_length, emb, ptab, w0, b0, eps0, w1, b1, eps1, x, h, flags)
 

@@ -390,15 +390,17 @@ int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, int64_t bea
 /* The chosen tokens into the groups' state (what cohere_dec_pick_embed does for the greedy choice): for beam b of group g
  * = groups[i], slot r = g * beams + b, with q = parent[i][b], t = token[i][b]: finished[r] = finished[q's] or t == eos or
  * total[i][b] is not above -inf; made[r] = made[q's] + (finished[q's] ? 0 : 1); score[r] = total[i][b]; pos[r] += 1;
- * out[r][pos[r]] = tok[r] = t; held[r] (may be null) = pos[r] + 1, the positions held once tok has been read. done[g] = 1 (and flags_host[g], pinned host memory, may be null) once all beams have
- * finished, once the best has and by_length is 0, and at pos >= limit[g]. The group dummy, and groups that are done, keep
- * their state. Then x, h [n_groups * beams, width] get the embedding of tok at pos, as cohere_dec_embed (emb [vocabulary,
- * width], ptab [positions, width]; indexes out of range are brought into it). A group is named once (the dummy any
+ * out[r][pos[r]] = tok[r] = t; held[r] (may be null) = pos[r] + 1, the positions held once tok has been read. done[g] = 1
+ * (and flags_host[g], pinned host memory, may be null) once all beams have finished, once the best has and by_length is 0,
+ * and at pos >= limit[g]. The group dummy, and groups that are done, keep their state. Then x, h [n_groups * beams, width]
+ * get the embedding of tok at pos, as cohere_dec_embed (emb [vocabulary, width], ptab [positions, width]; indexes out of
+ * range are brought into it). A group is named once (the dummy any
  * number of times). */
 int cohere_dec_beam_advance(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
                             const int64_t* token, const float* total, int64_t slots, int64_t dummy, int64_t* tok,
                             int32_t* pos, int32_t* held, float* score, uint8_t* finished,
-                            int32_t* made, uint8_t* done, const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos, int32_t by_length,
+                            int32_t* made, uint8_t* done, const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos,
+                            int32_t by_length,
                             const uint16_t* emb, int64_t vocabulary, const uint16_t* ptab, int64_t positions,
                             const uint16_t* w0, const uint16_t* b0, float eps0, const uint16_t* w1, const uint16_t* b1,
                             float eps1, uint16_t* x, uint16_t* h, int64_t width, uint8_t* flags_host, void* stream);
