@@ -42,35 +42,43 @@ struct Tile {
 template <int TM>
 DEVI Tile tile_of(const PagedArgs& p, int w) {
   Tile t;
-  int i = w;
   t.x0 = 0;
+  t.rows = 0;
   if (p.starts) {
     const int lane = lane_id();
-    int count = 0;
-    for (int i0 = 0; i0 < p.S; i0 += 64) {
-      const int at = i0 + lane;
-      const int64_t a = at < p.S ? min(max(p.starts[at], 0), p.R) : 0;
-      count += __popcll(__ballot(at < p.S && a * p.ratio / TM + at <= w));
+    int i, a, b;
+    if (p.S < 64) {  // all of it in one round trip
+      const int start = min(max(p.starts[min(lane, p.S)], 0), p.R), slot = p.active[min(lane, p.S - 1)];
+      i = __popcll(__ballot(lane < p.S && (int64_t)start * p.ratio / TM + lane <= w)) - 1;
+      if (i < 0) return t;
+      a = __builtin_amdgcn_readlane(start, i);
+      b = max(__builtin_amdgcn_readlane(start, i + 1), a);
+      t.slot = __builtin_amdgcn_readlane(slot, i);
+    } else {
+      int count = 0;
+      for (int i0 = 0; i0 < p.S; i0 += 64) {
+        const int at = i0 + lane;
+        const int64_t start = at < p.S ? min(max(p.starts[at], 0), p.R) : 0;
+        count += __popcll(__ballot(at < p.S && start * p.ratio / TM + at <= w));
+      }
+      i = count - 1;
+      if (i < 0) return t;
+      a = min(max(p.starts[i], 0), p.R);
+      b = min(max(p.starts[i + 1], a), p.R);
+      t.slot = p.active[i];
     }
-    i = count - 1;
-    if (i < 0) {
-      t.rows = 0;
-      return t;
-    }
-    const int a = min(max(p.starts[i], 0), p.R), b = min(max(p.starts[i + 1], a), p.R);
     t.first = a;
     t.c = b - a;
     t.x0 = (w - ((int)((int64_t)a * p.ratio / TM) + i)) * TM;
   } else {
-    const int tiles = (p.ratio + TM - 1) / TM;
-    i = w / tiles;
+    const int tiles = (p.ratio + TM - 1) / TM, i = w / tiles;
     t.x0 = (w - i * tiles) * TM;
     t.first = i;
     t.c = 1;
+    t.slot = p.active[i];
   }
   const int64_t left = (int64_t)t.c * p.ratio - t.x0;
   t.rows = left < TM ? (left > 0 ? (int)left : 0) : TM;
-  t.slot = p.active[i];
   t.ok = (unsigned)t.slot < (unsigned)p.slots;
   t.slot = t.ok ? t.slot : 0;
   return t;
