@@ -47,8 +47,22 @@ DEVI uint64_t wave_max_u64(uint64_t v) {
   return v;
 }
 DEVI double wave_sum_d(double v) {
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  const auto moved = [](double x, auto ctrl) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, decltype(ctrl)::value, 0xF, 0xF, false),
+                   hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), decltype(ctrl)::value, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  v += moved(v, std::integral_constant<int, DPP_XOR1>{});
+  v += moved(v, std::integral_constant<int, DPP_XOR2>{});
+  v += moved(v, std::integral_constant<int, DPP_ROR4>{});
+  v += moved(v, std::integral_constant<int, DPP_ROR8>{});
+  const auto lane = [&](int i) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), i) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, i));
+  };
+  return (lane(15) + lane(31)) + (lane(47) + lane(63));
 }
 
 // of the first n lanes' keys (0: none, the others different) the place of this lane's among them
@@ -437,47 +451,49 @@ struct ReorderArgs {
   char *k, *v;
   float *ks, *vs;
   int G, B, W, OUT, NS, L, pages, shift, KV, bytes;  // NS: states a row, bytes of a vector held
-  uint32_t chunks;                                   // of 16 bytes of a page in part filled, all layers, keys and values
+  int tables, columns;  // blocks of 256 columns: of the tables, of all rows (tables, tokens, states)
+  uint32_t chunks;      // of 16 bytes of a page in part filled, all layers, keys and values
 };
 
-// Block 0 of a group moves its rows of the tables, a thread a column of all B beams; the others move what the page in part
-// filled holds, a thread 16 bytes of all B beams: read before any is written, so that nothing has to wait for anything.
+// The first `columns` blocks of a group move its rows of the tables, tokens and states, a thread a column of all B beams;
+// the others move what the page in part filled holds, a thread 16 bytes of all B beams: read before any is written, so that
+// nothing has to wait for anything. Four round trips one behind the other: group, its state, the pages, what they hold.
 template <int MB>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) {
   const int i = blockIdx.y, g = a.groups[i], B = a.B, tid = threadIdx.x;
-  if ((unsigned)g >= (unsigned)a.G || (a.done && a.done[g])) return;
-  const int64_t slot0 = (int64_t)g * B;
-  const int n = max(a.n[slot0], 0);
   int from[MB];
   bool moved = false;
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
-    const int q = b < B ? a.parent[(int64_t)i * B + b] : b;
-    from[b] = (unsigned)q < (unsigned)B ? q : b;
+    const int q = a.parent[(int64_t)i * B + min(b, B - 1)];
+    from[b] = b < B && (unsigned)q < (unsigned)B ? q : b;
     moved |= from[b] != b;
   }
-  if (!moved) return;
-  if (blockIdx.x == 0) {
-    const auto move = [&](auto* rows, int width, int count) {
+  const bool there = (unsigned)g < (unsigned)a.G;
+  const int64_t slot0 = (int64_t)(there ? g : 0) * B;
+  const int n = max(a.n[slot0], 0);
+  const bool done = a.done && a.done[there ? g : 0];
+  if (!there || done || !moved) return;
+  if ((int)blockIdx.x < a.columns) {
+    const auto move = [&](auto* rows, int width, int c, int count) {
       using T = std::remove_reference_t<decltype(*rows)>;
-      for (int c = tid; c < count; c += 256) {
-        T x[MB];
+      if (c >= count) return;
+      T x[MB];
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
-          if (b < B) x[b] = rows[(slot0 + from[b]) * width + c];
+      for (int b = 0; b < MB; ++b) x[b] = rows[(slot0 + (b < B ? from[b] : 0)) * width + c];
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
-          if (b < B && from[b] != b) rows[(slot0 + b) * width + c] = x[b];
-      }
+      for (int b = 0; b < MB; ++b)
+        if (b < B && from[b] != b) rows[(slot0 + b) * width + c] = x[b];
     };
-    if (a.table) move(a.table, a.W, min(n >> a.shift, a.W));
-    if (a.tokens) move(a.tokens, a.OUT, min(n, a.OUT));
-    if (a.states) move(a.states, a.NS, a.NS);
+    const int block = blockIdx.x, tokens = a.tokens ? (a.OUT + 255) / 256 : 0;
+    if (block < a.tables) move(a.table, a.W, block * 256 + tid, min(n >> a.shift, a.W));
+    else if (block < a.tables + tokens) move(a.tokens, a.OUT, (block - a.tables) * 256 + tid, min(n, a.OUT));
+    else move(a.states, a.NS, (block - a.tables - tokens) * 256 + tid, a.NS);
     return;
   }
   const int filled = n & ((1 << a.shift) - 1), place = n >> a.shift;
   if (filled == 0 || place >= a.W) return;
-  const uint32_t c = (blockIdx.x - 1) * 256 + tid;
+  const uint32_t c = (blockIdx.x - a.columns) * 256 + tid;
   if (c >= a.chunks) return;
   const int part = (int)(c & (a.bytes / 16 - 1));  // 16 of bf16, 8 of int8
   uint32_t rest = c >> (a.bytes == 256 ? 4 : 3);
@@ -651,12 +667,16 @@ extern "C" int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, 
   const int bytes = bits == 16 ? 256 : 128;
   // a page of one position is never in part filled
   COHERE_REQUIRE(!k || kv_heads <= TOP / (2 * 256 * 16) / L, "dec_beam_reorder: too many layers and heads");
-  const int64_t chunks = k && shift > 0 ? L * 2 * kv_heads * P * (bytes / 16) : 0, blocks = 1 + (chunks + 255) / 256;
+  const int64_t chunks = k && shift > 0 ? L * 2 * kv_heads * P * (bytes / 16) : 0;
+  const auto blocks = [](int64_t of) { return (of + 255) / 256; };
+  const int64_t tables = table ? blocks(width) : 0,
+                columns = tables + (tokens ? blocks(OUT) : 0) + (states ? blocks(n_states) : 0);
   const ReorderArgs a{groups, parent, n, done, table, tokens, states, static_cast<char*>(k), static_cast<char*>(v),
                       bits == 8 ? ks : nullptr, bits == 8 ? vs : nullptr, (int)slots, (int)beams, (int)width, (int)OUT,
                       (int)n_states, (int)L, (int)pages, shift < 0 ? 0 : shift, (int)kv_heads, bytes,
-                      (uint32_t)chunks};
-  const dim3 grid((unsigned)blocks, (unsigned)n_groups);
+                      (int)tables, (int)columns, (uint32_t)chunks};
+  const dim3 grid((unsigned)(columns + blocks(chunks)), (unsigned)n_groups);
+  if (grid.x == 0) return 0;  // nothing that could move
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (beams <= 4) beam_reorder_kernel<4><<<grid, 256, 0, s>>>(a);
   else if (beams <= 8) beam_reorder_kernel<8><<<grid, 256, 0, s>>>(a);

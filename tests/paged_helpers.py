@@ -180,14 +180,17 @@ def close(got, want, bound):
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, worst {float((err / bound)[bad].max()):.3f} x bound"
 
 
-def select64(logits, groups, score, finished, made, norm, pad):
-    """(parent, token, total) by the definition, in 64 bits; logits on the CPU."""
+def select64(logits, groups, score, finished, made, norm, pad, ranks=None):
+    """(parent, token, total) by the definition, in 64 bits; logits on the CPU. ranks: a list that gets every group's
+    (beams, V) ranks."""
     n, (G, B), V = len(groups), score.shape, logits.shape[1]
     parent, token = torch.zeros(n, B, dtype=torch.int32), torch.zeros(n, B, dtype=torch.int64)
     out = torch.zeros(n, B, dtype=torch.float64)
     for i, g in enumerate(groups.tolist()):
         if not 0 <= g < G:
             parent[i], token[i], out[i] = torch.arange(B), pad, -math.inf
+            if ranks is not None:
+                ranks.append(None)
             continue
         total = np.full((B, V), -np.inf)
         rank = np.full((B, V), -np.inf)
@@ -206,6 +209,8 @@ def select64(logits, groups, score, finished, made, norm, pad):
                 rank[b] = total[b] * float(norm[at])
         total, rank = np.nan_to_num(total, nan=-np.inf, posinf=np.inf, neginf=-np.inf), \
             np.nan_to_num(rank, nan=-np.inf, posinf=np.inf, neginf=-np.inf)
+        if ranks is not None:
+            ranks.append(rank)
         best = np.argsort(-rank.reshape(-1), kind="stable")[:B]
         parent[i], token[i] = torch.from_numpy((best // V).astype(np.int32)), torch.from_numpy(best % V)
         out[i] = torch.from_numpy(total.reshape(-1)[best])
