@@ -88,7 +88,7 @@ paged_chunk_kernel(const PagedArgs p) {
   const int hi = row_ok ? (t.x0 + t.rows - 1) / p.ratio + 1 : 0;  // the chunk's tokens that the tile's last row sees
   const int np = (n + KT - 1) / KT, nb = np + (hi + KT - 1) / KT;
   // as many parts as there are for `least` tiles each
-  const int parts = max(1, min(nsp, (nb + p.least - 1) / p.least));
+  const int parts = max(1, min(nsp, nb / p.least));
   if (sp >= parts) return;
   const int chunk = (nb + parts - 1) / parts, start = min(nb, sp * chunk), end = min(nb, start + chunk);
   const int P1 = (1 << p.shift) - 1;
@@ -438,10 +438,10 @@ int64_t chunk_workgroups(const PagedArgs& p) {
 }
 
 void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
-  // Tiles that a part has at least: few where there are few workgroups (4 x 24 tokens over 1 K, 8 parts asked for: 14.9 us,
-  // with 12 tiles 19.4), else enough that a part's start and the joining are small beside it (9 ragged sequences of up to
-  // 3 K, 4 asked for: 90 us, with 4 tiles 95; 2048 tokens over nothing, 2 asked for: 75, no parts 62).
-  p.least = chunk_workgroups(p) < 256 ? 4 : 12;
+  // Tiles that a part has at least: few where there are few workgroups (17 tokens over 8 K, int8, 32 parts asked for: 21 us,
+  // with 10 tiles 32), else enough that a part's start and the joining are small beside it, few enough that long and short
+  // tiles even out (9 ragged sequences of up to 3 K, int8, 2 asked for, with 4, 10 and 16: 86, 82 and 91; in bf16 67, 66, 64).
+  p.least = chunk_workgroups(p) < 256 ? 3 : 10;
   const dim3 grid((unsigned)chunk_workgroups(p), (unsigned)p.parts);
   if (q8 && p.shift >= 4) paged_chunk_kernel<true, true><<<grid, W * 64, 0, s>>>(p);
   else if (q8) paged_chunk_kernel<true, false><<<grid, W * 64, 0, s>>>(p);

@@ -364,10 +364,11 @@ int cohere_dec_gather_paged_q8(const int32_t* slot_of, const int32_t* pos_of, in
  * logits bf16 [n * beams, ld] is its beam b. Candidates (b, v): total = score[g][b] + l[v] - max l - log sum exp(l -
  * max l), NaN logits counted as -inf (a row of nothing else gives -inf), infinite ones as the largest finite number; a
  * finished beam has total = score[g][b] for v = pad and -inf for the others. Ranked by total * norm[min(made[g][b] +
- * (finished ? 0 : 1), norm_len - 1)] (norm fp32, positive; null: by total), in 64 bits (the logarithms to 1e-10), then by the
- * lowest b * V + v; a NaN counts as -inf. The best `beams` of them, best first, into row i of parent int32, token int64 and total fp32 [n,
- * beams]. A group out of range gets parents 0 .., tokens pad and totals -inf. V % 8 == 0, V >= beams, 0 <= pad < V, n *
- * beams <= 65535. work: cohere_dec_beam_select_work(n * beams, V, beams) bytes, 8-byte aligned, of one call at a time. */
+ * (finished ? 0 : 1), norm_len - 1)] (norm fp32, positive; null: by total), in 64 bits (the logarithms to 1e-10), then by
+ * the lowest b * V + v; a NaN counts as -inf. The best `beams` of them, best first, into row i of parent int32, token int64
+ * and total fp32 [n, beams]. A group out of range gets parents 0 .., tokens pad and totals -inf. V % 8 == 0, V >= beams, 0
+ * <= pad < V, n * beams <= 65535. work: cohere_dec_beam_select_work(n * beams, V, beams) bytes, 8-byte aligned, of one call
+ * at a time. */
 int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V, const int32_t* groups,
                            int64_t slots, const float* score, const uint8_t* finished, const int32_t* made,
                            const float* norm, int64_t norm_len, int64_t pad, int32_t* parent, int64_t* token, float* total,
