@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __
   const float* base = part + head * nsp * (HD + 2);
   const float2 ml = *reinterpret_cast<const float2*>(base + min(lane, nsp - 1) * (HD + 2) + HD);
   const int r = (int)(head / H);
-  if (r < starts[0] || r >= starts[S]) return;
+  if (starts && (r < starts[0] || r >= starts[S])) return;
   if (lane_value(ml.y, 0) < 0.f) return;  // one part, which wrote the outputs
   const bool in = lane < nsp && ml.x != -INFINITY;
   const float M = wave_max64(in ? ml.x : -INFINITY), w = in ? exp2_hw(ml.x - M) : 0.f;

@@ -257,6 +257,24 @@ def test_long_context(gpu):
     _check(c, 1)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("ratio", [2, 17, 40])
+def test_splits_without_starts(gpu, bits, ratio):
+    """A row a sequence in several parts, of few and of many heads to a key head."""
+    c = Paged(ratio, [0, 7, 300, 1500], [1, 1, 1, 1], 1, ratio, 16, bits)
+    for splits in (2, 5, 16):
+        _check(c, splits, starts=None, weights_bf16=ratio > 16)
+
+
+@pytest.mark.parametrize("ratio", [2, 8])
+@pytest.mark.parametrize("copies", [12, 13, 30])
+def test_many_sequences(gpu, ratio, copies):
+    """60 to 150 sequences, some without a row, in both kernels."""
+    c = Paged(copies, [0, 5, 33, 64, 17] * copies, [3, 0, 20, 1, 7] * copies, 1, ratio, 16, 16, front=2, back=3)
+    _check(c, weights_bf16=True)
+    _check(c, 3, weights_bf16=True)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.07, 1e-30])
 def test_scales(gpu, scale):
     """Scales that turn the order of the scores round, or leave nothing of it."""
