@@ -33,8 +33,6 @@ class BeamDecoder(StreamDecoder):
     """StreamDecoder with `beams` hypotheses (1..16) a slot; buckets count slots. length_penalty: 0 ranks by the sum of
     log probabilities, 1 by their mean. page: positions a page (a power of two up to 256). kv_bits: 16 or 8."""
 
-    BUCKETS = (1, 2, 4, 8, 12, 16, 24, 32)
-
     def __init__(self, model, slots: int = 32, max_new_tokens: int = 448, max_prompt: int = 16, max_audio_s: float = 36.0,
                  buckets=None, int8: bool = False, frames: int | None = None, capture: bool = True,
                  fused: bool | None = None, chunk: int = 4, kv_bits: int | None = None, penalties: bool = False,

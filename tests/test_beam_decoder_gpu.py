@@ -175,6 +175,31 @@ def test_requests_do_not_depend_on_each_other(gpu):
         assert torch.equal(dec.out[rows].cpu(), want[i]) and torch.equal(dec.score[SLOTS[i]].cpu(), scores[i])
 
 
+def test_as_many_requests_as_slots(gpu):
+    """The buckets that are there by default hold as many requests as the service's default slots; a request's tokens are
+    the same among many."""
+    few = _decoder(gpu)
+    b = _start(few)
+    for _ in range(8):
+        few.step(b)
+    few.stream.synchronize()
+    want = [few.tokens(s).cpu() for s in SLOTS]
+    dec = _decoder(gpu, slots=128, buckets=None, capture=False)
+    assert dec.bucket(128) == 128
+    n = 101
+    for i in range(n):
+        dec.fill_cross(_memory(dec, [FRAMES[i % 3]], seed=i % 3), [FRAMES[i % 3]], [i], projected=True)
+    dec.stream.wait_stream(torch.cuda.current_stream())
+    dec.admit(list(range(n)), [PROMPTS[i % 3] for i in range(n)], [FRAMES[i % 3] for i in range(n)])
+    b = dec.set_active(list(range(n)))
+    assert b == 112
+    for _ in range(8):
+        dec.step(b)
+    dec.stream.synchronize()
+    for i in range(n):
+        assert torch.equal(dec.tokens(i).cpu(), want[i % 3]), i
+
+
 def test_scores_are_the_hypotheses_own(gpu):
     """Each hypothesis read token by token by a greedy decoder gives its score: the sum of its tokens' log probabilities.
     The two decoders' logits differ by the order of fp32 sums in the attentions, which moves bf16 roundings behind it: a
