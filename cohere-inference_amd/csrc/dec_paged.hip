@@ -680,11 +680,12 @@ extern "C" int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs,
   // Parts until the GPU is full, and then, where they stay long, until long and short sequences even out. Few-row kernel,
   // of 256 CUs x 2 workgroups: 1 x 8 heads over 64 K positions in 1, 16 and 64 parts 564, 50 and 44 us; 32 x 8 (x 4) over 1
   // .. 16 K, int8, 1, 2 and 8 parts 187, 152 and 126; 64 x 8 over up to 1 K 21, 2 parts 25. Kernel of 128 rows: 256 tokens
-  // over 32 K 606, 16 parts 72, 32 63; 9 ragged sequences of up to 3 K 106, 2 parts 85; 8 x 512 tokens over nothing 26, 2 31.
+  // over 32 K 606, 16 parts 72, 32 63; 8 x 512 tokens over nothing 25, 2 parts 31.
   const int64_t ratio = heads / kv_heads;
   const bool many = many_rows(rows, seqs, ratio);
   const int64_t wgs = tiles_for(rows, seqs, ratio, many ? 128 : 16, rows != seqs) * kv_heads;
   const int64_t full = many ? 256 : 512, most = many ? 1024 : 2048, least = 192, longer = many ? 768 : 1024;
+  if (many && wgs >= 192 && wgs <= 448) return 1;  // workgroups of two groups of waves
   int64_t n = 1;
   while (n < 64 && wgs * 2 * n <= most && T / (2 * n) >= (wgs * n < full ? least : longer)) n *= 2;
   return n;

@@ -53,12 +53,14 @@ DEVI uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(LDS_AS c
 // the wave's LDS operations done, and its loads
 DEVI void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <bool Q8, bool BIG>
-__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// G: groups of W waves, each with every G-th tile and buffers of its own, whose results meet in LDS
+template <bool Q8, bool BIG, int G>
+__global__ void __launch_bounds__(G * W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_chunk_kernel(const PagedArgs p) {
-  __shared__ __attribute__((aligned(16))) char kbuf[2][KT * 256], vbuf[2][KT * 256];
-  __shared__ __attribute__((aligned(16))) float sscale[Q8 ? 2 : 1][2][Q8 ? KT : 1];  // of a tile's keys and values
-  const int lane = lane_id(), wave = wave_id(), col = lane & 31, half = lane >> 5;
+  __shared__ __attribute__((aligned(16))) char kbuf[G * 2][KT * 256], vbuf[G * 2][KT * 256];
+  __shared__ __attribute__((aligned(16))) float sscale[Q8 ? G * 2 : 1][2][Q8 ? KT : 1];  // of a tile's keys and values
+  const int lane = lane_id(), col = lane & 31, half = lane >> 5;
+  const int wave = G == 1 ? wave_id() : wave_id() % W, group = G == 1 ? 0 : wave_id() / W;
   const int kvh = blockIdx.x % p.KV, sp = blockIdx.y, nsp = p.parts;
   // a chunk's last tiles first: they see the most keys, and what starts last ends last
   const Tile t = tile_of<TM>(p, gridDim.x / p.KV - 1 - blockIdx.x / p.KV);
@@ -114,8 +116,8 @@ paged_chunk_kernel(const PagedArgs p) {
   const auto piece_k = [&](int i) { return (uint32_t)((lane & 15) ^ (i * 4 + k4)) * 16; };
   const auto issue = [&](int b, int entry, uint64_t live, int buf) {
     const int t0 = first_of(b);
-    const uint32_t kdst = __builtin_amdgcn_readfirstlane(lds_address(kbuf[buf])) + kk0 * 256,
-                   vdst = __builtin_amdgcn_readfirstlane(lds_address(vbuf[buf])) + kk0 * 256;
+    const uint32_t kdst = __builtin_amdgcn_readfirstlane(lds_address(kbuf[group * 2 + buf])) + kk0 * 256,
+                   vdst = __builtin_amdgcn_readfirstlane(lds_address(vbuf[group * 2 + buf])) + kk0 * 256;
     if (b >= np) {  // of the chunk's tokens
       const uint32_t stride = (uint32_t)p.ldq * 2, bytes = (uint32_t)max(min(hi - t0 - kk0, 16), 0) * stride;
       const int64_t at = (int64_t)(t0 + kk0) * stride;
@@ -202,7 +204,7 @@ paged_chunk_kernel(const PagedArgs p) {
               w[k] = pack_bf2((float)(int8_t)y, (float)(int8_t)(y >> 8));
             }
             const int sw = z ? (kk & 3) << 2 : kk & 15;
-            char* dst = (z ? vbuf : kbuf)[buf] + kk * 256;
+            char* dst = (z ? vbuf : kbuf)[group * 2 + buf] + kk * 256;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
               *reinterpret_cast<uint4*>(dst + ((((lane & 7) * 2 + c) ^ sw) * 16)) =
@@ -210,7 +212,7 @@ paged_chunk_kernel(const PagedArgs p) {
           }
         }
       }
-      if (lane < 32) sscale[buf][lane >> 4][wave * 16 + (lane & 15)] = sr;
+      if (lane < 32) sscale[group * 2 + buf][lane >> 4][wave * 16 + (lane & 15)] = sr;
     }
   };
 
@@ -225,7 +227,7 @@ paged_chunk_kernel(const PagedArgs p) {
   // a tile's products; OWN: of the chunk's tokens
   constexpr int AHEAD = Q8 ? 4 : 6;  // keys' pieces on their way from LDS
   const auto read_k = [&](v8bf (&kf)[AHEAD], int buf, int j) {
-    kf[j % AHEAD] = *reinterpret_cast<const v8bf*>(kbuf[buf] + ((j >> 3) * 32 + col) * 256 +
+    kf[j % AHEAD] = *reinterpret_cast<const v8bf*>(kbuf[group * 2 + buf] + ((j >> 3) * 32 + col) * 256 +
                                                    ((((j & 7) * 2 + half) ^ (col & 15)) * 16));
   };
   const auto tile = [&](int b, int buf, uint64_t live, v8bf (&kf)[AHEAD], auto own) {
@@ -242,7 +244,7 @@ paged_chunk_kernel(const PagedArgs p) {
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
         const int kk = half * 4 + ((lane & 15) >> 2), c = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-        const char* src = vbuf[buf] + (u * 16 + kk) * 256 + ((c ^ ((kk & 3) << 2)) * 16) + (lane & 1) * 8;
+        const char* src = vbuf[group * 2 + buf] + (u * 16 + kk) * 256 + ((c ^ ((kk & 3) << 2)) * 16) + (lane & 1) * 8;
         const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)src);
         const v4s d = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)(src + 8 * 256));
         vf[u & 1][dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(a, d, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -252,12 +254,12 @@ paged_chunk_kernel(const PagedArgs p) {
     const auto read_ks = [&](int z) {
       if constexpr (Q8)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) ks[g] = *reinterpret_cast<const v4f*>(&sscale[buf][0][z * 32 + g * 8 + half * 4]);
+        for (int g = 0; g < 4; ++g) ks[g] = *reinterpret_cast<const v4f*>(&sscale[group * 2 + buf][0][z * 32 + g * 8 + half * 4]);
     };
     const auto read_vs = [&](int u) {
       if constexpr (Q8)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) vs[u & 1][g] = *reinterpret_cast<const v4f*>(&sscale[buf][1][u * 16 + g * 8 + half * 4]);
+        for (int g = 0; g < 2; ++g) vs[u & 1][g] = *reinterpret_cast<const v4f*>(&sscale[group * 2 + buf][1][u * 16 + g * 8 + half * 4]);
     };
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
@@ -343,41 +345,70 @@ paged_chunk_kernel(const PagedArgs p) {
     }
   };
 
-  int entry = 0;
+  int entry = 0, b = start + group;
   uint64_t next = 0;
-  if (start < end) {
-    entry = start == 0 ? entry0 : entry_of(start);
-    next = live_of(start, entry);
-    issue(start, entry, next, 0);
+  if (b < end) {
+    entry = b == 0 ? entry0 : entry_of(b);
+    next = live_of(b, entry);
+    issue(b, entry, next, 0);
   }
   if (sp == 0 && row_ok) {
-    Append<Q8, W, 8> own;
-    for (int i = 0; own.load(p, t, n, kvh, TM, i); i += 8) own.store(p, n, kvh);
+    Append<Q8, G * W, 8 / G> own;
+    for (int i = 0; own.load(p, t, n, kvh, TM, i); i += 8 / G) own.store(p, n, kvh);
   }
-  if (start < end) {
-    convert(start, 0);
-    entry = start + 1 < end ? entry_of(start + 1) : 0;
+  if (b < end) {
+    convert(b, 0);
+    entry = b + G < end ? entry_of(b + G) : 0;
   }
-  const auto tiles = [&](int b, int to, auto own) {
-    for (; b < to; ++b) {
-      const int buf = (b - start) & 1;
+  int buf = 0;
+  const auto tiles = [&](int to, auto own) {
+    for (; b < to; b += G, buf ^= 1) {
       asm volatile("" : "+v"(entry));  // waited for here, not behind the next tile's loads
       tile_barrier();                  // this tile is in LDS, and no wave reads the other buffer any more
       const uint64_t live = next;
       v8bf kf[AHEAD];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) read_k(kf, buf, j);
-      if (b + 1 < end) {
-        next = live_of(b + 1, entry);
-        issue(b + 1, entry, next, buf ^ 1);
-        if (b + 2 < end) entry = entry_of(b + 2);
+      if (b + G < end) {
+        next = live_of(b + G, entry);
+        issue(b + G, entry, next, buf ^ 1);
+        if (b + 2 * G < end) entry = entry_of(b + 2 * G);
       }
       tile(b, buf, live, kf, own);
-      if (b + 1 < end) convert(b + 1, buf ^ 1);
+      if (b + G < end) convert(b + G, buf ^ 1);
     }
   };
-  tiles(start, min(end, np), std::false_type{});
-  tiles(max(start, np), end, std::true_type{});
+  tiles(min(end, np), std::false_type{});
+  tiles(end, std::true_type{});
+  if constexpr (G == 2) {
+    // every wave has passed as many barriers; the second group's results go through the buffers, which nobody reads now
+    if (group == 1 && (end - start) % 2) tile_barrier();
+    tile_barrier();
+    v4f* outputs = reinterpret_cast<v4f*>(kbuf) + wave * 16 * 64 + lane;
+    float* rest = reinterpret_cast<float*>(vbuf) + wave * 3 * 64 + lane;
+    if (group == 1) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        outputs[j * 64] = v4f{acc[j >> 2][(j & 3) * 4], acc[j >> 2][(j & 3) * 4 + 1], acc[j >> 2][(j & 3) * 4 + 2],
+                              acc[j >> 2][(j & 3) * 4 + 3]};
+      rest[0] = base;
+      rest[64] = l;
+      rest[128] = bad ? 1.f : 0.f;
+    }
+    tile_barrier();
+    if (group == 1) return;
+    const float other = rest[0], to = fmaxf(base, other), mine = base == -INFINITY ? 0.f : exp2_hw(base - to),
+                its = other == -INFINITY ? 0.f : exp2_hw(other - to);
+    l = l * mine + rest[64] * its;
+    base = to;
+    bad |= rest[128] != 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const v4f o = outputs[j * 64];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[j >> 2][(j & 3) * 4 + k] = acc[j >> 2][(j & 3) * 4 + k] * mine + o[k] * its;
+    }
+  }
   l = xor32_sum(l);
   if (wave * 32 + col < t.rows) {
     if (__builtin_expect(bad, 0)) {
@@ -441,12 +472,19 @@ void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
   // Tiles that a part has at least: few where there are few workgroups (17 tokens over 8 K, int8, 32 parts asked for: 21 us,
   // with 10 tiles 32), else enough that a part's start and the joining are small beside it, few enough that long and short
   // tiles even out (9 ragged sequences of up to 3 K, int8, 2 asked for, with 4, 10 and 16: 86, 82 and 91; in bf16 67, 66, 64).
-  p.least = chunk_workgroups(p) < 256 ? 3 : 10;
-  const dim3 grid((unsigned)chunk_workgroups(p), (unsigned)p.parts);
-  if (q8 && p.shift >= 4) paged_chunk_kernel<true, true><<<grid, W * 64, 0, s>>>(p);
-  else if (q8) paged_chunk_kernel<true, false><<<grid, W * 64, 0, s>>>(p);
-  else if (p.shift >= 4) paged_chunk_kernel<false, true><<<grid, W * 64, 0, s>>>(p);
-  else paged_chunk_kernel<false, false><<<grid, W * 64, 0, s>>>(p);
+  const int64_t wgs = chunk_workgroups(p);
+  p.least = wgs < 256 ? 3 : 10;
+  const dim3 grid((unsigned)wgs, (unsigned)p.parts);
+  // Two groups of waves a workgroup (it then has a CU to itself) where there are few workgroups and no parts: the longest
+  // tile takes half as long, and its results meet without a way through memory. 9 ragged sequences 52 us, in bf16 with one
+  // group 65 and in 2 parts 67 (int8 82, 107 and 82); 8 x 512 tokens over nothing 22 and 25; 512 workgroups of one length 92
+  // and 83.
+  const bool two = p.parts == 1 && wgs <= 448;
+#define CHUNK(Q, BIG) \
+  (two ? paged_chunk_kernel<Q, BIG, 2><<<grid, 2 * W * 64, 0, s>>>(p) : paged_chunk_kernel<Q, BIG, 1><<<grid, W * 64, 0, s>>>(p))
+  if (q8) p.shift >= 4 ? CHUNK(true, true) : CHUNK(true, false);
+  else p.shift >= 4 ? CHUNK(false, true) : CHUNK(false, false);
+#undef CHUNK
 }
 
 }  // namespace cohere_paged

@@ -292,6 +292,14 @@ def test_parts_of_a_tiles_own_number(gpu, bits):
         _check(c, splits, weights_bf16=True)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("page", [16, 2])
+def test_many_chunks_at_once(gpu, bits, page):
+    """So many workgroups that each has one group of waves (the tests of few chunks have two)."""
+    c = Paged(18, [100, 0, 260] * 20, [17, 20, 0] * 20, 8, 2, page, bits)
+    _check(c, weights_bf16=True)
+
+
 def test_chunks_captured_while_positions_move(gpu):
     """A captured chunk whose sequences have other numbers of parts in every replay, its workspace left as it was."""
     from kernels.cuda_ext import ext
