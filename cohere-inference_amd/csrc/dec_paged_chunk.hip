@@ -235,7 +235,7 @@ paged_chunk_kernel(const PagedArgs p) {
     const int t0 = first_of(b);
     if (idle || (OWN && t0 > tok1)) return;  // no row of the wave's sees them
     const bool causal = OWN && t0 + KT - 1 > tok0;
-      // The order of these steps is this source's, kept by the fences: vector work stands between the matrix products, for the
+    // The order of these steps is this source's, kept by the fences: vector work stands between the matrix products, for the
     // other wave's products to run under, and what is read from LDS is asked for some products ahead.
     v16f s[2];  // scores, then weights, of 32 keys each
     // keys 16 u + 4 half + (lane % 16) / 4 (and 8 on), dimensions 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) ..
@@ -254,12 +254,14 @@ paged_chunk_kernel(const PagedArgs p) {
     const auto read_ks = [&](int z) {
       if constexpr (Q8)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) ks[g] = *reinterpret_cast<const v4f*>(&sscale[group * 2 + buf][0][z * 32 + g * 8 + half * 4]);
+        for (int g = 0; g < 4; ++g)
+          ks[g] = *reinterpret_cast<const v4f*>(&sscale[group * 2 + buf][0][z * 32 + g * 8 + half * 4]);
     };
     const auto read_vs = [&](int u) {
       if constexpr (Q8)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) vs[u & 1][g] = *reinterpret_cast<const v4f*>(&sscale[group * 2 + buf][1][u * 16 + g * 8 + half * 4]);
+        for (int g = 0; g < 2; ++g)
+          vs[u & 1][g] = *reinterpret_cast<const v4f*>(&sscale[group * 2 + buf][1][u * 16 + g * 8 + half * 4]);
     };
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
@@ -291,7 +293,8 @@ paged_chunk_kernel(const PagedArgs p) {
       for (int z = 0; z < 2; ++z) {
         // bit 8 (r / 4) + r % 4: key z 32 + 8 (r / 4) + 4 half + r % 4 is there, and not behind the query's token
         const int upto = causal ? tok - t0 - z * 32 : 31;
-        const uint32_t seen = (uint32_t)(live >> (z * 32)) & (upto < 0 ? 0u : ~0u >> max(31 - upto, 0)), mine = seen >> (half * 4);
+        const uint32_t seen = (uint32_t)(live >> (z * 32)) & (upto < 0 ? 0u : ~0u >> max(31 - upto, 0));
+        const uint32_t mine = seen >> (half * 4);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int kk = (r >> 2) * 8 + (r & 3);
@@ -481,7 +484,8 @@ void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
   // and 83.
   const bool two = p.parts == 1 && wgs <= 448;
 #define CHUNK(Q, BIG) \
-  (two ? paged_chunk_kernel<Q, BIG, 2><<<grid, 2 * W * 64, 0, s>>>(p) : paged_chunk_kernel<Q, BIG, 1><<<grid, W * 64, 0, s>>>(p))
+  (two ? paged_chunk_kernel<Q, BIG, 2><<<grid, 2 * W * 64, 0, s>>>(p)                                                       \
+       : paged_chunk_kernel<Q, BIG, 1><<<grid, W * 64, 0, s>>>(p))
   if (q8) p.shift >= 4 ? CHUNK(true, true) : CHUNK(true, false);
   else p.shift >= 4 ? CHUNK(false, true) : CHUNK(false, false);
 #undef CHUNK

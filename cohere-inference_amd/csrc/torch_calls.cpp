@@ -1,7 +1,7 @@
 // The entry points over 4-bit caches and pages, on logits and of beam search as Python functions of torch tensors: the
 // argument checks in C++, because in Python they take longer than the launch (a lone call 8.6 us of host time; here 4,
-// what a launch alone takes) and these calls are made once per layer and step. Bound to the C ABI's functions by address (bind), so that the
-// library is the one that kernels/cuda_ext.py loaded. A refused call raises RuntimeError.
+// what a launch alone takes) and these calls are made once per layer and step. Bound to the C ABI's functions by address
+// (bind), so that the library is the one that kernels/cuda_ext.py loaded. A refused call raises RuntimeError.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -454,7 +454,8 @@ void beam_advance(const Call& c) {
   launch([&] {
     return f_advance(ptr<int32_t>(groups), n, B, ptr<int32_t>(parent), ptr<int64_t>(token), ptr<float>(total), G, dummy,
                      ptr<int64_t>(tok), ptr<int32_t>(pos), ptr<int32_t>(held), ptr<float>(score), ptr<uint8_t>(finished),
-                     ptr<int32_t>(made), ptr<uint8_t>(done), ptr<int32_t>(limit), ptr<int64_t>(out), out.size(1), eos, by_length,
+                     ptr<int32_t>(made), ptr<uint8_t>(done), ptr<int32_t>(limit), ptr<int64_t>(out), out.size(1), eos,
+                     by_length,
                      ptr<uint16_t>(emb), emb.size(0), ptr<uint16_t>(ptab), ptab.size(0), ptr<uint16_t>(w0),
                      ptr<uint16_t>(b0), (float)eps0, ptr<uint16_t>(w1), ptr<uint16_t>(b1), (float)eps1, ptr<uint16_t>(x),
                      ptr<uint16_t>(h), w, ptr<uint8_t>(flags), st);
