@@ -686,10 +686,10 @@ extern "C" int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, 
 
 extern "C" int cohere_dec_beam_advance(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,
                                        const int64_t* token, const float* total, int64_t slots, int64_t dummy, int64_t* tok,
-                                       int32_t* pos, int32_t* held, float* score, uint8_t* finished,
-                                       int32_t* made, uint8_t* done, const int32_t* limit, int64_t* out, int64_t OUT,
-                                       int64_t eos, int32_t by_length, const uint16_t* emb, int64_t vocabulary, const uint16_t* ptab, int64_t positions,
-                                       const uint16_t* w0, const uint16_t* b0, float eps0, const uint16_t* w1,
+                                       int32_t* pos, int32_t* held, float* score, uint8_t* finished, int32_t* made,
+                                       uint8_t* done, const int32_t* limit, int64_t* out, int64_t OUT, int64_t eos,
+                                       int32_t by_length, const uint16_t* emb, int64_t vocabulary, const uint16_t* ptab,
+                                       int64_t positions, const uint16_t* w0, const uint16_t* b0, float eps0, const uint16_t* w1,
                                        const uint16_t* b1, float eps1, uint16_t* x, uint16_t* h, int64_t width,
                                        uint8_t* flags_host, void* stream) {
   cohere::clear_error();
