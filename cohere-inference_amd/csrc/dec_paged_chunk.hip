@@ -138,8 +138,8 @@ paged_chunk_kernel(const PagedArgs p) {
       const uint32_t keys = ok ? (uint32_t)max(min(n - t0 - kk0, 16), 0) : 0;
       if constexpr (Q8) {
         const auto from = [&](const void* pages, int size) {
-          return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(pages)) + vec * size, 0,
-                                                   keys * size, 0x00027000);
+          const v4i r = buffer_of(pages, vec * size, keys * size);  // scalar: the compiler does not see that it is
+          return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)(uint32_t)r[1] << 32 | (uint32_t)r[0]), 0, r[2], r[3]);
         };
         const auto kb = from(p.k, HD), vb = from(p.v, HD);
 #pragma unroll
