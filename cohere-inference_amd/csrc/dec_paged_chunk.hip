@@ -11,7 +11,7 @@
 // What bounds it: a tile's 32 products keep a SIMD's matrix core 1024 cycles and its 200 vector instructions (32 exponentials
 // at 8 cycles) about as long; a wave does one after the other, and two waves a SIMD, what the registers allow, overlap them
 // only in part. 4 x 2048 tokens x 32 heads behind 6 to 8 K positions: 1044 us, 1054 TFLOP/s (a large product of the library:
-// 1188); a tile alone on its CU takes 1.2 us, int8 1.9 (their conversion).
+// 1188); a tile alone on its CU takes 1.2 us, int8 1.7 (their conversion).
 // Maximum, sum and outputs of a query stay in lanes l % 32 = query. The base of a query's weights is set 2^8 above its
 // largest score and moves only when a score passes it, so that rescaling is rare and weights are at most 1.
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
@@ -268,7 +268,7 @@ paged_chunk_kernel(const PagedArgs p) {
     __builtin_amdgcn_sched_barrier(0);
     float mx = -INFINITY;
     // Within a wave nothing runs under a matrix product, another wave's vector work does: of the two waves of a SIMD the one
-    // with products alone to do goes first (4 x 2048 tokens 1068 -> 1050 us, int8 1457 -> 1348).
+    // with products alone to do goes first (4 x 2048 tokens 1068 -> 1050 us).
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -474,14 +474,13 @@ int64_t chunk_workgroups(const PagedArgs& p) {
 void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
   // Tiles that a part has at least: few where there are few workgroups (17 tokens over 8 K, int8, 32 parts asked for: 21 us,
   // with 10 tiles 32), else enough that a part's start and the joining are small beside it, few enough that long and short
-  // tiles even out (9 ragged sequences of up to 3 K, int8, 2 asked for, with 4, 10 and 16: 86, 82 and 91; in bf16 67, 66, 64).
+  // tiles even out (9 ragged sequences of up to 3 K, int8, 2 asked for, with 4, 10 and 16: 86, 82 and 91).
   const int64_t wgs = chunk_workgroups(p);
   p.least = wgs < 256 ? 3 : 10;
   const dim3 grid((unsigned)wgs, (unsigned)p.parts);
   // Two groups of waves a workgroup (it then has a CU to itself) where there are few workgroups and no parts: the longest
-  // tile takes half as long, and its results meet without a way through memory. 9 ragged sequences 52 us, in bf16 with one
-  // group 65 and in 2 parts 67 (int8 82, 107 and 82); 8 x 512 tokens over nothing 22 and 25; 512 workgroups of one length 92
-  // and 83.
+  // tile takes half as long, and its results meet without a way through memory. 9 ragged sequences in bf16 52 us, with one
+  // group 65, in 2 parts 67; 8 x 512 tokens over nothing 22 and 25; 512 workgroups of one length 92 and 83.
   const bool two = p.parts == 1 && wgs <= 448;
 #define CHUNK(Q, BIG) \
   (two ? paged_chunk_kernel<Q, BIG, 2><<<grid, 2 * W * 64, 0, s>>>(p)                                                       \
