@@ -325,16 +325,16 @@ int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, 
 
 /* Attention of a chunk of new tokens per sequence. Sequence i (0 .. seqs - 1) is slot s = active[i] with n[s] positions
  * held; its rows of q and out are starts[i] .. starts[i + 1] - 1 (int32 [seqs + 1], ascending, within 0 .. rows; starts
- * null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq] holds heads x 128 queries, then
- * kv_heads x 128 keys, then the values; query head h reads key head h / (heads / kv_heads). Row j of a sequence, position
- * n[s] + j, attends to positions 0 .. n[s] - 1 as the pages hold them and to rows 0 .. j of its sequence as given, whose
- * keys and values are appended at positions n[s] ..: out = softmax(q k^T scale) v, bf16 [rows, heads * 128]. Rows of a
- * slot out of range, or with n[s] < 0, get zeros, and nothing is appended. Rows in front of starts[0] or from
- * starts[seqs] on are left as they were. A page that is appended to belongs to one sequence of the call, and so does its
- * slot; full pages may be shared by any number. What a row does not attend to never shows in it, NaN and infinities
- * included. out must not overlap q. splits (1 .. 64) divides the keys over workgroups and needs part with rows x heads x
- * splits x 130 floats, of one call at a time. fp32 sums; the weights are held to 2^-17 of themselves, in bf16 (2^-9)
- * where a sequence and key head have more than 16 query rows on average. */
+ * null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq <= 2^24] holds heads x 128
+ * queries, then kv_heads x 128 keys, then the values; query head h reads key head h / (heads / kv_heads). Row j of a
+ * sequence, position n[s] + j, attends to positions 0 .. n[s] - 1 as the pages hold them and to rows 0 .. j of its
+ * sequence as given, whose keys and values are appended at positions n[s] ..: out = softmax(q k^T scale) v, bf16 [rows,
+ * heads * 128]. Rows of a slot out of range, or with n[s] < 0, get zeros, and nothing is appended. Rows in front of
+ * starts[0] or from starts[seqs] on are left as they were. A page that is appended to belongs to one sequence of the
+ * call, and so does its slot; full pages may be shared by any number. What a row does not attend to never shows in it,
+ * NaN and infinities included. out must not overlap q. splits (1 .. 64) divides the keys over workgroups and needs part
+ * with rows x heads x splits x 130 floats, of one call at a time. fp32 sums; the weights are held to 2^-17 of
+ * themselves, in bf16 (2^-9) where a sequence and key head have more than 16 query rows on average. */
 int cohere_dec_attention_paged(const int32_t* active, const int32_t* starts, int64_t seqs, const uint16_t* q, int64_t ldq,
                                int64_t rows, uint16_t* k, uint16_t* v, int64_t pages, int64_t P, const int32_t* table,
                                int64_t width, const int32_t* n, int64_t slots, int64_t heads, int64_t kv_heads,
