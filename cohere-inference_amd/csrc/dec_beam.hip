@@ -120,6 +120,7 @@ struct SelectArgs {
   float* total;
   char* work;
   int n, G, B, V, N, pad, parts;
+  int eos;  // -1: none
 };
 
 // A workgroup takes J * 2048 logits of a row: their maximum, the sum, and the B best. A wave finds its B best among few:
@@ -389,9 +390,13 @@ __global__ void __launch_bounds__(64 * MAXB) beam_merge_kernel(const SelectArgs 
     total = lane == 0 ? start : -INFINITY;
   } else {
     const int have = __popcll(__ballot(cur != 0));
+    const bool nothing = have == 0 && a.eos >= 0;  // it ends here, at no cost
     v = (int)~(uint32_t)cur;
     if (cur) total = start + ((double)logit_of((uint32_t)(cur >> 32)) - (double)M - log(S));
-    if (have < B) {  // the lowest indexes that have no key
+    if (nothing) {
+      v = lane == 0 ? a.eos : lane - 1 + (lane - 1 >= a.eos);
+      total = lane == 0 ? start : -INFINITY;
+    } else if (have < B) {  // the lowest indexes that have no key
       int free = 0;
       for (int u = 0, to = have; to < B; ++u) {
         if (__any(cur != 0 && v == u)) continue;
@@ -617,12 +622,13 @@ extern "C" int64_t cohere_dec_beam_select_work(int64_t rows, int64_t V, int64_t 
   return rows * select_parts(rows, V) * part_bytes((int)beams);
 }
 
-extern "C" int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V,
-                                      const int32_t* groups, int64_t slots, const float* score, const uint8_t* finished,
-                                      const int32_t* made, const float* norm, int64_t norm_len, int64_t pad,
-                                      int32_t* parent, int64_t* token, float* total, void* work, int64_t work_bytes,
-                                      void* stream) {
+extern "C" int cohere_dec_beam_select_eos(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V,
+                                          const int32_t* groups, int64_t slots, const float* score,
+                                          const uint8_t* finished, const int32_t* made, const float* norm,
+                                          int64_t norm_len, int64_t pad, int64_t eos, int32_t* parent, int64_t* token,
+                                          float* total, void* work, int64_t work_bytes, void* stream) {
   cohere::clear_error();
+  COHERE_REQUIRE(eos >= -1 && eos < V, "dec_beam_select: the end token must be in the vocabulary (-1: none)");
   COHERE_REQUIRE(n >= 0 && beams >= 1 && beams <= MAXB && n * beams <= 65535 && slots > 0 && slots * beams <= TOP,
                  "dec_beam_select: 1 to 16 beams, at most 65535 rows");
   COHERE_REQUIRE(V >= beams && V % 8 == 0 && V < (int64_t(1) << 30) && ld >= V && ld % 8 == 0 && pad >= 0 && pad < V,
@@ -635,13 +641,23 @@ extern "C" int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_
                  "dec_beam_select: work of dec_beam_select_work bytes");
   const int64_t rows = n * beams;
   const SelectArgs a{logits, ld, groups, score, finished, made, norm, parent, token, total, static_cast<char*>(work),
-                     (int)n, (int)slots, (int)beams, (int)V, (int)norm_len, (int)pad, (int)select_parts(rows, V)};
+                     (int)n, (int)slots, (int)beams, (int)V, (int)norm_len, (int)pad, (int)select_parts(rows, V),
+                     (int)eos};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)a.parts, (unsigned)rows);
   if (select_j(rows, V) == 8) beam_parts_kernel<8><<<grid, 256, 0, s>>>(a);
   else beam_parts_kernel<1><<<grid, 256, 0, s>>>(a);
   beam_merge_kernel<<<(unsigned)n, (unsigned)beams * 64, 0, s>>>(a);
   return cohere::check_launch("dec_beam_select");
+}
+
+extern "C" int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V,
+                                      const int32_t* groups, int64_t slots, const float* score, const uint8_t* finished,
+                                      const int32_t* made, const float* norm, int64_t norm_len, int64_t pad,
+                                      int32_t* parent, int64_t* token, float* total, void* work, int64_t work_bytes,
+                                      void* stream) {
+  return cohere_dec_beam_select_eos(logits, ld, n, beams, V, groups, slots, score, finished, made, norm, norm_len, pad, -1,
+                                    parent, token, total, work, work_bytes, stream);
 }
 
 extern "C" int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, int64_t beams, const int32_t* parent,

@@ -24,7 +24,7 @@ decltype(&cohere_dec_attention_paged) f_paged;
 decltype(&cohere_dec_attention_paged_q8) f_paged_q8;
 decltype(&cohere_dec_gather_paged) f_gather_paged;
 decltype(&cohere_dec_gather_paged_q8) f_gather_paged_q8;
-decltype(&cohere_dec_beam_select) f_select;
+decltype(&cohere_dec_beam_select_eos) f_select;
 decltype(&cohere_dec_beam_reorder) f_reorder;
 decltype(&cohere_dec_beam_advance) f_advance;
 decltype(&cohere_last_error) f_error;
@@ -364,7 +364,7 @@ void beam_select(const Call& c) {
   const Tensor &logits = c.tensor(0), &groups = c.tensor(1), &score = c.tensor(2), &finished = c.tensor(3),
                &parent = c.tensor(7), &token = c.tensor(8), &total = c.tensor(9), &work = c.tensor(10);
   const Tensor *made = c.maybe(4), *norm = c.maybe(5);
-  const int64_t pad = c.whole(6), n = groups.numel();
+  const int64_t pad = c.whole(6), eos = c.whole(11), n = groups.numel();
   c.need(score.dim() == 2 && score.size(0) > 0 && score.size(1) >= 1 && score.size(1) <= 16, "score (groups, 1 to 16 beams)");
   const int64_t G = score.size(0), B = score.size(1);
   c.need(logits.dim() == 2 && logits.scalar_type() == at::kBFloat16 && logits.size(0) == n * B && logits.stride(1) == 1,
@@ -381,7 +381,7 @@ void beam_select(const Call& c) {
   launch([&] {
     return f_select(ptr<uint16_t>(logits), logits.stride(0), n, B, logits.size(1), ptr<int32_t>(groups), G,
                     ptr<float>(score), ptr<uint8_t>(finished), ptr<int32_t>(made), ptr<float>(norm),
-                    norm ? norm->numel() : 0, pad, ptr<int32_t>(parent), ptr<int64_t>(token), ptr<float>(total),
+                    norm ? norm->numel() : 0, pad, eos, ptr<int32_t>(parent), ptr<int64_t>(token), ptr<float>(total),
                     work.data_ptr(), work.numel(), st);
   });
 }
@@ -493,7 +493,7 @@ ENTRY("dec_attention_paged", paged, 11)
 ENTRY("dec_attention_paged_q8", paged_q8, 13)
 ENTRY("dec_gather_paged", gather_pages, 6)
 ENTRY("dec_gather_paged_q8", gather_pages_q8, 8)
-ENTRY("dec_beam_select", beam_select, 11)
+ENTRY("dec_beam_select", beam_select, 12)
 ENTRY("dec_beam_reorder", beam_reorder, 11)
 ENTRY("dec_beam_advance", beam_advance, 27)
 
@@ -516,7 +516,7 @@ PyObject* bind(PyObject*, PyObject* addresses) {
   at("cohere_dec_attention_paged_q8", f_paged_q8);
   at("cohere_dec_gather_paged", f_gather_paged);
   at("cohere_dec_gather_paged_q8", f_gather_paged_q8);
-  at("cohere_dec_beam_select", f_select);
+  at("cohere_dec_beam_select_eos", f_select);
   at("cohere_dec_beam_reorder", f_reorder);
   at("cohere_dec_beam_advance", f_advance);
   PyObject* c = PyImport_ImportModule("torch._C");

@@ -10,7 +10,8 @@ weights and cross-attention caches of kernels.stream_decoder.StreamDecoder, with
 
 Pages hold one position by default: nothing is ever copied then (with longer pages a step copies what the page in part
 filled holds, ext.dec_beam_reorder). The hypotheses of a slot are ranked by the sum of their tokens' log probabilities, by
-length_penalty divided by (tokens made) ^ length_penalty; ended ones stay among them. A slot is done once its best
+length_penalty divided by (tokens made) ^ length_penalty; ended ones stay among them. One whose rules leave it no token ends
+with the end token at no cost, as a row of StreamDecoder does. A slot is done once its best
 hypothesis has ended (without length_penalty: no other can pass it), once all have, or at its token limit.
 
     dec = BeamDecoder(model, beams=4, slots=16, int8=True)
@@ -105,12 +106,13 @@ class BeamDecoder(StreamDecoder):
         bufs, logits = self._buffers(rows), self.logits[:rows]
         parent, token, total = self.parent[:b], self.token[:b], self.total[:b]
         layers = range(len(self.blocks))
+        eos = self.eos if 0 <= self.eos < self.head.n else -1
         return (self._layers(bufs, [self._paged(i, act, None, self.pos, bufs.qkv, bufs.att) for i in layers],
                              [self._cross(i, slot_of, bufs.q, bufs.att) for i in layers])
                 + self._head(bufs, logits) + self._rules(act, logits)
                 + [lambda: ext.dec_beam_select(logits, groups, self.score, self.ended,
                                                None if self.norm is None else self.made, self.norm, self.pad, parent,
-                                               token, total, self.work),
+                                               token, total, self.work, eos),
                    lambda: ext.dec_beam_reorder(groups, parent, self.held, self.finished, self.table, self.out,
                                                 self.gstate, self.self_k, self.self_v, self.self_ks, self.self_vs),
                    lambda: ext.dec_beam_advance(groups, parent, token, total, self.dummy, self.tok, self.pos, self.held,

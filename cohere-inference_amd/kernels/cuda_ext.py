@@ -45,8 +45,8 @@ EXPORTS = ("cohere_gemm_i8", "cohere_gemm_sp", "cohere_quantize_rows", "cohere_l
            "cohere_piece_rows", "cohere_dec_attention_q4", "cohere_dec_attention_q4_splits", "cohere_dec_scatter_kv_q4",
            "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4", "cohere_dec_logits", "cohere_dec_attention_paged",
            "cohere_dec_attention_paged_q8", "cohere_dec_attention_paged_splits", "cohere_dec_gather_paged",
-           "cohere_dec_gather_paged_q8", "cohere_dec_beam_select", "cohere_dec_beam_select_work",
-           "cohere_dec_beam_reorder", "cohere_dec_beam_advance")
+           "cohere_dec_gather_paged_q8", "cohere_dec_beam_select", "cohere_dec_beam_select_eos",
+           "cohere_dec_beam_select_work", "cohere_dec_beam_reorder", "cohere_dec_beam_advance")
 
 
 def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
@@ -89,6 +89,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "cohere_dec_gather_paged": [P, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, P],
         "cohere_dec_gather_paged_q8": [P, P, I64, P, I64, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
         "cohere_dec_beam_select": [P, I64, I64, I64, I64, P, I64, P, P, P, P, I64, I64, P, P, P, P, I64, P],
+        "cohere_dec_beam_select_eos": [P, I64, I64, I64, I64, P, I64, P, P, P, P, I64, I64, I64, P, P, P, P, I64, P],
         "cohere_dec_beam_reorder": [P, I64, I64, P, P, P, I64, P, I64, P, I64, P, I64, P, P, P, P, I64, I64, I64, I64, I32,
                                     P],
         "cohere_dec_beam_advance": [P, I64, I64, P, P, P, I64, I64, P, P, P, P, P, P, P, P, P, I64, I64, I32, P, I64, P, I64,
@@ -148,7 +149,7 @@ def _ptr(t: torch.Tensor | None):
 # the functions that csrc/torch_calls.cpp calls with torch tensors
 CALLS = ("cohere_dec_attention_q4", "cohere_dec_scatter_kv_q4", "cohere_dec_gather_kv_q4", "cohere_gemm_kv_q4",
          "cohere_dec_logits", "cohere_dec_attention_paged", "cohere_dec_attention_paged_q8", "cohere_dec_gather_paged",
-         "cohere_dec_gather_paged_q8", "cohere_dec_beam_select", "cohere_dec_beam_reorder", "cohere_dec_beam_advance",
+         "cohere_dec_gather_paged_q8", "cohere_dec_beam_select_eos", "cohere_dec_beam_reorder", "cohere_dec_beam_advance",
          "cohere_last_error")
 
 
@@ -753,13 +754,14 @@ class _Ext:
         """Bytes of dec_beam_select's workspace."""
         return int(self._lib.cohere_dec_beam_select_work(int(rows), int(V), int(beams)))
 
-    def dec_beam_select(self, logits, groups, score, finished, made, norm, pad, parent, token, total, work):
+    def dec_beam_select(self, logits, groups, score, finished, made, norm, pad, parent, token, total, work, eos=-1):
         """The best continuations over a group's beams and the vocabulary: logits bf16 (n B, V), row i B + b beam b of
         group groups[i]; score fp32, finished uint8 and made int32 (groups, B). Candidates (b, v) have score + log
         softmax(l)[v]; a finished beam has pad alone, with its score. Ranked by total x norm[tokens made] (norm fp32; made
         and norm None: by total), the lowest b V + v first where equal. parent int32, token int64, total fp32 (n, B): the
-        B best, best first. work: uint8 of dec_beam_select_work(n B, V, B) bytes, of one call at a time."""
-        _calls.dec_beam_select(logits, groups, score, finished, made, norm, pad, parent, token, total, work)
+        B best, best first. work: uint8 of dec_beam_select_work(n B, V, B) bytes, of one call at a time. eos: what ends a
+        beam whose logits hold nothing above -inf, its score unchanged (-1: it has candidates of -inf alone)."""
+        _calls.dec_beam_select(logits, groups, score, finished, made, norm, pad, parent, token, total, work, eos)
 
     def dec_beam_reorder(self, groups, parent, n, done, table, tokens, states, k, v, ks, vs):
         """Every beam takes over its parent's history in place (slots: group x B + beam): table entries of full pages,

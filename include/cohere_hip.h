@@ -373,6 +373,14 @@ int cohere_dec_beam_select(const uint16_t* logits, int64_t ld, int64_t n, int64_
                            int64_t slots, const float* score, const uint8_t* finished, const int32_t* made,
                            const float* norm, int64_t norm_len, int64_t pad, int32_t* parent, int64_t* token, float* total,
                            void* work, int64_t work_bytes, void* stream);
+/* The same, but where nothing is left for a beam that goes on (score above -inf, not finished, no logit above -inf: a mask
+ * that allows nothing) it ends, as a row of cohere_dec_pick does: total = score[g][b] for v = eos (0 <= eos < V) and -inf
+ * for the others. eos -1: no such token, cohere_dec_beam_select. */
+int cohere_dec_beam_select_eos(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V,
+                               const int32_t* groups, int64_t slots, const float* score, const uint8_t* finished,
+                               const int32_t* made, const float* norm, int64_t norm_len, int64_t pad, int64_t eos,
+                               int32_t* parent, int64_t* token, float* total, void* work, int64_t work_bytes,
+                               void* stream);
 int64_t cohere_dec_beam_select_work(int64_t rows, int64_t V, int64_t beams);
 
 /* Every beam takes over its parent's history, in place: row b of group g = groups[i] (slot g * beams + b) gets of row
