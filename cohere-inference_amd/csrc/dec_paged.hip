@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
   // the tile's blocks: of the chunk's tokens up to its last one, then of the positions held; wave w has every W-th
   const int last = p.starts ? (t.x0 + t.rows - 1) / p.ratio : 0, nr = last / KB + 1;
   int n = 0, nb = 0, start = 0, end = 0, b = wave;
+  float rise = 0.f;
   bool row_ok = false;
   const int held = p.n[t.slot];  // on its way
   const auto bounds = [&]() {
@@ -64,6 +65,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     row_ok = n >= 0;
     n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
     nb = row_ok ? nr + (n + KB - 1) / KB : 0;
+    rise = rise_of((uint32_t)n + last + 1);
   };
   if constexpr (SPLIT) {  // without parts nothing up to the first loads waits for n
     bounds();
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        d[h][i] = exp2_hw(d[h][i] - to);
+        d[h][i] = exp2_hw(d[h][i] - to - rise);
         l += d[h][i];
       }
   };
@@ -166,6 +168,9 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
 
   // the chunk's own blocks, as given; bad: of the wave's some values are infinite or NaN
   bool bad = false;
+  if constexpr (!SPLIT) {
+    if (!single) bounds();  // the weights' rise
+  }
   for (; !single && b < (SPLIT ? min(end, nr) : nr); b += W) {
     const int j0 = b * KB;
     const auto own_row = [&](int j) { return rowkv + (int64_t)min(j, t.c - 1) * p.ldq; };
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     }
     dot = xor32_sum(xor16_sum(dot)) * p.scale;
     m = dot == dot ? dot : -INFINITY;  // maxima pass over a NaN, the sum keeps it
-    const float e = dot == -INFINITY ? 0.f : exp2_hw(dot - m);  // 1, but for scores that are not finite
+    const float e = dot == -INFINITY ? 0.f : exp2_hw(dot - m - rise);
     l = grp == 0 ? e : 0.f;
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
     if (nsp == 1) {
       float o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = L == 0.f ? 0.f : O[i] / L;
+      for (int i = 0; i < 4; ++i) o[i] = L == 0.f ? 0.f : mean_of(O[i], O[i] / L);
       *reinterpret_cast<uint2*>(p.out + at * HD + dim) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
     } else {
       float* part = p.part + (at * nsp + sp) * (HD + 2);  // parts are 520 bytes apart: 8-byte stores
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
   for (int i = 0; i < N; ++i)
     if (grp + CG * i < nsp) o = __builtin_fmaf(lane_value(w, grp + CG * i), v[i], o);
   if constexpr (CG == 1) {
-    out[head * HD + d] = f2bf(L == 0.f ? 0.f : o / L);
+    out[head * HD + d] = f2bf(L == 0.f ? 0.f : mean_of(o, o / L));
   } else {
     __shared__ float so[CG][HD];
     so[grp][d] = o;
@@ -485,7 +490,7 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
       float O = 0.f;
 #pragma unroll
       for (int g = 0; g < CG; ++g) O += so[g][d];
-      out[head * HD + d] = f2bf(L == 0.f ? 0.f : O / L);
+      out[head * HD + d] = f2bf(L == 0.f ? 0.f : mean_of(O, O / L));
     }
   }
 }
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __
         o1 = __builtin_fmaf(wi, v[i].y, o1);
       }
   }
-  *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(o0 / L, o1 / L);
+  *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(mean_of(o0, o0 / L), mean_of(o1, o1 / L));
 }
 
 // ---- reading back ------------------------------------------------------------------------------------------------------

@@ -13,7 +13,8 @@
 // only in part. 4 x 2048 tokens x 32 heads behind 6 to 8 K positions: 1044 us, 1054 TFLOP/s (a large product of the library:
 // 1188); a tile alone on its CU takes 1.2 us, int8 1.7 (their conversion).
 // Maximum, sum and outputs of a query stay in lanes l % 32 = query. The base of a query's weights is set 2^8 above its
-// largest score and moves only when a score passes it, so that rescaling is rare and weights are at most 1.
+// largest score and the number of keys above that (rise_of), and moves only when a score passes the latter, so that
+// rescaling is rare.
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
 // need three products for one).
 #include "paged.h"
@@ -88,6 +89,7 @@ paged_chunk_kernel(const PagedArgs p) {
   const bool row_ok = n >= 0;
   n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
   const int hi = row_ok ? (t.x0 + t.rows - 1) / p.ratio + 1 : 0;  // the chunk's tokens that the tile's last row sees
+  const float rise = rise_of((uint32_t)n + hi);
   const int np = (n + KT - 1) / KT, nb = np + (hi + KT - 1) / KT;
   // as many parts as there are for `least` tiles each
   const int parts = max(1, min(nsp, nb / p.least));
@@ -305,7 +307,7 @@ paged_chunk_kernel(const PagedArgs p) {
     }
 #pragma unroll
     for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
-    mx = xor32_max(mx) * scale;
+    mx = xor32_max(mx) * scale + rise;
     if (__any(mx > base)) {
       const float to = mx > base ? mx + RISE : base, a = to == -INFINITY ? 1.f : exp2_hw(base - to);
       l *= a;
@@ -438,7 +440,7 @@ paged_chunk_kernel(const PagedArgs p) {
         for (int g = 0; g < 4; ++g) {
           float o[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = l == 0.f ? 0.f : acc[dt][4 * g + k] * inv;
+          for (int k = 0; k < 4; ++k) o[k] = l == 0.f ? 0.f : mean_of(acc[dt][4 * g + k], acc[dt][4 * g + k] * inv);
           *reinterpret_cast<uint2*>(dst + dt * 32 + g * 8) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
         }
     } else {

@@ -32,6 +32,17 @@ struct PagedArgs {
 
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Weights are at most 2^-rise of a row's number of keys, so that their sum is below 1 and that of weight x value no larger
+// than the largest value: with weights up to 1 two of the type's largest would be infinite before the division.
+DEVI float rise_of(uint32_t keys) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint((float)(32 - __clz((int)keys)))));
+}
+// a mean is no larger than the type's largest; the sums' roundings must not make it so
+DEVI float mean_of(float sum, float mean) {
+  constexpr float TOP = 0x1.fep127f;
+  return fabsf(mean) > TOP && fabsf(sum) < INFINITY ? copysignf(TOP, mean) : mean;
+}
+
 // One workgroup's sequence and tile of TM query rows (x = token * ratio + head of the key head's): sequence i has the
 // tiles base(i) .. , base(i) = floor(starts[i] ratio / TM) + i, which leaves each at least the tiles that it needs, so that
 // neither the host nor a prefix sum has to know the chunks. Tiles without rows end at once.
