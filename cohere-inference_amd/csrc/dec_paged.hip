@@ -435,11 +435,14 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))
       L += mw == -INFINITY ? sl[w][r] : exp2_hw(mw - MM) * sl[w][r];
       O += *reinterpret_cast<const v4f*>(region + w * REGION + (r * LD + dim) * 4);
     }
-    if (__builtin_expect(left_out && row_ok, 0)) {  // the row sees what was left out up to its own token
-      const int from = SPLIT ? start * KB : 0, to = min(tk + 1, SPLIT ? end * KB : t.c);
-      for (int j = from; j < to; ++j)
+    const bool finite = fabsf(O[0]) < INFINITY && fabsf(O[1]) < INFINITY && fabsf(O[2]) < INFINITY && fabsf(O[3]) < INFINITY;
+    if (__builtin_expect((left_out || !finite) && row_ok && fabsf(L) < INFINITY, 0)) {
+      v4f s = {0.f, 0.f, 0.f, 0.f};  // of the part's keys that the row sees: up to its own token, and those held
+      for (int j = start * KB, to = min(tk + 1, end * KB); j < to; ++j) add_given(s, rowkv + p.KV * HD, p.ldq, j, dim);
+      for (int j = max(start - nr, 0) * KB, to = min((int64_t)n, (int64_t)(end - nr) * KB); j < to; ++j)
+        add_held<Q8>(s, p, row, kvh, j, dim);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) O[i] += not_finite(rowkv[(int64_t)j * p.ldq + p.KV * HD + dim + i]);
+      for (int i = 0; i < 4; ++i) O[i] = s[i] == 0.f ? O[i] : s[i];
     }
     const int64_t at = (int64_t)(t.first + tk) * p.H + kvh * p.ratio + (xr - tk * p.ratio);
     if (nsp == 1) {
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
   float o = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (grp + CG * i < nsp) o = __builtin_fmaf(lane_value(w, grp + CG * i), v[i], o);
+    if (grp + CG * i < nsp) o = add_part(lane_value(w, grp + CG * i), v[i], o);
   if constexpr (CG == 1) {
     out[head * HD + d] = f2bf(L == 0.f ? 0.f : mean_of(o, o / L));
   } else {
@@ -523,8 +526,8 @@ __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __
     for (int i = 0; i < N; ++i)
       if (i0 + i < last && there >> (i0 + i) & 1) {  // in the others nothing has to have been written
         const float wi = lane_value(w, i0 + i);
-        o0 = __builtin_fmaf(wi, v[i].x, o0);
-        o1 = __builtin_fmaf(wi, v[i].y, o1);
+        o0 = add_part(wi, v[i].x, o0);
+        o1 = add_part(wi, v[i].y, o1);
       }
   }
   *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(mean_of(o0, o0 / L), mean_of(o1, o1 / L));

@@ -416,19 +416,30 @@ paged_chunk_kernel(const PagedArgs p) {
   }
   l = xor32_sum(l);
   if (wave * 32 + col < t.rows) {
-    if (__builtin_expect(bad, 0)) {
-      // of the part's tiles of the chunk's tokens those that some row of the wave's does not see whole
-      const int from = max((tok0 + 1) / KT, max(start - np, 0)) * KT, to = min(tok + 1, (end - np) * KT);
+    float zero = 0.f;  // NaN, if an output is not finite
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(acc[dt][r], 0.f, zero);
+    if (__builtin_expect((bad || zero != 0.f) && fabsf(l) < INFINITY, 0)) {
+      v4f s[16];  // of the part's keys that the row sees: those held, and up to its own token
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-      for (int j = from; j < to; ++j) {
-        const uint16_t* src = rowkv + (int64_t)j * p.ldq + p.KV * HD + half * 4;
+      for (int j = start * KT, to = (int)min((int64_t)n, (int64_t)end * KT); j < to; ++j)
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int i = 0; i < 16; ++i) add_held<Q8>(s[i], p, row, kvh, j, i * 8 + half * 4);
+#pragma unroll 1
+      for (int j = max(start - np, 0) * KT, to = min(tok + 1, (end - np) * KT); j < to; ++j)
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
+        for (int i = 0; i < 16; ++i) add_given(s[i], rowkv + p.KV * HD, p.ldq, j, i * 8 + half * 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[dt][4 * g + k] += not_finite(src[dt * 32 + g * 8 + k]);
-      }
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = (i & 3) * 4 + k;
+          acc[i >> 2][r] = s[i][k] == 0.f ? acc[i >> 2][r] : s[i][k];
+        }
     }
     const int64_t at = (int64_t)(t.first + tok) * p.H + head;
     if (parts == 1) {

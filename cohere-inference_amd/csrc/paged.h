@@ -122,7 +122,7 @@ DEVI void unpack8(const uint4& u, float (&f)[8]) {
 }
 
 // Infinities and NaN among a chunk's own values: 0 x them is NaN, where a query does not see the key. They leave the product
-// (made zeros; whether there were any in the wave), and are added to the outputs of the rows that see them at the end.
+// (made zeros; whether there were any in the wave), and come back to the outputs of the rows that see them at the end.
 template <int N>
 DEVI bool leave_out(v8bf (&v)[N]) {
   const auto marks = [](int w) { return ((uint32_t)w & 0x7f807f80u) + 0x00800080u; };  // bits 15, 31: exponent of all ones
@@ -144,7 +144,28 @@ DEVI bool leave_out(v8bf (&v)[N]) {
   return some;
 }
 // the value, if it is infinite or NaN
-DEVI float not_finite(uint32_t h) { return (h & 0x7f80u) == 0x7f80u ? __uint_as_float(h << 16) : 0.f; }
+DEVI float not_finite(float x) { return fabsf(x) < INFINITY ? 0.f : x; }
+
+// Outputs that infinite or NaN values have reached: in the products they meet weights that are rounded to 0 and remainders of
+// weights, and become NaN, where the definition has them whole. These outputs are the sums of such values alone, which are
+// read once more: 4 dimensions from `dim` on, of token j as given (rowv: the chunk's first values) or of position t held.
+DEVI void add_given(v4f& s, const uint16_t* rowv, int64_t ldq, int j, int dim) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] += not_finite(__uint_as_float((uint32_t)rowv[j * ldq + dim + i] << 16));
+}
+template <bool Q8>
+DEVI void add_held(v4f& s, const PagedArgs& p, const int32_t* row, int kvh, int t, int dim) {
+  const int page = row[t >> p.shift];
+  if ((unsigned)page >= (unsigned)p.pages) return;
+  const int64_t vec = (((int64_t)page * p.KV + kvh) << p.shift) + (t & ((1 << p.shift) - 1));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Q8) s[i] += not_finite((float)static_cast<const int8_t*>(p.v)[vec * HD + dim + i] * p.vs[vec]);
+    else s[i] += not_finite(__uint_as_float((uint32_t)static_cast<const uint16_t*>(p.v)[vec * HD + dim + i] << 16));
+  }
+}
+// a part's output by its weight; one that is not finite however small that is
+DEVI float add_part(float w, float v, float o) { return fabsf(v) < INFINITY ? __builtin_fmaf(w, v, o) : o + v; }
 
 // a vector (16 lanes, 8 values each, u) as it is held, at vector `vec` of the pages; every lane takes part, `live` writes
 template <bool Q8>
