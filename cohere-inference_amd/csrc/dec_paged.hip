@@ -6,7 +6,7 @@
 //                        go into the pages at n ..
 //   dec_gather_paged     keys and values of (slot, position) pairs as bf16 rows
 #include "cohere_hip.h"
-#include "paged.h"
+#include "paged_rows.h"
 
 #include <string>
 #include <type_traits>
@@ -15,455 +15,26 @@ namespace {
 
 using namespace cohere_paged;
 
-// ---- attention, few query rows -----------------------------------------------------------------------------------------
-// A workgroup takes 16 query rows of a (sequence, key head) and one part of the keys; its waves take blocks of 32 keys in
-// turn, each by itself:
-//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16, twice 16 keys: lane (key l % 16, l / 16) loads 16-byte pieces of its keys, and
-//   gets of the result the scores of query l % 16 with keys 4 (l / 16) + i in register i. bf16 products are exact in fp32.
-//   O^T = V^T P^T on the same instruction, 32 keys at once: the weights as they stand are its B operand (the order of the
-//   32 keys is free, and taken as the lanes hold them); V^T comes from the wave's own 8 KB of LDS, into which the loads go
-//   straight (int8: through registers, converted), by the transposing read. A weight is held as the sum of two bf16 numbers
-//   (to 2^-17 of itself), two products.
-// The maximum, the sum and the outputs of a query stay in lanes l % 16 = query: a new maximum rescales without any move.
-// Why not fp32 products, which need no LDS and no second bf16 number: 16 keys would keep a SIMD's matrix core 1024 cycles
-// where this takes 128, and a wave alone took 2570 cycles for 16 keys.
-constexpr int KB = 32;
-typedef short v4s __attribute__((ext_vector_type(4)));
-
-// what absent values are read from
-__device__ __attribute__((aligned(16))) uint32_t zero_row[4];
-
-// 16 bytes a lane from `offset` + `more` behind a buffer's start, zeros behind its end, into LDS at dst + 16 lane
-DEVI void buffer_to_lds(__amdgpu_buffer_rsrc_t r, int offset, int more, char* dst) {
-#ifdef __HIP_DEVICE_COMPILE__  // the host's pass refuses the builtin
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_AS void*)dst, 16, offset, more, 0, 0);
-#endif
-}
-
+// ---- attention of a token per sequence --------------------------------------------------------------------------------
 template <bool Q8, bool BIG, bool SPLIT, int W>
 __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))) paged_rows_kernel(const PagedArgs p) {
-  constexpr int LD = HD + 4, REGION = 16 * LD * 4;  // a wave's values (32 x 256 bytes), later its outputs
-  static_assert(REGION >= KB * 256 && REGION % 256 == 0, "a wave's region");
-  __shared__ __attribute__((aligned(256))) char region[W * REGION];
-  __shared__ float sm[W][16], sl[W][16];
-  __shared__ int sbad[W];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, grp = lane >> 4;
-  const int kvh = blockIdx.x % p.KV, sp = SPLIT ? blockIdx.y : 0, nsp = SPLIT ? p.parts : 1;
-  const Tile t = tile_of<16>(p, blockIdx.x / p.KV);
-  if (t.rows == 0) return;
-  char* sv = region + wave * REGION;
-  const int32_t* row = p.table + (int64_t)t.slot * p.W;
-  const int P1 = (1 << p.shift) - 1;
-  // the tile's blocks: of the chunk's tokens up to its last one, then of the positions held; wave w has every W-th
-  const int last = p.starts ? (t.x0 + t.rows - 1) / p.ratio : 0, nr = last / KB + 1;
-  int n = 0, nb = 0, start = 0, end = 0, b = wave;
-  float rise = 0.f;
-  bool row_ok = false;
-  const int held = p.n[t.slot];  // on its way
-  const auto bounds = [&]() {
-    n = t.ok ? held : -1;
-    row_ok = n >= 0;
-    n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
-    nb = row_ok ? nr + (n + KB - 1) / KB : 0;
-    rise = rise_of((uint32_t)n + last + 1);
-  };
-  if constexpr (SPLIT) {  // without parts nothing up to the first loads waits for n
-    bounds();
-    const int chunk = (nb + nsp - 1) / nsp;
-    start = min(nb, sp * chunk);
-    end = min(nb, start + chunk);
-    b = start + wave;
-  }
-  // The first of the wave's blocks of positions held, and the pages of these. BIG (pages of 16 or more): of half h of the
-  // k-th one in lane 2 (k % 32) + h. Else one a key (lane % 32), one block ahead.
-  const int b0 = b >= nr ? b : b + (nr - b + W - 1) / W * W;
-  const auto entry_of = [&](int block) {
-    const int64_t at = BIG ? (int64_t)(block + (lane >> 1) * W - nr) * KB + (lane & 1) * 16
-                           : (int64_t)(block - nr) * KB + (lane & 31);
-    return row[min(at >> p.shift, (int64_t)p.W - 1)];
-  };
-  int entry = entry_of(b0);
-
-  // the lane's query row (the tile's last one repeated), its token and head
-  const int x = t.x0 + min(col, t.rows - 1), tok = p.starts ? x / p.ratio : 0,
-            head = kvh * p.ratio + (x - tok * p.ratio);
-  // the dimensions that a lane holds of a product's step s: as 16-byte loads of int8 or bf16 vectors bring them
-  const auto dims = [&](int s) { return Q8 ? (s >> 1) * 64 + grp * 16 + (s & 1) * 8 : s * 32 + grp * 8; };
-  v8bf qf[4];
-  {
-    const uint16_t* qp = p.q + (int64_t)(t.first + tok) * p.ldq + head * HD;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) qf[s] = *reinterpret_cast<const v8bf*>(qp + dims(s));
-  }
-
-  const uint16_t* rowkv = p.q + (int64_t)t.first * p.ldq + (p.H + kvh) * HD;
-  // A chunk of one token has one key of its own, which every row sees: its score is the first maximum and its value the
-  // first outputs, without a product; the loads are made here, and waited for behind the first block's.
-  const bool single = t.c == 1, first = single && b == 0;
-  v8bf k1[4];
-  uint2 v1[8];
-  if (first) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) k1[s] = *reinterpret_cast<const v8bf*>(rowkv + dims(s));
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) v1[dt] = *reinterpret_cast<const uint2*>(rowkv + p.KV * HD + dt * 16 + grp * 4);
-  }
-
-  v4f acc[8];  // dimensions 16 dt + 4 grp + i of query col in acc[dt][i]
-#pragma unroll
-  for (int dt = 0; dt < 8; ++dt) acc[dt] = v4f{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-
-  // scores d of the lane's query with keys 16 h + 4 grp + i become weights; m, l, acc follow
-  const auto softmax = [&](v4f (&d)[2]) {
-    float mx = fmaxf(fmaxf(fmaxf(d[0][0], d[0][1]), fmaxf(d[0][2], d[0][3])),
-                     fmaxf(fmaxf(d[1][0], d[1][1]), fmaxf(d[1][2], d[1][3])));
-    mx = xor32_max(xor16_max(mx));
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, mx), a = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
-      l *= a;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) acc[dt] *= a;
-      m = mn;
-    }
-    const float to = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        d[h][i] = exp2_hw(d[h][i] - to - rise);
-        l += d[h][i];
-      }
-  };
-  // Values lie in LDS as bf16: key k's 16-byte pieces c at 256 k + 16 (c ^ 2 (k % 8)), so that the transposing reads, 16
-  // keys' 32 bytes each, meet no bank twice.
-  v8bf vf[8];
-  const auto read_v = [&]() {
-    const int k = grp * 4 + (col >> 2), at = k * 256 + (k & 7) * 32 + (col & 3) * 8;
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-      const char* src = sv + (at ^ (dt * 32));
-      const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)src);
-      const v4s c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4s*)(src + 16 * 256));
-      vf[dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, before other values are on their way
-  };
-  // weights as the product's B operand, twice: rounded, and what that left
-  const auto products = [&](const v4f (&d)[2]) {
-    v4i hi, lo;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float a = d[k >> 1][(k & 1) * 2], c = d[k >> 1][(k & 1) * 2 + 1];
-      hi[k] = (int)pack_bf2(a, c);
-      lo[k] = (int)pack_bf2(a - __uint_as_float((uint32_t)hi[k] << 16), c - __uint_as_float((uint32_t)hi[k] & 0xffff0000u));
-    }
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt)
-      acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[dt], __builtin_bit_cast(v8bf, hi), acc[dt], 0, 0, 0);
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt)
-      acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[dt], __builtin_bit_cast(v8bf, lo), acc[dt], 0, 0, 0);
-  };
-
-  // the chunk's own blocks, as given; bad: of the wave's some values are infinite or NaN
-  bool bad = false;
-  if constexpr (!SPLIT) {
-    if (!single) bounds();  // the weights' rise
-  }
-  for (; !single && b < (SPLIT ? min(end, nr) : nr); b += W) {
-    const int j0 = b * KB;
-    const auto own_row = [&](int j) { return rowkv + (int64_t)min(j, t.c - 1) * p.ldq; };
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = i * 4 + grp;
-      const char* at = reinterpret_cast<const char*>(own_row(j0 + k) + p.KV * HD) + (col ^ ((k & 7) * 2)) * 16;
-      at = j0 + k < t.c ? at : reinterpret_cast<const char*>(zero_row);
-      __builtin_amdgcn_global_load_lds(at, (LDS_AS void*)(sv + i * 4 * 256), 16, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    v4f d[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint16_t* kp = own_row(j0 + h * 16 + col);
-      d[h] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const v8bf*>(kp + dims(s)), qf[s], d[h], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[h][i] = j0 + h * 16 + grp * 4 + i <= tok ? d[h][i] * p.scale : -INFINITY;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    softmax(d);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    read_v();
-    bad |= leave_out(vf);
-    products(d);
-  }
-
-  // Positions held. A block's keys and values on their way. BIG: through buffers of a half (nothing, where it has no page),
-  // addressed by constants; else an absent page's keys read page 0, and its values zeros.
-  constexpr int VEC = Q8 ? HD : 2 * HD, KS = Q8 ? 2 : 4;  // bytes of a vector, loads of a key
-  v4i kf[2][KS], vr[Q8 ? 4 : 1];
-  v4f ks[2], vs[2];
-  uint32_t there = 0;  // keys with a page
-  int pages_of = 0;
-  int64_t base[2];
-  const auto rsrc = [&](const void* pages, int h, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(pages)) + base[h] * bytes, 0,
-                                             there >> (16 * h) & 1 ? 16 * bytes : 0, 0x00027000);
-  };
-  const auto vec_of = [&](int block, int k) {  // vectors are counted in 32 bits
-    return (((uint32_t)__shfl(pages_of, k, 64) * (uint32_t)p.KV + kvh) << p.shift) + (((block - nr) * KB + k) & P1);
-  };
-  const auto load_k = [&](int block, bool any) {  // any: the block is one
-    if constexpr (BIG) {
-      there = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int page = __builtin_amdgcn_readlane(entry, ((block - b0) / W & 31) * 2 + h);
-        const bool ok = any & ((unsigned)page < (unsigned)p.pages);
-        base[h] = (((int64_t)(ok ? page : 0) * p.KV + kvh) << p.shift) + (((block - nr) * KB + h * 16) & P1);
-        there |= ok ? 0xffffu << (16 * h) : 0u;
-      }
-    } else {
-      const bool ok = any && (unsigned)entry < (unsigned)p.pages;
-      there = (uint32_t)__ballot(ok);  // lanes 32 .. hold the same
-      pages_of = ok ? entry : 0;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (BIG) {
-        const auto r = rsrc(p.k, h, VEC);
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-          kf[h][s] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, col * VEC + grp * 16 + s * 64, 0, 0));
-        if constexpr (Q8) {
-          ks[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rsrc(p.ks, h, 4), grp * 16, 0, 0));
-          vs[h] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rsrc(p.vs, h, 4), grp * 16, 0, 0));
-        }
-      } else {
-        const char* at = static_cast<const char*>(p.k) + (uint64_t)vec_of(block, h * 16 + col) * VEC;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) kf[h][s] = *reinterpret_cast<const v4i*>(at + grp * 16 + s * 64);
-        if constexpr (Q8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t vec = vec_of(block, h * 16 + grp * 4 + i);
-            ks[h][i] = p.ks[vec];
-            vs[h][i] = p.vs[vec];
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-      }
-    }
-  };
-  const auto load_v = [&](int block) {
-    if constexpr (Q8) {  // 8 keys a load, 16 dimensions a lane
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (BIG)
-          vr[i] = __builtin_bit_cast(
-              v4i, __builtin_amdgcn_raw_buffer_load_b128(rsrc(p.v, i >> 1, VEC), lane * 16 + (i & 1) * 8 * VEC, 0, 0));
-        else
-          vr[i] = *reinterpret_cast<const v4i*>(static_cast<const char*>(p.v) +
-                                                (uint64_t)vec_of(block, i * 8 + (lane >> 3)) * VEC + (lane & 7) * 16);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = i * 4 + grp, c = col ^ ((k & 7) * 2);
-        if constexpr (BIG) {
-          buffer_to_lds(rsrc(p.v, i >> 2, VEC), grp * VEC + c * 16, (i & 3) * 4 * VEC, sv + i * 4 * 256);
-        } else {
-          const char* at = static_cast<const char*>(p.v) + (uint64_t)vec_of(block, k) * VEC + c * 16;
-          at = there >> k & 1 ? at : reinterpret_cast<const char*>(zero_row);
-          __builtin_amdgcn_global_load_lds(at, (LDS_AS void*)(sv + i * 4 * 256), 16, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);  // one address after the other: together they would take 16 registers
-        }
-      }
-    }
-  };
-  load_k(b0, true);
-  load_v(b0);
-  if constexpr (!BIG) entry = entry_of(b0 + W);
-  if constexpr (!SPLIT) {
-    bounds();
-    end = nb;
-  }
-  Append<Q8, W, 2> own;  // 16 tokens at most: two steps
-  const bool writes = sp == 0 && row_ok && own.load(p, t, n, kvh, 16, 0);
-  if (first) {
-    float dot = 0.f;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      float a[8], c[8];
-      unpack8(__builtin_bit_cast(uint4, qf[s]), a);
-      unpack8(__builtin_bit_cast(uint4, k1[s]), c);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(a[i], c[i], dot);
-    }
-    dot = xor32_sum(xor16_sum(dot)) * p.scale;
-    m = dot == dot ? dot : -INFINITY;  // maxima pass over a NaN, the sum keeps it
-    const float e = dot == -INFINITY ? 0.f : exp2_hw(dot - m - rise);
-    l = grp == 0 ? e : 0.f;
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt)
-      acc[dt] = e * v4f{__uint_as_float(v1[dt].x << 16), __uint_as_float(v1[dt].x & 0xffff0000u),
-                        __uint_as_float(v1[dt].y << 16), __uint_as_float(v1[dt].y & 0xffff0000u)};
-  }
-
-  // Each block's loads are made under the products of the one before it.
-  for (b = b0; b < end; b += W) {
-    const int left = n - (b - nr) * KB;
-    const uint32_t live = (left < KB ? ~0u >> (KB - left) : ~0u) & there;
-    v4f d[2], vscale[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      d[h] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        v4i w;
-        if constexpr (Q8) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int y = kf[h][s >> 1][(s & 1) * 2 + (k >> 1)];
-            w[k] = (int)pack_bf2((float)(int8_t)(y >> (16 * (k & 1))), (float)(int8_t)(y >> (16 * (k & 1) + 8)));
-          }
-        } else {
-          w = kf[h][s];
-        }
-        d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), qf[s], d[h], 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[h][i] *= Q8 ? ks[h][i] * p.scale : p.scale;
-    }
-    if constexpr (Q8) {  // values from the registers into LDS
-      vscale[0] = vs[0];
-      vscale[1] = vs[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = i * 8 + (lane >> 3);
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int y = vr[i][j >> 1] >> (16 * (j & 1));
-          w[j] = pack_bf2((float)(int8_t)y, (float)(int8_t)(y >> 8));
-        }
-        char* dst = sv + k * 256 + (((lane & 7) ^ (k & 7)) * 32);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(dst + 16) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-    }
-    if (live != ~0u) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = live >> (h * 16 + grp * 4 + i) & 1;
-          d[h][i] = in ? d[h][i] : -INFINITY;
-          if constexpr (Q8) vscale[h][i] = in ? vscale[h][i] : 0.f;
-        }
-      if constexpr (!Q8) {  // what lies behind the last position may be NaN, and 0 x it too
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll 1
-        for (int k = grp; k < KB; k += 4)
-          if (!(live >> k & 1)) *reinterpret_cast<uint4*>(sv + k * 256 + col * 16) = make_uint4(0, 0, 0, 0);
-      }
-    }
-    read_v();
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (BIG) {
-      if (__builtin_expect(((b + W - b0) / W & 31) == 0, 0)) entry = entry_of(b + W);
-    }
-    load_k(b + W, b + W < end);
-    load_v(b + W);
-    if constexpr (!BIG) entry = entry_of(b + 2 * W);
-    __builtin_amdgcn_sched_barrier(0);
-    softmax(d);
-    if constexpr (Q8) {
-      d[0] *= vscale[0];
-      d[1] *= vscale[1];
-    }
-    products(d);
-  }
-  if (!row_ok) {
-    m = -INFINITY;
-    l = 0.f;
-  }
-
-  if (writes) own.store(p, n, kvh);
-
-  // the waves' results meet: each wave's outputs by its share of the largest maximum, summed by all threads
-  l = xor32_sum(xor16_sum(l));
-  if (lane == 0) sbad[wave] = bad;
-  if (grp == 0) {
-    sm[wave][col] = m;
-    sl[wave][col] = l;
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads into the region
-  __syncthreads();
-  float M = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w][col]);
-  const float f = m == -INFINITY ? 0.f : exp2_hw(m - M);
-  if (col < t.rows) {
-    float* dst = reinterpret_cast<float*>(sv) + col * LD + grp * 4;
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-      v4f o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = m == -INFINITY ? 0.f : f * acc[dt][i];  // a wave without keys has outputs of 0
-      *reinterpret_cast<v4f*>(dst + dt * 16) = o;
-    }
-  }
-  __syncthreads();
-  int left_out = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) left_out |= sbad[w];
-  const int dim = (tid & 31) * 4;  // 32 threads a row, 4 dimensions each
-  for (int r = tid >> 5; r < t.rows; r += W * 2) {
-    const int xr = t.x0 + r, tk = p.starts ? xr / p.ratio : 0;
-    float MM = -INFINITY, L = 0.f;
-    v4f O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < W; ++w) MM = fmaxf(MM, sm[w][r]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float mw = sm[w][r];
-      L += mw == -INFINITY ? sl[w][r] : exp2_hw(mw - MM) * sl[w][r];
-      O += *reinterpret_cast<const v4f*>(region + w * REGION + (r * LD + dim) * 4);
-    }
-    const bool finite = fabsf(O[0]) < INFINITY && fabsf(O[1]) < INFINITY && fabsf(O[2]) < INFINITY && fabsf(O[3]) < INFINITY;
-    if (__builtin_expect((left_out || !finite) && row_ok && fabsf(L) < INFINITY, 0)) {
-      v4f s = {0.f, 0.f, 0.f, 0.f};  // of the part's keys that the row sees: up to its own token, and those held
-      for (int j = start * KB, to = min(tk + 1, end * KB); j < to; ++j) add_given(s, rowkv + p.KV * HD, p.ldq, j, dim);
-      for (int j = max(start - nr, 0) * KB, to = min((int64_t)n, (int64_t)(end - nr) * KB); j < to; ++j)
-        add_held<Q8>(s, p, row, kvh, j, dim);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) O[i] = s[i] == 0.f ? O[i] : s[i];
-    }
-    const int64_t at = (int64_t)(t.first + tk) * p.H + kvh * p.ratio + (xr - tk * p.ratio);
-    if (nsp == 1) {
-      float o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = L == 0.f ? 0.f : mean_of(O[i], O[i] / L);
-      *reinterpret_cast<uint2*>(p.out + at * HD + dim) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
-    } else {
-      float* part = p.part + (at * nsp + sp) * (HD + 2);  // parts are 520 bytes apart: 8-byte stores
-      *reinterpret_cast<float2*>(part + dim) = make_float2(O[0], O[1]);
-      *reinterpret_cast<float2*>(part + dim + 2) = make_float2(O[2], O[3]);
-      if (dim == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(MM, L);
-    }
-  }
+  __shared__ FewRows<W> lds;
+  const int i = blockIdx.x / p.KV;
+  Tile t;
+  t.first = i;
+  t.c = 1;
+  t.x0 = 0;
+  t.rows = p.ratio;
+  t.slot = p.active[i];
+  t.ok = (unsigned)t.slot < (unsigned)p.slots;
+  t.slot = t.ok ? t.slot : 0;
+  few_rows<Q8, BIG, SPLIT, W>(p, t, blockIdx.x % p.KV, lds);
 }
 
-// The parts of a (row, head), for rows of the sequences: every wave finds the maximum, the parts' weights (lane s part s's)
-// and the sum; CG groups of 128 threads sum N parts each, all their loads in flight at once.
+// The parts of a (row, head): every wave finds the maximum, the parts' weights (lane s part s's) and the sum; CG groups of 128
+// threads sum N parts each, all their loads in flight at once.
 template <int CG, int N>
-__global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __restrict__ part, const int32_t* starts, int S,
-                                                                int H, int nsp, uint16_t* out) {
+__global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __restrict__ part, int nsp, uint16_t* out) {
   const int64_t head = blockIdx.x;
   const int tid = threadIdx.x, lane = lane_id(), d = tid & (HD - 1), grp = wave_id() >> 1;
   const float* base = part + head * nsp * (HD + 2);
@@ -472,10 +43,6 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
   float v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = base[min(grp + CG * i, nsp - 1) * (HD + 2) + d];
-  if (starts) {
-    const int r = blockIdx.x / H;
-    if (r < starts[0] || r >= starts[S]) return;
-  }
   const float M = wave_max64(lane < nsp ? ms : -INFINITY);
   const float w = lane < nsp && ms != -INFINITY ? exp2_hw(ms - M) : 0.f;
   const float L = wave_sum64(lane < nsp ? (ms == -INFINITY ? ls : w * ls) : 0.f);
@@ -498,8 +65,8 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
   }
 }
 
-// The same behind the kernel of many rows, whose rows have parts of their own number: a wave a (row, head), which reads those
-// parts alone that it has, N at a time.
+// The same behind the kernel of chunks, for rows of the sequences, which may have parts of their own number: a wave a (row,
+// head), which reads those parts alone that it has, N at a time.
 template <int N>
 __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __restrict__ part, const int32_t* starts, int S,
                                                                  int64_t count, int H, int nsp, uint16_t* out) {
@@ -614,9 +181,6 @@ void launch_rows(const PagedArgs& p, dim3 grid, hipStream_t s) {
   else paged_rows_kernel<Q8, false, false, W><<<grid, W * 64, 0, s>>>(p);
 }
 
-// whether a call goes to the kernel of 128 query rows a workgroup: more than 16 rows per sequence and key head on average
-bool many_rows(int64_t rows, int64_t seqs, int64_t ratio) { return rows * ratio > 16 * seqs; }
-
 template <bool Q8>
 int attention_entry(PagedArgs p, int64_t rows, int64_t seqs, int64_t slots, int64_t heads, int64_t kv_heads, int64_t width,
                     int64_t pages, int64_t P, int64_t splits, int64_t part_len, void* stream, const char* name) {
@@ -640,21 +204,21 @@ int attention_entry(PagedArgs p, int64_t rows, int64_t seqs, int64_t slots, int6
   p.R = (int)rows; p.S = (int)seqs; p.slots = (int)slots; p.W = (int)width; p.pages = (int)pages; p.shift = shift;
   p.H = (int)heads; p.KV = (int)kv_heads; p.ratio = (int)(heads / kv_heads); p.parts = (int)splits;
   p.scale *= LOG2E;
-  const int64_t wgs = tiles_for(rows, seqs, p.ratio, 16, p.starts != nullptr) * kv_heads;
+  // Which kernel a sequence goes to hangs on it alone, and so do its bits: up to 16 query rows a key head few_rows, in a
+  // kernel of its own where every sequence is one token, else in the chunks' kernel, which finds out how long each is.
+  const bool chunks = p.starts || p.ratio > FEW;
+  const int64_t wgs = chunks ? chunk_workgroups(p) : seqs * kv_heads;
   COHERE_REQUIRE(wgs <= TOP && rows * heads <= TOP, nm + ": too many rows and heads");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)wgs, (unsigned)splits);
-  const bool many = many_rows(rows, seqs, p.ratio) && p.scale != 0.f;
-  if (many) launch_chunk(p, Q8, s);
-  else launch_rows<Q8>(p, grid, s);
-  const unsigned hs = (unsigned)(rows * heads);
-  const unsigned hs4 = (hs + 3) / 4;
-  if (many && splits > 4)
+  if (chunks) launch_chunk(p, Q8, s);
+  else launch_rows<Q8>(p, dim3((unsigned)wgs, (unsigned)splits), s);
+  const unsigned hs = (unsigned)(rows * heads), hs4 = (hs + 3) / 4;
+  if (chunks && splits > 4)
     paged_combine_many_kernel<16><<<hs4, 256, 0, s>>>(p.part, p.starts, p.S, hs, p.H, p.parts, p.out);
-  else if (many && splits > 1)
+  else if (chunks && splits > 2)
     paged_combine_many_kernel<4><<<hs4, 256, 0, s>>>(p.part, p.starts, p.S, hs, p.H, p.parts, p.out);
-  else if (splits > 4) paged_combine_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
-  else if (splits > 1) paged_combine_kernel<1, 4><<<hs, HD, 0, s>>>(p.part, p.starts, p.S, p.H, p.parts, p.out);
+  else if (!chunks && splits > 4) paged_combine_kernel<4, 16><<<hs, 4 * HD, 0, s>>>(p.part, p.parts, p.out);
+  else if (!chunks && splits > 1) paged_combine_kernel<1, 4><<<hs, HD, 0, s>>>(p.part, p.parts, p.out);
   return cohere::check_launch(name);
 }
 
@@ -687,17 +251,23 @@ int gather_entry(GatherArgs p, int64_t rows, int64_t slots, int64_t width, int64
 
 extern "C" int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t T) {
   if (rows <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || T <= 0) return 1;
+  const int64_t ratio = heads / kv_heads;
+  const bool many = rows * ratio > FEW * seqs;
+  const int64_t wgs = tiles_for(rows, seqs, ratio, many ? 128 : FEW, rows != seqs) * kv_heads;
+  int64_t n = 1, full = 512, most = 2048, longer = 1024;
+  if (many) {
+    // Two parts are one workgroup's groups of waves. Chunks of 128 tokens over nothing, 64 to 256 workgroups, in 1 and 2 parts
+    // 12.9 to 14.0 and 13.5 to 14.6 us, 320 17.5 and 26; of 512 tokens 25 and 22; of 100 over 2 K, 224, 336 and 456
+    // workgroups, 51 and 43, 67 and 46, 78 and 94; 168, 2 and 4 parts 42 and 35, 224 43 and 49.
+    if (T < 384 || wgs > 448) return 1;
+    if (T < 768 || wgs >= 192) return 2;
+    n = 4; full = 256; most = 1024; longer = 768;
+  }
   // Parts until the GPU is full, and then, where they stay long, until long and short sequences even out. Few-row kernel,
   // of 256 CUs x 2 workgroups: 1 x 8 heads over 64 K positions in 1, 16 and 64 parts 564, 50 and 44 us; 32 x 8 (x 4) over 1
   // .. 16 K, int8, 1, 2 and 8 parts 187, 152 and 126; 64 x 8 over up to 1 K 21, 2 parts 25. Kernel of 128 rows: 256 tokens
-  // over 32 K 606, 16 parts 72, 32 63; 8 x 512 tokens over nothing 25, 2 parts 31.
-  const int64_t ratio = heads / kv_heads;
-  const bool many = many_rows(rows, seqs, ratio);
-  const int64_t wgs = tiles_for(rows, seqs, ratio, many ? 128 : 16, rows != seqs) * kv_heads;
-  const int64_t full = many ? 256 : 512, most = many ? 1024 : 2048, least = 192, longer = many ? 768 : 1024;
-  if (many && wgs >= 192 && wgs <= 448) return 1;  // workgroups of two groups of waves
-  int64_t n = 1;
-  while (n < 64 && wgs * 2 * n <= most && T / (2 * n) >= (wgs * n < full ? least : longer)) n *= 2;
+  // over 32 K 606, 16 parts 72, 32 63; 6 x 100 over 2 K, 1, 2 and 4 parts 50, 41 and 29.
+  while (n < 64 && wgs * 2 * n <= most && T / (2 * n) >= (wgs * n < full ? 192 : longer)) n *= 2;
   return n;
 }
 

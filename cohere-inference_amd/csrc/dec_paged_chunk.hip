@@ -1,7 +1,8 @@
-// dec_attention_paged for chunks of many query rows (paged.h states the pages' form; dec_paged.hip has the few-row kernel
-// and the entry points), for gfx950.
+// dec_attention_paged for chunks (paged.h states the pages' form; dec_paged.hip has the kernel of single tokens and the entry
+// points), for gfx950. A workgroup whose sequence has at most 16 query rows to a key head does paged_rows.h's work on it: how
+// a sequence is worked on must not hang on what else is in the call, and only the GPU knows how long each is.
 //
-// A workgroup takes 128 query rows of a (sequence, key head), 32 a wave, and one part of the keys, 64 at a time: of the
+// Else a workgroup takes 128 query rows of a (sequence, key head), 32 a wave, and one part of the keys, 64 at a time: of the
 // positions held, then of the chunk's own tokens. A tile's keys and values lie in LDS as bf16 (bf16 pages straight from
 // memory, int8 ones converted on the way: codes are exact in bf16, their scales go into the scores and weights); two tiles,
 // so that the next one's loads run under this one's products.
@@ -17,33 +18,33 @@
 // rescaling is rare.
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
 // need three products for one).
-#include "paged.h"
+#include "paged_rows.h"
 
 namespace {
 
 using namespace cohere_paged;
 
 constexpr int KT = 64, TM = 128, W = 4;
+// tiles that a part has at least, so that its start and the joining pay (17 tokens over 8 K, int8, 32 parts asked for: 21 us,
+// with 10 32)
+constexpr int LEAST = 3;
 constexpr float RISE = 8.f;
-
-// what absent keys are read from
-__device__ __attribute__((aligned(16))) uint4 zero_row[1];
-
-typedef short v4s __attribute__((ext_vector_type(4)));
 
 // 16 bytes a lane from src into LDS at dst + 16 lane. Written out, because for the builtin the compiler waits for all such
 // copies in front of the next LDS read, whichever buffer that is of; the waits are tile_barrier's. No register is written,
-// and the compiler's own counts of loads in flight stay safe: more are in flight than it counts, so it waits for more. m0 is
-// used by nothing else in these kernels.
+// and the compiler's own counts of loads in flight stay safe: more are in flight than it counts, so it waits for more.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: nothing lives in it across these, and now nothing is taken to
 DEVI void copy_to_lds(const void* src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
 }
 // the same through a buffer: from `offset` behind its start, zeros behind its end. Five wait states lie between a vector
 // instruction's write of a scalar register and a memory instruction's read of it.
 DEVI void buffer_to_lds(v4i buffer, uint32_t offset, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(offset), "s"(buffer)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 DEVI v4i buffer_of(const void* base, int64_t offset, uint32_t bytes) {
   const uint64_t at = (uint64_t)base + offset;
   const auto uniform = [](uint32_t x) { return (int)__builtin_amdgcn_readfirstlane((int)x); };
@@ -54,18 +55,25 @@ DEVI uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(LDS_AS c
 // the wave's LDS operations done, and its loads
 DEVI void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// G: groups of W waves, each with every G-th tile and buffers of its own, whose results meet in LDS
-template <bool Q8, bool BIG, int G>
+// G: groups of W waves, each with every G-th tile and buffers of its own, whose results meet in LDS (p.parts is 2 then, and
+// there are none in memory); SPLIT: up to p.parts parts
+template <bool Q8, bool BIG, bool SPLIT, int G>
 __global__ void __launch_bounds__(G * W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_chunk_kernel(const PagedArgs p) {
-  __shared__ __attribute__((aligned(16))) char kbuf[G * 2][KT * 256], vbuf[G * 2][KT * 256];
+  __shared__ __attribute__((aligned(256))) char buffers[2][G * 2][KT * 256];
+  auto &kbuf = buffers[0], &vbuf = buffers[1];
   __shared__ __attribute__((aligned(16))) float sscale[Q8 ? G * 2 : 1][2][Q8 ? KT : 1];  // of a tile's keys and values
   const int lane = lane_id(), col = lane & 31, half = lane >> 5;
   const int wave = G == 1 ? wave_id() : wave_id() % W, group = G == 1 ? 0 : wave_id() / W;
-  const int kvh = blockIdx.x % p.KV, sp = blockIdx.y, nsp = p.parts;
+  const int kvh = blockIdx.x % p.KV, sp = SPLIT ? blockIdx.y : 0, nsp = SPLIT ? p.parts : 1;
   // a chunk's last tiles first: they see the most keys, and what starts last ends last
   const Tile t = tile_of<TM>(p, gridDim.x / p.KV - 1 - blockIdx.x / p.KV);
   if (t.rows == 0) return;
+  if ((int64_t)t.c * p.ratio <= FEW) {
+    static_assert(sizeof(FewRows<G * W>) <= sizeof(buffers), "the few-row body's LDS");
+    few_rows<Q8, BIG, SPLIT, G * W>(p, t, kvh, *reinterpret_cast<FewRows<G * W>*>(buffers));
+    return;
+  }
   // the lane's query row (the tile's last one repeated), its token and head
   const int x = t.x0 + min(wave * 32 + col, t.rows - 1), tok = x / p.ratio, head = kvh * p.ratio + (x - tok * p.ratio);
   const bool idle = wave * 32 >= t.rows;  // no row of the wave's
@@ -82,7 +90,7 @@ paged_chunk_kernel(const PagedArgs p) {
       qf[s] = __builtin_bit_cast(v8bf, u);
     }
   }
-  const float scale = fabsf(p.scale);
+  const float scale = p.scale == 0.f ? 0x1p-149f : fabsf(p.scale);  // 0 x -inf, a key that is not there, would be NaN
   int n = t.ok ? p.n[t.slot] : -1;
   const int32_t* row = p.table + (int64_t)t.slot * p.W;
   const int entry0 = row[min(lane >> p.shift, p.W - 1)];  // of a first part's first tile, on its way beside n
@@ -91,8 +99,8 @@ paged_chunk_kernel(const PagedArgs p) {
   const int hi = row_ok ? (t.x0 + t.rows - 1) / p.ratio + 1 : 0;  // the chunk's tokens that the tile's last row sees
   const float rise = rise_of((uint32_t)n + hi);
   const int np = (n + KT - 1) / KT, nb = np + (hi + KT - 1) / KT;
-  // as many parts as there are for `least` tiles each
-  const int parts = max(1, min(nsp, nb / p.least));
+  // as many parts as there are for LEAST tiles each
+  const int parts = SPLIT ? max(1, min(nsp, nb / LEAST)) : 1;
   if (sp >= parts) return;
   const int chunk = (nb + parts - 1) / parts, start = min(nb, sp * chunk), end = min(nb, start + chunk);
   const int P1 = (1 << p.shift) - 1;
@@ -183,7 +191,7 @@ paged_chunk_kernel(const PagedArgs p) {
         const int kk = kk0 + i * 4 + k4;
         const int64_t at = vec_of(t0, entry, kk) * (2 * HD);
         const bool there = live >> kk & 1;
-        const char* zero = reinterpret_cast<const char*>(zero_row);
+        const char* zero = reinterpret_cast<const char*>(zeros);
         copy_to_lds(there ? static_cast<const char*>(p.k) + at + piece_k(i) : zero, kdst + i * 1024);
         copy_to_lds(there ? static_cast<const char*>(p.v) + at + piece_v : zero, vdst + i * 1024);
       }
@@ -484,20 +492,15 @@ int64_t chunk_workgroups(const PagedArgs& p) {
   return tiles_for(p.R, p.S, p.ratio, TM, p.starts != nullptr) * p.KV;
 }
 
-void launch_chunk(PagedArgs p, bool q8, hipStream_t s) {
-  // Tiles that a part has at least: few where there are few workgroups (17 tokens over 8 K, int8, 32 parts asked for: 21 us,
-  // with 10 tiles 32), else enough that a part's start and the joining are small beside it, few enough that long and short
-  // tiles even out (9 ragged sequences of up to 3 K, int8, 2 asked for, with 4, 10 and 16: 86, 82 and 91).
-  const int64_t wgs = chunk_workgroups(p);
-  p.least = wgs < 256 ? 3 : 10;
-  const dim3 grid((unsigned)wgs, (unsigned)p.parts);
-  // Two groups of waves a workgroup (it then has a CU to itself) where there are few workgroups and no parts: the longest
-  // tile takes half as long, and its results meet without a way through memory. 9 ragged sequences in bf16 52 us, with one
-  // group 65, in 2 parts 67; 8 x 512 tokens over nothing 22 and 25; 512 workgroups of one length 92 and 83.
-  const bool two = p.parts == 1 && wgs <= 448;
+void launch_chunk(const PagedArgs& p, bool q8, hipStream_t s) {
+  // Two parts are two groups of waves of one workgroup (it then has a CU to itself): the longest tile takes half as long, and
+  // its results meet without a way through memory. 9 ragged sequences in bf16 52 us, in one part 65, in two through memory
+  // 67; 8 x 512 tokens over nothing 22 and 25; 512 workgroups of one length 92 and 83.
+  const dim3 grid((unsigned)chunk_workgroups(p), p.parts > 2 ? (unsigned)p.parts : 1);
 #define CHUNK(Q, BIG) \
-  (two ? paged_chunk_kernel<Q, BIG, 2><<<grid, 2 * W * 64, 0, s>>>(p)                                                       \
-       : paged_chunk_kernel<Q, BIG, 1><<<grid, W * 64, 0, s>>>(p))
+  (p.parts == 1   ? paged_chunk_kernel<Q, BIG, false, 1><<<grid, W * 64, 0, s>>>(p)     \
+   : p.parts == 2 ? paged_chunk_kernel<Q, BIG, false, 2><<<grid, 2 * W * 64, 0, s>>>(p) \
+                  : paged_chunk_kernel<Q, BIG, true, 1><<<grid, W * 64, 0, s>>>(p))
   if (q8) p.shift >= 4 ? CHUNK(true, true) : CHUNK(true, false);
   else p.shift >= 4 ? CHUNK(false, true) : CHUNK(false, false);
 #undef CHUNK

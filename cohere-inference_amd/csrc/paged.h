@@ -1,4 +1,4 @@
-// Caches in pages, as the kernels over them share it (dec_paged.hip, dec_paged_chunk.hip).
+// Caches in pages, as the kernels over them share it (dec_paged.hip, dec_paged_chunk.hip, paged_rows.h).
 //
 // Pages (pages, KV, P, 128), P a power of two up to 256; position t of slot s is in page table[s][t / P] at t % P. A
 // table entry outside 0 .. pages - 1 is an absent page: its positions are neither read nor written. 16 bits: bf16. 8 bits:
@@ -14,7 +14,10 @@ namespace cohere_paged {
 
 constexpr int HD = 128;  // head size
 constexpr float LOG2E = 1.4426950408889634f;
-typedef float v2f __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+// what absent keys and values are read from
+static __device__ __attribute__((aligned(16))) uint32_t zeros[4];
 
 struct PagedArgs {
   const int32_t *active, *starts;  // starts null: sequence i is row i
@@ -27,7 +30,7 @@ struct PagedArgs {
   float scale;  // times log2(e): scores are powers of two
   uint16_t* out;  // (rows, H * 128)
   float* part;    // (rows, H, parts, 130) when split: outputs, maximum (power of two), sum
-  int parts, least;  // least: tiles of a part, many rows
+  int parts;
 };
 
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -230,8 +233,8 @@ struct Append {
   }
 };
 
-// the kernel for chunks of many query rows (dec_paged_chunk.hip)
+// the kernel for chunks (dec_paged_chunk.hip)
 int64_t chunk_workgroups(const PagedArgs& p);
-void launch_chunk(PagedArgs p, bool q8, hipStream_t s);
+void launch_chunk(const PagedArgs& p, bool q8, hipStream_t s);
 
 }  // namespace cohere_paged

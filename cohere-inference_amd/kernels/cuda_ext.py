@@ -732,7 +732,8 @@ class _Ext:
         positions n[slot].. (n is left to the caller). Slots out of range or with n < 0 get zeros; rows outside
         starts[0]..starts[-1] - 1 are left as they were. A slot, and a page that is appended to, belong to one sequence
         of the call. splits > 1 needs part (rows x H x splits x 130 floats, of one call at a time); out must not overlap
-        q."""
+        q. Weights are held to 2^-17, in bf16 (2^-9) for a sequence with more than 16 query rows to a key head; with the
+        same splits, and starts in both calls or in neither, a sequence's rows are the same bits whatever is beside it."""
         _calls.dec_attention_paged(active, starts, q, k, v, table, n, scale, splits, part, out)
 
     def dec_attention_paged_q8(self, active, starts, q, k, v, ks, vs, table, n, scale, splits, part, out):

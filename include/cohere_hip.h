@@ -332,10 +332,11 @@ int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, 
  * heads * 128]. Rows of a slot out of range, or with n[s] < 0, get zeros, and nothing is appended. Rows in front of
  * starts[0] or from starts[seqs] on are left as they were. A page that is appended to belongs to one sequence of the
  * call, and so does its slot; full pages may be shared by any number. What a row does not attend to never shows in it,
- * NaN and infinities included. out must not overlap q. splits (1 .. 64) divides the keys over workgroups; above 1 it
- * needs part with rows x heads x splits x 130 floats, of one call at a time. fp32 sums, of weights so small that a mean of
- * values up to the type's largest is finite (what values below 2^-70 add may lose digits); the weights are held to 2^-17 of
- * themselves, in bf16 (2^-9) where a sequence and key head have more than 16 query rows on average. */
+ * NaN and infinities included. out must not overlap q. splits (1 .. 64) divides the keys; above 1 it needs part with
+ * rows x heads x splits x 130 floats, of one call at a time. fp32 sums, of weights so small that a mean of values up to the
+ * type's largest is finite (what values below 2^-70 add may lose digits). The weights are held to 2^-17 of themselves, in
+ * bf16 (2^-9) for a sequence with more than 16 query rows to a key head, tokens x heads / kv_heads. With the same splits, and
+ * starts in both calls or in neither, a sequence's rows are the same bits whatever is beside it. */
 int cohere_dec_attention_paged(const int32_t* active, const int32_t* starts, int64_t seqs, const uint16_t* q, int64_t ldq,
                                int64_t rows, uint16_t* k, uint16_t* v, int64_t pages, int64_t P, const int32_t* table,
                                int64_t width, const int32_t* n, int64_t slots, int64_t heads, int64_t kv_heads,
