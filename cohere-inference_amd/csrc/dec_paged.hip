@@ -49,9 +49,15 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
   float o = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (grp + CG * i < nsp) o = add_part(lane_value(w, grp + CG * i), v[i], o);
+    if (grp + CG * i < nsp) o = __builtin_fmaf(lane_value(w, grp + CG * i), v[i], o);
+  if (__builtin_expect(!(fabsf(o) < INFINITY), 0)) {
+    o = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (grp + CG * i < nsp) o = add_part(lane_value(w, grp + CG * i), v[i], o);
+  }
   if constexpr (CG == 1) {
-    out[head * HD + d] = f2bf(L == 0.f ? 0.f : mean_of(o, o / L));
+    out[head * HD + d] = f2bf(L == 0.f ? 0.f : within(o, L) / L);
   } else {
     __shared__ float so[CG][HD];
     so[grp][d] = o;
@@ -60,7 +66,7 @@ __global__ void __launch_bounds__(CG * HD) paged_combine_kernel(const float* __r
       float O = 0.f;
 #pragma unroll
       for (int g = 0; g < CG; ++g) O += so[g][d];
-      out[head * HD + d] = f2bf(L == 0.f ? 0.f : mean_of(O, O / L));
+      out[head * HD + d] = f2bf(L == 0.f ? 0.f : within(O, L) / L);
     }
   }
 }
@@ -84,20 +90,25 @@ __global__ void __launch_bounds__(256) paged_combine_many_kernel(const float* __
   float o0 = 0.f, o1 = 0.f;
   const uint64_t there = __ballot(in);
   const int last = 64 - __clzll(there);
-  for (int i0 = 0; i0 < last; i0 += N) {
-    float2 v[N];
+  const auto join = [&](auto add) {
+    o0 = o1 = 0.f;
+    for (int i0 = 0; i0 < last; i0 += N) {
+      float2 v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = *reinterpret_cast<const float2*>(base + min(i0 + i, last - 1) * (HD + 2) + lane * 2);
+      for (int i = 0; i < N; ++i)
+        v[i] = *reinterpret_cast<const float2*>(base + min(i0 + i, last - 1) * (HD + 2) + lane * 2);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i0 + i < last && there >> (i0 + i) & 1) {  // in the others nothing has to have been written
-        const float wi = lane_value(w, i0 + i);
-        o0 = add_part(wi, v[i].x, o0);
-        o1 = add_part(wi, v[i].y, o1);
-      }
-  }
-  *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(mean_of(o0, o0 / L), mean_of(o1, o1 / L));
+      for (int i = 0; i < N; ++i)
+        if (i0 + i < last && there >> (i0 + i) & 1) {  // in the others nothing has to have been written
+          const float wi = lane_value(w, i0 + i);
+          o0 = add(wi, v[i].x, o0);
+          o1 = add(wi, v[i].y, o1);
+        }
+    }
+  };
+  join([](float a, float x, float o) { return __builtin_fmaf(a, x, o); });
+  if (__builtin_expect(__any(!(fabsf(o0) + fabsf(o1) < INFINITY)), 0)) join(add_part);
+  *reinterpret_cast<uint32_t*>(out + head * HD + lane * 2) = L == 0.f ? 0u : pack_bf2(within(o0, L) / L, within(o1, L) / L);
 }
 
 // ---- reading back ------------------------------------------------------------------------------------------------------
@@ -257,8 +268,8 @@ extern "C" int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs,
   int64_t n = 1, full = 512, most = 2048, longer = 1024;
   if (many) {
     // Two parts are one workgroup's groups of waves. Chunks of 128 tokens over nothing, 64 to 256 workgroups, in 1 and 2 parts
-    // 12.9 to 14.0 and 13.5 to 14.6 us, 320 17.5 and 26; of 512 tokens 25 and 22; of 100 over 2 K, 224, 336 and 456
-    // workgroups, 51 and 43, 67 and 46, 78 and 94; 168, 2 and 4 parts 42 and 35, 224 43 and 49.
+    // 11.0 to 12.1 and 12.8 to 13.7 us, 320 15.8 and 24; of 512 tokens 25 and 22; of 100 over 2 K, 224, 336 and 456
+    // workgroups, 49 and 42, 64 and 46, 77 and 92; 168, 2 and 4 parts 41 and 35, 224 42 and 49.
     if (T < 384 || wgs > 448) return 1;
     if (T < 768 || wgs >= 192) return 2;
     n = 4; full = 256; most = 1024; longer = 768;
@@ -266,7 +277,7 @@ extern "C" int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs,
   // Parts until the GPU is full, and then, where they stay long, until long and short sequences even out. Few-row kernel,
   // of 256 CUs x 2 workgroups: 1 x 8 heads over 64 K positions in 1, 16 and 64 parts 564, 50 and 44 us; 32 x 8 (x 4) over 1
   // .. 16 K, int8, 1, 2 and 8 parts 187, 152 and 126; 64 x 8 over up to 1 K 21, 2 parts 25. Kernel of 128 rows: 256 tokens
-  // over 32 K 606, 16 parts 72, 32 63; 6 x 100 over 2 K, 1, 2 and 4 parts 50, 41 and 29.
+  // over 32 K 606, 16 parts 72, 32 63; 6 x 100 over 2 K, 1, 2 and 4 parts 48, 41 and 29.
   while (n < 64 && wgs * 2 * n <= most && T / (2 * n) >= (wgs * n < full ? 192 : longer)) n *= 2;
   return n;
 }

@@ -136,9 +136,9 @@ paged_chunk_kernel(const PagedArgs p) {
       asm volatile("" : "+v"(first));  // the offsets are made here: kept over the tiles they would take 8 registers
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t offset = (i * 4 + first) * stride;
-        buffer_to_lds(kb, offset + piece_k(i), kdst + i * 1024);
-        buffer_to_lds(vb, offset + piece_v, vdst + i * 1024);
+        const uint32_t offset = (i * 4 + first) * stride, c = lane & 15;
+        buffer_to_lds(kb, offset + (c ^ (i * 4 + first)) * 16, kdst + i * 1024);
+        buffer_to_lds(vb, offset + (c ^ first << 2) * 16, vdst + i * 1024);
       }
       sr = 1.f;
     } else if constexpr (BIG) {  // the wave's keys are one page's
@@ -154,8 +154,8 @@ paged_chunk_kernel(const PagedArgs p) {
         const auto kb = from(p.k, HD), vb = from(p.v, HD);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          kr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, lane * 16 + i * 1024, 0, 0));
-          vr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vb, lane * 16 + i * 1024, 0, 0));
+          kr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, lane * 16, i * 1024, 0));
+          vr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vb, lane * 16, i * 1024, 0));
         }
         const int at = (lane & 15) * 4;
         const uint32_t ks = __builtin_amdgcn_raw_buffer_load_b32(from(p.ks, 4), at, 0, 0),
@@ -424,12 +424,12 @@ paged_chunk_kernel(const PagedArgs p) {
   }
   l = xor32_sum(l);
   if (wave * 32 + col < t.rows) {
-    float zero = 0.f;  // NaN, if an output is not finite
+    float size[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(acc[dt][r], 0.f, zero);
-    if (__builtin_expect((bad || zero != 0.f) && fabsf(l) < INFINITY, 0)) {
+      for (int dt = 0; dt < 4; ++dt) size[dt] += fabsf(acc[dt][r]);
+    if (__builtin_expect((bad || !((size[0] + size[1]) + (size[2] + size[3]) <= TOP * l)) && fabsf(l) < INFINITY, 0)) {
       v4f s[16];  // of the part's keys that the row sees: those held, and up to its own token
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -446,7 +446,7 @@ paged_chunk_kernel(const PagedArgs p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int r = (i & 3) * 4 + k;
-          acc[i >> 2][r] = s[i][k] == 0.f ? acc[i >> 2][r] : s[i][k];
+          acc[i >> 2][r] = s[i][k] == 0.f ? within(acc[i >> 2][r], l) : s[i][k];
         }
     }
     const int64_t at = (int64_t)(t.first + tok) * p.H + head;
@@ -459,7 +459,7 @@ paged_chunk_kernel(const PagedArgs p) {
         for (int g = 0; g < 4; ++g) {
           float o[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = l == 0.f ? 0.f : mean_of(acc[dt][4 * g + k], acc[dt][4 * g + k] * inv);
+          for (int k = 0; k < 4; ++k) o[k] = l == 0.f ? 0.f : acc[dt][4 * g + k] * inv;
           *reinterpret_cast<uint2*>(dst + dt * 32 + g * 8) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
         }
     } else {

@@ -40,10 +40,12 @@ DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 DEVI float rise_of(uint32_t keys) {
   return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint((float)(32 - __clz((int)keys)))));
 }
-// a mean is no larger than the type's largest; the sums' roundings must not make it so
-DEVI float mean_of(float sum, float mean) {
-  constexpr float TOP = 0x1.fep127f;
-  return fabsf(mean) > TOP && fabsf(sum) < INFINITY ? copysignf(TOP, mean) : mean;
+// A mean is no larger than the type's largest, and the sums' roundings must not make it so: a finite sum o of weight x value,
+// `weights` the sum of weights. Whether any of several is too large, or not finite, is seen at their magnitudes' sum.
+constexpr float TOP = 0x1.fep127f;
+DEVI float within(float o, float weights) {
+  const float most = TOP * weights;
+  return fabsf(o) > most && fabsf(o) < INFINITY ? copysignf(most, o) : o;
 }
 
 // One workgroup's sequence and tile of TM query rows (x = token * ratio + head of the key head's): sequence i has the

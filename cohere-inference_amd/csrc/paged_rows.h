@@ -428,20 +428,20 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
       L += mw == -INFINITY ? sl[w][r] : exp2_hw(mw - MM) * sl[w][r];
       O += *reinterpret_cast<const v4f*>(region + w * REGION + (r * LD + dim) * 4);
     }
-    const bool finite = fabsf(O[0]) < INFINITY && fabsf(O[1]) < INFINITY && fabsf(O[2]) < INFINITY && fabsf(O[3]) < INFINITY;
-    if (__builtin_expect((left_out || !finite) && row_ok && fabsf(L) < INFINITY, 0)) {
+    const float size = (fabsf(O[0]) + fabsf(O[1])) + (fabsf(O[2]) + fabsf(O[3]));
+    if (__builtin_expect((left_out || !(size <= TOP * L)) && row_ok && fabsf(L) < INFINITY, 0)) {
       v4f s = {0.f, 0.f, 0.f, 0.f};  // of the part's keys that the row sees: up to its own token, and those held
       for (int j = 0, to = start == 0 && end > 0 ? tk + 1 : 0; j < to; ++j) add_given(s, rowkv + p.KV * HD, p.ldq, j, dim);
       for (int j = max(start - nr, 0) * KB, to = min((int64_t)n, (int64_t)(end - nr) * KB); j < to; ++j)
         add_held<Q8>(s, p, row, kvh, j, dim);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) O[i] = s[i] == 0.f ? O[i] : s[i];
+      for (int i = 0; i < 4; ++i) O[i] = s[i] == 0.f ? within(O[i], L) : s[i];
     }
     const int64_t at = (int64_t)(t.first + tk) * p.H + kvh * p.ratio + (r - tk * p.ratio);
     if (nsp == 1) {
       float o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = L == 0.f ? 0.f : mean_of(O[i], O[i] / L);
+      for (int i = 0; i < 4; ++i) o[i] = L == 0.f ? 0.f : O[i] / L;
       *reinterpret_cast<uint2*>(p.out + at * HD + dim) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
     } else {
       float* part = p.part + (at * nsp + sp) * (HD + 2);  // parts are 520 bytes apart: 8-byte stores
