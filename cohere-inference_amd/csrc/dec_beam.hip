@@ -13,6 +13,7 @@
 #include "common.h"
 #include "rows.h"
 
+#include <algorithm>
 #include <string>
 #include <type_traits>
 
@@ -617,9 +618,17 @@ constexpr int64_t TOP = 0x7fffffff;
 
 }  // namespace
 
+// what a call of so many rows needs
+static int64_t select_work(int64_t rows, int64_t V, int64_t beams) {
+  return rows * select_parts(rows, V) * part_bytes((int)beams);
+}
+
 extern "C" int64_t cohere_dec_beam_select_work(int64_t rows, int64_t V, int64_t beams) {
   if (rows <= 0 || V <= 0 || beams < 1 || beams > MAXB) return 0;
-  return rows * select_parts(rows, V) * part_bytes((int)beams);
+  // the most rows whose workgroups take 2048 logits each: they have the more parts
+  const int64_t most = 255 / ((V + 16383) / 16384);
+  const int64_t need = select_work(rows, V, beams);
+  return rows > most && most > 0 ? std::max(need, select_work(most, V, beams)) : need;
 }
 
 extern "C" int cohere_dec_beam_select_eos(const uint16_t* logits, int64_t ld, int64_t n, int64_t beams, int64_t V,
@@ -637,7 +646,7 @@ extern "C" int cohere_dec_beam_select_eos(const uint16_t* logits, int64_t ld, in
                  "dec_beam_select: bad pointer");
   COHERE_REQUIRE(!norm || (made && norm_len > 0 && norm_len <= TOP), "dec_beam_select: norm needs made");
   if (n == 0) return 0;
-  COHERE_REQUIRE(work && al(work, 8) && work_bytes >= cohere_dec_beam_select_work(n * beams, V, beams),
+  COHERE_REQUIRE(work && al(work, 8) && work_bytes >= select_work(n * beams, V, beams),
                  "dec_beam_select: work of dec_beam_select_work bytes");
   const int64_t rows = n * beams;
   const SelectArgs a{logits, ld, groups, score, finished, made, norm, parent, token, total, static_cast<char*>(work),

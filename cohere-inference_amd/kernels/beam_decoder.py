@@ -80,8 +80,7 @@ class BeamDecoder(StreamDecoder):
         self.parent = torch.zeros(bm, B, **i32)
         self.token = torch.zeros(bm, B, device=dev, dtype=torch.long)
         self.total = torch.zeros(bm, B, device=dev)
-        self.work = torch.empty(max(ext.dec_beam_select_work(b * B, self.head.n, B) for b in self.buckets), device=dev,
-                                dtype=torch.uint8)
+        self.work = torch.empty(ext.dec_beam_select_work(bm * B, self.head.n, B), device=dev, dtype=torch.uint8)
 
     def _idle_rows(self) -> torch.Tensor:
         return self._rows(self.groups).reshape(-1)

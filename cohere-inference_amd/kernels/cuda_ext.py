@@ -752,7 +752,7 @@ class _Ext:
         _calls.dec_gather_paged_q8(slot_of, pos_of, table, k, v, ks, vs, kv)
 
     def dec_beam_select_work(self, rows, V, beams) -> int:
-        """Bytes of dec_beam_select's workspace."""
+        """Bytes of dec_beam_select's workspace for up to `rows` rows, fewer ones too."""
         return int(self._lib.cohere_dec_beam_select_work(int(rows), int(V), int(beams)))
 
     def dec_beam_select(self, logits, groups, score, finished, made, norm, pad, parent, token, total, work, eos=-1):

@@ -383,6 +383,7 @@ int cohere_dec_beam_select_eos(const uint16_t* logits, int64_t ld, int64_t n, in
                                const int32_t* made, const float* norm, int64_t norm_len, int64_t pad, int64_t eos,
                                int32_t* parent, int64_t* token, float* total, void* work, int64_t work_bytes,
                                void* stream);
+/* Bytes of work for a call of up to `rows` rows (n * beams), fewer ones too. */
 int64_t cohere_dec_beam_select_work(int64_t rows, int64_t V, int64_t beams);
 
 /* Every beam takes over its parent's history, in place: row b of group g = groups[i] (slot g * beams + b) gets of row
