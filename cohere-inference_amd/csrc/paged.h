@@ -94,7 +94,7 @@ DEVI Tile tile_of(const PagedArgs& p, int w) {
     t.slot = p.active[i];
   }
   const int64_t left = (int64_t)t.c * p.ratio - t.x0;
-  t.rows = left < TM ? (left > 0 ? (int)left : 0) : TM;
+  t.rows = t.x0 < 0 ? 0 : left < TM ? (left > 0 ? (int)left : 0) : TM;  // below 0: starts that do not ascend
   t.ok = (unsigned)t.slot < (unsigned)p.slots;
   t.slot = t.ok ? t.slot : 0;
   return t;

@@ -324,8 +324,8 @@ int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, 
  * width * P <= 2^30; offsets into the pages are 64 bits wide. 16-byte aligned pages, rows and outputs. */
 
 /* Attention of a chunk of new tokens per sequence. Sequence i (0 .. seqs - 1) is slot s = active[i] with n[s] positions
- * held; its rows of q and out are starts[i] .. starts[i + 1] - 1 (int32 [seqs + 1], ascending, within 0 .. rows; starts
- * null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq <= 2^24] holds heads x 128
+ * held; its rows of q and out are starts[i] .. starts[i + 1] - 1 (int32 [seqs + 1], ascending, within 0 .. rows,
+ * else some rows are left out; starts null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq <= 2^24] holds heads x 128
  * queries, then kv_heads x 128 keys, then the values; query head h reads key head h / (heads / kv_heads). Row j of a
  * sequence, position n[s] + j, attends to positions 0 .. n[s] - 1 as the pages hold them and to rows 0 .. j of its
  * sequence as given, whose keys and values are appended at positions n[s] ..: out = softmax(q k^T scale) v, bf16 [rows,

@@ -77,6 +77,21 @@ def test_few_rows_hold_weights_to_2_17(gpu, bits, splits, ratio, page, chunk):
         assert same_bits(a, b)
 
 
+@pytest.mark.parametrize("starts", [[9, 0, 200], [150, 40, 30], [200, 200, 0], [-5, 7, 1000], [2 ** 31 - 1, 0, -2 ** 31]])
+def test_starts_that_do_not_ascend(gpu, starts):
+    """Nothing outside the rows that are there is read or written: neighbours of out stay as they were."""
+    from kernels.cuda_ext import ext
+
+    c = Paged(70, [30, 20], [100, 100], 2, 3, 16, 16)
+    q, guard = c.q.contiguous().cuda(), torch.full((c.rows + 64, c.H * D), 7.0, dtype=BF, device="cuda")
+    args = (c.k.cuda(), c.v.cuda(), c.table.cuda(), c.n.cuda(), c.scale)
+    for splits in (1, 2, 3):
+        part = torch.empty(c.rows * c.H * splits * 130, device="cuda") if splits > 1 else None
+        ext.dec_attention_paged(c.active.cuda(), torch.tensor(starts, dtype=torch.int32).cuda(), q, *args, splits, part,
+                                guard[32:-32])
+        assert (guard[:32] == 7).all() and (guard[-32:] == 7).all()
+
+
 @pytest.mark.parametrize("kv_bits", [16, 8])
 def test_prompts_of_any_length_do_not_depend_on_each_other(gpu, kv_bits):
     """What the pages hold of a prompt, and the hypotheses behind it, are the same bits alone and beside others."""
