@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(256) beam_advance_kernel(const AdvanceArgs a) 
         a.tok[slot0 + b] = t;
         a.pos[slot0 + b] = p;
         if (a.held) a.held[slot0 + b] = p + 1;
-        if (p < a.OUT) a.out[(slot0 + b) * a.OUT + p] = t;
+        if ((unsigned)p < (unsigned)a.OUT) a.out[(slot0 + b) * a.OUT + p] = t;
         if (lane == 0 && end) {
           a.done[g] = 1;
           if (a.flags) a.flags[g] = 1;

@@ -402,7 +402,7 @@ int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, int64_t bea
 /* The chosen tokens into the groups' state (what cohere_dec_pick_embed does for the greedy choice): for beam b of group g
  * = groups[i], slot r = g * beams + b, with q = parent[i][b], t = token[i][b]: finished[r] = finished[q's] or t == eos or
  * total[i][b] is not above -inf; made[r] = made[q's] + (finished[q's] ? 0 : 1); score[r] = total[i][b]; pos[r] += 1;
- * out[r][pos[r]] = tok[r] = t; held[r] (may be null) = pos[r] + 1, the positions held once tok has been read. done[g] = 1
+ * out[r][pos[r]] = tok[r] = t (out where there is such a position); held[r] (may be null) = pos[r] + 1, the positions held once tok has been read. done[g] = 1
  * (and flags_host[g], pinned host memory, may be null) once all beams have finished, once the best has and by_length is 0,
  * and at pos >= limit[g]. The group dummy, and groups that are done, keep their state. Then x, h [n_groups * beams, width]
  * get the embedding of tok at pos, as cohere_dec_embed (emb [vocabulary, width], ptab [positions, width]; indexes out of

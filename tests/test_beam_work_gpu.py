@@ -1,4 +1,4 @@
-"""dec_beam_select with one workspace for batches of every size."""
+"""dec_beam_select with one workspace for batches of every size; dec_beam_advance at the ends of its rows."""
 
 from __future__ import annotations
 
@@ -28,3 +28,27 @@ def test_one_workspace_for_all_batches(gpu):
         assert torch.equal(token.cpu(), want[1]) and torch.equal(parent.cpu(), want[0])
         err = (total.cpu().double() - want[2]).abs()
         assert (err <= 2.0 ** -24 * want[2].abs() * (1 + 2.0 ** -20) + 2.0 ** -32).all()
+
+
+def test_advance_at_positions_that_out_does_not_have(gpu):
+    """Positions below zero and behind the last one: the state moves on, and no row's tokens change."""
+    from kernels.cuda_ext import ext
+
+    G, B, OUT, width = 3, 2, 6, 256
+    groups = torch.arange(G, dtype=torch.int32).cuda()
+    parent, token = torch.zeros(G, B, dtype=torch.int32).cuda(), torch.full((G, B), 9).cuda()
+    total = torch.full((G, B), -1.0).cuda()
+    pos = torch.tensor([-40, -40, 5, 5, 3, 3], dtype=torch.int32)
+    guard = torch.full((G * B + 16, OUT), 7).cuda()  # rows of other memory around out
+    tok, score = torch.zeros(G * B, dtype=torch.int64).cuda(), torch.zeros(G, B).cuda()
+    ended, made = torch.zeros(G, B, dtype=torch.uint8).cuda(), torch.zeros(G, B, dtype=torch.int32).cuda()
+    done, limit = torch.zeros(G, dtype=torch.uint8).cuda(), torch.full((G,), 100, dtype=torch.int32).cuda()
+    emb, ptab = torch.ones(16, width, dtype=BF).cuda(), torch.ones(8, width, dtype=BF).cuda()
+    ln = torch.ones(width, dtype=BF).cuda()
+    x, h = (torch.empty(G * B, width, dtype=BF).cuda() for _ in range(2))
+    pos_d = pos.cuda()
+    ext.dec_beam_advance(groups, parent, token, total, G, tok, pos_d, None, score, ended, made, done, limit, guard[8:-8], 3,
+                         False, emb, ptab, ln, ln, 1e-5, ln, ln, 1e-5, x, h, None)
+    want = torch.full((G * B + 16, OUT), 7)
+    want[8 + 4:8 + 6, 4] = 9
+    assert torch.equal(guard.cpu(), want) and torch.equal(pos_d.cpu(), pos + 1)
