@@ -5,17 +5,17 @@
 // Else a workgroup takes 128 query rows of a (sequence, key head), 32 a wave, and one part of the keys, 64 at a time: of the
 // positions held, then of the chunk's own tokens. A tile's keys and values lie in LDS as bf16 (bf16 pages straight from
 // memory, int8 ones converted on the way: codes are exact in bf16, their scales go into the scores and weights); two tiles,
-// so that the next one's loads run under this one's products.
+// so that the next one's loads run under this one's products. (Not those of int8 pages yet: a lane chooses between the scales
+// of keys and values as soon as it has asked for them, which waits for the wave's loads.)
 //   S^T = K Q^T on v_mfma_f32_32x32x16_bf16: queries in registers, a lane's result is 16 keys of query l % 32.
 //   O^T = V^T P^T on the same instruction: the weights as they stand are its B operand (the order of the 16 keys of a
 //   product is free, and taken as the lanes hold them), V^T comes through the transposing LDS read.
 // What bounds it: a tile's 32 products keep a SIMD's matrix core 1024 cycles and its 200 vector instructions (32 exponentials
 // at 8 cycles) about as long; a wave does one after the other, and two waves a SIMD, what the registers allow, overlap them
 // only in part. 4 x 2048 tokens x 32 heads behind 6 to 8 K positions: 1044 us, 1054 TFLOP/s (a large product of the library:
-// 1188); a tile alone on its CU takes 1.2 us, int8 1.7 (their conversion).
-// Maximum, sum and outputs of a query stay in lanes l % 32 = query. The base of a query's weights is set 2^8 above its
-// largest score and the number of keys above that (rise_of), and moves only when a score passes the latter, so that
-// rescaling is rare.
+// 1188); a tile alone on its CU takes 1.2 us, int8 1.7 (that wait, and their conversion).
+// Maximum, sum and outputs of a query stay in lanes l % 32 = query. The base of a query's weights is set 2^8 above what its
+// largest score needs (bits_of), and moves only when a score needs more, so that rescaling is rare.
 // Rounded to fewer bits: the weights, to bf16 for the second product (off by at most 2^-9 of themselves; exact ones would
 // need three products for one).
 #include "paged_rows.h"
@@ -34,7 +34,7 @@ constexpr float RISE = 8.f;
 // copies in front of the next LDS read, whichever buffer that is of; the waits are tile_barrier's. No register is written,
 // and the compiler's own counts of loads in flight stay safe: more are in flight than it counts, so it waits for more.
 #pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: nothing lives in it across these, and now nothing is taken to
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved, and named so that nothing is taken to live in it
 DEVI void copy_to_lds(const void* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
 }
@@ -97,7 +97,7 @@ paged_chunk_kernel(const PagedArgs p) {
   const bool row_ok = n >= 0;
   n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
   const int hi = row_ok ? (t.x0 + t.rows - 1) / p.ratio + 1 : 0;  // the chunk's tokens that the tile's last row sees
-  const float rise = rise_of((uint32_t)n + hi);
+  const float rise = (float)bits_of((uint32_t)n + hi);
   const int np = (n + KT - 1) / KT, nb = np + (hi + KT - 1) / KT;
   // as many parts as there are for LEAST tiles each
   const int parts = SPLIT ? max(1, min(nsp, nb / LEAST)) : 1;

@@ -35,11 +35,9 @@ struct PagedArgs {
 
 DEVI float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Weights are at most 2^-rise of a row's number of keys, so that their sum is below 1 and that of weight x value no larger
+// Weights are at most 2^-bits_of(a row's number of keys), so that their sum is below 1 and that of weight x value no larger
 // than the largest value: with weights up to 1 two of the type's largest would be infinite before the division.
-DEVI float rise_of(uint32_t keys) {
-  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint((float)(32 - __clz((int)keys)))));
-}
+DEVI int bits_of(uint32_t keys) { return __builtin_amdgcn_readfirstlane(32 - __clz((int)keys)); }
 // A mean is no larger than the type's largest, and the sums' roundings must not make it so: a finite sum o of weight x value,
 // `weights` the sum of weights. Whether any of several is too large, or not finite, is seen at their magnitudes' sum.
 constexpr float TOP = 0x1.fep127f;

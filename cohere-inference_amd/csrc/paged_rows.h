@@ -52,7 +52,7 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
   const int P1 = (1 << p.shift) - 1;
   // the blocks: of the chunk's own tokens, 16 at most, then of the positions held; wave w has every W-th
   int n = 0, nb = 0, start = 0, end = 0, b = wave;
-  float rise = 0.f;
+  float most = 0.f;  // a weight's
   bool row_ok = false;
   const int held = p.n[t.slot];  // on its way
   const auto bounds = [&]() {
@@ -60,7 +60,7 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
     row_ok = n >= 0;
     n = (int)min((int64_t)max(n, 0), (int64_t)p.W << p.shift);
     nb = row_ok ? nr + (n + KB - 1) / KB : 0;
-    rise = rise_of((uint32_t)n + t.c);
+    most = __uint_as_float((uint32_t)(127 - bits_of((uint32_t)n + t.c)) << 23);
   };
   if constexpr (SPLIT) {  // without parts nothing up to the first loads waits for n
     bounds();
@@ -126,7 +126,7 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        d[h][i] = exp2_hw(d[h][i] - to - rise);
+        d[h][i] = exp2_hw(d[h][i] - to) * most;
         l += d[h][i];
       }
   };
@@ -164,7 +164,7 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
   // the chunk's own tokens, as given; bad: some of their values are infinite or NaN
   bool bad = false;
   if (!single && b == 0) {
-    if constexpr (!SPLIT) bounds();  // the weights' rise
+    if constexpr (!SPLIT) bounds();  // what a weight is at most
     const auto own_row = [&](int j) { return rowkv + (int64_t)min(j, t.c - 1) * p.ldq; };
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -298,7 +298,7 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
     }
     dot = xor32_sum(xor16_sum(dot)) * p.scale;
     m = dot == dot ? dot : -INFINITY;  // maxima pass over a NaN, the sum keeps it
-    const float e = dot == -INFINITY ? 0.f : exp2_hw(dot - m - rise);
+    const float e = dot == -INFINITY ? 0.f : exp2_hw(dot - m) * most;
     l = grp == 0 ? e : 0.f;
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
