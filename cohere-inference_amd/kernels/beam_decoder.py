@@ -32,7 +32,8 @@ from kernels.stream_decoder import Grammar, Rules, StreamDecoder
 
 class BeamDecoder(StreamDecoder):
     """StreamDecoder with `beams` hypotheses (1..16) a slot; buckets count slots. length_penalty: 0 ranks by the sum of
-    log probabilities, 1 by their mean. page: positions a page (a power of two up to 256). kv_bits: 16 or 8."""
+    log probabilities, 1 by their mean. page: positions a page (a power of two up to 256). kv_bits: 16 or 8. A request's
+    hypotheses do not depend on the others admitted or stepped with it."""
 
     def __init__(self, model, slots: int = 32, max_new_tokens: int = 448, max_prompt: int = 16, max_audio_s: float = 36.0,
                  buckets=None, int8: bool = False, frames: int | None = None, capture: bool = True,

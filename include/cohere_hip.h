@@ -324,10 +324,10 @@ int cohere_dec_logits(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, 
  * width * P <= 2^30; offsets into the pages are 64 bits wide. 16-byte aligned pages, rows and outputs. */
 
 /* Attention of a chunk of new tokens per sequence. Sequence i (0 .. seqs - 1) is slot s = active[i] with n[s] positions
- * held; its rows of q and out are starts[i] .. starts[i + 1] - 1 (int32 [seqs + 1], ascending, within 0 .. rows,
- * else some rows are left out; starts null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq <= 2^24] holds heads x 128
- * queries, then kv_heads x 128 keys, then the values; query head h reads key head h / (heads / kv_heads). Row j of a
- * sequence, position n[s] + j, attends to positions 0 .. n[s] - 1 as the pages hold them and to rows 0 .. j of its
+ * held; its rows of q and out are starts[i] .. starts[i + 1] - 1 (int32 [seqs + 1], ascending, within 0 .. rows, else
+ * some rows are left out; starts null: row i alone, rows == seqs). A sequence without rows is nothing. q [rows, ldq <=
+ * 2^24] holds heads x 128 queries, then kv_heads x 128 keys, then the values; query head h reads key head h / (heads /
+ * kv_heads). Row j of a sequence, position n[s] + j, attends to positions 0 .. n[s] - 1 as the pages hold them and to rows 0 .. j of its
  * sequence as given, whose keys and values are appended at positions n[s] ..: out = softmax(q k^T scale) v, bf16 [rows,
  * heads * 128]. Rows of a slot out of range, or with n[s] < 0, get zeros, and nothing is appended. Rows in front of
  * starts[0] or from starts[seqs] on are left as they were. A page that is appended to belongs to one sequence of the
@@ -347,7 +347,8 @@ int cohere_dec_attention_paged_q8(const int32_t* active, const int32_t* starts, 
                                   int64_t heads, int64_t kv_heads, float scale, int64_t splits, float* part,
                                   int64_t part_len, uint16_t* out, void* stream);
 
-/* The number of splits that fills the GPU for such a call over up to T positions (1 for sizes that it would refuse). */
+/* The number of splits that fills the GPU for such a call over up to T positions, the longest sequence's (1 for sizes that
+ * it would refuse). */
 int64_t cohere_dec_attention_paged_splits(int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t T);
 
 /* What the pages of all layers, k, v (L, pages, kv_heads, P, 128) and scales (L, pages, kv_heads, P), hold of position
@@ -402,9 +403,9 @@ int cohere_dec_beam_reorder(const int32_t* groups, int64_t n_groups, int64_t bea
 /* The chosen tokens into the groups' state (what cohere_dec_pick_embed does for the greedy choice): for beam b of group g
  * = groups[i], slot r = g * beams + b, with q = parent[i][b], t = token[i][b]: finished[r] = finished[q's] or t == eos or
  * total[i][b] is not above -inf; made[r] = made[q's] + (finished[q's] ? 0 : 1); score[r] = total[i][b]; pos[r] += 1;
- * out[r][pos[r]] = tok[r] = t (out where there is such a position); held[r] (may be null) = pos[r] + 1, the positions held once tok has been read. done[g] = 1
- * (and flags_host[g], pinned host memory, may be null) once all beams have finished, once the best has and by_length is 0,
- * and at pos >= limit[g]. The group dummy, and groups that are done, keep their state. Then x, h [n_groups * beams, width]
+ * out[r][pos[r]] = tok[r] = t (out where there is such a position); held[r] (may be null) = pos[r] + 1, the positions held
+ * once tok has been read. done[g] = 1 (and flags_host[g], pinned host memory, may be null) once all beams have finished,
+ * once the best has and by_length is 0, and at pos >= limit[g]. The group dummy, and groups that are done, keep their state. Then x, h [n_groups * beams, width]
  * get the embedding of tok at pos, as cohere_dec_embed (emb [vocabulary, width], ptab [positions, width]; indexes out of
  * range are brought into it). A group is named once (the dummy any
  * number of times). */
