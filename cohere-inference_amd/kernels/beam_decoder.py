@@ -90,12 +90,11 @@ class BeamDecoder(StreamDecoder):
 
     def _paged(self, i: int, act, starts, n, qkv, out):
         """Layer i's self-attention over pages (and the append) of rows qkv."""
-        k, v = self.self_k[i], self.self_v[i]
+        k, v, table, scale = self.self_k[i], self.self_v[i], self.table, self.scale
         if self.kv_bits == 8:
             ks, vs = self.self_ks[i], self.self_vs[i]
-            return lambda: ext.dec_attention_paged_q8(act, starts, qkv, k, v, ks, vs, self.table, n, self.scale, 1, None,
-                                                      out)
-        return lambda: ext.dec_attention_paged(act, starts, qkv, k, v, self.table, n, self.scale, 1, None, out)
+            return lambda: ext.dec_attention_paged_q8(act, starts, qkv, k, v, ks, vs, table, n, scale, 1, None, out)
+        return lambda: ext.dec_attention_paged(act, starts, qkv, k, v, table, n, scale, 1, None, out)
 
     def _cross(self, i: int, slot_of, q, out):
         return super()._attention(i, False, slot_of, q, 1, out)
@@ -106,19 +105,18 @@ class BeamDecoder(StreamDecoder):
         bufs, logits = self._buffers(rows), self.logits[:rows]
         parent, token, total = self.parent[:b], self.token[:b], self.total[:b]
         layers = range(len(self.blocks))
-        eos = self.eos if 0 <= self.eos < self.head.n else -1
+        select = (self.score, self.ended, None if self.norm is None else self.made, self.norm, self.pad, parent, token,
+                  total, self.work, self.eos if 0 <= self.eos < self.head.n else -1)
+        reorder = (self.held, self.finished, self.table, self.out, self.gstate, self.self_k, self.self_v, self.self_ks,
+                   self.self_vs)
+        advance = (self.dummy, self.tok, self.pos, self.held, self.score, self.ended, self.made, self.finished, self.limit,
+                   self.out, self.eos, self.norm is not None, *self._embedding(), bufs.x, bufs.hn, self.flags)
         return (self._layers(bufs, [self._paged(i, act, None, self.pos, bufs.qkv, bufs.att) for i in layers],
                              [self._cross(i, slot_of, bufs.q, bufs.att) for i in layers])
                 + self._head(bufs, logits) + self._rules(act, logits)
-                + [lambda: ext.dec_beam_select(logits, groups, self.score, self.ended,
-                                               None if self.norm is None else self.made, self.norm, self.pad, parent,
-                                               token, total, self.work, eos),
-                   lambda: ext.dec_beam_reorder(groups, parent, self.held, self.finished, self.table, self.out,
-                                                self.gstate, self.self_k, self.self_v, self.self_ks, self.self_vs),
-                   lambda: ext.dec_beam_advance(groups, parent, token, total, self.dummy, self.tok, self.pos, self.held,
-                                                self.score, self.ended, self.made, self.finished, self.limit, self.out,
-                                                self.eos, self.norm is not None, self.embed, self.pos_table,
-                                                *self.emb_ln, *self.blocks[0].norms[0], bufs.x, bufs.hn, self.flags)])
+                + [lambda: ext.dec_beam_select(logits, groups, *select),
+                   lambda: ext.dec_beam_reorder(groups, parent, *reorder),
+                   lambda: ext.dec_beam_advance(groups, parent, token, total, *advance)])
 
     @property
     def _embeds_ahead(self) -> bool:
@@ -222,8 +220,7 @@ class BeamDecoder(StreamDecoder):
         w = self.width
         bufs = types.SimpleNamespace(x=new(w), hn=new(w), att=new(w), qkv=new(3 * w), q=new(w), proj=new(w),
                                      ffn=new(self.blocks[0].fc1.n))
-        ext.dec_embed(every, tok, pos_d, self.embed, self.pos_table, *self.emb_ln, *self.blocks[0].norms[0], bufs.x,
-                      bufs.hn)
+        ext.dec_embed(every, tok, pos_d, *self._embedding(), bufs.x, bufs.hn)
         nothing = torch.zeros_like(self.pos)  # nothing is held yet
         layers = range(len(self.blocks))
         ops = self._layers(bufs, [self._paged(i, first, starts_d, nothing, bufs.qkv, bufs.att) for i in layers],

@@ -15,7 +15,9 @@ as a fixed list of launches over preallocated buffers and captured into one HIP 
 
 from __future__ import annotations
 
+import contextlib
 import dataclasses
+import gc
 import math
 import types
 
@@ -156,6 +158,20 @@ class Rules:
 
 
 # ---- the decoder and its captured step ------------------------------------------------------------------------------
+
+@contextlib.contextmanager
+def _no_collection():
+    """No garbage collection in the block: the end of another graph, of anything in a cycle, is an error while one is
+    captured (it waits for the GPU), which ends the process."""
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if was:
+            gc.enable()
+
+
 
 class _Projection:
     """One decoder linear bound to its skinny kernel: int8 weights in prepare_w8's layout through dec_w8_linear, or
@@ -329,6 +345,11 @@ class StreamDecoder:
         if capture:
             self._capture()
 
+    def __del__(self):
+        # what is still queued on the decoder's stream reads and writes buffers that are about to be freed
+        with contextlib.suppress(Exception):
+            self.stream.synchronize()
+
     def _cache(self, slots: int, t: int):
         """A cache of every layer and its scales (None in 16 bits): (layer, slot, head, position, ..), or pages."""
         dims, dev = (len(self.blocks), slots, self.h, t), dict(device=self.device)
@@ -362,21 +383,29 @@ class StreamDecoder:
             k, v, ks, vs, n = self.self_k[i], self.self_v[i], self.self_ks, self.self_vs, self.pos
         else:
             k, v, ks, vs, n = self.cross_k[i], self.cross_v[i], self.cross_ks, self.cross_vs, self.cross_len
+        scale, part = self.scale, self.part
         if self.kv_bits == 4:
             ks, vs = ks[i], vs[i]
-            return lambda: ext.dec_attention_q4(self_attn, act, q, k, v, ks, vs, n, self.scale, splits, self.part, out)
+            return lambda: ext.dec_attention_q4(self_attn, act, q, k, v, ks, vs, n, scale, splits, part, out)
         if self.kv_bits == 8:
             ks, vs = ks[i], vs[i]
-            return lambda: ext.dec_attention_q8(self_attn, act, q, k, v, ks, vs, n, self.scale, splits, self.part,
-                                                out)
-        return lambda: ext.dec_attention(self_attn, act, q, k, v, n, self.scale, splits, self.part, out)
+            return lambda: ext.dec_attention_q8(self_attn, act, q, k, v, ks, vs, n, scale, splits, part, out)
+        return lambda: ext.dec_attention(self_attn, act, q, k, v, n, scale, splits, part, out)
 
     def _program(self, b: int) -> list:
         """The step for the first b active rows (reference stream_decoder.py:176-199): embedding + first LayerNorm,
         per layer self-attention (qkv, attention over the slot's cache, o, residual + LayerNorm), cross-attention (q,
         attention over the slot's frames, o, residual + LayerNorm) and feed-forward (fc1 + ReLU, fc2, residual + the
-        next LayerNorm), then the head, the greedy pick and the end flags' copy to the host."""
+        next LayerNorm), then the head, the greedy pick and the end flags' copy to the host.
+
+        The launches hold tensors and weights, not the decoder: in a cycle with its program it would live on until a
+        garbage collection, which may come while a graph is captured, where its own graphs' end is an error that ends
+        the process."""
         act, bufs, logits = self.active[:b], self._buffers(b), self.logits[:b]
+        state = (self.dummy, self.tok, self.pos, self.finished, self.forced, self.plen, self.limit, self.out, self.pad,
+                 self.eos)
+        embedding = self._embedding()
+        flags, finished = self.flags, self.finished
         self_attn = [self._attention(i, True, act, bufs.qkv, 1, bufs.att) for i in range(len(self.blocks))]
         cross = [self._attention(i, False, act, bufs.q, self._splits(b), bufs.att) for i in range(len(self.blocks))]
         ops = self._layers(bufs, self_attn, cross) + self._head(bufs, logits) + self._rules(act, logits)
@@ -384,14 +413,15 @@ class StreamDecoder:
             # the pick computes the next step's embedding of its row and writes the end flags to the host itself. The
             # same bits as the unfused step. The step's own embedding comes from the previous step's pick, or from
             # step() when the rows changed.
-            return ops + [lambda: ext.dec_pick_embed(logits, act, self.dummy, self.tok, self.pos, self.finished,
-                                                     self.forced, self.plen, self.limit, self.out, self.pad, self.eos,
-                                                     self.embed, self.pos_table, *self.emb_ln, *self.blocks[0].norms[0],
-                                                     bufs.x, bufs.hn, self.flags)]
-        return [lambda: self._embed(b)] + ops + [
-            lambda: ext.dec_pick(logits, act, self.dummy, self.tok, self.pos, self.finished, self.forced, self.plen,
-                                 self.limit, self.out, self.pad, self.eos),
-            lambda: self.flags.copy_(self.finished, non_blocking=True)]
+            return ops + [lambda: ext.dec_pick_embed(logits, act, *state, *embedding, bufs.x, bufs.hn, flags)]
+        tok, pos = self.tok, self.pos
+        return [lambda: ext.dec_embed(act, tok, pos, *embedding, bufs.x, bufs.hn)] + ops + [
+            lambda: ext.dec_pick(logits, act, *state),
+            lambda: flags.copy_(finished, non_blocking=True)]
+
+    def _embedding(self) -> tuple:
+        """The embedding's tables and LayerNorms, and the first layer's."""
+        return (self.embed, self.pos_table, *self.emb_ln, *self.blocks[0].norms[0])
 
     def _buffers(self, rows: int) -> types.SimpleNamespace:
         """The step buffers of the first `rows` rows."""
@@ -433,23 +463,23 @@ class StreamDecoder:
         return ops
 
     def _head(self, bufs, logits) -> list:
+        head, ln = self.head, self.final_ln
         if self.fused:
-            return [lambda: self.head.fused(bufs.x, logits, ln=self.final_ln)]
-        return [lambda: self.head(bufs.hn, logits)]
+            return [lambda: head.fused(bufs.x, logits, ln=ln)]
+        return [lambda: head(bufs.hn, logits)]
 
     def _rules(self, act, logits) -> list:
         """The requests' rules on the logits, in place (nothing where the decoder was built without any)."""
         if not self.rules_on:
             return []
-        return [lambda: ext.dec_logits(logits, logits, act, self.pos, self.out, self.first, self.plen, self.pen,
-                                       self.bias, self.bias_of, self.mask, self.classes, self.trans, self.start,
-                                       self.gstate)]
+        rules = (self.pos, self.out, self.first, self.plen, self.pen, self.bias, self.bias_of, self.mask, self.classes,
+                 self.trans, self.start, self.gstate)
+        return [lambda: ext.dec_logits(logits, logits, act, *rules)]
 
     def _embed(self, b: int) -> None:
         """The embedding and first LayerNorm of the bucket's active rows (x, hn), on the current stream."""
         rows = b * self.beams
-        ext.dec_embed(self.active[:rows], self.tok, self.pos, self.embed, self.pos_table, *self.emb_ln,
-                      *self.blocks[0].norms[0], self.x[:rows], self.hn[:rows])
+        ext.dec_embed(self.active[:rows], self.tok, self.pos, *self._embedding(), self.x[:rows], self.hn[:rows])
 
     @property
     def _embeds_ahead(self) -> bool:
@@ -475,13 +505,13 @@ class StreamDecoder:
                 self._run(b)
                 self.stream.synchronize()
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=self.stream):
+                with _no_collection(), torch.cuda.graph(g, stream=self.stream):
                     for op in self.programs[b]:  # the program only: step() adds the embedding when the rows change
                         op()
                 self.graphs[b] = g
                 if self.chunk > 1:
                     g = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(g, stream=self.stream):
+                    with _no_collection(), torch.cuda.graph(g, stream=self.stream):
                         for _ in range(self.chunk):
                             for op in self.programs[b]:
                                 op()
