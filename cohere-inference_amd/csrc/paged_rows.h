@@ -24,7 +24,7 @@ template <int W>
 struct FewRows {
   static constexpr int LD = HD + 4, REGION = FEW * LD * 4;  // a wave's values (32 x 256 bytes), later its outputs
   static_assert(REGION >= KB * 256 && REGION % 256 == 0, "a wave's region");
-  alignas(256) char region[W][REGION];
+  alignas(256) char region[W * REGION];
   float m[W][FEW], l[W][FEW];
   int bad[W];
 };
@@ -44,7 +44,7 @@ DEVI void few_rows(const PagedArgs& p, const Tile& t, int kvh, FewRows<W>& lds) 
   auto& sm = lds.m;
   auto& sl = lds.l;
   auto& sbad = lds.bad;
-  char* const region = lds.region[0];
+  char* const region = lds.region;
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), col = lane & 15, grp = lane >> 4;
   const int sp = SPLIT ? blockIdx.y : 0, nsp = SPLIT ? p.parts : 1;
   char* sv = region + wave * REGION;
